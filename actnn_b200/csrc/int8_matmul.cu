@@ -1,0 +1,319 @@
+// Matrix product of 8-bit integers with a scale for each token and each output channel:
+//
+//   out[t, n] = (sum_k x[t, k] * w[n, k]) * token_scale[t] * channel_scale[n] + bias[n]
+//
+// The sum is exact (int32; k <= 131072 keeps it below 2^31), the scales and the bias are applied in fp32 and rounded once.
+//
+// The tensor cores compute tiles of 128 channels (the rows of the accumulator, one lane of tensor memory each) by up to 256
+// tokens (its columns): the operand with 128 rows is the weight, so that few tokens waste no work, and a thread of the
+// epilogue has one channel, whose scale and bias stay in registers while 32 lanes write 32 neighbouring outputs of a token.
+// A block is a pipeline: one thread requests tiles of both operands (128 bytes of the reduction a stage, swizzled for the
+// matrix instructions), one issues the matrix instructions, eight warps scale and write one accumulator while the next one
+// fills.  Where the tiles are too few for the SMs, the reduction is split over the blocks of a cluster, which add their
+// integer sums through distributed shared memory: order does not matter to them.
+//
+// Every wait is bounded.  A block whose wait runs out writes nothing more, is counted (the counter of the bulk waits), lets
+// its copies and instructions end and leaves.
+#include <atomic>
+
+#include "activation.cuh"
+#include "tcgen05.cuh"
+
+namespace actnn {
+namespace {
+
+constexpr int kMmThreads = 320;                 // 8 epilogue warps, one for the copies, one for the matrix instructions
+constexpr int kMmEpilogue = 256;
+constexpr int kMmStagesMost = 8;
+constexpr int kMmStageK = 128;                  // bytes of the reduction in a stage
+constexpr int kMmChannels = 128;
+constexpr int kMmSmem = 212 * 1024;             // of the SM's 227 KB: stages, and 1 KB to align them
+
+struct MmArgs {
+  const float *token_scale, *channel_scale;
+  const void* bias;
+  void* out;
+  int64_t T, N;
+  int K, tokens, stages, k_blocks, splits;      // tokens: columns of a tile
+  int channel_tiles, tiles, columns;            // columns: of tensor memory, a buffer
+};
+
+struct MmShared {
+  uint64_t full[kMmStagesMost], empty[kMmStagesMost], sum_full[2], sum_empty[2], drained;
+  uint32_t tmem;
+  int dead;
+  float scale[2][256];
+};
+
+// Waits for a phase; false once this or another wait of the block has run out.
+ACTNN_DEV bool mm_wait(uint32_t bar, uint32_t parity, MmShared& s, unsigned* gave_up) {
+  volatile int* dead = &s.dead;
+  for (uint32_t i = 0; i < kBulkWaitTries; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (*dead) return false;
+  }
+  *dead = 1;
+  if (gave_up) atomicAdd(gave_up, 1u);
+  return false;
+}
+
+template <typename T, bool SPLIT>
+__global__ void __launch_bounds__(kMmThreads, 1)
+int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens, const MmArgs a,
+                   unsigned* gave_up) {
+  extern __shared__ uint8_t dynamic_s[];
+  __shared__ MmShared s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t stage0 = (smem_addr(dynamic_s) + 1023u) & ~1023u;
+  const uint32_t a_bytes = kMmChannels * kMmStageK, stage_bytes = a_bytes + a.tokens * kMmStageK;
+  const uint32_t split = SPLIT ? cluster_rank() : 0;
+  const int k_first = SPLIT ? (int)((int64_t)split * a.k_blocks / a.splits) : 0;
+  const int k_end = SPLIT ? (int)((int64_t)(split + 1) * a.k_blocks / a.splits) : a.k_blocks;
+  const int first_tile = SPLIT ? blockIdx.x / a.splits : blockIdx.x, tile_step = SPLIT ? a.tiles : gridDim.x;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < a.stages; ++i) {
+      mbar_init(smem_addr(&s.full[i]), 1);
+      mbar_init(smem_addr(&s.empty[i]), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_addr(&s.sum_full[i]), 1);
+      mbar_init(smem_addr(&s.sum_empty[i]), kMmEpilogue / 32);
+    }
+    mbar_init(smem_addr(&s.drained), 1);
+    s.dead = 0;
+    mbar_init_fence();
+  }
+  const uint32_t columns = SPLIT ? a.columns : 2 * a.columns;
+  if (warp == 9) tmem_alloc(smem_addr(&s.tmem), columns);
+  tmem_fence_before_sync();
+  __syncthreads();
+  tmem_fence_after_sync();
+  const uint32_t tmem = s.tmem;
+
+  if (warp == 8) {                                              // ---------------- copies
+    if (lane == 0) {
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+        const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
+        for (int k = k_first; k < k_end; ++k) {
+          if (!(ok = mm_wait(smem_addr(&s.empty[stage]), phase ^ 1, s, gave_up))) break;
+          const uint32_t bar = smem_addr(&s.full[stage]), dst = stage0 + stage * stage_bytes;
+          mbar_expect_tx(bar, stage_bytes);
+          tile_load(dst, &weights, k * kMmStageK, ct * kMmChannels, bar);
+          tile_load(dst + a_bytes, &tokens, k * kMmStageK, tt * a.tokens, bar);
+          ++issued;
+          if (++stage == a.stages) stage = 0, phase ^= 1;
+        }
+      }
+      if (!ok) {                                                // what was requested still lands in this block's memory
+        for (int i = 0; i < a.stages && i < issued; ++i) {
+          if (--stage < 0) stage = a.stages - 1, phase ^= 1;
+          mbar_wait(smem_addr(&s.full[stage]), phase);
+        }
+      }
+    }
+  } else if (warp == 9) {                                       // ---------------- matrix instructions
+    if (lane == 0) {
+      const uint32_t instruction = int8_instruction(a.tokens);
+      int stage = 0, buf = 0;
+      uint32_t phase = 0, buf_phase = 0;
+      bool ok = true;
+      for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+        if (!(ok = mm_wait(smem_addr(&s.sum_empty[buf]), buf_phase ^ 1, s, gave_up))) break;
+        tmem_fence_after_sync();
+        const uint32_t d = tmem + buf * a.columns;
+        for (int k = k_first; k < k_end; ++k) {
+          if (!(ok = mm_wait(smem_addr(&s.full[stage]), phase, s, gave_up))) break;
+          tmem_fence_after_sync();
+          const uint32_t at = stage0 + stage * stage_bytes;
+          const uint64_t da = rows128_descriptor(at), db = rows128_descriptor(at + a_bytes);
+#pragma unroll
+          for (int i = 0; i < kMmStageK / 32; ++i)              // 32 bytes further along the rows: 2 in units of 16 bytes
+            mma_int8(d, da + 2 * i, db + 2 * i, instruction, k > k_first || i > 0);
+          mma_commit(smem_addr(&s.empty[stage]));
+          if (++stage == a.stages) stage = 0, phase ^= 1;
+        }
+        if (!ok) break;
+        mma_commit(smem_addr(&s.sum_full[buf]));
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+      }
+      mma_commit(smem_addr(&s.drained));
+      mbar_wait(smem_addr(&s.drained), 0);
+    }
+    __syncwarp();
+  } else {                                                      // ---------------- epilogue
+    const int quarter = warp & 3, half = warp >> 2;
+    int buf = 0;
+    uint32_t buf_phase = 0;
+    for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
+      const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
+      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + quarter * 32 + lane;
+      if constexpr (!SPLIT) {
+        if ((int)threadIdx.x < a.tokens) s.scale[buf][threadIdx.x] = t0 + threadIdx.x < a.T ? __ldg(a.token_scale + t0 + threadIdx.x) : 0.f;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+      }
+      const float w = n < a.N ? __ldg(a.channel_scale + n) : 0.f;
+      const float b = n < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
+      const bool ok = mm_wait(smem_addr(&s.sum_full[buf]), buf_phase, s, lane == 0 ? gave_up : nullptr);
+      if (__any_sync(kFull, !ok)) break;
+      tmem_fence_after_sync();
+      const uint32_t d = tmem + buf * a.columns + ((uint32_t)(quarter * 32) << 16);
+      for (int c = half * 16; c < a.tokens; c += 32) {
+        uint32_t r[16];
+        tmem_load16(d + c, r);
+        tmem_load_wait();
+        if constexpr (SPLIT) {                                  // [column][channel] over the stages, which are done with
+          const uint32_t p = stage0 + c * (kMmChannels * 4) + (quarter * 32 + lane) * 4;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            asm volatile("st.shared.u32 [%0], %1;" :: "r"(p + i * kMmChannels * 4), "r"(r[i]) : "memory");
+        } else {
+          T* o = reinterpret_cast<T*>(a.out) + (t0 + c) * a.N + n;
+          const int left = (int)min((int64_t)16, a.T - t0 - c);
+          if (n < a.N) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (i < left) o[i * a.N] = from_float<T>(fmaf((float)(int)r[i] * s.scale[buf][c + i], w, b));
+          }
+        }
+      }
+      if constexpr (!SPLIT) {
+        tmem_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_addr(&s.sum_empty[buf]));
+        if (++buf == 2) buf = 0, buf_phase ^= 1;
+      }
+    }
+  }
+  if constexpr (SPLIT) {
+    __syncwarp();
+    cluster_sync();
+    if (warp < 8 && !s.dead) {
+      const int tt = first_tile / a.channel_tiles, ct = first_tile - tt * a.channel_tiles;
+      const int ch = threadIdx.x & 127;
+      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + ch;
+      const float w = n < a.N ? __ldg(a.channel_scale + n) : 0.f;
+      const float b = n < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
+      for (int c = (int)split + a.splits * (threadIdx.x >> 7); c < a.tokens && t0 + c < a.T; c += 2 * a.splits) {
+        int sum = 0;
+        for (int k = 0; k < a.splits; ++k) sum += peer_load(stage0 + c * (kMmChannels * 4) + ch * 4, k);
+        if (n < a.N)
+          reinterpret_cast<T*>(a.out)[(t0 + c) * a.N + n] = from_float<T>(fmaf((float)sum * __ldg(a.token_scale + t0 + c), w, b));
+      }
+    }
+    cluster_sync();                                             // nobody leaves while its sums are read
+  }
+  tmem_fence_before_sync();
+  __syncthreads();
+  if (warp == 9) tmem_free(tmem, columns);
+}
+
+// ------------------------------------------------------------------ host
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiled encode_tiled() {
+  static std::atomic<EncodeTiled> fn{nullptr};
+  EncodeTiled f = fn.load(std::memory_order_acquire);
+  if (!f) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult found;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
+        found != cudaDriverEntryPointSuccess) {
+      cudaGetLastError();
+      return nullptr;
+    }
+    f = (EncodeTiled)p;
+    fn.store(f, std::memory_order_release);
+  }
+  return f;
+}
+// Rows of K bytes, `ld` bytes apart, in boxes of 128 bytes by `box` rows; zeros where a box reaches past the matrix.
+bool map_rows(CUtensorMap* m, const void* p, int64_t K, int64_t rows, int64_t ld, int box) {
+  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
+  const cuuint32_t boxes[2] = {(cuuint32_t)kMmStageK, (cuuint32_t)box}, ones[2] = {1, 1};
+  const EncodeTiled f = encode_tiled();
+  return f && f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+void plan(MmArgs& a) {
+  const int sms = device_info().sm_count;
+  const int64_t token_tiles = (a.T + 255) / 256;
+  a.tokens = (int)(((a.T + token_tiles - 1) / token_tiles + 15) / 16 * 16);
+  a.channel_tiles = (int)((a.N + kMmChannels - 1) / kMmChannels);
+  a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
+  a.k_blocks = (a.K + kMmStageK - 1) / kMmStageK;
+  a.splits = 1;
+  while (a.splits < 8 && (int64_t)a.tiles * a.splits * 2 <= sms && a.k_blocks >= a.splits * 2 * 2) a.splits *= 2;
+  a.columns = 32;
+  while (a.columns < a.tokens) a.columns *= 2;
+  a.stages = (kMmSmem - 1024) / ((kMmChannels + a.tokens) * kMmStageK);
+  if (a.stages > kMmStagesMost) a.stages = kMmStagesMost;
+}
+
+template <typename T, bool SPLIT> int launch(const CUtensorMap& w, const CUtensorMap& x, const MmArgs& a, cudaStream_t stream) {
+  auto* kernel = int8_matmul_kernel<T, SPLIT>;
+  static std::atomic<uint64_t> raised{0};                       // devices whose limit of dynamic shared memory is raised
+  int dev = 0;
+  cudaGetDevice(&dev);
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (!(raised.load(std::memory_order_acquire) & bit)) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmSmem) != cudaSuccess) return check_launch(), ACTNN_ERR_LAUNCH;
+    raised.fetch_or(bit, std::memory_order_release);
+  }
+  const int sms = device_info().sm_count;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(SPLIT ? a.tiles * a.splits : a.tiles < sms ? a.tiles : sms);
+  cfg.blockDim = dim3(kMmThreads);
+  cfg.dynamicSmemBytes = kMmSmem;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = SPLIT ? a.splits : 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  unsigned* gave_up = bulk_wait_counter();
+  if (cudaLaunchKernelEx(&cfg, kernel, w, x, a, gave_up) != cudaSuccess) {
+    cudaGetLastError();
+    return ACTNN_ERR_LAUNCH;
+  }
+  return check_launch();
+}
+template <typename T> int launch_typed(const CUtensorMap& w, const CUtensorMap& x, const MmArgs& a, cudaStream_t stream) {
+  return a.splits > 1 ? launch<T, true>(w, x, a, stream) : launch<T, false>(w, x, a, stream);
+}
+
+}  // namespace
+}  // namespace actnn
+
+using namespace actnn;
+
+extern "C" int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8_t* weights, const float* channel_scale,
+                                 const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens,
+                                 int64_t ld_weights, int dtype, actnn_stream_t stream) {
+  if (T < 0 || N < 0 || K < 1 || K > 131072 || T > 0x7fffff00 || N > 0x7fffff00 || ld_tokens < K || ld_weights < K ||
+      ld_tokens > ((int64_t)1 << 39) || ld_weights > ((int64_t)1 << 39)) return ACTNN_ERR_SHAPE;
+  if (dtype < ACTNN_F32 || dtype > ACTNN_BF16) return ACTNN_ERR_DTYPE;
+  if (T == 0 || N == 0) return ACTNN_OK;
+  if (!tokens || !token_scale || !weights || !channel_scale || !out) return ACTNN_ERR_NULL;
+  if (!aligned(tokens, 16) || !aligned(weights, 16) || ld_tokens % 16 != 0 || ld_weights % 16 != 0) return ACTNN_ERR_ALIGN;
+  const int size = dtype_size(dtype);
+  if (!aligned(token_scale, 4) || !aligned(channel_scale, 4) || !aligned(bias, size) || !aligned(out, size)) return ACTNN_ERR_ALIGN;
+  MmArgs a{};
+  a.token_scale = token_scale; a.channel_scale = channel_scale; a.bias = bias; a.out = out;
+  a.T = T; a.N = N; a.K = (int)K;
+  if ((N + kMmChannels - 1) / kMmChannels * ((T + 15) / 16) > 0x7fffffff) return ACTNN_ERR_SHAPE;
+  plan(a);
+  CUtensorMap w, x;
+  if (!map_rows(&w, weights, K, N, ld_weights, kMmChannels) || !map_rows(&x, tokens, K, T, ld_tokens, a.tokens)) return ACTNN_ERR_LAUNCH;
+  switch (dtype) {
+    case ACTNN_F32: return launch_typed<float>(w, x, a, (cudaStream_t)stream);
+    case ACTNN_F16: return launch_typed<__half>(w, x, a, (cudaStream_t)stream);
+    default: return launch_typed<__nv_bfloat16>(w, x, a, (cudaStream_t)stream);
+  }
+}

@@ -1,0 +1,83 @@
+// The 5th-generation tensor core, tensor memory and tiled bulk copies, as thin wrappers of the PTX instructions.
+#pragma once
+
+#include <cuda.h>
+
+#include "common.cuh"
+
+namespace actnn {
+#ifdef __CUDACC__
+
+// ------------------------------------------------------------------ barriers
+ACTNN_DEV void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
+
+// ------------------------------------------------------------------ tiled copies
+// A box of a rank-2 tensor to shared memory; x (elements of the contiguous dimension) starts on 16 bytes.
+ACTNN_DEV void tile_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+               :: "r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+ACTNN_DEV void tensor_map_prefetch(const CUtensorMap* map) {
+  asm volatile("prefetch.tensormap [%0];" :: "l"(map) : "memory");
+}
+
+// ------------------------------------------------------------------ tensor memory
+// One whole warp allocates (a power of two of columns, 32 at least), and the same warp frees.
+ACTNN_DEV void tmem_alloc(uint32_t dst_smem, uint32_t columns) {
+  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(dst_smem), "r"(columns) : "memory");
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+ACTNN_DEV void tmem_free(uint32_t addr, uint32_t columns) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+}
+ACTNN_DEV void tmem_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+ACTNN_DEV void tmem_fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+// 16 columns of the warp's 32 lanes (the quarter that its number modulo four names): column i of lane l in r[i] of lane l.
+ACTNN_DEV void tmem_load16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+                 "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+               : "r"(addr));
+}
+ACTNN_DEV void tmem_load_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// ------------------------------------------------------------------ matrix instructions
+// Shared-memory operand whose rows of 128 bytes run along the reduction, swizzled in 128-byte lines: eight rows are 1024
+// bytes, and 1024 bytes further come the next eight.  `addr` on 1024 bytes (plus the offset along the reduction).
+ACTNN_DEV uint64_t rows128_descriptor(uint32_t addr) {
+  return (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
+         ((uint64_t)2 << 61);
+}
+// Signed 8-bit operands, 32-bit integer sums: 128 rows of A, n rows of B (16, or 32 to 256 in steps of 16).
+ACTNN_DEV uint32_t int8_instruction(int n) {
+  return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
+}
+// D[128, n] (+)= A[128, 32] B[n, 32]^T, issued by one thread.
+ACTNN_DEV void mma_int8(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+               :: "r"(d), "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add) : "memory");
+}
+// The barrier is arrived at once all matrix instructions that this thread issued before are done.
+ACTNN_DEV void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+}
+
+// ------------------------------------------------------------------ clusters
+ACTNN_DEV uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+ACTNN_DEV void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+ACTNN_DEV int32_t peer_load(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  int32_t v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  return v;
+}
+#endif
+}  // namespace actnn

@@ -1,0 +1,161 @@
+// 8-bit codes of rows (tokens, or output channels of a weight): one scale a row.
+//
+//   a = max |x|,  scale = a * (1 / 127),  code = rint(x * (127 * (1 / a)))
+//
+// A row is read once where the threads that share it can hold it in registers (up to 32 elements each), else twice, the
+// second time from the L2.  Bound by HBM: 2 + 1 bytes an element of a 16-bit type.
+#include "activation.cuh"
+
+namespace actnn {
+namespace {
+
+constexpr int kRowThreads = 256;
+constexpr int kHeld = 4;                               // vectors of eight that a thread holds
+
+// The largest of `most` over the LANES threads of a row; LANES = 32 (a warp per row) or kRowThreads.
+template <int LANES> ACTNN_DEV uint32_t row_max(uint32_t most) {
+  most = __reduce_max_sync(kFull, most);
+  if constexpr (LANES > 32) {
+    __shared__ uint32_t warp_most[LANES / 32];
+    if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
+    __syncthreads();
+    most = warp_most[0];
+#pragma unroll
+    for (int i = 1; i < LANES / 32; ++i) most = max(most, warp_most[i]);
+  }
+  return most;
+}
+
+// VEC: rows of x are whole aligned vectors of eight.  codes: rows `ldc` bytes apart (a multiple of 8), zero from cols to ldc.
+template <typename T, int LANES, bool VEC>
+__global__ void __launch_bounds__(kRowThreads)
+row_codes_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scale, int64_t rows, int64_t cols,
+                 int64_t ldx, int64_t ldc) {
+  const int lane = threadIdx.x % LANES;
+  const int64_t row = (int64_t)blockIdx.x * (kRowThreads / LANES) + threadIdx.x / LANES;
+  if (row >= rows) return;                             // whole warps; never with LANES > 32
+  const T* p = x + row * ldx;
+  int8_t* q = codes + row * ldc;
+  float f[kHeld][8];
+  uint32_t most = 0;
+  auto load = [&](int64_t e, float (&v)[8]) {
+    if constexpr (VEC) {
+      if (e < cols) {
+        unpack_vec(load_vec<T, 8>(p + e), v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = e + i < cols ? to_float(__ldg(p + e + i)) : 0.f;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) load((int64_t)(k * LANES + lane) * 8, f[k]);
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k)
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, abs_bits(f[k][i]));
+  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < cols; e += LANES * 8) {
+    float v[8];
+    load(e, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, abs_bits(v[i]));
+  }
+  const float a = largest(row_max<LANES>(most));
+  const float inv = code_factor(a);
+  if (lane == 0) scale[row] = code_step(a);
+  auto store = [&](int64_t e, const float (&v)[8]) {
+    uint32_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = code_bits(v[i], inv);
+    store_codes<8>(q + e, c);
+  };
+#pragma unroll
+  for (int k = 0; k < kHeld; ++k) {
+    const int64_t e = (int64_t)(k * LANES + lane) * 8;
+    if (e < ldc) store(e, f[k]);
+  }
+  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < ldc; e += LANES * 8) {
+    float v[8];
+    load(e, v);
+    store(e, v);
+  }
+}
+
+// code * scale, eight elements a thread.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(kRowThreads)
+row_decode_kernel(const int8_t* __restrict__ codes, const float* __restrict__ scale, T* __restrict__ out, int64_t rows, int64_t cols,
+                  int64_t ldc, int64_t octs) {
+  const int64_t i = (int64_t)blockIdx.x * kRowThreads + threadIdx.x;
+  const int64_t row = i / octs, e = (i - row * octs) * 8;
+  if (row >= rows) return;
+  const float s = __ldg(scale + row);
+  float f[8];
+  if constexpr (VEC) {
+    unpack_codes(load_codes<8>(codes + row * ldc + e), f);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] *= s;
+    store_vec<T, 8>(out + row * cols + e, f);
+  } else {
+    for (int j = 0; j < 8 && e + j < cols; ++j) out[row * cols + e + j] = from_float<T>((float)codes[row * ldc + e + j] * s);
+  }
+}
+
+template <typename T>
+int encode(const void* x, int8_t* codes, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc, cudaStream_t s) {
+  const bool vec = cols % 8 == 0 && ldx % 8 == 0 && aligned(x, 16);
+  // a warp holds 1024 elements; up to twice that its re-read costs less than a block's barrier
+  const bool warp = cols <= 2048;
+  const int64_t grid = warp ? (rows + kRowThreads / 32 - 1) / (kRowThreads / 32) : rows;
+  if (grid > 0x7fffffff) return ACTNN_ERR_SHAPE;
+  auto* kernel = warp ? (vec ? row_codes_kernel<T, 32, true> : row_codes_kernel<T, 32, false>)
+                      : (vec ? row_codes_kernel<T, kRowThreads, true> : row_codes_kernel<T, kRowThreads, false>);
+  kernel<<<(unsigned)grid, kRowThreads, 0, s>>>((const T*)x, codes, scale, rows, cols, ldx, ldc);
+  return check_launch();
+}
+template <typename T>
+int decode(const int8_t* codes, const float* scale, void* out, int64_t rows, int64_t cols, int64_t ldc, cudaStream_t s) {
+  const bool vec = cols % 8 == 0 && ldc % 8 == 0 && aligned(codes, 8) && aligned(out, 16);
+  const int64_t octs = (cols + 7) / 8, grid = (rows * octs + kRowThreads - 1) / kRowThreads;
+  if (grid > 0x7fffffff) return ACTNN_ERR_SHAPE;
+  auto* kernel = vec ? row_decode_kernel<T, true> : row_decode_kernel<T, false>;
+  kernel<<<(unsigned)grid, kRowThreads, 0, s>>>(codes, scale, (T*)out, rows, cols, ldc, octs);
+  return check_launch();
+}
+
+}  // namespace
+}  // namespace actnn
+
+using namespace actnn;
+
+extern "C" int actnn_row_codes(const void* x, int8_t* codes, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc,
+                               int dtype, actnn_stream_t stream) {
+  if (rows < 0 || cols < 0 || cols > ((int64_t)1 << 31) || rows > ((int64_t)1 << 40) || (rows > 1 && ldx < cols) || ldc < cols ||
+      ldc % 16 != 0 || ldc - cols >= 16) return ACTNN_ERR_SHAPE;
+  if (dtype < ACTNN_F32 || dtype > ACTNN_BF16) return ACTNN_ERR_DTYPE;
+  if (rows == 0 || cols == 0) return ACTNN_OK;
+  if (!x || !codes || !scale) return ACTNN_ERR_NULL;
+  if (!aligned(x, dtype_size(dtype)) || !aligned(codes, 16) || !aligned(scale, 4)) return ACTNN_ERR_ALIGN;
+  switch (dtype) {
+    case ACTNN_F32: return encode<float>(x, codes, scale, rows, cols, ldx, ldc, (cudaStream_t)stream);
+    case ACTNN_F16: return encode<__half>(x, codes, scale, rows, cols, ldx, ldc, (cudaStream_t)stream);
+    default: return encode<__nv_bfloat16>(x, codes, scale, rows, cols, ldx, ldc, (cudaStream_t)stream);
+  }
+}
+
+extern "C" int actnn_row_decode(const int8_t* codes, const float* scale, void* out, int64_t rows, int64_t cols, int64_t ldc,
+                                int dtype, actnn_stream_t stream) {
+  if (rows < 0 || cols < 0 || cols > ((int64_t)1 << 31) || rows > ((int64_t)1 << 40) || (rows > 1 && ldc < cols)) return ACTNN_ERR_SHAPE;
+  if (dtype < ACTNN_F32 || dtype > ACTNN_BF16) return ACTNN_ERR_DTYPE;
+  if (rows == 0 || cols == 0) return ACTNN_OK;
+  if (!codes || !scale || !out) return ACTNN_ERR_NULL;
+  if (!aligned(out, dtype_size(dtype)) || !aligned(scale, 4)) return ACTNN_ERR_ALIGN;
+  switch (dtype) {
+    case ACTNN_F32: return decode<float>(codes, scale, out, rows, cols, ldc, (cudaStream_t)stream);
+    case ACTNN_F16: return decode<__half>(codes, scale, out, rows, cols, ldc, (cudaStream_t)stream);
+    default: return decode<__nv_bfloat16>(codes, scale, out, rows, cols, ldc, (cudaStream_t)stream);
+  }
+}

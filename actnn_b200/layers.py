@@ -16,7 +16,11 @@ from torch.nn.modules.utils import _pair, _single, _triple
 
 from . import ops
 from .conf import config
+from .cpp_extension import checkpoint as ext_checkpoint
+from .cpp_extension import group_norm as ext_group_norm
+from .cpp_extension import int8 as ext_int8
 from .cpp_extension import quantization as ext_quantization
+from .cpp_extension._checks import activation_kind
 from .qbnscheme import QBNScheme
 from .qscheme import QScheme
 
@@ -270,3 +274,95 @@ class QAvgPool2d(_AvgPoolNd):
                       "for avg_pool2d is not implemented.")
         return ext_quantization.act_quantized_max_pool2d(input, self.kernel_size, self.stride, self.padding,
                                                          (1, 1), self.ceil_mode, False)
+
+
+# ------------------------------------------------------------------------- token operators (no counterpart in the reference)
+class QInt8Linear(nn.Linear):
+    """A linear layer whose product runs in 8-bit integers, with a scale for each token and each output channel.
+
+    In training the weight is coded in every step and the codes of the input are what the backward pass keeps.  For serving,
+    ``freeze()`` codes the weight once: until ``unfreeze()`` (or ``train()``) the forward pass reads those codes alone, whatever
+    happens to ``weight``."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        super().__init__(in_features, out_features, bias)
+        self.frozen = None
+
+    def freeze(self):
+        self.frozen = ext_int8.quantize_rows(self.weight.detach())
+        return self
+
+    def unfreeze(self):
+        self.frozen = None
+        return self
+
+    def train(self, mode: bool = True):
+        if mode:
+            self.unfreeze()
+        return super().train(mode)
+
+    def _apply(self, fn, recurse=True):
+        self.frozen = None                    # the weight moves or changes its type: freeze again
+        return super()._apply(fn, recurse)
+
+    def forward(self, input):
+        if self.frozen is not None:
+            if torch.is_grad_enabled() and input.requires_grad:
+                raise RuntimeError("QInt8Linear is frozen: no gradient passes through it (call unfreeze() first)")
+            return ext_int8.linear(input, *self.frozen, None if self.bias is None else self.bias.detach())
+        return ops.int8_linear.apply(input, self.weight, self.bias)
+
+
+class _QActivation(nn.Module):
+    _name = "none"
+    _gated = False
+
+    def forward(self, input):
+        if not torch.is_grad_enabled() or not input.requires_grad:
+            return ext_checkpoint.activation_forward(input, self._name, self._gated, save=False)[0]
+        return (ops.glu if self._gated else ops.activation).apply(input, self._name)
+
+    def extra_repr(self):
+        return self._name
+
+
+class QSiLU(_QActivation):
+    """``x * sigmoid(x)`` that keeps its input in 8 bits."""
+    _name = "silu"
+
+
+class QGELU(_QActivation):
+    """GELU, ``approximate`` as in ``nn.GELU``, that keeps its input in 8 bits."""
+
+    def __init__(self, approximate: str = "none"):
+        super().__init__()
+        if approximate not in ("none", "tanh"):
+            raise ValueError("approximate must be 'none' or 'tanh', got %r" % (approximate,))
+        self._name = "gelu" if approximate == "none" else "gelu_tanh"
+
+
+class QGLU(_QActivation):
+    """``f(gate) * up`` of the two halves of the last dimension, ``activation`` one of "silu", "gelu", "gelu_tanh", "relu"."""
+    _gated = True
+
+    def __init__(self, activation: str = "silu"):
+        super().__init__()
+        activation_kind(activation)
+        self._name = activation
+
+
+class QGroupNorm(nn.GroupNorm):
+    """Group norm with an activation behind it, on channels-last tensors, that keeps its input in 8 bits."""
+
+    def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation: Optional[str] = None):
+        super().__init__(num_groups, num_channels, eps, affine)
+        activation_kind(activation)
+        self.activation = activation or "none"
+
+    def forward(self, input):
+        if not torch.is_grad_enabled() or not (input.requires_grad or (self.weight is not None and self.weight.requires_grad)):
+            return ext_group_norm.inference(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+        return ops.group_norm.apply(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
+
+    def extra_repr(self):
+        return super().extra_repr() + ", activation=" + self.activation

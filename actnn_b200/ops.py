@@ -26,6 +26,9 @@ from torch.nn.modules.utils import _pair, _single, _triple
 
 from .conf import config
 from .cpp_extension import backward_func as ext_backward_func
+from .cpp_extension import checkpoint as ext_checkpoint
+from .cpp_extension import group_norm as ext_group_norm
+from .cpp_extension import int8 as ext_int8
 from .cpp_extension import minimax as ext_minimax  # noqa: F401  (kept under the name the reference imports)
 from .cpp_extension import quantization as ext_quantization
 from .qbnscheme import QBNScheme
@@ -627,3 +630,115 @@ class adaptive_avg_pool2d(Function):
         input_shape = ctx.saved
         repeat_size = [int(x / y) for x, y in zip(input_shape, grad_output.shape)]
         return grad_output.repeat(repeat_size) / np.prod(repeat_size), None
+
+
+# ---------------------------------------------------------------------------------------
+# token operators: rows of channels with 8-bit copies (the reference has no counterpart)
+# ---------------------------------------------------------------------------------------
+def _keep(tensor):
+    """A saved tensor as the swap levels keep it."""
+    return swap_to_cpu(tensor) if config.swap else tensor
+
+
+def _kept(saved):
+    return saved if isinstance(saved, torch.Tensor) and saved.is_cuda else swap_to_gpu(saved)
+
+
+class int8_linear(Function):
+    """``x @ weight.T + bias`` in 8-bit integers: rows of ``x`` and of ``weight`` are coded on the way (scale per token, scale per
+    output channel), and the codes are all that is kept.  The gradients are those of the product of the decoded matrices, passed
+    straight through the rounding; like those of ``linear`` they are dense products in the activation's type."""
+
+    @staticmethod
+    def forward(ctx, input, weight, bias=None):
+        input, weight, bias = _autocast_inputs(input, weight, bias)
+        with _autocast_off():
+            if weight.dim() != 2 or input.dim() < 1 or input.shape[-1] != weight.shape[1]:
+                raise RuntimeError("shapes %s and %s cannot be multiplied" % (tuple(input.shape), tuple(weight.shape)))
+            codes, scale = ext_int8.quantize_rows(input)
+            wcodes, wscale = ext_int8.quantize_rows(weight)
+            output = ext_int8.matmul(codes, scale, wcodes, wscale, bias, input.dtype)
+            ctx.saved = (_keep(codes) if ctx.needs_input_grad[1] else None, scale, wcodes if ctx.needs_input_grad[0] else None, wscale)
+            ctx.other_args = (input.dtype, input.shape, weight.dtype, None if bias is None else bias.dtype)
+            return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        codes, scale, wcodes, wscale = ctx.saved
+        dtype, shape, wdtype, bdtype = ctx.other_args
+        with _autocast_off():
+            go = grad_output.reshape(-1, grad_output.shape[-1]) if grad_output.dim() != 2 else grad_output
+            grad_input = grad_weight = grad_bias = None
+            if ctx.needs_input_grad[0]:
+                grad_input = go.mm(ext_int8.dequantize_rows(wcodes, wscale, dtype)).view(shape)
+            if ctx.needs_input_grad[1]:
+                x = ext_int8.dequantize_rows(_kept(codes), scale, dtype)
+                grad_weight = go.t().mm(x.view(-1, shape[-1])).to(wdtype)
+            if bdtype is not None and ctx.needs_input_grad[2]:
+                grad_bias = go.sum(0).to(bdtype)
+        return grad_input, grad_weight, grad_bias
+
+
+class activation(Function):
+    """An activation function ("relu", "silu", "gelu", "gelu_tanh") that keeps its input in 8 bits."""
+    gated = False
+
+    @classmethod
+    def run_forward(cls, ctx, input, name):
+        ctx.name = name
+        if not config.compress_activation:
+            ctx.saved = None
+            ctx.save_for_backward(input)
+            return ext_checkpoint.activation_forward(input, name, cls.gated, save=False)[0]
+        output, codes, scale = ext_checkpoint.activation_forward(input, name, cls.gated, save=ctx.needs_input_grad[0])
+        ctx.saved = None if codes is None else (_keep(codes), scale)
+        return output
+
+    @classmethod
+    def run_backward(cls, ctx, grad_output):
+        if ctx.saved is None:
+            return ext_checkpoint.activation_backward(grad_output, ctx.name, x=ctx.saved_tensors[0], gated=cls.gated), None
+        codes, scale = ctx.saved
+        return ext_checkpoint.activation_backward(grad_output, ctx.name, _kept(codes), scale, gated=cls.gated), None
+
+    @staticmethod
+    def forward(ctx, input, name):
+        return activation.run_forward(ctx, input, name)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return activation.run_backward(ctx, grad_output)
+
+
+class glu(activation):
+    """The gated form: ``f(gate) * up`` of the two halves of the last dimension, both kept in 8 bits."""
+    gated = True
+
+    @staticmethod
+    def forward(ctx, input, name):
+        return glu.run_forward(ctx, input, name)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return glu.run_backward(ctx, grad_output)
+
+
+class group_norm(Function):
+    """Group norm followed by an activation function ("none" for none), on channels-last tensors, its input kept in 8 bits."""
+
+    @staticmethod
+    def forward(ctx, input, num_groups, weight=None, bias=None, eps=1e-5, name="none"):
+        output, saved, stats = ext_group_norm.forward(input, num_groups, weight, bias, eps, name, config.compress_activation)
+        ctx.save_for_backward(weight, bias, *(() if config.compress_activation else (saved,)))
+        ctx.saved = (_keep(saved) if config.compress_activation else None, stats)
+        ctx.other_args = (num_groups, name)
+        return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        weight, bias, *exact = ctx.saved_tensors
+        codes, stats = ctx.saved
+        groups, name = ctx.other_args
+        needs = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
+        gx, gw, gb = ext_group_norm.backward(grad_output, exact[0] if exact else _kept(codes), stats, groups, weight, bias, name, needs)
+        return gx, None, None if gw is None else gw.to(weight.dtype), None if gb is None else gb.to(bias.dtype), None, None

@@ -421,6 +421,64 @@ int actnn_batch_norm_backward_elemt(const void* x, const void* grad_out, const f
                                     void* workspace, int64_t workspace_bytes, actnn_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * 8-bit codes of rows (tokens, or the output channels of a weight), one float32 scale a row:
+ * a = max |x| of the row (at least 1e-30), scale = a * (1/127), code = rint(x * (127 * (1/a))), half to even,
+ * each step one rounded fp32 operation.  A row with a NaN or an infinity decodes to NaN.
+ * `codes`: rows `ld_codes` bytes apart, the least multiple of 16 that holds `cols`, zero behind the
+ * end; rows of x are `ld_x` elements apart (vector loads where x is on 16 bytes and cols and ld_x are
+ * multiples of 8).  actnn_row_decode writes code * scale, [rows, cols] contiguous.
+ * The reference has no counterpart (its codes are per group of 256 with a minimum,
+ * actnn/actnn/cpp_extension/quantization_cuda_kernel.cu:86-142). */
+int actnn_row_codes(const void* x, int8_t* codes, float* scale, int64_t rows, int64_t cols, int64_t ld_x,
+                    int64_t ld_codes, int dtype, actnn_stream_t stream);
+int actnn_row_decode(const int8_t* codes, const float* scale, void* out, int64_t rows, int64_t cols,
+                     int64_t ld_codes, int dtype, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * out[t, n] = (sum_k tokens[t, k] * weights[n, k]) * token_scale[t] * channel_scale[n] + bias[n]
+ * on the integer tensor cores; the sum is exact (int32), out is [T, N] contiguous of `dtype`, rounded
+ * once.  `bias` (of `dtype`) may be NULL.  Rows of codes start on 16 bytes: pointers and ld_* (bytes)
+ * are multiples of 16, and what lies between K and ld is not read as data.  1 <= K <= 131072.
+ * A block whose bounded wait runs out leaves its outputs unwritten and counts the event
+ * (actnn_bulk_wait_failures).  The reference has no counterpart (its layers compute in the
+ * activation's type, actnn/actnn/ops.py:408-428). */
+int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8_t* weights,
+                      const float* channel_scale, const void* bias, void* out, int64_t T, int64_t N, int64_t K,
+                      int64_t ld_tokens, int64_t ld_weights, int dtype, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Activation functions whose backward pass reads an 8-bit copy of the input.  `kind`: 0 identity, 1 ReLU,
+ * 2 SiLU, 3 GELU (erf), 4 GELU (tanh form).  x is [rows, cols]; with `gated` it is [rows, 2 * cols] and
+ * y = f(x[:, :cols]) * x[:, cols:].  y and grad_y are [rows, cols]; all contiguous.
+ * With b = ceil(rows * cols / 256): `codes` has 256 * b bytes (gated: twice that, the gate's first), `scale`
+ * b values (gated: 2 * b); 256 consecutive elements share a scale, coded as in actnn_row_codes.  NULL codes
+ * and scale: nothing is saved, and the backward pass reads x instead (x may be NULL when codes are given).
+ * The form without gate wants x, y, grad_y and grad_x on 16 bytes.  The reference has no counterpart (of its
+ * activation functions ReLU saves one bit, actnn/actnn/cpp_extension/quantization.cc:106-124). */
+int actnn_act_forward(const void* x, void* y, int8_t* codes, float* scale, int64_t rows, int64_t cols, int gated,
+                      int kind, int dtype, actnn_stream_t stream);
+int actnn_act_backward(const void* grad_y, const void* x, const int8_t* codes, const float* scale, void* grad_x,
+                       int64_t rows, int64_t cols, int gated, int kind, int dtype, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Group norm with an activation (`kind` as above) on channels-last data [N, S, C], G groups of C / G channels:
+ * y = f((x - mean) * rstd * gamma + beta), statistics over S * C / G elements, biased variance.
+ * `codes` [N, S, C] (NULL: not saved) are 127 steps either way of the middle of each (sample, group)'s range;
+ * `stats` float32 [N, G, 4] = mean, rstd, middle, half of the range (NULL only without codes: inference).
+ * The backward pass computes with the decoded input, or with x where codes are NULL.  gamma, beta float32 or
+ * NULL; grad_gamma, grad_beta (float32, NULL: not wanted) are sums over samples and positions.  Results are
+ * reproducible (fixed order of summation).  Workspace: 16-byte aligned, actnn_group_norm_workspace bytes.
+ * The reference has no counterpart (its norms are batch norms, actnn/actnn/ops.py:444-500). */
+int actnn_group_norm_workspace(int64_t N, int64_t S, int64_t C, int64_t G, int64_t* bytes);
+int actnn_group_norm_forward(const void* x, const float* gamma, const float* beta, void* y, int8_t* codes,
+                             float* stats, int64_t N, int64_t S, int64_t C, int64_t G, double eps, int kind,
+                             int dtype, void* workspace, int64_t workspace_bytes, actnn_stream_t stream);
+int actnn_group_norm_backward(const void* grad_y, const void* x, const int8_t* codes, const float* stats,
+                              const float* gamma, const float* beta, void* grad_x, float* grad_gamma,
+                              float* grad_beta, int64_t N, int64_t S, int64_t C, int64_t G, int kind, int dtype,
+                              void* workspace, int64_t workspace_bytes, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * How many bulk-copy waits gave up on the current device since the library was loaded.
  * The opt-in staged pack kernels (environment ACTNN_STAGED_PACK=1) copy their inputs into
  * shared memory with the bulk-copy engine and bound every wait on the completion barrier;
