@@ -55,6 +55,9 @@ def _run(x, groups, weight, bias, eps, activation, codes_wanted, stats_wanted):
 
 def inference(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
     """The output alone."""
+    nat = _lib.native()
+    if nat:
+        return nat.group_norm_value(x, groups, weight, bias, eps, "none" if activation is None else activation)
     return _run(x, groups, weight, bias, eps, activation, False, False)[0]
 
 

@@ -105,6 +105,9 @@ def _check_product(x, weight_codes, bias, dtype):
 
 def linear(x, weight_codes, weight_scale, bias=None):
     """A linear layer on a weight kept as codes: the tokens ``x`` ``[.., K]`` are coded row by row, the result has their type."""
+    nat = _lib.native()
+    if nat:
+        return nat.int8_linear(x, weight_codes, weight_scale, bias)
     check_cuda_values(x, "x")
     _check_codes(weight_codes, weight_scale, "weight_codes")
     _check_product(x, weight_codes, bias, x.dtype)

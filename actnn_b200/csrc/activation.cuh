@@ -2,8 +2,8 @@
 //
 // A code stands for code * scale, |code| <= 127, half to even:  scale = a * (1 / 127),  code = rint(x * (127 * (1 / a))),  a the
 // largest magnitude of what shares the scale, at least kTiny.  Every step is one rounded fp32 operation in this order, so codes
-// are reproducible to the bit.  a is found on the bit patterns of |x|: a NaN is larger than an infinity there, so neither is
-// lost, and everything that shares a scale with one decodes to NaN (a = inf: 0 * inf; a = NaN: NaN).
+// are reproducible to the bit.  a is found on the bit patterns of |x|, where infinities and NaNs are above all numbers; it
+// becomes a NaN then, and so does the scale: everything that shares it decodes to NaN.
 #pragma once
 
 #include "common.cuh"
@@ -112,9 +112,11 @@ template <typename T, int V> ACTNN_DEV void store_vec(T* p, const float (&f)[V])
 }
 
 // ------------------------------------------------------------------ codes
-// The largest magnitude, as bits of its absolute value; kTiny at least.
+// The largest magnitude from the bits of the largest absolute value: kTiny at least, a NaN where it is not finite.
 ACTNN_DEV uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-ACTNN_DEV float largest(uint32_t bits) { return __uint_as_float(max(bits, __float_as_uint(kTiny))); }
+ACTNN_DEV float largest(uint32_t bits) {
+  return __uint_as_float(bits >= 0x7f800000u ? 0x7fffffffu : max(bits, __float_as_uint(kTiny)));
+}
 
 ACTNN_DEV float code_factor(float a) { return __fmul_rn(__frcp_rn(a), 127.f); }
 ACTNN_DEV float code_step(float a) { return __fmul_rn(a, 1.f / 127.f); }

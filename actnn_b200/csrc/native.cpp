@@ -281,6 +281,173 @@ Tensor relu_backward(const Tensor& grad_in, const Tensor& mask) {
 }
 
 // with_minmax: also min and max of every 256 outputs, not differentiable
+// ---------------------------------------------------------------------------------------- token operators
+constexpr const char* kNames[] = {"none", "relu", "silu", "gelu", "gelu_tanh"};
+int activation_kind(const std::string& name) {
+  for (int i = 0; i < 5; ++i)
+    if (name == kNames[i]) return i;
+  TORCH_CHECK(false, "activation must be one of gelu, gelu_tanh, none, relu, silu, got '", name, "'");
+}
+void check_values(const Tensor& t, const char* name) {
+  TORCH_CHECK(t.is_cuda(), name, " must be a CUDA tensor!");
+  TORCH_CHECK(t.scalar_type() == at::kFloat || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16, "The type of ", name,
+              " is not correct!");
+}
+bool on16(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+Tensor on_16_bytes(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return on16(c) ? c : c.clone(at::MemoryFormat::Contiguous);
+}
+int64_t row_bytes(int64_t k) { return (k + 15) / 16 * 16; }
+
+// A matrix of the rows of x and the elements between them; copied only where the rows do not lie evenly.
+std::pair<Tensor, int64_t> as_rows(const Tensor& x) {
+  const int64_t k = x.size(-1);
+  if (x.dim() == 2 && (x.stride(1) == 1 || k == 1) && (x.size(0) <= 1 || x.stride(0) >= k)) return {x, x.size(0) > 1 ? x.stride(0) : k};
+  return {x.contiguous(), k};
+}
+// The same for codes, whose rows start on 16 bytes.
+std::pair<Tensor, int64_t> code_rows(const Tensor& codes) {
+  const int64_t k = codes.size(-1);
+  Tensor c = codes.dim() == 2 ? codes : codes.reshape({k ? codes.numel() / k : 0, k});
+  int64_t ld = c.size(0) > 1 ? c.stride(0) : row_bytes(k);
+  if ((c.stride(1) != 1 && k > 1) || ld % 16 || ld < k || !on16(c)) {
+    ld = row_bytes(k);
+    Tensor padded = at::zeros({c.size(0), ld}, c.options());
+    padded.narrow(1, 0, k).copy_(c);
+    c = padded.narrow(1, 0, k);
+  }
+  return {c, ld};
+}
+struct RowCodes { Tensor codes, scale; int64_t rows, k, ld; };       // codes: [rows, ld]
+RowCodes row_codes(const Tensor& x) {
+  const auto [flat, ldx] = as_rows(x);
+  const int64_t k = x.size(-1), rows = k ? x.numel() / k : 0, ld = row_bytes(k);
+  RowCodes r{make({rows, ld}, at::kChar, x), make({rows}, at::kFloat, x), rows, k, ld};
+  check(actnn_row_codes(flat.data_ptr(), r.codes.data_ptr<int8_t>(), r.scale.data_ptr<float>(), rows, k, ldx, ld,
+                        dtype_id(x.scalar_type()), stream()),
+        "actnn_row_codes");
+  return r;
+}
+Tensor row_decode(const RowCodes& r, at::ScalarType t) {
+  Tensor out = make({r.rows, r.k}, t, r.codes);
+  check(actnn_row_decode(r.codes.data_ptr<int8_t>(), r.scale.data_ptr<float>(), out.data_ptr(), r.rows, r.k, r.ld, dtype_id(t), stream()),
+        "actnn_row_decode");
+  return out;
+}
+std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
+  std::vector<int64_t> s = x.sizes().vec();
+  s.back() = n;
+  return s;
+}
+void check_bias(const OptTensor& bias, const Tensor& x, int64_t n) {
+  if (!bias.has_value() || !bias->defined()) return;
+  check_values(*bias, "bias");
+  TORCH_CHECK(bias->device() == x.device(), "bias is on ", bias->device(), ", expected ", x.device());
+  TORCH_CHECK(bias->dim() == 1 && bias->size(0) == n, "The dimension of bias is not correct!");
+}
+constexpr int64_t kMostK = 131072;
+
+Tensor int8_linear(const Tensor& x, const Tensor& codes, const Tensor& scale, const OptTensor& bias) {
+  check_values(x, "x");
+  TORCH_CHECK(codes.is_cuda(), "weight_codes must be a CUDA tensor!");
+  TORCH_CHECK(codes.scalar_type() == at::kChar && scale.scalar_type() == at::kFloat,
+              "The type of weight_codes is not correct! (int8 codes, float32 scales)");
+  TORCH_CHECK(codes.dim() == 2 && scale.dim() == 1 && scale.size(0) == codes.size(0), "The dimension of weight_codes is not correct!");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == codes.size(1), "shapes ", x.sizes(), " and ", codes.sizes(), " cannot be multiplied");
+  const int64_t n = codes.size(0), k = codes.size(1);
+  TORCH_CHECK(k <= kMostK, "a product over ", k, " values may overflow its 32-bit sum; at most ", kMostK, " are accepted");
+  TORCH_CHECK(codes.device() == x.device() && scale.device() == x.device(), "the weight is on ", codes.device(), ", the tokens on ", x.device());
+  check_bias(bias, x, n);
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = make(with_last(x, n), x.scalar_type(), x);
+  const bool with = bias.has_value() && bias->defined();
+  const Tensor b = with ? bias->to(x.scalar_type()).contiguous() : Tensor();
+  if (k == 0) return with ? out.copy_(b) : out.zero_();
+  const auto [flat, ldx] = as_rows(x);
+  const auto [w, ldw] = code_rows(codes);
+  const Tensor s = scale.contiguous();
+  const int64_t rows = x.numel() / k;
+  int64_t bytes = 0;
+  check(actnn_int8_linear_workspace(rows, k, &bytes), "actnn_int8_linear_workspace");
+  Tensor ws;
+  if (bytes) ws = make({bytes}, at::kByte, x);
+  check(actnn_int8_linear(flat.data_ptr(), w.data_ptr<int8_t>(), s.data_ptr<float>(), with ? b.data_ptr() : nullptr, out.data_ptr(), rows, n,
+                          k, ldx, ldw, dtype_id(x.scalar_type()), bytes ? ws.data_ptr() : nullptr, bytes, stream()),
+        "actnn_int8_linear");
+  return out;
+}
+
+// (y, codes, scale); the latter undefined unless `save`
+std::tuple<Tensor, Tensor, Tensor> act_forward(const Tensor& x_in, int kind, bool gated, bool save) {
+  check_values(x_in, "x");
+  int64_t cols = x_in.dim() ? x_in.size(-1) : 1;
+  TORCH_CHECK(!gated || (x_in.dim() >= 1 && cols % 2 == 0), "a gated activation splits its last dimension in two, got shape ", x_in.sizes());
+  if (gated) cols /= 2;
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const Tensor x = on_16_bytes(x_in);
+  Tensor y = gated ? make(with_last(x, cols), x.scalar_type(), x) : make(x.sizes(), x.scalar_type(), x), codes, scale;
+  const int64_t blocks = (y.numel() + 255) / 256 * (gated ? 2 : 1);
+  if (save) codes = make({blocks * 256}, at::kChar, x), scale = make({blocks}, at::kFloat, x);
+  if (y.numel())
+    check(actnn_act_forward(x.data_ptr(), y.data_ptr(), save ? codes.data_ptr<int8_t>() : nullptr, save ? scale.data_ptr<float>() : nullptr,
+                            y.numel() / cols, cols, gated, kind, dtype_id(x.scalar_type()), stream()),
+          "actnn_act_forward");
+  return {y, codes, scale};
+}
+Tensor act_backward(const Tensor& grad, const Tensor& x_in, const Tensor& codes, const Tensor& scale, int kind, bool gated) {
+  c10::cuda::CUDAGuard guard(grad.device());
+  const Tensor dy = on_16_bytes(grad);
+  const int64_t cols = dy.dim() ? dy.size(-1) : 1;
+  Tensor x, out = gated ? make(with_last(dy, 2 * cols), dy.scalar_type(), dy) : make(dy.sizes(), dy.scalar_type(), dy);
+  if (!codes.defined()) x = on_16_bytes(x_in);
+  if (dy.numel())
+    check(actnn_act_backward(dy.data_ptr(), x.defined() ? x.data_ptr() : nullptr, codes.defined() ? codes.data_ptr<int8_t>() : nullptr,
+                             codes.defined() ? scale.data_ptr<float>() : nullptr, out.data_ptr(), dy.numel() / cols, cols, gated, kind,
+                             dtype_id(dy.scalar_type()), stream()),
+          "actnn_act_backward");
+  return out;
+}
+
+// x as contiguous [N, ..., C]
+Tensor channels_behind(const Tensor& x) { return x.movedim(1, -1).contiguous(); }
+OptTensor norm_parameter(const OptTensor& p, const char* name, const Tensor& x) {
+  if (!p.has_value() || !p->defined()) return std::nullopt;
+  check_values(*p, name);
+  TORCH_CHECK(p->device() == x.device(), name, " is on ", p->device(), ", expected ", x.device());
+  TORCH_CHECK(p->dim() == 1 && p->size(0) == x.size(1), name, " must have one value for each of the ", x.size(1), " channels");
+  return as_f32(p->detach());
+}
+Tensor norm_workspace(const Tensor& x, int64_t n, int64_t s, int64_t c, int64_t groups) {
+  int64_t bytes = 0;
+  check(actnn_group_norm_workspace(n, s, c, groups, &bytes), "actnn_group_norm_workspace");
+  return make({bytes}, at::kByte, x);
+}
+struct NormForward { Tensor y, last, codes, stats; };
+NormForward norm_forward(const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps, int kind, bool codes,
+                         bool stats) {
+  check_values(x, "x");
+  TORCH_CHECK(x.dim() >= 2, "The dimension of x is not correct!");
+  const int64_t n = x.size(0), c = x.size(1);
+  TORCH_CHECK(groups >= 1 && c >= 1 && c % groups == 0, c, " channels cannot be split into ", groups, " groups");
+  c10::cuda::CUDAGuard guard(x.device());
+  NormForward r;
+  r.last = channels_behind(x);
+  int64_t s = 1;
+  for (int64_t i = 2; i < x.dim(); ++i) s *= x.size(i);
+  const OptTensor w = norm_parameter(weight, "weight", x), b = norm_parameter(bias, "bias", x);
+  Tensor y = make(r.last.sizes(), x.scalar_type(), x);
+  if (codes) r.codes = make(r.last.sizes(), at::kChar, x);
+  if (stats) r.stats = make({n, groups, 4}, at::kFloat, x);
+  const Tensor ws = norm_workspace(x, n, s, c, groups);
+  check(actnn_group_norm_forward(r.last.data_ptr(), (const float*)ptr(w), (const float*)ptr(b), y.data_ptr(),
+                                 codes ? r.codes.data_ptr<int8_t>() : nullptr, stats ? r.stats.data_ptr<float>() : nullptr, n, s, c, groups,
+                                 eps, kind, dtype_id(x.scalar_type()), ws.data_ptr(), ws.numel(), stream()),
+        "actnn_group_norm_forward");
+  r.y = y.movedim(-1, 1);
+  return r;
+}
+
 struct Relu : torch::autograd::Function<Relu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, bool with_minmax) {
     c10::cuda::CUDAGuard guard(x.device());
@@ -375,6 +542,113 @@ struct MaxPool : torch::autograd::Function<MaxPool> {
   }
 };
 
+// x, weight, bias -> x weight^T + bias in 8-bit integers; the codes of both operands are kept
+struct Int8Linear : torch::autograd::Function<Int8Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    check_values(x, "x");
+    check_values(weight, "weight");
+    TORCH_CHECK(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "shapes ", x.sizes(), " and ", weight.sizes(),
+                " cannot be multiplied");
+    TORCH_CHECK(weight.device() == x.device(), "the weight is on ", weight.device(), ", the tokens on ", x.device());
+    const int64_t n = weight.size(0), k = weight.size(1);
+    TORCH_CHECK(k <= kMostK, "a product over ", k, " values may overflow its 32-bit sum; at most ", kMostK, " are accepted");
+    check_bias(bias, x, n);
+    const bool with = bias.has_value() && bias->defined();
+    c10::cuda::CUDAGuard guard(x.device());
+    const RowCodes cx = row_codes(x), cw = row_codes(weight);
+    Tensor out = make(with_last(x, n), x.scalar_type(), x);
+    const Tensor b = with ? bias->to(x.scalar_type()).contiguous() : Tensor();
+    if (k == 0)
+      with ? out.copy_(b) : out.zero_();
+    else
+      check(actnn_int8_matmul(cx.codes.data_ptr<int8_t>(), cx.scale.data_ptr<float>(), cw.codes.data_ptr<int8_t>(), cw.scale.data_ptr<float>(),
+                              with ? b.data_ptr() : nullptr, out.data_ptr(), cx.rows, n, k, cx.ld, cw.ld, dtype_id(x.scalar_type()), stream()),
+            "actnn_int8_matmul");
+    ctx->save_for_backward({cx.codes, cx.scale, cw.codes, cw.scale});
+    ctx->saved_data["sizes"] = x.sizes();
+    ctx->saved_data["n"] = n;
+    ctx->saved_data["x"] = x.scalar_type();
+    ctx->saved_data["w"] = weight.scalar_type();
+    ctx->saved_data["b"] = with ? (int64_t)bias->scalar_type() : (int64_t)-1;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t k = sizes.back(), n = ctx->saved_data["n"].toInt();
+    const auto type = ctx->saved_data["x"].toScalarType();
+    const RowCodes cx{saved[0], saved[1], saved[0].size(0), k, saved[0].size(1)}, cw{saved[2], saved[3], n, k, saved[2].size(1)};
+    c10::cuda::CUDAGuard guard(cx.codes.device());
+    c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);       // products in the types of the forward pass
+    const Tensor go = grads[0].reshape({n ? grads[0].numel() / n : (k ? cx.rows : 0), n});
+    Tensor gx, gw, gb;
+    if (ctx->needs_input_grad(0)) gx = k ? go.mm(row_decode(cw, type)).view(sizes) : at::zeros(sizes, go.options());
+    if (ctx->needs_input_grad(1))
+      gw = k ? go.t().mm(row_decode(cx, type)).to(ctx->saved_data["w"].toScalarType())
+             : at::zeros({n, k}, go.options().dtype(ctx->saved_data["w"].toScalarType()));
+    const int64_t bias_type = ctx->saved_data["b"].toInt();
+    if (bias_type >= 0 && ctx->needs_input_grad(2)) gb = go.sum(0).to((at::ScalarType)bias_type);
+    return {gx, gw, gb};
+  }
+};
+
+// `compress` false: the input itself is kept
+struct Activation : torch::autograd::Function<Activation> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t kind, bool gated, bool compress) {
+    auto [y, codes, scale] = act_forward(x, (int)kind, gated, compress);
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["gated"] = gated;
+    ctx->saved_data["compress"] = compress;
+    if (compress) ctx->save_for_backward({codes, scale});
+    else ctx->save_for_backward({x});
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool compress = ctx->saved_data["compress"].toBool();
+    return {act_backward(grads[0], compress ? Tensor() : saved[0], compress ? saved[0] : Tensor(), compress ? saved[1] : Tensor(),
+                         (int)ctx->saved_data["kind"].toInt(), ctx->saved_data["gated"].toBool()),
+            Tensor(), Tensor(), Tensor()};
+  }
+};
+
+struct GroupNorm : torch::autograd::Function<GroupNorm> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t groups, const OptTensor& weight, const OptTensor& bias, double eps,
+                        int64_t kind, bool compress) {
+    NormForward r = norm_forward(x, groups, weight, bias, eps, (int)kind, compress, true);
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["kind"] = kind;
+    ctx->saved_data["compress"] = compress;
+    ctx->save_for_backward({compress ? r.codes : x, r.stats, weight.has_value() ? *weight : Tensor(), bias.has_value() ? *bias : Tensor()});
+    return r.y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const bool compress = ctx->saved_data["compress"].toBool();
+    const Tensor &weight = saved[2], &bias = saved[3];
+    const Tensor dy = grads[0];
+    c10::cuda::CUDAGuard guard(dy.device());
+    const Tensor last = channels_behind(dy), x = compress ? Tensor() : channels_behind(saved[0]);
+    const int64_t n = dy.size(0), c = dy.size(1), groups = ctx->saved_data["groups"].toInt();
+    int64_t s = 1;
+    for (int64_t i = 2; i < dy.dim(); ++i) s *= dy.size(i);
+    const OptTensor w = as_f32(weight), b = as_f32(bias);
+    Tensor gx = make(last.sizes(), last.scalar_type(), last), gw, gb;
+    if (weight.defined() && ctx->needs_input_grad(1)) gw = make({c}, at::kFloat, last);                    // counted without absent ones
+    if (bias.defined() && ctx->needs_input_grad(weight.defined() ? 2 : 1)) gb = make({c}, at::kFloat, last);
+    const Tensor ws = norm_workspace(last, n, s, c, groups);
+    check(actnn_group_norm_backward(last.data_ptr(), compress ? nullptr : x.data_ptr(), compress ? saved[0].data_ptr<int8_t>() : nullptr,
+                                    saved[1].data_ptr<float>(), (const float*)ptr(w), (const float*)ptr(b), gx.data_ptr(),
+                                    gw.defined() ? gw.data_ptr<float>() : nullptr, gb.defined() ? gb.data_ptr<float>() : nullptr, n, s, c,
+                                    groups, (int)ctx->saved_data["kind"].toInt(), dtype_id(last.scalar_type()), ws.data_ptr(), ws.numel(),
+                                    stream()),
+          "actnn_group_norm_backward");
+    if (gw.defined()) gw = gw.to(weight.scalar_type());
+    if (gb.defined()) gb = gb.to(bias.scalar_type());
+    return {gx.movedim(-1, 1), Tensor(), gw, gb, Tensor(), Tensor(), Tensor()};
+  }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -388,6 +662,20 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("transpose16", &transpose16);
   m.def("sample_sumsq", &sample_sumsq);
   m.def("mean_sample_sumsq", &mean_sample_sumsq);
+  m.def("int8_linear", &int8_linear);
+  m.def("int8_linear_train", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return Int8Linear::apply(x, w, b); });
+  m.def("activation", [](const Tensor& x, const std::string& name, bool gated, bool compress) {
+    return Activation::apply(x, activation_kind(name), gated, compress);
+  });
+  m.def("activation_value", [](const Tensor& x, const std::string& name, bool gated) {
+    return std::get<0>(act_forward(x, activation_kind(name), gated, false));
+  });
+  m.def("group_norm", [](const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps, const std::string& name,
+                         bool compress) { return GroupNorm::apply(x, groups, w, b, eps, activation_kind(name), compress); });
+  m.def("group_norm_value", [](const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps,
+                               const std::string& name) {
+    return norm_forward(x, groups, w, b, eps, activation_kind(name), false, false).y;
+  });
   m.def("relu", [](const Tensor& x) { return Relu::apply(x, false)[0]; });
   m.def("relu_minmax", [](const Tensor& x) { return Relu::apply(x, true); });
   m.def("dropout", [](const Tensor& x, double p) { return Dropout::apply(x, p); });

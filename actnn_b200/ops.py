@@ -24,6 +24,7 @@ import torch.nn.functional as F
 from torch.autograd.function import Function
 from torch.nn.modules.utils import _pair, _single, _triple
 
+from . import _lib
 from .conf import config
 from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import checkpoint as ext_checkpoint
@@ -644,14 +645,9 @@ def _kept(saved):
     return saved if isinstance(saved, torch.Tensor) and saved.is_cuda else swap_to_gpu(saved)
 
 
-class int8_linear(Function):
-    """``x @ weight.T + bias`` in 8-bit integers: rows of ``x`` and of ``weight`` are coded on the way (scale per token, scale per
-    output channel), and the codes are all that is kept.  The gradients are those of the product of the decoded matrices, passed
-    straight through the rounding; like those of ``linear`` they are dense products in the activation's type."""
-
+class _Int8Linear(Function):
     @staticmethod
     def forward(ctx, input, weight, bias=None):
-        input, weight, bias = _autocast_inputs(input, weight, bias)
         with _autocast_off():
             if weight.dim() != 2 or input.dim() < 1 or input.shape[-1] != weight.shape[1]:
                 raise RuntimeError("shapes %s and %s cannot be multiplied" % (tuple(input.shape), tuple(weight.shape)))
@@ -679,66 +675,90 @@ class int8_linear(Function):
         return grad_input, grad_weight, grad_bias
 
 
-class activation(Function):
-    """An activation function ("relu", "silu", "gelu", "gelu_tanh") that keeps its input in 8 bits."""
-    gated = False
+class int8_linear:
+    """``x @ weight.T + bias`` in 8-bit integers: rows of ``x`` and of ``weight`` are coded on the way (scale per token, scale per
+    output channel), and the codes are all that is kept.  The gradients are those of the product of the decoded matrices, passed
+    straight through the rounding; like those of ``linear`` they are dense products in the activation's type."""
 
-    @classmethod
-    def run_forward(cls, ctx, input, name):
-        ctx.name = name
+    @staticmethod
+    def apply(input, weight, bias=None):
+        input, weight, bias = _autocast_inputs(input, weight, bias)
+        nat = _lib.native()
+        if nat and not config.swap:
+            return nat.int8_linear_train(input, weight, bias)
+        return _Int8Linear.apply(input, weight, bias)
+
+
+class _Activation(Function):
+    @staticmethod
+    def forward(ctx, input, name, gated):
+        ctx.name, ctx.gated, ctx.codes = name, gated, None
         if not config.compress_activation:
-            ctx.saved = None
             ctx.save_for_backward(input)
-            return ext_checkpoint.activation_forward(input, name, cls.gated, save=False)[0]
-        output, codes, scale = ext_checkpoint.activation_forward(input, name, cls.gated, save=ctx.needs_input_grad[0])
-        ctx.saved = None if codes is None else (_keep(codes), scale)
+            return ext_checkpoint.activation_forward(input, name, gated, save=False)[0]
+        output, codes, scale = ext_checkpoint.activation_forward(input, name, gated)
+        ctx.codes = _keep(codes), scale
         return output
 
-    @classmethod
-    def run_backward(cls, ctx, grad_output):
-        if ctx.saved is None:
-            return ext_checkpoint.activation_backward(grad_output, ctx.name, x=ctx.saved_tensors[0], gated=cls.gated), None
-        codes, scale = ctx.saved
-        return ext_checkpoint.activation_backward(grad_output, ctx.name, _kept(codes), scale, gated=cls.gated), None
-
-    @staticmethod
-    def forward(ctx, input, name):
-        return activation.run_forward(ctx, input, name)
-
     @staticmethod
     def backward(ctx, grad_output):
-        return activation.run_backward(ctx, grad_output)
+        if ctx.codes is None:
+            grad = ext_checkpoint.activation_backward(grad_output, ctx.name, x=ctx.saved_tensors[0], gated=ctx.gated)
+        else:
+            codes, scale = ctx.codes
+            grad = ext_checkpoint.activation_backward(grad_output, ctx.name, _kept(codes), scale, gated=ctx.gated)
+        return grad, None, None
 
 
-class glu(activation):
+def _activation(input, name, gated):
+    nat = _lib.native()
+    if nat and not config.swap:
+        return nat.activation(input, name, gated, config.compress_activation)
+    return _Activation.apply(input, name, gated)
+
+
+class activation:
+    """An activation function ("none", "relu", "silu", "gelu", "gelu_tanh") that keeps its input in 8 bits."""
+
+    @staticmethod
+    def apply(input, name):
+        return _activation(input, name, False)
+
+
+class glu:
     """The gated form: ``f(gate) * up`` of the two halves of the last dimension, both kept in 8 bits."""
-    gated = True
 
     @staticmethod
-    def forward(ctx, input, name):
-        return glu.run_forward(ctx, input, name)
+    def apply(input, name):
+        return _activation(input, name, True)
+
+
+class _GroupNorm(Function):
+    @staticmethod
+    def forward(ctx, input, num_groups, weight, bias, eps, name):
+        compress = config.compress_activation
+        output, saved, stats = ext_group_norm.forward(input, num_groups, weight, bias, eps, name, compress)
+        ctx.save_for_backward(weight, bias, None if compress else input)
+        ctx.codes = _keep(saved) if compress else None
+        ctx.other_args = (num_groups, name, stats)
+        return output
 
     @staticmethod
     def backward(ctx, grad_output):
-        return glu.run_backward(ctx, grad_output)
+        weight, bias, input = ctx.saved_tensors
+        groups, name, stats = ctx.other_args
+        saved = _kept(ctx.codes) if input is None else input.movedim(1, -1).contiguous()
+        gx, gw, gb = ext_group_norm.backward(grad_output, saved, stats, groups, weight, bias, name,
+                                             (ctx.needs_input_grad[2], ctx.needs_input_grad[3]))
+        return gx, None, None if gw is None else gw.to(weight.dtype), None if gb is None else gb.to(bias.dtype), None, None
 
 
-class group_norm(Function):
+class group_norm:
     """Group norm followed by an activation function ("none" for none), on channels-last tensors, its input kept in 8 bits."""
 
     @staticmethod
-    def forward(ctx, input, num_groups, weight=None, bias=None, eps=1e-5, name="none"):
-        output, saved, stats = ext_group_norm.forward(input, num_groups, weight, bias, eps, name, config.compress_activation)
-        ctx.save_for_backward(weight, bias, *(() if config.compress_activation else (saved,)))
-        ctx.saved = (_keep(saved) if config.compress_activation else None, stats)
-        ctx.other_args = (num_groups, name)
-        return output
-
-    @staticmethod
-    def backward(ctx, grad_output):
-        weight, bias, *exact = ctx.saved_tensors
-        codes, stats = ctx.saved
-        groups, name = ctx.other_args
-        needs = ctx.needs_input_grad[2], ctx.needs_input_grad[3]
-        gx, gw, gb = ext_group_norm.backward(grad_output, exact[0] if exact else _kept(codes), stats, groups, weight, bias, name, needs)
-        return gx, None, None if gw is None else gw.to(weight.dtype), None if gb is None else gb.to(bias.dtype), None, None
+    def apply(input, num_groups, weight=None, bias=None, eps=1e-5, name="none"):
+        nat = _lib.native()
+        if nat and not config.swap:
+            return nat.group_norm(input, num_groups, weight, bias, eps, "none" if name is None else name, config.compress_activation)
+        return _GroupNorm.apply(input, num_groups, weight, bias, eps, name)

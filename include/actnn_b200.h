@@ -447,6 +447,17 @@ int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8
                       int64_t ld_tokens, int64_t ld_weights, int dtype, actnn_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * A linear layer on a weight kept as codes: x [T, K] of `dtype`, rows `ld_x` elements apart, is coded as by
+ * actnn_row_codes and multiplied as by actnn_int8_matmul, with the same result.  Up to eight tokens (whose codes
+ * fit 48 KB) in one launch; otherwise `workspace`, 16-byte aligned, takes the codes:
+ * actnn_int8_linear_workspace bytes (0: may be NULL).  The reference has no counterpart
+ * (actnn/actnn/ops.py:408-428 computes in the activation's type). */
+int actnn_int8_linear_workspace(int64_t T, int64_t K, int64_t* bytes);
+int actnn_int8_linear(const void* x, const int8_t* weights, const float* channel_scale, const void* bias, void* out,
+                      int64_t T, int64_t N, int64_t K, int64_t ld_x, int64_t ld_weights, int dtype, void* workspace,
+                      int64_t workspace_bytes, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * Activation functions whose backward pass reads an 8-bit copy of the input.  `kind`: 0 identity, 1 ReLU,
  * 2 SiLU, 3 GELU (erf), 4 GELU (tanh form).  x is [rows, cols]; with `gated` it is [rows, 2 * cols] and
  * y = f(x[:, :cols]) * x[:, cols:].  y and grad_y are [rows, cols]; all contiguous.
