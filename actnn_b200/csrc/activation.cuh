@@ -61,6 +61,8 @@ template <typename T, int V> ACTNN_DEV Vec<T, V> load_vec(const T* p) {
   Vec<T, V> r;
   if constexpr (V == 1) {
     r.v = __ldg(p);
+  } else if constexpr (V * sizeof(T) == 4) {
+    asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
   } else if constexpr (V * sizeof(T) == 8) {
     asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
   } else {
@@ -99,7 +101,9 @@ template <typename T, int V> ACTNN_DEV void store_vec(T* p, const float (&f)[V])
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) w[i] = pair_from_float(f[2 * i], f[2 * i + 1], T());
     }
-    if constexpr (V * sizeof(T) == 8) {
+    if constexpr (V * sizeof(T) == 4) {
+      asm volatile("st.global.u32 [%0], %1;" :: "l"(p), "r"(w[0]) : "memory");
+    } else if constexpr (V * sizeof(T) == 8) {
       asm volatile("st.global.v2.u32 [%0], {%1,%2};" :: "l"(p), "r"(w[0]), "r"(w[1]) : "memory");
     } else {
 #pragma unroll
@@ -134,11 +138,12 @@ ACTNN_DEV void unpack_codes4(uint32_t w, float (&f)[4]) {
   f[3] = __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - 8388736.f;
 }
 
-// V codes (V = 1, 4 or 8) in and out of memory, and as floats
+// V codes (V = 1, 2, 4 or 8) in and out of memory, and as floats
 template <int V> struct Codes { uint32_t w[(V + 3) / 4]; };
 template <int V> ACTNN_DEV Codes<V> load_codes(const int8_t* p) {
   Codes<V> r;
   if constexpr (V == 1) r.w[0] = (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(p));
+  else if constexpr (V == 2) r.w[0] = (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(p));
   else if constexpr (V == 4) asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
   else asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(r.w[0]), "=r"(r.w[1]) : "l"(p));
   return r;
@@ -146,6 +151,11 @@ template <int V> ACTNN_DEV Codes<V> load_codes(const int8_t* p) {
 template <int V> ACTNN_DEV void unpack_codes(const Codes<V>& r, float (&f)[V]) {
   if constexpr (V == 1) {
     f[0] = (float)(int8_t)r.w[0];
+  } else if constexpr (V == 2) {
+    float q[4];
+    unpack_codes4(r.w[0], q);
+    f[0] = q[0];
+    f[1] = q[1];
   } else {
 #pragma unroll
     for (int i = 0; i < V / 4; ++i) {
@@ -160,6 +170,8 @@ template <int V> ACTNN_DEV void unpack_codes(const Codes<V>& r, float (&f)[V]) {
 template <int V> ACTNN_DEV void store_codes(int8_t* p, const uint32_t (&c)[V]) {
   if constexpr (V == 1) {
     *reinterpret_cast<uint8_t*>(p) = (uint8_t)c[0];
+  } else if constexpr (V == 2) {
+    *reinterpret_cast<uint16_t*>(p) = (uint16_t)__byte_perm(c[0], c[1], 0x0040);
   } else if constexpr (V == 4) {
     *reinterpret_cast<uint32_t*>(p) = pack_codes4(c[0], c[1], c[2], c[3]);
   } else {

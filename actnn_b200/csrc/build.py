@@ -16,8 +16,9 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SOURCES = ["api.cu", "codec_mixed.cu", "codec_single.cu", "codec_generic.cu", "codec_column.cu", "codec_ragged.cu",
            "compress_mixed.cu", "stats.cu", "mask_ops.cu",
            "maxpool.cu", "batch_norm.cu", "bn_column.cu", "layout.cu",
-           "token_codes.cu", "int8_matmul.cu", "int8_few.cu", "act_checkpoint.cu", "group_norm.cu"]
-HEADERS = ["common.cuh", "quant_math.cuh", "mixed_bundle.cuh", "column.cuh", "flat_runs.cuh", "activation.cuh", "tcgen05.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
+           "token_codes.cu", "int8_matmul.cu", "int8_few.cu", "act_checkpoint.cu",
+           "group_norm.cu", "group_norm_f16.cu", "group_norm_bf16.cu"]
+HEADERS = ["common.cuh", "quant_math.cuh", "mixed_bundle.cuh", "column.cuh", "flat_runs.cuh", "activation.cuh", "tcgen05.cuh", "group_norm.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
 LIB = os.path.join(HERE, "libactnn_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",
