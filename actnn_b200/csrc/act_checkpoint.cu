@@ -24,38 +24,31 @@ template <bool GATED> ACTNN_DEV int64_t input_of_oct(int64_t oct, const GluShape
   return (oct + (int64_t)fast_div((uint32_t)oct, g.oct_cols) * g.oct_cols.d) * 8;
 }
 
-ACTNN_DEV void codes_of(const float (&f)[8], uint32_t most, int8_t* codes, float* scale, int lane) {
-  const float a = largest(most);
+ACTNN_DEV void codes_of(const float2 (&f)[4], uint32_t most, int8_t* codes, float* scale, int lane) {
+  const float a = largest(__reduce_max_sync(kFull, most));
   const float inv = code_factor(a);
-  uint32_t c[8];
+  float2 c[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = code_bits(f[i], inv);
+  for (int i = 0; i < 4; ++i) c[i] = code_bits(f[i], make_float2(inv, inv));
   store_codes<8>(codes, c);
   if (lane == 0) *scale = code_step(a);
 }
-ACTNN_DEV uint32_t most_of(const float (&f)[8]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(f[i]));
-  return __reduce_max_sync(kFull, m);
-}
 
 // Eight elements, or the first `count` of them and zeros.
-template <typename T> ACTNN_DEV void load_some(const T* p, int count, float (&f)[8]) {
-  if (count >= 8) {
-    unpack_vec(load_vec<T, 8>(p), f);
-  } else {
+template <typename T> ACTNN_DEV Vec<T, 8> load_some(const T* p, int count) {
+  if (count >= 8) return load_vec<T, 8>(p);
+  Vec<T, 8> r;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = i < count ? to_float(p[i]) : 0.f;
-  }
+  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(r.w)[i] = i < count ? p[i] : from_float<T>(0.f);
+  return r;
 }
-template <typename T> ACTNN_DEV void store_some(T* p, int count, const float (&f)[8]) {
+template <typename T> ACTNN_DEV void store_some(T* p, int count, const float2 (&f)[4]) {
   if (count >= 8) {
     store_vec<T, 8>(p, f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (i < count) p[i] = from_float<T>(f[i]);
+      if (i < count) p[i] = from_float<T>(i & 1 ? f[i / 2].y : f[i / 2].x);
   }
 }
 
@@ -72,16 +65,20 @@ act_forward_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restric
   const int64_t oct = b * 32 + lane;
   const int64_t left = numel - oct * 8;
   const int count = left >= 8 ? 8 : left > 0 ? (int)left : 0;
-  float f[8], u[8], out[8];
+  float2 f[4], u[4], out[4];
   const int64_t at = count > 0 ? input_of_oct<GATED>(oct, g) : 0;
-  load_some(x + at, count, f);
-  if constexpr (GATED) load_some(x + at + g.cols, count, u);
+  const Vec<T, 8> fv = load_some(x + at, count), uv = GATED ? load_some(x + at + g.cols, count) : fv;
+  unpack_vec(fv, f);
+  if constexpr (GATED) unpack_vec(uv, u);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) out[i] = act_value<KIND, P>(f[i]) * (GATED ? u[i] : 1.f);
+  for (int i = 0; i < 4; ++i) {
+    out[i] = act_value<KIND, P>(f[i]);
+    if constexpr (GATED) out[i] = f_mul(out[i], u[i]);
+  }
   if (count > 0) store_some(y + oct * 8, count, out);
   if constexpr (SAVE) {
-    codes_of(f, most_of(f), codes + oct * 8, scale + b, lane);
-    if constexpr (GATED) codes_of(u, most_of(u), codes + (blocks * 32 + oct) * 8, scale + blocks + b, lane);
+    codes_of(f, most_of(fv), codes + oct * 8, scale + b, lane);
+    if constexpr (GATED) codes_of(u, most_of(uv), codes + (blocks * 32 + oct) * 8, scale + blocks + b, lane);
   }
 }
 
@@ -98,30 +95,32 @@ act_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const int
   if (left <= 0) return;
   const int count = left >= 8 ? 8 : (int)left;
   const int64_t at = input_of_oct<GATED>(oct, g);
-  float f[8], u[8], d[8], df[8], du[8];
-  load_some(dy + oct * 8, count, d);
+  float2 f[4], u[4], d[4], df[4], du[4];
+  const Vec<T, 8> dv = load_some(dy + oct * 8, count);
   if constexpr (CODES) {
-    const Codes<8> cf = load_codes<8>(codes + oct * 8);
-    const float s = __ldg(scale + b);
+    const Codes<8> cf = load_codes<8>(codes + oct * 8), cu = GATED ? load_codes<8>(codes + (blocks * 32 + oct) * 8) : cf;
+    const float sf = __ldg(scale + b), su = GATED ? __ldg(scale + blocks + b) : sf;
     unpack_codes(cf, f);
+    if constexpr (GATED) unpack_codes(cu, u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] *= s;
-    if constexpr (GATED) {
-      const Codes<8> cu = load_codes<8>(codes + (blocks * 32 + oct) * 8);
-      const float su = __ldg(scale + blocks + b);
-      unpack_codes(cu, u);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) u[i] *= su;
+    for (int i = 0; i < 4; ++i) {
+      f[i] = f_mul(f[i], make_float2(sf, sf));
+      if constexpr (GATED) u[i] = f_mul(u[i], make_float2(su, su));
     }
   } else {
-    load_some(x + at, count, f);
-    if constexpr (GATED) load_some(x + at + g.cols, count, u);
+    const Vec<T, 8> fv = load_some(x + at, count), uv = GATED ? load_some(x + at + g.cols, count) : fv;
+    unpack_vec(fv, f);
+    if constexpr (GATED) unpack_vec(uv, u);
   }
+  unpack_vec(dv, d);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 v = act_both<KIND, P>(f[i]);
-    df[i] = d[i] * (GATED ? u[i] : 1.f) * v.y;
-    du[i] = d[i] * v.x;
+  for (int i = 0; i < 4; ++i) {
+    float2 value;
+    df[i] = f_mul(d[i], act_slope<KIND, P>(f[i], GATED ? &value : nullptr));
+    if constexpr (GATED) {
+      df[i] = f_mul(df[i], u[i]);
+      du[i] = f_mul(d[i], value);
+    }
   }
   store_some(dx + at, count, df);
   if constexpr (GATED) store_some(dx + at + g.cols, count, du);
@@ -152,10 +151,13 @@ glu_forward_any_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __res
   if constexpr (SAVE) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const float a = largest(most_of(half ? u : f)), inv = code_factor(a);
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = max(most, abs_bits(half ? u[j] : f[j]));
+      const float a = largest(__reduce_max_sync(kFull, most)), inv = code_factor(a);
       int8_t* c = codes + (half * blocks + b) * 256 + lane;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) c[32 * j] = (int8_t)code_bits(half ? u[j] : f[j], inv);
+      for (int j = 0; j < 8; ++j) c[32 * j] = (int8_t)__float_as_uint(code_bits(half ? u[j] : f[j], inv));
       if (lane == 0) scale[half * blocks + b] = code_step(a);
     }
   }
@@ -185,9 +187,9 @@ glu_backward_any_kernel(const T* __restrict__ dy, const T* __restrict__ x, const
         u = to_float(x[at + cols]);
       }
       const float d = to_float(dy[first + 32 * j]);
-      const float2 v = act_both<KIND, P>(f);
-      dx[at] = from_float<T>(d * u * v.y);
-      dx[at + cols] = from_float<T>(d * v.x);
+      float value;
+      dx[at] = from_float<T>(d * act_slope<KIND, P>(f, &value) * u);
+      dx[at + cols] = from_float<T>(d * value);
     }
     for (col += 32; col >= cols; col -= cols) ++row;
   }

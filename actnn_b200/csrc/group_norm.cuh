@@ -100,11 +100,79 @@ ACTNN_DEV int lanes_for(int entries) { return entries >= 32 ? 32 : entries <= 1 
 
 constexpr float kInf = __builtin_huge_valf();
 
+// Minimum and maximum of vectors.  Pairs of a 16-bit type are compared as they are.
+template <typename T, int V> struct Extremes {
+  float lo = kInf, hi = -kInf;
+  ACTNN_DEV void take(const Vec<T, V>&, const typename Many<V>::F (&f)[Many<V>::N]) {
+#pragma unroll
+    for (int i = 0; i < Many<V>::N; ++i)
+      f_each(f[i], [&](float v) {
+        lo = min_nan(lo, v);
+        hi = max_nan(hi, v);
+        return v;
+      });
+  }
+  ACTNN_DEV float lowest() const { return lo; }
+  ACTNN_DEV float highest() const { return hi; }
+};
+ACTNN_DEV uint32_t min2_nan(uint32_t a, uint32_t b, __half) {
+  uint32_t r;
+  asm("min.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+ACTNN_DEV uint32_t max2_nan(uint32_t a, uint32_t b, __half) {
+  uint32_t r;
+  asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+ACTNN_DEV uint32_t min2_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+  uint32_t r;
+  asm("min.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+ACTNN_DEV uint32_t max2_nan(uint32_t a, uint32_t b, __nv_bfloat16) {
+  uint32_t r;
+  asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <typename T, int V> struct Extremes16 {
+  uint32_t lo, hi;                                   // infinities: 0x7c00 in float16, 0x7f80 in bfloat16
+  ACTNN_DEV Extremes16() {
+    lo = pair_from_float(make_float2(kInf, kInf), T());
+    hi = lo | 0x80008000u;
+  }
+  ACTNN_DEV void take(const Vec<T, V>& w, const float2 (&)[Many<V>::N]) {
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      lo = min2_nan(lo, w.w[i], T());
+      hi = max2_nan(hi, w.w[i], T());
+    }
+  }
+  ACTNN_DEV float lowest() const {
+    const float2 p = pair_to_float(lo, T());
+    return min_nan(p.x, p.y);
+  }
+  ACTNN_DEV float highest() const {
+    const float2 p = pair_to_float(hi, T());
+    return max_nan(p.x, p.y);
+  }
+};
+
+template <int V> struct Extremes<__half, V> : Extremes16<__half, V> {};
+template <int V> struct Extremes<__nv_bfloat16, V> : Extremes16<__nv_bfloat16, V> {};
+template <> struct Extremes<__half, 1> : Extremes<float, 1> {
+  ACTNN_DEV void take(const Vec<__half, 1>&, const float (&f)[1]) { Extremes<float, 1>::take(Vec<float, 1>(), f); }
+};
+template <> struct Extremes<__nv_bfloat16, 1> : Extremes<float, 1> {
+  ACTNN_DEV void take(const Vec<__nv_bfloat16, 1>&, const float (&f)[1]) { Extremes<float, 1>::take(Vec<float, 1>(), f); }
+};
+
 // ------------------------------------------------------------------ statistics
 // A block per sample, run of positions and run of channels.  out[((n * G + group) * chunks + chunk) * parts + part].
 template <typename T, int V>
 __global__ void __launch_bounds__(kGnThreads)
 gn_stats_kernel(const T* __restrict__ x, Part* __restrict__ out, const GnShape g) {
+  using F = typename Many<V>::F;
   __shared__ float4 part_s[kGnThreads];
   const BlockAt at = block_at(g);
   const int c0 = tile_first(g, at.tile), width = tile_end(g, at.tile) - c0;
@@ -119,18 +187,19 @@ gn_stats_kernel(const T* __restrict__ x, Part* __restrict__ out, const GnShape g
       const float items = (float)(count * V);
       const T* p = x + (at.n * g.S + first + r) * g.C + c0 + v * V;
       const float shift = to_float(p[0]);
-      float s = 0.f, q = 0.f, lo = kInf, hi = -kInf;
+      F s2 = f_both<F>(0.f), q2 = f_both<F>(0.f);
+      const F off = f_both<F>(-shift);
+      Extremes<T, V> ex;
       auto take = [&](const Vec<T, V>& w) {
-        float f[V];
+        F f[Many<V>::N];
         unpack_vec(w, f);
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float d = f[i] - shift;
-          s += d;
-          q = fmaf(d, d, q);
-          lo = min_nan(lo, f[i]);
-          hi = max_nan(hi, f[i]);
+        for (int i = 0; i < Many<V>::N; ++i) {
+          const F d = f_add(f[i], off);
+          s2 = f_add(s2, d);
+          q2 = f_fma(d, d, q2);
         }
+        ex.take(w, f);
       };
       for (; count >= kGnAheadStats; count -= kGnAheadStats) {
         Vec<T, V> w[kGnAheadStats];
@@ -140,7 +209,8 @@ gn_stats_kernel(const T* __restrict__ x, Part* __restrict__ out, const GnShape g
         for (int i = 0; i < kGnAheadStats; ++i) take(w[i]);
       }
       for (; count > 0; --count, p += step) take(load_vec<T, V>(p));
-      mine = make_float4(fmaf(items, shift, s), q - s * (s / items), lo, hi);
+      const float s = f_sum(s2), q = f_sum(q2);
+      mine = make_float4(fmaf(items, shift, s), q - s * (s / items), ex.lowest(), ex.highest());
     }
     part_s[threadIdx.x] = mine;
   }
@@ -210,22 +280,39 @@ ACTNN_DEV float4 join_stats(const Part* __restrict__ p, bool in, const GnShape& 
   return make_float4(mean, 1.f / sqrtf(var + g.eps), mid, half);
 }
 
+// A constant for each channel of a thread.
+template <int V> struct Row {
+  typename Many<V>::F f[Many<V>::N];
+  ACTNN_DEV void set(int i, float v) {
+    if constexpr (V == 1) f[0] = v;
+    else if (i & 1) f[i / 2].y = v;
+    else f[i / 2].x = v;
+  }
+  ACTNN_DEV float get(int i) const {
+    if constexpr (V == 1) return f[0];
+    else return i & 1 ? f[i / 2].y : f[i / 2].x;
+  }
+};
+
 // ------------------------------------------------------------------ output and codes
 template <typename T, int V, int KIND, bool SAVE>
 ACTNN_DEV void gn_apply(const T* __restrict__ p, T* __restrict__ y, int8_t* __restrict__ codes, int64_t count, int64_t step,
-                        const float (&a)[V], const float (&b)[V], float mid, float inv) {
+                        const Row<V>& a, const Row<V>& b, float mid, float inv) {
+  using F = typename Many<V>::F;
   constexpr bool P = sizeof(T) == 4;
+  constexpr int N = Many<V>::N;
+  const F off = f_both<F>(-mid), factor = f_both<F>(inv);
   auto put = [&](const Vec<T, V>& w) {
-    float f[V], o[V];
+    F f[N], o[N];
     unpack_vec(w, f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = act_value<KIND, P>(fmaf(f[i], a[i], b[i]));
+    for (int i = 0; i < N; ++i) o[i] = act_value<KIND, P>(f_fma(f[i], a.f[i], b.f[i]));
     store_vec<T, V>(y, o);
     y += step;
     if constexpr (SAVE) {
-      uint32_t c[V];
+      F c[N];
 #pragma unroll
-      for (int i = 0; i < V; ++i) c[i] = code_bits(__fsub_rn(f[i], mid), inv);
+      for (int i = 0; i < N; ++i) c[i] = code_bits(f_add(f[i], off), factor);
       store_codes<V>(codes, c);
       codes += step;
     }
@@ -268,11 +355,12 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
   if (r >= R || first + r >= end) return;
   const int c = c0 + v * V;
   const float4 st = group_s[c / g.cpg - g0];
-  float a[V], b[V];
+  Row<V> a, b;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    a[i] = st.y * (gamma ? __ldg(gamma + c + i) : 1.f);
-    b[i] = (beta ? __ldg(beta + c + i) : 0.f) - st.x * a[i];
+    const float w = st.y * (gamma ? __ldg(gamma + c + i) : 1.f);
+    a.set(i, w);
+    b.set(i, (beta ? __ldg(beta + c + i) : 0.f) - st.x * w);
   }
   const float mid = st.z, inv = code_factor(st.w);
   const int64_t off = (at.n * g.S + first + r) * g.C + c, count = (end - first - r + R - 1) / R, step = (int64_t)R * g.C;
@@ -293,34 +381,36 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
 template <typename T, int V, bool CODES> struct Kept {
   Vec<T, V> w;
   ACTNN_DEV void load(const T* x, const int8_t*, int64_t at) { w = load_vec<T, V>(x + at); }
-  ACTNN_DEV void get(float (&f)[V], float mean) const {
+  ACTNN_DEV void get(typename Many<V>::F (&f)[Many<V>::N], float mean) const {
     unpack_vec(w, f);
 #pragma unroll
-    for (int i = 0; i < V; ++i) f[i] -= mean;
+    for (int i = 0; i < Many<V>::N; ++i) f[i] = f_add(f[i], f_both<typename Many<V>::F>(-mean));
   }
   static ACTNN_DEV float2 line(const float4& st) { return make_float2(st.y, 0.f); }
 };
 template <typename T, int V> struct Kept<T, V, true> {
   Codes<V> w;
   ACTNN_DEV void load(const T*, const int8_t* codes, int64_t at) { w = load_codes<V>(codes + at); }
-  ACTNN_DEV void get(float (&f)[V], float) const { unpack_codes<V>(w, f); }
+  ACTNN_DEV void get(typename Many<V>::F (&f)[Many<V>::N], float) const { unpack_codes<V>(w, f); }
   static ACTNN_DEV float2 line(const float4& st) { return make_float2(code_step(st.w) * st.y, (st.z - st.x) * st.y); }
 };
 
 template <typename T, int V, int KIND, bool CODES>
 ACTNN_DEV void gn_sums(const T* __restrict__ dy, const T* __restrict__ x, const int8_t* __restrict__ codes, int64_t at, int64_t count,
-                       int64_t step, float mean, const float (&za)[V], const float (&zb)[V], float (&s1)[V], float (&s2)[V]) {
-  constexpr bool P = sizeof(T) == 4;
+                       int64_t step, float mean, const Row<V>& za, const Row<V>& zb, Row<V>& s1, Row<V>& s2) {
+  using F = typename Many<V>::F;
   using K = Kept<T, V, CODES>;
+  constexpr bool P = sizeof(T) == 4;
+  constexpr int N = Many<V>::N;
   auto take = [&](const Vec<T, V>& w, const K& k) {
-    float d[V], f[V];
+    F d[N], f[N];
     unpack_vec(w, d);
     k.get(f, mean);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float dz = d[i] * act_both<KIND, P>(fmaf(f[i], za[i], zb[i])).y;
-      s1[i] += dz;
-      s2[i] = fmaf(dz, f[i], s2[i]);
+    for (int i = 0; i < N; ++i) {
+      const F dz = f_mul(d[i], act_slope<KIND, P>(f_fma(f[i], za.f[i], zb.f[i])));
+      s1.f[i] = f_add(s1.f[i], dz);
+      s2.f[i] = f_fma(dz, f[i], s2.f[i]);
     }
   };
   for (; count >= kGnAhead; count -= kGnAhead) {
@@ -356,13 +446,14 @@ gn_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const
     const int c = c0 + v * V;
     const float4 st = __ldg(reinterpret_cast<const float4*>(stats) + at.n * g.G + c / g.cpg);
     const float2 l = Kept<T, V, CODES>::line(st);
-    float za[V], zb[V], s1[V], s2[V];
+    Row<V> za, zb, s1, s2;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const float w = gamma ? __ldg(gamma + c + i) : 1.f;
-      za[i] = w * l.x;
-      zb[i] = fmaf(w, l.y, beta ? __ldg(beta + c + i) : 0.f);
-      s1[i] = s2[i] = 0.f;
+      za.set(i, w * l.x);
+      zb.set(i, fmaf(w, l.y, beta ? __ldg(beta + c + i) : 0.f));
+      s1.set(i, 0.f);
+      s2.set(i, 0.f);
     }
     const int64_t first = at.chunk * g.rows, end = min(g.S, first + g.rows), off = (at.n * g.S + first + r) * g.C + c;
     const int64_t count = first + r < end ? (end - first - r + R - 1) / R : 0, step = (int64_t)R * g.C;
@@ -374,7 +465,7 @@ gn_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const
       default: gn_sums<T, V, kActGeluTanh, CODES>(dy, x, codes, off, count, step, st.x, za, zb, s1, s2); break;
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) part_s[r * width + v * V + i] = make_float2(s1[i], fmaf(l.x, s2[i], l.y * s1[i]));
+    for (int i = 0; i < V; ++i) part_s[r * width + v * V + i] = make_float2(s1.get(i), fmaf(l.x, s2.get(i), l.y * s1.get(i)));
   }
   __syncthreads();
   for (int c = threadIdx.x; c < width; c += blockDim.x) {
@@ -389,19 +480,22 @@ gn_backward_sums_kernel(const T* __restrict__ dy, const T* __restrict__ x, const
 
 template <typename T, int V, int KIND, bool CODES>
 ACTNN_DEV void gn_grad(const T* __restrict__ dy, const T* __restrict__ x, const int8_t* __restrict__ codes, T* __restrict__ dx,
-                       int64_t at, int64_t count, int64_t step, float mean, const float (&za)[V], const float (&zb)[V],
-                       const float (&k1)[V], float k2, float k3) {
-  constexpr bool P = sizeof(T) == 4;
+                       int64_t at, int64_t count, int64_t step, float mean, const Row<V>& za, const Row<V>& zb, const Row<V>& k1,
+                       float k2, float k3) {
+  using F = typename Many<V>::F;
   using K = Kept<T, V, CODES>;
+  constexpr bool P = sizeof(T) == 4;
+  constexpr int N = Many<V>::N;
+  const F slope = f_both<F>(k2), level = f_both<F>(k3);
   int64_t to = at;
   auto put = [&](const Vec<T, V>& w, const K& k) {
-    float d[V], f[V];
+    F d[N], f[N];
     unpack_vec(w, d);
     k.get(f, mean);
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float dz = d[i] * act_both<KIND, P>(fmaf(f[i], za[i], zb[i])).y;
-      d[i] = fmaf(dz, k1[i], fmaf(f[i], k2, k3));
+    for (int i = 0; i < N; ++i) {
+      const F dz = f_mul(d[i], act_slope<KIND, P>(f_fma(f[i], za.f[i], zb.f[i])));
+      d[i] = f_fma(dz, k1.f[i], f_fma(f[i], slope, level));
     }
     store_vec<T, V>(dx + to, d);
     to += step;
@@ -458,13 +552,13 @@ gn_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const int8
   const int c = c0 + v * V;
   const float4 st = __ldg(reinterpret_cast<const float4*>(stats) + at.n * g.G + c / g.cpg);
   const float2 l = Kept<T, V, CODES>::line(st), m = means_s[c / g.cpg - g0];
-  float za[V], zb[V], k1[V];
+  Row<V> za, zb, k1;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
     const float w = gamma ? __ldg(gamma + c + i) : 1.f;
-    za[i] = w * l.x;
-    zb[i] = fmaf(w, l.y, beta ? __ldg(beta + c + i) : 0.f);
-    k1[i] = st.y * w;
+    za.set(i, w * l.x);
+    zb.set(i, fmaf(w, l.y, beta ? __ldg(beta + c + i) : 0.f));
+    k1.set(i, st.y * w);
   }
   const float k2 = -st.y * m.y * l.x, k3 = -st.y * fmaf(m.y, l.y, m.x);
   const int64_t off = (at.n * g.S + first + r) * g.C + c, count = (end - first - r + R - 1) / R, step = (int64_t)R * g.C;

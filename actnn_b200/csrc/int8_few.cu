@@ -58,23 +58,17 @@ int8_few_kernel(const T* __restrict__ x, const int8_t* __restrict__ weights, con
   if (threadIdx.x < TOK) most_s[threadIdx.x] = 0;
   __syncthreads();
   const T* p = x + t * ldx;
-  auto load = [&](int e, float (&f)[8]) {
-    if (vec && e + 8 <= K) {
-      unpack_vec(load_vec<T, 8>(p + e), f);
-    } else {
+  auto load = [&](int e) {
+    if (vec && e + 8 <= K) return load_vec<T, 8>(p + e);
+    Vec<T, 8> v;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = e + i < K ? to_float(__ldg(p + e + i)) : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = e + i < K ? __ldg(p + e + i) : from_float<T>(0.f);
+    return v;
   };
   if (t < tokens) {
     uint32_t most = 0;
 #pragma unroll 4
-    for (int e = member * 8; e < K; e += kTeam * 8) {
-      float f[8];
-      load(e, f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) most = max(most, abs_bits(f[i]));
-    }
+    for (int e = member * 8; e < K; e += kTeam * 8) most = max(most, most_of(load(e)));
     most = __reduce_max_sync(kFull, most);
     if (lane == 0) atomicMax(&most_s[t], most);
   }
@@ -84,12 +78,11 @@ int8_few_kernel(const T* __restrict__ x, const int8_t* __restrict__ weights, con
     int8_t* q = reinterpret_cast<int8_t*>(codes_s) + (size_t)t * pieces * 512;
 #pragma unroll 4
     for (int e = member * 8; e < pieces * 512; e += kTeam * 8) {
-      float f[8];
-      load(e, f);
-      uint32_t c[8];
+      float2 f[4];
+      unpack_vec(load(e), f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = code_bits(f[i], inv);
-      store_codes<8>(q + e, c);
+      for (int i = 0; i < 4; ++i) f[i] = code_bits(f[i], make_float2(inv, inv));
+      store_codes<8>(q + e, f);
     }
   }
   __syncthreads();

@@ -36,52 +36,36 @@ row_codes_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __r
   if (row >= rows) return;                             // whole warps; never with LANES > 32
   const T* p = x + row * ldx;
   int8_t* q = codes + row * ldc;
-  float f[kHeld][8];
-  uint32_t most = 0;
-  auto load = [&](int64_t e, float (&v)[8]) {
-    if constexpr (VEC) {
-      if (e < cols) {
-        unpack_vec(load_vec<T, 8>(p + e), v);
-      } else {
+  Vec<T, 8> held[kHeld];
+  auto load = [&](int64_t e) {
+    if (VEC && e < cols) return load_vec<T, 8>(p + e);
+    Vec<T, 8> v;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = e + i < cols ? to_float(__ldg(p + e + i)) : 0.f;
-    }
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && e + i < cols ? __ldg(p + e + i) : from_float<T>(0.f);
+    return v;
   };
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k) load((int64_t)(k * LANES + lane) * 8, f[k]);
+  for (int k = 0; k < kHeld; ++k) held[k] = load((int64_t)(k * LANES + lane) * 8);
+  uint32_t most = 0;
 #pragma unroll
-  for (int k = 0; k < kHeld; ++k)
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, abs_bits(f[k][i]));
-  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < cols; e += LANES * 8) {
-    float v[8];
-    load(e, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) most = max(most, abs_bits(v[i]));
-  }
+  for (int k = 0; k < kHeld; ++k) most = max(most, most_of(held[k]));
+  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < cols; e += LANES * 8) most = max(most, most_of(load(e)));
   const float a = largest(row_max<LANES>(most));
   const float inv = code_factor(a);
   if (lane == 0) scale[row] = code_step(a);
-  auto store = [&](int64_t e, const float (&v)[8]) {
-    uint32_t c[8];
+  auto store = [&](int64_t e, const Vec<T, 8>& v) {
+    float2 f[4];
+    unpack_vec(v, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = code_bits(v[i], inv);
-    store_codes<8>(q + e, c);
+    for (int i = 0; i < 4; ++i) f[i] = code_bits(f[i], make_float2(inv, inv));
+    store_codes<8>(q + e, f);
   };
 #pragma unroll
   for (int k = 0; k < kHeld; ++k) {
     const int64_t e = (int64_t)(k * LANES + lane) * 8;
-    if (e < ldc) store(e, f[k]);
+    if (e < ldc) store(e, held[k]);
   }
-  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < ldc; e += LANES * 8) {
-    float v[8];
-    load(e, v);
-    store(e, v);
-  }
+  for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < ldc; e += LANES * 8) store(e, load(e));
 }
 
 // code * scale, eight elements a thread.
@@ -93,11 +77,11 @@ row_decode_kernel(const int8_t* __restrict__ codes, const float* __restrict__ sc
   const int64_t row = i / octs, e = (i - row * octs) * 8;
   if (row >= rows) return;
   const float s = __ldg(scale + row);
-  float f[8];
   if constexpr (VEC) {
+    float2 f[4];
     unpack_codes(load_codes<8>(codes + row * ldc + e), f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] *= s;
+    for (int j = 0; j < 4; ++j) f[j] = f_mul(f[j], make_float2(s, s));
     store_vec<T, 8>(out + row * cols + e, f);
   } else {
     for (int j = 0; j < 8 && e + j < cols; ++j) out[row * cols + e + j] = from_float<T>((float)codes[row * ldc + e + j] * s);
