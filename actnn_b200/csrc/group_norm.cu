@@ -1,38 +1,45 @@
 // Group norm with an activation, channels last: the float32 kernels, how the work is cut, and the C entry points.  The formulas
 // and kernels are in group_norm.cuh.
+#include <algorithm>
+
 #include "group_norm.cuh"
 
 namespace actnn {
 
-int gn_forward_f32(const GnCall& c, const GnShape& g) { return gn_forward_of<float>(c, g); }
-int gn_backward_f32(const GnCall& c, const GnShape& g) { return gn_backward_of<float>(c, g); }
+int gn_run_f32(const GnCall& c, const GnShape& g, bool forward) { return gn_run<float>(c, g, forward); }
 
 namespace {
 
-// Cuts the channels for vectors of g.V, which divides cpg.
-void cut_channels(GnShape& g) {
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+// Cuts the channels for vectors of g.V; false where they do not fit.
+bool cut_channels(GnShape& g) {
   const int most = kGnThreads * g.V;
+  if (g.C % g.V != 0) return false;
+  const int64_t whole = (int64_t)g.cpg / gcd(g.cpg, g.V) * g.V;            // whole vectors of whole groups
   g.parts = 1;
   if (g.C <= most) {
     g.tile = g.C;
-  } else if (g.cpg <= most) {
-    g.tile = most / g.cpg * g.cpg;
+  } else if (whole <= most) {
+    g.tile = (int)(most / whole * whole);
   } else {
+    if (g.cpg % g.V != 0) return false;
     g.tile = most;
     g.parts = (g.cpg + most - 1) / most;
     g.tiles = g.G * g.parts;
-    return;
+    return true;
   }
   g.tiles = (g.C + g.tile - 1) / g.tile;
+  return true;
 }
-// Runs of positions: enough blocks for kGnBlocks on every SM, kGnLeast positions a thread at least.
-constexpr int kGnLeast = 4, kGnBlocks = 8;
+// Runs of positions: as many blocks as keep the SMs supplied, but enough positions a thread that what a block does before and
+// after them is little: kGnMany of them, or kGnFew until every SM has a block.
+constexpr int kGnMany = 24, kGnFew = 4, kGnBlocks = 4;
 void cut_positions(GnShape& g, int64_t N) {
   const int R = kGnThreads / (g.tile / g.V);
-  const int64_t want = (int64_t)device_info().sm_count * kGnBlocks;
-  int64_t k = (want + N * g.tiles - 1) / (N * g.tiles);
-  const int64_t most = (g.S + (int64_t)R * kGnLeast - 1) / ((int64_t)R * kGnLeast);
-  if (k > most) k = most;
+  const int64_t sms = device_info().sm_count, others = N * g.tiles;
+  auto runs = [&](int64_t least) { return (g.S + R * least - 1) / (R * least); };
+  auto fill = [&](int64_t blocks) { return (blocks + others - 1) / others; };
+  int64_t k = std::max(std::min(runs(kGnMany), fill(sms * kGnBlocks)), std::min(runs(kGnFew), fill(sms)));
   if (k < 1) k = 1;
   g.rows = ((g.S + k - 1) / k + R - 1) / R * R;
   g.chunks = (int)((g.S + g.rows - 1) / g.rows);
@@ -40,22 +47,22 @@ void cut_positions(GnShape& g, int64_t N) {
 
 int gn_shape(GnShape& g, int64_t N, int64_t S, int64_t C, int64_t G) {
   if (N < 0 || S < 0 || C < 1 || G < 1 || C % G != 0 || C > (1 << 24)) return ACTNN_ERR_SHAPE;
-  if (S > ((int64_t)1 << 40) / C || (N > 0 && S * C > ((int64_t)1 << 42) / N)) return ACTNN_ERR_SHAPE;
+  if (S > ((int64_t)1 << 38) / C || (N > 0 && S * C > ((int64_t)1 << 38) / N)) return ACTNN_ERR_SHAPE;     // more than memory holds
   g.S = S;
   g.C = (int)C;
   g.G = (int)G;
   g.cpg = (int)(C / G);
   return ACTNN_OK;
 }
-// The widest vectors that the channels of a group and the pointers take; false where the grid would be too large.
+// The widest vectors that the channels and the pointers take; false where the grid would be too large.
 bool gn_cut(GnShape& g, int64_t N, int dtype, const void* const* io, int n_io, const void* codes) {
   for (g.V = 8; g.V > 1; g.V /= 2) {
     const int bytes = g.V * dtype_size(dtype) < 16 ? g.V * dtype_size(dtype) : 16;
-    bool ok = g.cpg % g.V == 0 && aligned(codes, g.V);
+    bool ok = aligned(codes, g.V);
     for (int i = 0; i < n_io; ++i) ok = ok && aligned(io[i], bytes);
-    if (ok) break;
+    if (ok && cut_channels(g)) break;
   }
-  cut_channels(g);
+  cut_channels(g);                                       // one element a thread always fits
   cut_positions(g, N);
   return N * g.chunks * g.tiles <= 0x7fffffff;
 }
@@ -64,8 +71,7 @@ int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
 int64_t gn_bytes(GnShape g, int64_t N) {
   int64_t most = 0;
   for (g.V = 8; g.V >= 1; g.V /= 2) {
-    if (g.cpg % g.V != 0) continue;
-    cut_channels(g);
+    if (!cut_channels(g)) continue;
     cut_positions(g, N);
     const int64_t fwd = N * g.G * g.chunks * g.parts * (int64_t)sizeof(Part), bwd = N * g.chunks * g.C * (int64_t)sizeof(float2);
     most = fwd > most ? fwd : most;
@@ -105,7 +111,7 @@ extern "C" int actnn_group_norm_forward(const void* x, const float* gamma, const
   c.x = x; c.gamma = gamma; c.beta = beta; c.out = y; c.codes = codes; c.stats = stats; c.workspace = workspace; c.N = N;
   c.kind = kind; c.stream = (cudaStream_t)stream;
   if (!gn_cut(g, N, dtype, io, 2, codes)) return ACTNN_ERR_SHAPE;
-  return dtype == ACTNN_F32 ? gn_forward_f32(c, g) : dtype == ACTNN_F16 ? gn_forward_f16(c, g) : gn_forward_bf16(c, g);
+  return dtype == ACTNN_F32 ? gn_run_f32(c, g, true) : dtype == ACTNN_F16 ? gn_run_f16(c, g, true) : gn_run_bf16(c, g, true);
 }
 
 extern "C" int actnn_group_norm_backward(const void* grad_y, const void* x, const int8_t* codes, const float* stats,
@@ -131,5 +137,5 @@ extern "C" int actnn_group_norm_backward(const void* grad_y, const void* x, cons
   c.x = x; c.dy = grad_y; c.gamma = gamma; c.beta = beta; c.out = grad_x; c.codes = (int8_t*)codes; c.stats = (float*)stats;
   c.dgamma = grad_gamma; c.dbeta = grad_beta; c.workspace = workspace; c.N = N; c.kind = kind; c.stream = (cudaStream_t)stream;
   if (!gn_cut(g, N, dtype, io, 3, codes)) return ACTNN_ERR_SHAPE;
-  return dtype == ACTNN_F32 ? gn_backward_f32(c, g) : dtype == ACTNN_F16 ? gn_backward_f16(c, g) : gn_backward_bf16(c, g);
+  return dtype == ACTNN_F32 ? gn_run_f32(c, g, false) : dtype == ACTNN_F16 ? gn_run_f16(c, g, false) : gn_run_bf16(c, g, false);
 }

@@ -2,6 +2,5 @@
 #include "group_norm.cuh"
 
 namespace actnn {
-int gn_forward_f16(const GnCall& c, const GnShape& g) { return gn_forward_of<__half>(c, g); }
-int gn_backward_f16(const GnCall& c, const GnShape& g) { return gn_backward_of<__half>(c, g); }
+int gn_run_f16(const GnCall& c, const GnShape& g, bool forward) { return gn_run<__half>(c, g, forward); }
 }  // namespace actnn
