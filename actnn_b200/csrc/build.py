@@ -18,7 +18,7 @@ SOURCES = ["api.cu", "codec_mixed.cu", "codec_single.cu", "codec_generic.cu", "c
            "maxpool.cu", "batch_norm.cu", "bn_column.cu", "layout.cu",
            "token_codes.cu", "int8_matmul.cu", "int8_few.cu", "act_checkpoint.cu",
            "group_norm.cu", "group_norm_f16.cu", "group_norm_bf16.cu"]
-HEADERS = ["common.cuh", "quant_math.cuh", "mixed_bundle.cuh", "column.cuh", "flat_runs.cuh", "activation.cuh", "tcgen05.cuh", "group_norm.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
+HEADERS = ["common.cuh", "quant_math.cuh", "mixed_bundle.cuh", "column.cuh", "flat_runs.cuh", "activation.cuh", "cluster.cuh", "tcgen05.cuh", "group_norm.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
 LIB = os.path.join(HERE, "libactnn_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -3,7 +3,7 @@
 
 #include <cuda.h>
 
-#include "common.cuh"
+#include "cluster.cuh"
 
 namespace actnn {
 #ifdef __CUDACC__
@@ -61,23 +61,6 @@ ACTNN_DEV void mma_int8(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction
 // The barrier is arrived at once all matrix instructions that this thread issued before are done.
 ACTNN_DEV void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
-}
-
-// ------------------------------------------------------------------ clusters
-ACTNN_DEV uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-ACTNN_DEV void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-ACTNN_DEV int32_t peer_load(uint32_t addr, uint32_t rank) {
-  uint32_t remote;
-  int32_t v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
-  return v;
 }
 #endif
 }  // namespace actnn
