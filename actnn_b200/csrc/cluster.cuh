@@ -1,4 +1,4 @@
-// Thread-block clusters: barriers and distributed shared memory.
+// Thread-block clusters: barriers and distributed shared memory; and launches that overlap with the one before.
 #pragma once
 
 #include "common.cuh"
@@ -17,11 +17,11 @@ ACTNN_DEV void cluster_sync() {
 ACTNN_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 ACTNN_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // From the shared memory of block `rank`, at the place that `addr` is in this block's.
-ACTNN_DEV int32_t peer_load(uint32_t addr, uint32_t rank) {
+ACTNN_DEV int4 peer_load4i(uint32_t addr, uint32_t rank) {
   uint32_t remote;
-  int32_t v;
+  int4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(remote) : "memory");
+  asm volatile("ld.shared::cluster.v4.s32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(remote) : "memory");
   return v;
 }
 ACTNN_DEV float4 peer_load4(uint32_t addr, uint32_t rank) {
@@ -31,5 +31,10 @@ ACTNN_DEV float4 peer_load4(uint32_t addr, uint32_t rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(remote) : "memory");
   return v;
 }
+
+// ------------------------------------------------------------------ launches that overlap
+// The next launch of the stream may begin (where it was launched to); and: all launches before this one are over.
+ACTNN_DEV void grid_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+ACTNN_DEV void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 #endif
 }  // namespace actnn

@@ -329,6 +329,12 @@ int pack_single_generic(bool fused, const void* data, const void* mn, const void
 int unpack_single_generic(const int8_t* packed, int bits, const void* scale, const void* mn, void* out, int64_t N,
                           int64_t G, int64_t gs, int dtype, int stat_dtype, cudaStream_t s);
 
+// int8_matmul.cu: actnn_int8_matmul; `early`: the launch before it on the stream is the one that makes the tokens' codes, which alone
+// it has to wait for.
+int int8_matmul_impl(const int8_t* tokens, const float* token_scale, const int8_t* weights, const float* channel_scale,
+                     const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens, int64_t ld_weights,
+                     int dtype, bool early, actnn_stream_t stream);
+
 static inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 #ifdef __CUDACC__

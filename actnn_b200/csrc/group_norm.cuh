@@ -1023,9 +1023,15 @@ template <auto KERNEL, typename... Args> bool gn_start(const GnCall& c, const Gn
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, KERNEL, args...) == cudaSuccess;
 }
-// The cut of one of two launches of KERNEL.
+// The cut of one of two launches of KERNEL, by the blocks of 256 threads that an SM holds of it.
 template <auto KERNEL> void gn_cut_for(GnShape& g, int64_t N, int smem, int extra) {
-  gn_cut_positions(g, N, (int64_t)device_info().sm_count * cached_blocks_per_sm((const void*)KERNEL, gn_threads(g), smem), extra);
+  static std::atomic<int> resident{0};
+  int n = resident.load(std::memory_order_acquire);
+  if (n == 0) {
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kGnThreads, smem) != cudaSuccess || n < 1) n = 1;
+    resident.store(n, std::memory_order_release);
+  }
+  gn_cut_positions(g, N, (int64_t)device_info().sm_count * n, extra);
 }
 
 template <typename T, int V, bool ONE, bool SAVE> bool gn_forward(const GnCall& c, const GnShape& g) {

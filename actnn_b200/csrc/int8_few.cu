@@ -33,6 +33,17 @@ ACTNN_DEV uint4 weight_piece(const int8_t* row, int k, int K) {
   return v;
 }
 
+// Eight elements that are read again soon: through the L1.
+template <typename T> ACTNN_DEV Vec<T, 8> load_again(const T* p) {
+  Vec<T, 8> r;
+#pragma unroll
+  for (int i = 0; i < (int)(sizeof(T) / 2); ++i) {
+    const uint4 v = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    r.w[4 * i] = v.x, r.w[4 * i + 1] = v.y, r.w[4 * i + 2] = v.z, r.w[4 * i + 3] = v.w;
+  }
+  return r;
+}
+
 // TOK: tokens the registers hold, T <= TOK.  Codes of a token in shared memory: `pieces` * 512 bytes, zeros from K on.
 template <typename T, int TOK>
 __global__ void __launch_bounds__(kFewThreads)
@@ -59,7 +70,7 @@ int8_few_kernel(const T* __restrict__ x, const int8_t* __restrict__ weights, con
   __syncthreads();
   const T* p = x + t * ldx;
   auto load = [&](int e) {
-    if (vec && e + 8 <= K) return load_vec<T, 8>(p + e);
+    if (vec && e + 8 <= K) return load_again<T>(p + e);
     Vec<T, 8> v;
 #pragma unroll
     for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = e + i < K ? __ldg(p + e + i) : from_float<T>(0.f);
@@ -67,7 +78,7 @@ int8_few_kernel(const T* __restrict__ x, const int8_t* __restrict__ weights, con
   };
   if (t < tokens) {
     uint32_t most = 0;
-#pragma unroll 4
+#pragma unroll 8
     for (int e = member * 8; e < K; e += kTeam * 8) most = max(most, most_of(load(e)));
     most = __reduce_max_sync(kFull, most);
     if (lane == 0) atomicMax(&most_s[t], most);
@@ -156,7 +167,12 @@ template <typename T> int few_typed(const FewCall& c) {
   return c.tokens == 1 ? few<T, 1>(c) : c.tokens == 2 ? few<T, 2>(c) : c.tokens <= 4 ? few<T, 4>(c) : few<T, 8>(c);
 }
 
-bool few_tokens(int64_t T, int64_t K) { return T <= kFewTokens && T * ((K + 511) / 512 * 512) <= kFewSmem; }
+// One launch for one token, and for up to eight while coding them in every block costs less than a launch of its own.  Measured,
+// one launch against two, us, at N = 4096: K = 2048, 8 tokens 7.2 / 7.8; K = 4096, 1 token 6.1 / 10.6, 4 tokens 8.9 / 10.6, 8 tokens
+// 11.5 / 10.6; N = K = 8192, 1 token 14.2 / 18.2, 2 tokens 20.5 / 18.2.
+bool few_tokens(int64_t T, int64_t K) {
+  return T <= kFewTokens && T * ((K + 511) / 512 * 512) <= kFewSmem && (T == 1 || (K <= 4096 && T * K <= 16384));
+}
 int64_t row_bytes(int64_t K) { return (K + 15) / 16 * 16; }
 
 }  // namespace
@@ -190,7 +206,7 @@ extern "C" int actnn_int8_linear(const void* x, const int8_t* weights, const flo
     int8_t* c = (int8_t*)workspace;
     float* s = (float*)(c + codes);
     if (int st = actnn_row_codes(x, c, s, T, K, ldx, row_bytes(K), dtype, stream)) return st;
-    return actnn_int8_matmul(c, s, weights, channel_scale, bias, out, T, N, K, row_bytes(K), ldw, dtype, stream);
+    return int8_matmul_impl(c, s, weights, channel_scale, bias, out, T, N, K, row_bytes(K), ldw, dtype, true, stream);
   }
   FewCall c{x, weights, channel_scale, bias, out, (int)T, (int)K, (int)((K + 511) / 512), N, ldx, ldw,
             ldx % 8 == 0 && aligned(x, 16), (cudaStream_t)stream};

@@ -24,7 +24,7 @@ namespace {
 
 constexpr int kMmThreads = 320;                 // 8 epilogue warps, one for the copies, one for the matrix instructions
 constexpr int kMmEpilogue = 256;
-constexpr int kMmStagesMost = 8;
+constexpr int kMmStagesMost = 8, kMmSplitsMost = 8;
 constexpr int kMmStageK = 128;                  // bytes of the reduction in a stage
 constexpr int kMmChannels = 128;
 constexpr int kMmSmem = 212 * 1024;             // of the SM's 227 KB: stages, and 1 KB to align them
@@ -36,6 +36,8 @@ struct MmArgs {
   int64_t T, N;
   int K, tokens, stages, k_blocks, splits;      // tokens: columns of a tile
   int channel_tiles, tiles, columns;            // columns: of tensor memory, a buffer
+  bool vectors;                                 // four outputs of a token at a time are aligned
+  bool early;                                   // the launch before this one makes the tokens' codes, and is not waited for sooner than they are read
 };
 
 struct MmShared {
@@ -93,21 +95,34 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
 
   if (warp == 8) {                                              // ---------------- copies
     if (lane == 0) {
-      int stage = 0, issued = 0;
+      int stage = 0, issued = 0, ahead = 0;
       uint32_t phase = 0;
       bool ok = true;
+      if (a.early) {                                            // weights of the first stages before the tokens are there
+        const int ct = first_tile % a.channel_tiles;
+        for (ahead = 0; ahead < a.stages && ahead < k_end - k_first; ++ahead) {
+          const uint32_t bar = smem_addr(&s.full[ahead]);
+          mbar_expect_tx(bar, stage_bytes);
+          tile_load(stage0 + ahead * stage_bytes, &weights, (k_first + ahead) * kMmStageK, ct * kMmChannels, bar);
+        }
+        grid_wait();
+      }
       for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
         const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
         for (int k = k_first; k < k_end; ++k) {
           if (!(ok = mm_wait(smem_addr(&s.empty[stage]), phase ^ 1, s, gave_up))) break;
           const uint32_t bar = smem_addr(&s.full[stage]), dst = stage0 + stage * stage_bytes;
-          mbar_expect_tx(bar, stage_bytes);
-          tile_load(dst, &weights, k * kMmStageK, ct * kMmChannels, bar);
+          if (issued >= ahead) {
+            mbar_expect_tx(bar, stage_bytes);
+            tile_load(dst, &weights, k * kMmStageK, ct * kMmChannels, bar);
+          }
           tile_load(dst + a_bytes, &tokens, k * kMmStageK, tt * a.tokens, bar);
           ++issued;
           if (++stage == a.stages) stage = 0, phase ^= 1;
         }
       }
+      for (; ahead > issued; --ahead)                           // given up before their tokens were asked for: the barrier stays open,
+        mbar_wait(smem_addr(&s.full[ahead - 1]), 0);            // the limit of the wait outlasts the copy
       if (!ok) {                                                // what was requested still lands in this block's memory
         for (int i = 0; i < a.stages && i < issued; ++i) {
           if (--stage < 0) stage = a.stages - 1, phase ^= 1;
@@ -146,6 +161,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
     __syncwarp();
   } else {                                                      // ---------------- epilogue
     const int quarter = warp & 3, half = warp >> 2;
+    if (a.early) grid_wait();
     int buf = 0;
     uint32_t buf_phase = 0;
     for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
@@ -191,17 +207,37 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync();
-    if (warp < 8 && !s.dead) {
+    if (warp < 8 && !s.dead) {                                  // a warp takes a column: 4 channels a lane, all blocks' sums at once
       const int tt = first_tile / a.channel_tiles, ct = first_tile - tt * a.channel_tiles;
-      const int ch = threadIdx.x & 127;
-      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + ch;
-      const float w = n < a.N ? __ldg(a.channel_scale + n) : 0.f;
-      const float b = n < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
-      for (int c = (int)split + a.splits * (threadIdx.x >> 7); c < a.tokens && t0 + c < a.T; c += 2 * a.splits) {
-        int sum = 0;
-        for (int k = 0; k < a.splits; ++k) sum += peer_load(stage0 + c * (kMmChannels * 4) + ch * 4, k);
-        if (n < a.N)
-          reinterpret_cast<T*>(a.out)[(t0 + c) * a.N + n] = from_float<T>(fmaf((float)sum * __ldg(a.token_scale + t0 + c), w, b));
+      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + lane * 4;
+      float w[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = n + i < a.N ? __ldg(a.channel_scale + n + i) : 0.f;
+        b[i] = n + i < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n + i]) : 0.f;
+      }
+      const int end = (int)min((int64_t)a.tokens, a.T - t0);
+#pragma unroll 2
+      for (int c = (int)split + a.splits * warp; c < end; c += 8 * a.splits) {
+        int4 part[kMmSplitsMost];
+        const float scale = __ldg(a.token_scale + t0 + c);
+#pragma unroll
+        for (int k = 0; k < kMmSplitsMost; ++k)
+          if (k < a.splits) part[k] = peer_load4i(stage0 + c * (kMmChannels * 4) + lane * 16, k);
+        int4 sum = part[0];
+#pragma unroll
+        for (int k = 1; k < kMmSplitsMost; ++k)
+          if (k < a.splits) sum.x += part[k].x, sum.y += part[k].y, sum.z += part[k].z, sum.w += part[k].w;
+        float2 out[2] = {make_float2(fmaf((float)sum.x * scale, w[0], b[0]), fmaf((float)sum.y * scale, w[1], b[1])),
+                         make_float2(fmaf((float)sum.z * scale, w[2], b[2]), fmaf((float)sum.w * scale, w[3], b[3]))};
+        T* o = reinterpret_cast<T*>(a.out) + (t0 + c) * a.N + n;
+        if (a.vectors && n + 4 <= a.N) {
+          store_vec<T, 4>(o, out);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (n + i < a.N) o[i] = from_float<T>(i & 1 ? out[i / 2].y : out[i / 2].x);
+        }
       }
     }
     cluster_sync();                                             // nobody leaves while its sums are read
@@ -247,8 +283,14 @@ void plan(MmArgs& a) {
   a.channel_tiles = (int)((a.N + kMmChannels - 1) / kMmChannels);
   a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
   a.k_blocks = (a.K + kMmStageK - 1) / kMmStageK;
+#ifdef MM_TUNE
+  if (getenv("MM_TOKENS")) a.tokens = atoi(getenv("MM_TOKENS")), a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
+#endif
   a.splits = 1;
   while (a.splits < 8 && (int64_t)a.tiles * a.splits * 2 <= sms && a.k_blocks >= a.splits * 2 * 2) a.splits *= 2;
+#ifdef MM_TUNE
+  if (getenv("MM_SPLITS")) a.splits = atoi(getenv("MM_SPLITS"));
+#endif
   a.columns = 32;
   while (a.columns < a.tokens) a.columns *= 2;
   a.stages = (kMmSmem - 1024) / ((kMmChannels + a.tokens) * kMmStageK);
@@ -271,12 +313,14 @@ template <typename T, bool SPLIT> int launch(const CUtensorMap& w, const CUtenso
   cfg.blockDim = dim3(kMmThreads);
   cfg.dynamicSmemBytes = kMmSmem;
   cfg.stream = stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = SPLIT ? a.splits : 1;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = a.early ? 2 : 1;
   unsigned* gave_up = bulk_wait_counter();
   if (cudaLaunchKernelEx(&cfg, kernel, w, x, a, gave_up) != cudaSuccess) {
     cudaGetLastError();
@@ -293,9 +337,9 @@ template <typename T> int launch_typed(const CUtensorMap& w, const CUtensorMap& 
 
 using namespace actnn;
 
-extern "C" int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8_t* weights, const float* channel_scale,
-                                 const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens,
-                                 int64_t ld_weights, int dtype, actnn_stream_t stream) {
+int actnn::int8_matmul_impl(const int8_t* tokens, const float* token_scale, const int8_t* weights, const float* channel_scale,
+                            const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens, int64_t ld_weights,
+                            int dtype, bool early, actnn_stream_t stream) {
   if (T < 0 || N < 0 || K < 1 || K > 131072 || T > 0x7fffff00 || N > 0x7fffff00 || ld_tokens < K || ld_weights < K ||
       ld_tokens > ((int64_t)1 << 39) || ld_weights > ((int64_t)1 << 39)) return ACTNN_ERR_SHAPE;
   if (dtype < ACTNN_F32 || dtype > ACTNN_BF16) return ACTNN_ERR_DTYPE;
@@ -307,6 +351,8 @@ extern "C" int actnn_int8_matmul(const int8_t* tokens, const float* token_scale,
   MmArgs a{};
   a.token_scale = token_scale; a.channel_scale = channel_scale; a.bias = bias; a.out = out;
   a.T = T; a.N = N; a.K = (int)K;
+  a.vectors = N % 4 == 0 && aligned(out, 4 * size < 16 ? 4 * size : 16);
+  a.early = early;
   if ((N + kMmChannels - 1) / kMmChannels * ((T + 15) / 16) > 0x7fffffff) return ACTNN_ERR_SHAPE;
   plan(a);
   CUtensorMap w, x;
@@ -316,4 +362,10 @@ extern "C" int actnn_int8_matmul(const int8_t* tokens, const float* token_scale,
     case ACTNN_F16: return launch_typed<__half>(w, x, a, (cudaStream_t)stream);
     default: return launch_typed<__nv_bfloat16>(w, x, a, (cudaStream_t)stream);
   }
+}
+
+extern "C" int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8_t* weights, const float* channel_scale,
+                                 const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens,
+                                 int64_t ld_weights, int dtype, actnn_stream_t stream) {
+  return int8_matmul_impl(tokens, token_scale, weights, channel_scale, bias, out, T, N, K, ld_tokens, ld_weights, dtype, false, stream);
 }

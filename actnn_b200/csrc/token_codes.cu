@@ -5,6 +5,7 @@
 // A row is read once where the threads that share it can hold it in registers (up to 32 elements each), else twice, the
 // second time from the L2.  Bound by HBM: 2 + 1 bytes an element of a 16-bit type.
 #include "activation.cuh"
+#include "cluster.cuh"
 
 namespace actnn {
 namespace {
@@ -12,16 +13,17 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kHeld = 4;                               // vectors of eight that a thread holds
 
-// The largest of `most` over the LANES threads of a row; LANES = 32 (a warp per row) or kRowThreads.
+// The largest of `most` over the LANES threads of a row; every thread of the block takes part.
 template <int LANES> ACTNN_DEV uint32_t row_max(uint32_t most) {
   most = __reduce_max_sync(kFull, most);
   if constexpr (LANES > 32) {
-    __shared__ uint32_t warp_most[LANES / 32];
+    __shared__ uint32_t warp_most[kRowThreads / 32];
     if ((threadIdx.x & 31) == 0) warp_most[threadIdx.x >> 5] = most;
     __syncthreads();
-    most = warp_most[0];
+    const int first = threadIdx.x / LANES * (LANES / 32);
+    most = warp_most[first];
 #pragma unroll
-    for (int i = 1; i < LANES / 32; ++i) most = max(most, warp_most[i]);
+    for (int i = 1; i < LANES / 32; ++i) most = max(most, warp_most[first + i]);
   }
   return most;
 }
@@ -32,8 +34,10 @@ __global__ void __launch_bounds__(kRowThreads)
 row_codes_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __restrict__ scale, int64_t rows, int64_t cols,
                  int64_t ldx, int64_t ldc) {
   const int lane = threadIdx.x % LANES;
-  const int64_t row = (int64_t)blockIdx.x * (kRowThreads / LANES) + threadIdx.x / LANES;
-  if (row >= rows) return;                             // whole warps; never with LANES > 32
+  const int64_t mine = (int64_t)blockIdx.x * (kRowThreads / LANES) + threadIdx.x / LANES;
+  const bool in = mine < rows;
+  const int64_t row = in ? mine : rows - 1;            // threads without a row do the last one again, and write nothing
+  grid_release();                                      // of the product that may follow: it waits for the end of this launch itself
   const T* p = x + row * ldx;
   int8_t* q = codes + row * ldc;
   Vec<T, 8> held[kHeld];
@@ -52,6 +56,7 @@ row_codes_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __r
   for (int64_t e = (int64_t)(kHeld * LANES + lane) * 8; e < cols; e += LANES * 8) most = max(most, most_of(load(e)));
   const float a = largest(row_max<LANES>(most));
   const float inv = code_factor(a);
+  if (!in) return;
   if (lane == 0) scale[row] = code_step(a);
   auto store = [&](int64_t e, const Vec<T, 8>& v) {
     float2 f[4];
@@ -91,12 +96,14 @@ row_decode_kernel(const int8_t* __restrict__ codes, const float* __restrict__ sc
 template <typename T>
 int encode(const void* x, int8_t* codes, float* scale, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc, cudaStream_t s) {
   const bool vec = cols % 8 == 0 && ldx % 8 == 0 && aligned(x, 16);
-  // a warp holds 1024 elements; up to twice that its re-read costs less than a block's barrier
-  const bool warp = cols <= 2048;
-  const int64_t grid = warp ? (rows + kRowThreads / 32 - 1) / (kRowThreads / 32) : rows;
+  // as few threads a row as hold it: 32 elements each
+  const int lanes = cols <= 1024 ? 32 : cols <= 2048 ? 64 : cols <= 4096 ? 128 : 256;
+  const int64_t per = kRowThreads / lanes, grid = (rows + per - 1) / per;
   if (grid > 0x7fffffff) return ACTNN_ERR_SHAPE;
-  auto* kernel = warp ? (vec ? row_codes_kernel<T, 32, true> : row_codes_kernel<T, 32, false>)
-                      : (vec ? row_codes_kernel<T, kRowThreads, true> : row_codes_kernel<T, kRowThreads, false>);
+  auto* kernel = lanes == 32 ? (vec ? row_codes_kernel<T, 32, true> : row_codes_kernel<T, 32, false>)
+                 : lanes == 64 ? (vec ? row_codes_kernel<T, 64, true> : row_codes_kernel<T, 64, false>)
+                 : lanes == 128 ? (vec ? row_codes_kernel<T, 128, true> : row_codes_kernel<T, 128, false>)
+                                : (vec ? row_codes_kernel<T, 256, true> : row_codes_kernel<T, 256, false>);
   kernel<<<(unsigned)grid, kRowThreads, 0, s>>>((const T*)x, codes, scale, rows, cols, ldx, ldc);
   return check_launch();
 }
