@@ -96,9 +96,10 @@ struct Place {
   int64_t n, first;                     // sample, first position of the block
   int rows;                             // positions of the block; less than one in the last blocks of a short cluster
   int chunk, tile, c0, width, vecs, R, r, c, count, g0;         // g0: the tile's first group
+  int full, more;                       // every row of threads has `full` positions, the first `more` of them one more
   int64_t at, step;                     // the thread's first element, and from one of its positions to the next
 };
-ACTNN_DEV int row_count(const Place& p, int r) { return r < p.rows ? (int)((uint32_t)(p.rows - r + p.R - 1) / (uint32_t)p.R) : 0; }
+ACTNN_DEV int row_count(const Place& p, int r) { return p.full + (r < p.more ? 1 : 0); }
 template <int V> ACTNN_DEV Place place_of(const GnShape& g) {
   Place p;
   const uint32_t a = fast_div(blockIdx.x, g.by_chunks), n = fast_div(a, g.by_tiles);
@@ -119,6 +120,8 @@ template <int V> ACTNN_DEV Place place_of(const GnShape& g) {
   p.c = p.c0 + (threadIdx.x - p.r * p.vecs) * V;
   p.first = p.chunk * g.rows;
   p.rows = (int)min(g.S - p.first, g.rows);
+  p.full = p.rows > 0 ? (int)((uint32_t)p.rows / (uint32_t)p.R) : 0;
+  p.more = p.rows > 0 ? p.rows - p.full * p.R : 0;
   p.count = p.r < p.R ? row_count(p, p.r) : 0;
   p.at = (p.n * g.S + p.first + p.r) * g.C + p.c;
   p.step = (int64_t)p.R * g.C;
@@ -167,7 +170,12 @@ ACTNN_DEV float lanes_max(float v, int L) {
   for (int o = L >> 1; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(kFull, v, o));
   return v;
 }
-ACTNN_DEV int lanes_for(int entries) { return entries >= 32 ? 32 : entries <= 1 ? 1 : 1 << (32 - __clz(entries - 1)); }
+// How many lanes share a group of `entries`: so many that none idles, and that the block has lanes for all `groups` at a time.
+ACTNN_DEV int lanes_for(int entries, int groups) {
+  const int wanted = entries >= 32 ? 32 : entries <= 1 ? 1 : 1 << (32 - __clz(entries - 1));
+  const int there = groups >= (int)blockDim.x ? 1 : 1 << (31 - __clz((int)blockDim.x / groups));
+  return min(wanted, min(there, 32));
+}
 
 constexpr float kInf = __builtin_huge_valf();
 
@@ -470,8 +478,10 @@ template <typename T, int V, bool ONE> struct ThreadStats {
 template <int V, int M, typename Give> ACTNN_DEV void join_block(const float4* cell_s, const Place& p, const GnShape& g, Give give) {
   const int cells = p.vecs * M, groups = g.parts == 1 ? (int)fast_div(p.width, g.by_cpg) : 1;
   const int cpg = g.parts == 1 ? (int)g.by_cells.d : cells, entries = p.R * cpg;       // cells of a group in a row of threads
+  const float items_full = (float)(p.full * (V / M)), items_more = (float)((p.full + 1) * (V / M));
+  const float per_full = 1.f / items_full, per_more = 1.f / items_more;
   auto row_of = [&](int e) { return g.parts == 1 ? (int)fast_div(e, g.by_cells) : e / cpg; };
-  const int L = lanes_for(entries), member = threadIdx.x & (L - 1), per = blockDim.x / L;
+  const int L = lanes_for(entries, groups), member = threadIdx.x & (L - 1), per = blockDim.x / L;
   for (int j0 = 0; j0 < groups; j0 += per) {
     const int j = j0 + threadIdx.x / L;
     const bool in = j < groups;
@@ -488,9 +498,10 @@ template <int V, int M, typename Give> ACTNN_DEV void join_block(const float4* c
     for (int e = member; in && e < entries; e += L) {
       const int er = row_of(e);
       const float4 q = cell_s[er * cells + j * cpg + (e - er * cpg)];
-      const float items = (float)(row_count(p, er) * (V / M));
+      const bool one_more = er < p.more;
+      const float items = one_more ? items_more : items_full;
       if (items > 0.f) {
-        const float d = q.x / items - mean;
+        const float d = q.x * (one_more ? per_more : per_full) - mean;
         m2 += fmaf(items * d, d, q.y);
       }
     }
@@ -635,7 +646,7 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
   Positions<T, V, Alone<T, V>> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Alone<T, V>>::kDepth);
   pos.start();
   const int g0 = p.g0, groups = g.parts == 1 ? (int)fast_div(p.width, g.by_cpg) : 1, count = g.first_chunks * g.first_parts;
-  const int L = lanes_for(count), per = blockDim.x / L, member = threadIdx.x & (L - 1);
+  const int L = lanes_for(count, groups), per = blockDim.x / L, member = threadIdx.x & (L - 1);
   for (int j0 = 0; j0 < groups; j0 += per) {
     const int j = j0 + threadIdx.x / L;
     const Part* q = parts + (p.n * g.G + g0 + (j < groups ? j : 0)) * count;
@@ -673,7 +684,7 @@ gn_forward_held_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
   __syncthreads();
   join_block<V, Stats::M>(cell_s, p, g, [&](int j, const Part& q) { own_s[j] = make_float4(q.mean, q.m2, q.lo, q.hi); });
   cluster_sync();
-  const int g0 = p.g0, groups = (int)fast_div(p.width, g.by_cpg), L = lanes_for(g.chunks), per = blockDim.x / L, member = threadIdx.x & (L - 1);
+  const int g0 = p.g0, groups = (int)fast_div(p.width, g.by_cpg), L = lanes_for(g.chunks, groups), per = blockDim.x / L, member = threadIdx.x & (L - 1);
   for (int j0 = 0; j0 < groups; j0 += per) {
     const int j = j0 + threadIdx.x / L;
     const uint32_t own = smem_addr(own_s + (j < groups ? j : 0));
@@ -844,7 +855,7 @@ ACTNN_DEV void grad_all(Positions<T, V, Kept<T, V, CODES>>& pos, const Line<T, V
 template <typename Load>
 ACTNN_DEV void group_means(float4* mean_s, const Place& p, const GnShape& g, const float* gamma, int runs, Load load) {
   const int groups = g.parts == 1 ? (int)fast_div(p.width, g.by_cpg) : 1, entries = runs * g.cpg;
-  const int L = lanes_for(entries), per = blockDim.x / L, member = threadIdx.x & (L - 1), gc0 = p.g0 * g.cpg;
+  const int L = lanes_for(entries, groups), per = blockDim.x / L, member = threadIdx.x & (L - 1), gc0 = p.g0 * g.cpg;
   for (int j0 = 0; j0 < groups; j0 += per) {
     const int j = j0 + threadIdx.x / L;
     float a = 0.f, b = 0.f;
