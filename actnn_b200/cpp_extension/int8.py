@@ -5,6 +5,8 @@ Rows of codes start on 16 bytes: ``quantize_rows`` returns a ``[.., K]`` view of
 A row that holds a NaN or an infinity decodes to NaN, its neighbours stay as they are.
 
 The reference computes its linear layers in the activation's type (actnn/actnn/ops.py:408-428) and has no counterpart."""
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -85,6 +87,21 @@ def matmul(codes, scale, weight_codes, weight_scale, bias=None, dtype=torch.bflo
     scale, weight_scale = scale.contiguous(), weight_scale.contiguous()
     _lib.call("actnn_int8_matmul", out, flat.data_ptr(), scale.data_ptr(), weights.data_ptr(), weight_scale.data_ptr(),
               _lib.ptr(bias), out.data_ptr(), flat.shape[0], n, k, ld, ld_w, _lib.dtype_id(dtype), _lib.stream_of(out))
+    return out
+
+
+def column_sums(x):
+    """The sums over the rows of a matrix, in float32 and rounded once: the gradient of a bias."""
+    check_cuda_values(x, "x")
+    if x.dim() != 2:
+        raise RuntimeError("The dimension of x is not correct!")
+    x = x.contiguous()
+    size = ctypes.c_int64(0)
+    _lib.call("actnn_column_sums_workspace", x, x.shape[0], x.shape[1], ctypes.addressof(size))
+    ws = _lib.scratch(x.device, size.value)
+    out = torch.empty(x.shape[1], dtype=x.dtype, device=x.device)
+    _lib.call("actnn_column_sums", x, x.data_ptr(), out.data_ptr(), x.shape[0], x.shape[1], _lib.dtype_id(x.dtype), ws.data_ptr(),
+              size.value, _lib.stream_of(x))
     return out
 
 

@@ -42,9 +42,9 @@ template <typename T> ACTNN_DEV Vec<T, 8> load_some(const T* p, int count) {
   for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(r.w)[i] = i < count ? p[i] : from_float<T>(0.f);
   return r;
 }
-template <typename T> ACTNN_DEV void store_some(T* p, int count, const float2 (&f)[4]) {
+template <typename T, bool STREAM> ACTNN_DEV void store_some(T* p, int count, const float2 (&f)[4]) {
   if (count >= 8) {
-    store_vec<T, 8>(p, f);
+    store_vec<T, 8, STREAM>(p, f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -75,7 +75,7 @@ act_forward_kernel(const T* __restrict__ x, T* __restrict__ y, int8_t* __restric
     out[i] = act_value<KIND, P>(f[i]);
     if constexpr (GATED) out[i] = f_mul(out[i], u[i]);
   }
-  if (count > 0) store_some(y + oct * 8, count, out);
+  if (count > 0) store_some<T, false>(y + oct * 8, count, out);
   if constexpr (SAVE) {
     codes_of(f, most_of(fv), codes + oct * 8, scale + b, lane);
     if constexpr (GATED) codes_of(u, most_of(uv), codes + (blocks * 32 + oct) * 8, scale + blocks + b, lane);
@@ -122,8 +122,9 @@ act_backward_kernel(const T* __restrict__ dy, const T* __restrict__ x, const int
       du[i] = f_mul(d[i], value);
     }
   }
-  store_some(dx + at, count, df);
-  if constexpr (GATED) store_some(dx + at + g.cols, count, du);
+  // evict-first stores: 16384 x 4096 gated bfloat16 81.3 -> 77.9 us; the output of the forward pass gains nothing by them
+  store_some<T, true>(dx + at, count, df);
+  if constexpr (GATED) store_some<T, true>(dx + at + g.cols, count, du);
 }
 
 // The gated form where a row is not a whole number of aligned vectors: element j * 32 + lane of a block is the lane's j-th, so

@@ -129,7 +129,8 @@ template <typename T, int V> ACTNN_DEV void unpack_vec(const Vec<T, V>& r, typen
     }
   }
 }
-template <typename T, int V> ACTNN_DEV void store_vec(T* p, const typename Many<V>::F (&f)[Many<V>::N]) {
+// STREAM: written once and not read soon (evict first).
+template <typename T, int V, bool STREAM = false> ACTNN_DEV void store_vec(T* p, const typename Many<V>::F (&f)[Many<V>::N]) {
   if constexpr (V == 1) {
     *p = from_float<T>(f[0]);
   } else {
@@ -150,7 +151,10 @@ template <typename T, int V> ACTNN_DEV void store_vec(T* p, const typename Many<
     } else {
 #pragma unroll
       for (int i = 0; i < (int)(V * sizeof(T) / 16); ++i)
-        asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};"
+        if constexpr (STREAM) asm volatile("st.global.cs.v4.u32 [%0], {%1,%2,%3,%4};"
+                     :: "l"(reinterpret_cast<char*>(p) + 16 * i), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
+                        "r"(w[4 * i + 3]) : "memory");
+        else asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};"
                      :: "l"(reinterpret_cast<char*>(p) + 16 * i), "r"(w[4 * i]), "r"(w[4 * i + 1]), "r"(w[4 * i + 2]),
                         "r"(w[4 * i + 3]) : "memory");
     }

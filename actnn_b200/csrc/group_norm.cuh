@@ -100,11 +100,12 @@ struct Place {
   int64_t at, step;                     // the thread's first element, and from one of its positions to the next
 };
 ACTNN_DEV int row_count(const Place& p, int r) { return p.full + (r < p.more ? 1 : 0); }
-template <int V> ACTNN_DEV Place place_of(const GnShape& g) {
+// BACK: from the last sample to the first, for a launch that reads what the one before it read: the end is still in the L2.
+template <int V, bool BACK = false> ACTNN_DEV Place place_of(const GnShape& g) {
   Place p;
-  const uint32_t a = fast_div(blockIdx.x, g.by_chunks), n = fast_div(a, g.by_tiles);
+  const uint32_t block = BACK ? gridDim.x - 1 - blockIdx.x : blockIdx.x, a = fast_div(block, g.by_chunks), n = fast_div(a, g.by_tiles);
   p.n = n;
-  p.chunk = (int)(blockIdx.x - a * (uint32_t)g.chunks);
+  p.chunk = (int)(block - a * (uint32_t)g.chunks);
   p.tile = (int)(a - n * (uint32_t)g.tiles);
   p.c0 = tile_first(g, p.tile);
   p.width = tile_end(g, p.tile) - p.c0;
@@ -642,7 +643,7 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
                   const float* __restrict__ beta, T* __restrict__ y, int8_t* __restrict__ codes, float* __restrict__ stats,
                   int kind, const GnShape g) {
   extern __shared__ float4 dynamic_s[];                   // tables, ring
-  const Place p = place_of<V>(g);
+  const Place p = place_of<V, true>(g);
   Positions<T, V, Alone<T, V>> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Alone<T, V>>::kDepth);
   pos.start();
   const int g0 = p.g0, groups = g.parts == 1 ? (int)fast_div(p.width, g.by_cpg) : 1, count = g.first_chunks * g.first_parts;
@@ -896,7 +897,7 @@ gn_backward_kernel(const T* __restrict__ dy, const void* __restrict__ kept, cons
                    const float* __restrict__ gamma, const float* __restrict__ beta, const float2* __restrict__ sums,
                    T* __restrict__ dx, int kind, const GnShape g) {
   extern __shared__ float4 dynamic_s[];                   // tables, ring
-  const Place p = place_of<V>(g);
+  const Place p = place_of<V, true>(g);
   Positions<T, V, Kept<T, V, CODES>> pos(dy, kept, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Kept<T, V, CODES>>::kDepth);
   pos.start();
   group_means(dynamic_s, p, g, gamma, g.first_chunks, [&](int k, int c) { return sums[(p.n * g.first_chunks + k) * g.C + c]; });

@@ -335,6 +335,18 @@ Tensor row_decode(const RowCodes& r, at::ScalarType t) {
         "actnn_row_decode");
   return out;
 }
+// The sums over the rows of a matrix.
+Tensor column_sums(const Tensor& x_in) {
+  const Tensor x = x_in.contiguous();
+  const int64_t rows = x.size(0), cols = x.size(1);
+  Tensor out = make({cols}, x.scalar_type(), x);
+  int64_t bytes = 0;
+  check(actnn_column_sums_workspace(rows, cols, &bytes), "actnn_column_sums_workspace");
+  Tensor ws = make({bytes}, at::kByte, x);
+  check(actnn_column_sums(x.data_ptr(), out.data_ptr(), rows, cols, dtype_id(x.scalar_type()), ws.data_ptr(), bytes, stream()),
+        "actnn_column_sums");
+  return out;
+}
 std::vector<int64_t> with_last(const Tensor& x, int64_t n) {
   std::vector<int64_t> s = x.sizes().vec();
   s.back() = n;
@@ -587,7 +599,7 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
       gw = k ? go.t().mm(row_decode(cx, type)).to(ctx->saved_data["w"].toScalarType())
              : at::zeros({n, k}, go.options().dtype(ctx->saved_data["w"].toScalarType()));
     const int64_t bias_type = ctx->saved_data["b"].toInt();
-    if (bias_type >= 0 && ctx->needs_input_grad(2)) gb = go.sum(0).to((at::ScalarType)bias_type);
+    if (bias_type >= 0 && ctx->needs_input_grad(2)) gb = column_sums(go).to((at::ScalarType)bias_type);
     return {gx, gw, gb};
   }
 };

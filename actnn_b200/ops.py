@@ -671,7 +671,7 @@ class _Int8Linear(Function):
                 x = ext_int8.dequantize_rows(_kept(codes), scale, dtype)
                 grad_weight = go.t().mm(x.view(-1, shape[-1])).to(wdtype)
             if bdtype is not None and ctx.needs_input_grad[2]:
-                grad_bias = go.sum(0).to(bdtype)
+                grad_bias = ext_int8.column_sums(go).to(bdtype)
         return grad_input, grad_weight, grad_bias
 
 

@@ -435,6 +435,14 @@ int actnn_row_decode(const int8_t* codes, const float* scale, void* out, int64_t
                      int64_t ld_codes, int dtype, actnn_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Sums over the rows of x [rows, cols], contiguous, in float32 and rounded once to `dtype`: the gradient of a
+ * linear layer's bias (grad_output.sum(0), actnn/actnn/ops.py:425).  Fixed order of summation; workspace of
+ * actnn_column_sums_workspace bytes, 4-byte aligned. */
+int actnn_column_sums_workspace(int64_t rows, int64_t cols, int64_t* bytes);
+int actnn_column_sums(const void* x, void* out, int64_t rows, int64_t cols, int dtype, void* workspace,
+                      int64_t workspace_bytes, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * out[t, n] = (sum_k tokens[t, k] * weights[n, k]) * token_scale[t] * channel_scale[n] + bias[n]
  * on the integer tensor cores; the sum is exact (int32), out is [T, N] contiguous of `dtype`, rounded
  * once.  `bias` (of `dtype`) may be NULL.  Rows of codes start on 16 bytes: pointers and ld_* (bytes)

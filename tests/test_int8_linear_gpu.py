@@ -222,6 +222,19 @@ def test_gradients(cuda_device, dtype, shape, n, with_bias):
         assert bool(((b.grad.double() - g.sum(0)).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,cols", [(0, 5), (1, 1), (3, 0), (31, 64), (33, 65), (700, 1000), (5000, 8), (64, 4104), (2, 20000)])
+def test_column_sums(cuda_device, dtype, rows, cols):
+    from actnn_b200.cpp_extension import int8
+    x = tokens(rows, cols, dtype)
+    got, ref = int8.column_sums(x), x.double().sum(0)
+    bound = UNIT[dtype] * ref.abs() + (rows + 8) * 2.0 ** -24 * x.double().abs().sum(0) + (2.0 ** -25 if dtype == torch.float16 else 0)
+    assert got.dtype == dtype and got.shape == (cols,) and bool(((got.double() - ref).abs() <= bound).all())
+    if rows > 2:
+        y = torch.cat([x, x], 1)[:, cols // 2:cols // 2 + cols]                      # strides and starts that no vector fits
+        assert torch.equal(int8.column_sums(y), int8.column_sums(y.contiguous()))
+
+
 def test_gradients_against_differences(cuda_device):
     """Along a direction that keeps every code (one common factor), the loss moves as the gradient says."""
     from actnn_b200 import ops

@@ -35,6 +35,17 @@ def test_row_codes(lib):
     assert call(*changed(args, _2=257)) == ALIGN
 
 
+def test_column_sums(lib):
+    size = ctypes.c_int64(0)
+    assert lib.actnn_column_sums_workspace(100, 40, ctypes.addressof(size)) == 0 and size.value > 0
+    assert lib.actnn_column_sums_workspace(100, 40, None) == NULL and lib.actnn_column_sums_workspace(-1, 40, ctypes.addressof(size)) == SHAPE
+    # x out, rows cols dtype, workspace bytes, stream
+    args, call = [256, 256, 100, 40, 1, 256, 1 << 20, None], lib.actnn_column_sums
+    assert call(*changed(args, _2=-1)) == SHAPE and call(*changed(args, _4=3)) == DTYPE and call(*changed(args, _3=0)) == 0
+    assert all(call(*changed(args, **{"_%d" % i: None})) == NULL for i in (0, 1, 5))
+    assert call(*changed(args, _0=257)) == ALIGN and call(*changed(args, _5=258)) == ALIGN and call(*changed(args, _6=16)) == CAPACITY
+
+
 def test_int8_matmul(lib):
     # tokens token_scale weights channel_scale bias out, T N K ld_tokens ld_weights dtype, stream
     args, call = [256] * 6 + [4, 8, 40, 48, 48, 1, None], lib.actnn_int8_matmul
