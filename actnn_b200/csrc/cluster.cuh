@@ -17,6 +17,15 @@ ACTNN_DEV void cluster_sync() {
 ACTNN_DEV void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
 ACTNN_DEV void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // From the shared memory of block `rank`, at the place that `addr` is in this block's.
+ACTNN_DEV uint32_t peer_addr(uint32_t addr, uint32_t rank) {
+  uint32_t remote;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(addr), "r"(rank));
+  return remote;
+}
+// Arrives at a barrier of the cluster.
+ACTNN_DEV void peer_arrive(uint32_t remote) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(remote) : "memory");
+}
 ACTNN_DEV int4 peer_load4i(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   int4 v;

@@ -27,6 +27,7 @@ constexpr int kMmEpilogue = 256;
 constexpr int kMmStagesMost = 8, kMmSplitsMost = 8;
 constexpr int kMmStageK = 128;                  // bytes of the reduction in a stage
 constexpr int kMmChannels = 128;
+constexpr int kMmStaging = 32 * 1024;           // outputs on their way: two buffers for each half of the epilogue's warps
 constexpr int kMmSmem = 212 * 1024;             // of the SM's 227 KB: stages, and 1 KB to align them
 
 struct MmArgs {
@@ -36,6 +37,8 @@ struct MmArgs {
   int64_t T, N;
   int K, tokens, stages, k_blocks, splits;      // tokens: columns of a tile
   int channel_tiles, tiles, columns;            // columns: of tensor memory, a buffer
+  bool pair;                                    // tiles of 256 channels by pairs of blocks
+  bool boxes;                                   // outputs leave as boxes of 128 channels
   bool vectors;                                 // four outputs of a token at a time are aligned
   bool early;                                   // the launch before this one makes the tokens' codes, and is not waited for sooner than they are read
 };
@@ -44,8 +47,16 @@ struct MmShared {
   uint64_t full[kMmStagesMost], empty[kMmStagesMost], sum_full[2], sum_empty[2], drained;
   uint32_t tmem;
   int dead;
-  float scale[2][256];
+  alignas(16) float scale[2][256];
 };
+
+// Tokens of a box: 8 KB of 128 channels.
+template <typename T> constexpr int box_tokens() { return kMmStaging / 4 / (kMmChannels * (int)sizeof(T)); }
+ACTNN_DEV void store_shared(uint32_t at, float v) { asm volatile("st.shared.f32 [%0], %1;" :: "r"(at), "f"(v) : "memory"); }
+ACTNN_DEV void store_shared(uint32_t at, __half v) { asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(__half_as_ushort(v)) : "memory"); }
+ACTNN_DEV void store_shared(uint32_t at, __nv_bfloat16 v) {
+  asm volatile("st.shared.u16 [%0], %1;" :: "r"(at), "h"(__bfloat16_as_ushort(v)) : "memory");
+}
 
 // Waits for a phase; false once this or another wait of the block has run out.
 ACTNN_DEV bool mm_wait(uint32_t bar, uint32_t parity, MmShared& s, unsigned* gave_up) {
@@ -59,19 +70,23 @@ ACTNN_DEV bool mm_wait(uint32_t bar, uint32_t parity, MmShared& s, unsigned* gav
   return false;
 }
 
-template <typename T, bool SPLIT>
+// SPLIT: the reduction is split over a cluster.  PAIR: a cluster of two blocks computes a tile of 256 channels, half of the channels
+// and half of the tokens' operand in each; the first one issues the matrix instructions, its barriers count the copies of both.
+template <typename T, bool SPLIT, bool PAIR>
 __global__ void __launch_bounds__(kMmThreads, 1)
-int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens, const MmArgs a,
-                   unsigned* gave_up) {
+int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens,
+                   const __grid_constant__ CUtensorMap outputs, const MmArgs a, unsigned* gave_up) {
   extern __shared__ uint8_t dynamic_s[];
   __shared__ MmShared s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t stage0 = (smem_addr(dynamic_s) + 1023u) & ~1023u;
-  const uint32_t a_bytes = kMmChannels * kMmStageK, stage_bytes = a_bytes + a.tokens * kMmStageK;
-  const uint32_t split = SPLIT ? cluster_rank() : 0;
+  const uint32_t rank = SPLIT || PAIR ? cluster_rank() : 0, split = SPLIT ? rank : 0;
+  const int load_tokens = PAIR ? a.tokens / 2 : a.tokens, tile_channels = PAIR ? 2 * kMmChannels : kMmChannels;
+  const uint32_t a_bytes = kMmChannels * kMmStageK, stage_bytes = a_bytes + load_tokens * kMmStageK;
   const int k_first = SPLIT ? (int)((int64_t)split * a.k_blocks / a.splits) : 0;
   const int k_end = SPLIT ? (int)((int64_t)(split + 1) * a.k_blocks / a.splits) : a.k_blocks;
-  const int first_tile = SPLIT ? blockIdx.x / a.splits : blockIdx.x, tile_step = SPLIT ? a.tiles : gridDim.x;
+  const int first_tile = SPLIT ? blockIdx.x / a.splits : PAIR ? blockIdx.x / 2 : blockIdx.x;
+  const int tile_step = SPLIT ? a.tiles : PAIR ? gridDim.x / 2 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < a.stages; ++i) {
@@ -80,16 +95,17 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_addr(&s.sum_full[i]), 1);
-      mbar_init(smem_addr(&s.sum_empty[i]), kMmEpilogue / 32);
+      mbar_init(smem_addr(&s.sum_empty[i]), (PAIR ? 2 : 1) * kMmEpilogue / 32);
     }
     mbar_init(smem_addr(&s.drained), 1);
     s.dead = 0;
     mbar_init_fence();
   }
   const uint32_t columns = SPLIT ? a.columns : 2 * a.columns;
-  if (warp == 9) tmem_alloc(smem_addr(&s.tmem), columns);
+  if (warp == 9) tmem_alloc<PAIR>(smem_addr(&s.tmem), columns);
   tmem_fence_before_sync();
   __syncthreads();
+  if constexpr (PAIR) cluster_sync();                           // both blocks have their barriers and their tensor memory
   tmem_fence_after_sync();
   const uint32_t tmem = s.tmem;
 
@@ -98,12 +114,20 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       int stage = 0, issued = 0, ahead = 0;
       uint32_t phase = 0;
       bool ok = true;
+      // Requests one operand of a stage; of a pair, the first block's barrier counts.
+      auto request = [&](int stage, uint32_t offset, const CUtensorMap* map, int k, int row) {
+        const uint32_t dst = stage0 + stage * stage_bytes + offset, bar = smem_addr(&s.full[stage]);
+        if constexpr (PAIR) tile_load_pair(dst, map, k * kMmStageK, row, peer_addr(bar, 0));
+        else tile_load(dst, map, k * kMmStageK, row, bar);
+      };
+      auto expect = [&](int stage) {
+        if (!PAIR || rank == 0) mbar_expect_tx(smem_addr(&s.full[stage]), PAIR ? 2 * stage_bytes : stage_bytes);
+      };
       if (a.early) {                                            // weights of the first stages before the tokens are there
         const int ct = first_tile % a.channel_tiles;
-        for (ahead = 0; ahead < a.stages && ahead < k_end - k_first; ++ahead) {
-          const uint32_t bar = smem_addr(&s.full[ahead]);
-          mbar_expect_tx(bar, stage_bytes);
-          tile_load(stage0 + ahead * stage_bytes, &weights, (k_first + ahead) * kMmStageK, ct * kMmChannels, bar);
+        for (ahead = 0; first_tile < a.tiles && ahead < a.stages && ahead < k_end - k_first; ++ahead) {
+          expect(ahead);
+          request(ahead, 0, &weights, k_first + ahead, ct * tile_channels + (int)rank * kMmChannels * PAIR);
         }
         grid_wait();
       }
@@ -111,28 +135,31 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
         const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
         for (int k = k_first; k < k_end; ++k) {
           if (!(ok = mm_wait(smem_addr(&s.empty[stage]), phase ^ 1, s, gave_up))) break;
-          const uint32_t bar = smem_addr(&s.full[stage]), dst = stage0 + stage * stage_bytes;
           if (issued >= ahead) {
-            mbar_expect_tx(bar, stage_bytes);
-            tile_load(dst, &weights, k * kMmStageK, ct * kMmChannels, bar);
+            expect(stage);
+            request(stage, 0, &weights, k, ct * tile_channels + (int)rank * kMmChannels * PAIR);
           }
-          tile_load(dst + a_bytes, &tokens, k * kMmStageK, tt * a.tokens, bar);
+          request(stage, a_bytes, &tokens, k, tt * a.tokens + (int)rank * load_tokens * PAIR);
           ++issued;
           if (++stage == a.stages) stage = 0, phase ^= 1;
         }
       }
-      for (; ahead > issued; --ahead)                           // given up before their tokens were asked for: the barrier stays open,
-        mbar_wait(smem_addr(&s.full[ahead - 1]), 0);            // the limit of the wait outlasts the copy
-      if (!ok) {                                                // what was requested still lands in this block's memory
-        for (int i = 0; i < a.stages && i < issued; ++i) {
+      if (!ok) {
+        // What was requested still lands in this block's memory.  Where no barrier of this block tells (a pair's second block; a
+        // stage whose tokens were never asked for), the limit of a wait outlasts it: `drained` has no second phase.
+        if (PAIR || ahead > issued) {
+          mbar_wait(smem_addr(&s.drained), 0);
+          mbar_wait(smem_addr(&s.drained), 1);
+        }
+        for (int i = 0; !PAIR && i < a.stages && i < issued; ++i) {
           if (--stage < 0) stage = a.stages - 1, phase ^= 1;
           mbar_wait(smem_addr(&s.full[stage]), phase);
         }
       }
     }
   } else if (warp == 9) {                                       // ---------------- matrix instructions
-    if (lane == 0) {
-      const uint32_t instruction = int8_instruction(a.tokens);
+    if (lane == 0 && (!PAIR || rank == 0)) {
+      const uint32_t instruction = int8_instruction(tile_channels, a.tokens);
       int stage = 0, buf = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
@@ -147,26 +174,26 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
           const uint64_t da = rows128_descriptor(at), db = rows128_descriptor(at + a_bytes);
 #pragma unroll
           for (int i = 0; i < kMmStageK / 32; ++i)              // 32 bytes further along the rows: 2 in units of 16 bytes
-            mma_int8(d, da + 2 * i, db + 2 * i, instruction, k > k_first || i > 0);
-          mma_commit(smem_addr(&s.empty[stage]));
+            mma_int8<PAIR>(d, da + 2 * i, db + 2 * i, instruction, k > k_first || i > 0);
+          mma_commit<PAIR>(smem_addr(&s.empty[stage]));
           if (++stage == a.stages) stage = 0, phase ^= 1;
         }
         if (!ok) break;
-        mma_commit(smem_addr(&s.sum_full[buf]));
+        mma_commit<PAIR>(smem_addr(&s.sum_full[buf]));
         if (++buf == 2) buf = 0, buf_phase ^= 1;
       }
-      mma_commit(smem_addr(&s.drained));
+      mma_commit<PAIR>(smem_addr(&s.drained));
       mbar_wait(smem_addr(&s.drained), 0);
     }
     __syncwarp();
   } else {                                                      // ---------------- epilogue
     const int quarter = warp & 3, half = warp >> 2;
     if (a.early) grid_wait();
-    int buf = 0;
+    int buf = 0, box_buf = 0;
     uint32_t buf_phase = 0;
     for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
       const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
-      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + quarter * 32 + lane;
+      const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * tile_channels + rank * kMmChannels * PAIR + quarter * 32 + lane;
       if constexpr (!SPLIT) {
         if ((int)threadIdx.x < a.tokens) s.scale[buf][threadIdx.x] = t0 + threadIdx.x < a.T ? __ldg(a.token_scale + t0 + threadIdx.x) : 0.f;
         asm volatile("bar.sync 1, 256;" ::: "memory");
@@ -177,6 +204,35 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       if (__any_sync(kFull, !ok)) break;
       tmem_fence_after_sync();
       const uint32_t d = tmem + buf * a.columns + ((uint32_t)(quarter * 32) << 16);
+      if (!SPLIT && a.boxes) {
+        // The warps of a half turn kBoxTokens columns into rows of 128 channels in shared memory, which one thread sends off as a
+        // box while the next ones are made.
+        constexpr int kBoxTokens = box_tokens<T>();
+        for (int c = half * kBoxTokens; c < a.tokens; c += 2 * kBoxTokens) {
+          const uint32_t box = stage0 + a.stages * stage_bytes + (half * 2 + box_buf) * (kMmStaging / 4);
+          if ((threadIdx.x & 127) == 0) tile_store_read<1>();                       // the buffer's last box has been read
+          asm volatile("bar.sync %0, 128;" :: "r"(2 + half) : "memory");
+#pragma unroll
+          for (int k = 0; k < kBoxTokens; k += 16) {
+            uint32_t r[16];
+            tmem_load16(d + c + k, r);
+            tmem_load_wait();
+#pragma unroll
+            for (int i = 0; i < 16; i += 4) {
+              const float4 q = *reinterpret_cast<const float4*>(&s.scale[buf][c + k + i]);
+              const float sc[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                store_shared(box + ((k + i + j) * kMmChannels + quarter * 32 + lane) * sizeof(T),
+                             from_float<T>(fmaf((float)(int)r[i + j] * sc[j], w, b)));
+            }
+          }
+          tile_store_fence();
+          asm volatile("bar.sync %0, 128;" :: "r"(2 + half) : "memory");
+          if ((threadIdx.x & 127) == 0) tile_store(&outputs, (int)(n - lane), (int)(t0 + c), box);
+          box_buf ^= 1;
+        }
+      } else
       for (int c = half * 16; c < a.tokens; c += 32) {
         uint32_t r[16];
         tmem_load16(d + c, r);
@@ -199,11 +255,15 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       if constexpr (!SPLIT) {
         tmem_fence_before_sync();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_addr(&s.sum_empty[buf]));
+        if (lane == 0) {
+          if constexpr (PAIR) peer_arrive(peer_addr(smem_addr(&s.sum_empty[buf]), 0));
+          else mbar_arrive(smem_addr(&s.sum_empty[buf]));
+        }
         if (++buf == 2) buf = 0, buf_phase ^= 1;
       }
     }
   }
+  if (!SPLIT && a.boxes && warp < 8 && (threadIdx.x & 127) == 0) tile_store_done();
   if constexpr (SPLIT) {
     __syncwarp();
     cluster_sync();
@@ -244,7 +304,8 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   }
   tmem_fence_before_sync();
   __syncthreads();
-  if (warp == 9) tmem_free(tmem, columns);
+  if constexpr (PAIR) cluster_sync();                           // neither block's memory or barriers are used by the other any more
+  if (warp == 9) tmem_free<PAIR>(tmem, columns);
 }
 
 // ------------------------------------------------------------------ host
@@ -276,6 +337,18 @@ bool map_rows(CUtensorMap* m, const void* p, int64_t K, int64_t rows, int64_t ld
                 CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Outputs [T, N] in boxes of 128 channels by the tokens of a box.
+bool map_outputs(CUtensorMap* m, void* p, int64_t N, int64_t T, int dtype, int box) {
+  const int size = dtype_size(dtype);
+  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T}, strides[1] = {(cuuint64_t)(N * size)};
+  const cuuint32_t boxes[2] = {(cuuint32_t)kMmChannels, (cuuint32_t)box}, ones[2] = {1, 1};
+  const CUtensorMapDataType type = dtype == ACTNN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dtype == ACTNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  const EncodeTiled f = encode_tiled();
+  return f && f(m, type, 2, p, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 void plan(MmArgs& a) {
   const int sms = device_info().sm_count;
   const int64_t token_tiles = (a.T + 255) / 256;
@@ -291,14 +364,25 @@ void plan(MmArgs& a) {
 #ifdef MM_TUNE
   if (getenv("MM_SPLITS")) a.splits = atoi(getenv("MM_SPLITS"));
 #endif
+  // Pairs read half as much of the tokens' operand, which is what 256 columns want more of than the L2 gives (96 bytes a clock and SM);
+  // where there are tiles enough for them.
+  const int pairs = (int)((a.N + 2 * kMmChannels - 1) / (2 * kMmChannels)) * (int)((a.T + 255) / 256);
+  a.pair = a.splits == 1 && a.T > 128 && (pairs + sms / 2 - 1) / (sms / 2) <= (a.tiles + sms - 1) / sms;
+#ifdef MM_TUNE
+  if (getenv("MM_PAIR")) a.pair = atoi(getenv("MM_PAIR"));
+#endif
+  a.boxes = a.boxes && a.splits == 1;
+  if (a.pair || a.boxes) a.tokens = (a.tokens + 31) / 32 * 32;
+  if (a.pair) a.channel_tiles = (int)((a.N + 2 * kMmChannels - 1) / (2 * kMmChannels));
+  a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
   a.columns = 32;
   while (a.columns < a.tokens) a.columns *= 2;
-  a.stages = (kMmSmem - 1024) / ((kMmChannels + a.tokens) * kMmStageK);
+  a.stages = (kMmSmem - 1024 - (a.boxes ? kMmStaging : 0)) / ((kMmChannels + (a.pair ? a.tokens / 2 : a.tokens)) * kMmStageK);
   if (a.stages > kMmStagesMost) a.stages = kMmStagesMost;
 }
 
-template <typename T, bool SPLIT> int launch(const CUtensorMap& w, const CUtensorMap& x, const MmArgs& a, cudaStream_t stream) {
-  auto* kernel = int8_matmul_kernel<T, SPLIT>;
+template <typename T, bool SPLIT, bool PAIR> int launch(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& y, const MmArgs& a, cudaStream_t stream) {
+  auto* kernel = int8_matmul_kernel<T, SPLIT, PAIR>;
   static std::atomic<uint64_t> raised{0};                       // devices whose limit of dynamic shared memory is raised
   int dev = 0;
   cudaGetDevice(&dev);
@@ -309,27 +393,27 @@ template <typename T, bool SPLIT> int launch(const CUtensorMap& w, const CUtenso
   }
   const int sms = device_info().sm_count;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(SPLIT ? a.tiles * a.splits : a.tiles < sms ? a.tiles : sms);
+  cfg.gridDim = dim3(SPLIT ? a.tiles * a.splits : PAIR ? 2 * (a.tiles < sms / 2 ? a.tiles : sms / 2) : a.tiles < sms ? a.tiles : sms);
   cfg.blockDim = dim3(kMmThreads);
   cfg.dynamicSmemBytes = kMmSmem;
   cfg.stream = stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = SPLIT ? a.splits : 1;
+  at[0].val.clusterDim.x = SPLIT ? a.splits : PAIR ? 2 : 1;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = a.early ? 2 : 1;
   unsigned* gave_up = bulk_wait_counter();
-  if (cudaLaunchKernelEx(&cfg, kernel, w, x, a, gave_up) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, w, x, y, a, gave_up) != cudaSuccess) {
     cudaGetLastError();
     return ACTNN_ERR_LAUNCH;
   }
   return check_launch();
 }
-template <typename T> int launch_typed(const CUtensorMap& w, const CUtensorMap& x, const MmArgs& a, cudaStream_t stream) {
-  return a.splits > 1 ? launch<T, true>(w, x, a, stream) : launch<T, false>(w, x, a, stream);
+template <typename T> int launch_typed(const CUtensorMap& w, const CUtensorMap& x, const CUtensorMap& y, const MmArgs& a, cudaStream_t stream) {
+  return a.pair ? launch<T, false, true>(w, x, y, a, stream) : a.splits > 1 ? launch<T, true, false>(w, x, y, a, stream) : launch<T, false, false>(w, x, y, a, stream);
 }
 
 }  // namespace
@@ -353,14 +437,16 @@ int actnn::int8_matmul_impl(const int8_t* tokens, const float* token_scale, cons
   a.T = T; a.N = N; a.K = (int)K;
   a.vectors = N % 4 == 0 && aligned(out, 4 * size < 16 ? 4 * size : 16);
   a.early = early;
+  a.boxes = N * size % 16 == 0 && aligned(out, 16);
   if ((N + kMmChannels - 1) / kMmChannels * ((T + 15) / 16) > 0x7fffffff) return ACTNN_ERR_SHAPE;
   plan(a);
-  CUtensorMap w, x;
-  if (!map_rows(&w, weights, K, N, ld_weights, kMmChannels) || !map_rows(&x, tokens, K, T, ld_tokens, a.tokens)) return ACTNN_ERR_LAUNCH;
+  CUtensorMap w, x, y{};
+  if (a.boxes && !map_outputs(&y, out, N, T, dtype, kMmStaging / 4 / (kMmChannels * size))) return ACTNN_ERR_LAUNCH;
+  if (!map_rows(&w, weights, K, N, ld_weights, kMmChannels) || !map_rows(&x, tokens, K, T, ld_tokens, a.pair ? a.tokens / 2 : a.tokens)) return ACTNN_ERR_LAUNCH;
   switch (dtype) {
-    case ACTNN_F32: return launch_typed<float>(w, x, a, (cudaStream_t)stream);
-    case ACTNN_F16: return launch_typed<__half>(w, x, a, (cudaStream_t)stream);
-    default: return launch_typed<__nv_bfloat16>(w, x, a, (cudaStream_t)stream);
+    case ACTNN_F32: return launch_typed<float>(w, x, y, a, (cudaStream_t)stream);
+    case ACTNN_F16: return launch_typed<__half>(w, x, y, a, (cudaStream_t)stream);
+    default: return launch_typed<__nv_bfloat16>(w, x, y, a, (cudaStream_t)stream);
   }
 }
 
