@@ -349,32 +349,45 @@ bool map_outputs(CUtensorMap* m, void* p, int64_t N, int64_t T, int dtype, int b
                 CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// The cut: tokens of a tile, blocks that share a reduction, pairs or single blocks, by what they are expected to take (us): a
+// stage's bytes at what an SM gets from the L2 or its matrix instructions, the epilogue, and what a wave spends besides.  The
+// constants are fitted to times of all cuts for 16 to 16384 tokens, 500 to 16384 channels and reductions over 1000 to 8192, e.g.
+// 200 x 4096 x 4096: 208 tokens shared by four 12.4, by two 15.5, 64 tokens alone 14.2; 512 x 4096 x 4096: 128 tokens alone 15.1,
+// 256 shared by two 17.2; pairs or single blocks, 16384 x 4096 x 8192 360 / 390, 16384 x 1024 x 1024 23.0 / 21.5.
 void plan(MmArgs& a) {
+  constexpr double kBytes = 100e3, kColumns = 950.;            // a microsecond: bytes of an SM, columns of a stage
   const int sms = device_info().sm_count;
-  const int64_t token_tiles = (a.T + 255) / 256;
-  a.tokens = (int)(((a.T + token_tiles - 1) / token_tiles + 15) / 16 * 16);
-  a.channel_tiles = (int)((a.N + kMmChannels - 1) / kMmChannels);
-  a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
+  const int64_t least = (a.T + 255) / 256;
+  const bool boxes = a.boxes;
   a.k_blocks = (a.K + kMmStageK - 1) / kMmStageK;
-#ifdef MM_TUNE
-  if (getenv("MM_TOKENS")) a.tokens = atoi(getenv("MM_TOKENS")), a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
-#endif
-  a.splits = 1;
-  while (a.splits < 8 && (int64_t)a.tiles * a.splits * 2 <= sms && a.k_blocks >= a.splits * 2 * 2) a.splits *= 2;
-#ifdef MM_TUNE
-  if (getenv("MM_SPLITS")) a.splits = atoi(getenv("MM_SPLITS"));
-#endif
-  // Pairs read half as much of the tokens' operand, which is what 256 columns want more of than the L2 gives (96 bytes a clock and SM);
-  // where there are tiles enough for them.
-  const int pairs = (int)((a.N + 2 * kMmChannels - 1) / (2 * kMmChannels)) * (int)((a.T + 255) / 256);
-  a.pair = a.splits == 1 && a.T > 128 && (pairs + sms / 2 - 1) / (sms / 2) <= (a.tiles + sms - 1) / sms;
-#ifdef MM_TUNE
-  if (getenv("MM_PAIR")) a.pair = atoi(getenv("MM_PAIR"));
-#endif
-  a.boxes = a.boxes && a.splits == 1;
-  if (a.pair || a.boxes) a.tokens = (a.tokens + 31) / 32 * 32;
-  if (a.pair) a.channel_tiles = (int)((a.N + 2 * kMmChannels - 1) / (2 * kMmChannels));
-  a.tiles = (int)(a.channel_tiles * ((a.T + a.tokens - 1) / a.tokens));
+  double best = -1.;
+  auto offer = [&](int tokens, int splits, bool pair) {
+    const int step = boxes || pair ? 32 : 16;
+    tokens = splits > 1 ? (tokens + 15) / 16 * 16 : (tokens + step - 1) / step * step;
+    if (tokens > 256) return;
+    const int channels = pair ? 2 * kMmChannels : kMmChannels;
+    const int64_t channel_tiles = (a.N + channels - 1) / channels, tiles = channel_tiles * ((a.T + tokens - 1) / tokens);
+    const int64_t blocks = tiles * splits * (pair ? 2 : 1), waves = (blocks + sms - 1) / sms;
+    if (splits > 1 && blocks > sms) return;
+    const double load = (kMmChannels + (pair ? tokens / 2 : tokens)) * kMmStageK / kBytes, multiply = tokens / kColumns;
+    const double stages = (a.k_blocks + splits - 1) / splits * (load > multiply ? load : multiply);
+    const double time = (double)waves * (stages + (splits > 1 ? 1.7 + tokens * 0.0075 : tokens * 0.006) + (pair ? 2. : 0.5));
+    if (best >= 0. && time >= best) return;
+    best = time;
+    a.tokens = tokens;
+    a.splits = splits;
+    a.pair = pair;
+    a.channel_tiles = (int)channel_tiles;
+    a.tiles = (int)tiles;
+  };
+  for (const int64_t more : {1, 2, 3, 4, 6, 8}) {
+    const int tokens = (int)((a.T + least * more - 1) / (least * more));
+    if (more > 1 && tokens < 16) break;
+    for (int splits = 1; splits <= kMmSplitsMost && a.k_blocks >= 2 * splits; splits *= 2) offer(tokens, splits, false);
+    if (a.k_blocks < 2) offer(tokens, 1, false);
+    if (tokens > 64) offer(tokens, 1, true);
+  }
+  a.boxes = boxes && a.splits == 1;
   a.columns = 32;
   while (a.columns < a.tokens) a.columns *= 2;
   a.stages = (kMmSmem - 1024 - (a.boxes ? kMmStaging : 0)) / ((kMmChannels + (a.pair ? a.tokens / 2 : a.tokens)) * kMmStageK);

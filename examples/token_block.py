@@ -34,11 +34,12 @@ class TokenBlock(nn.Module):
 
 def kept_bytes(model, x):
     """Bytes of activations that the forward pass leaves for the backward pass."""
-    torch.cuda.synchronize()
-    before = torch.cuda.memory_allocated()
+    def held():
+        return torch.cuda.memory_stats()["requested_bytes.all.current"]      # without what the allocator adds to a block
+
+    before = held()
     y = model(x)
-    torch.cuda.synchronize()
-    return torch.cuda.memory_allocated() - before - y.numel() * y.element_size()
+    return held() - before - y.numel() * y.element_size()
 
 
 def train(steps=50, level="L3", device="cuda", dtype=torch.bfloat16, seed=0):
