@@ -50,7 +50,7 @@ bool hold_positions(GnShape& g, int64_t N, int size, int kept) {
   return false;
 #endif
   const int V = g.V;
-  if (V < 2 || V * size < 4 || (kept > 0 && V * kept < 4)) return false;
+  if (V < 2 || V * size < 4 || (kept > 0 && V * kept < 4)) return false;   // what the asynchronous copy does not know
   const int64_t sms = device_info().sm_count, whole = (int64_t)g.cpg / gcd(g.cpg, V) * V;
   for (const int segment : {kGnSegment, kGnSegment / 2}) {
     GnShape h = g;

@@ -219,9 +219,11 @@ template <int BYTES> ACTNN_DEV void from_shared(uint32_t src, uint32_t* w) {
 }
 
 // The positions of a thread, in places of its own: `places` of them for every thread of the block from `shared` on.
-template <typename T, int V, typename K> struct Positions {
+// SUMS: for a pass that writes nothing of a position's size.
+template <typename T, int V, typename K, bool SUMS> struct Positions {
   static constexpr int A = V * sizeof(T), B = K::kBytes;
-  static constexpr bool kAsync = V > 1 && A >= 4 && (B == 0 || B >= 4);        // the asynchronous copy knows 4, 8 and 16 bytes
+  static constexpr bool kAsync = V > 1 && A >= (SUMS ? 8 : 4) && (B == 0 || B >= 4);        // the asynchronous copy knows 4, 8 and 16 bytes
+  static constexpr int kAhead = SUMS ? 8 : 4;
   static constexpr int kDepth = B == 0 ? 8 : 6;                                // positions of a ring
   static constexpr int kPlace = kAsync ? kGnThreads * (A + B) : 0;             // bytes of a position of all threads
   using Words = typename K::Words;
@@ -284,10 +286,21 @@ template <typename T, int V, typename K> struct Positions {
         }
       }
     } else {
-#pragma unroll 4
-      for (int i = 0; i < count; ++i) {
-        const Words k = K::load(b + i * step_b);
-        take(load_vec<T, V>((const T*)(a + i * step_a)), k);
+      int i = 0;
+      for (; i + kAhead <= count; i += kAhead) {          // kAhead requests before the first is used
+        Vec<T, V> w[kAhead];
+        Words k[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j, a += step_a, b += step_b) {
+          w[j] = load_vec<T, V>((const T*)a);
+          k[j] = K::load(b);
+        }
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) take(w[j], k[j]);
+      }
+      for (; i < count; ++i, a += step_a, b += step_b) {
+        const Words k = K::load(b);
+        take(load_vec<T, V>((const T*)a), k);
       }
     }
   }
@@ -575,8 +588,8 @@ template <typename T, int V, bool ONE, int KIND, bool SAVE> struct Apply {
 };
 // The second half of the forward pass: group_s holds mean, rstd, mid and half range of the tile's groups; HELD: the positions
 // are in shared memory.
-template <typename T, int V, bool ONE, bool SAVE, bool HELD>
-ACTNN_DEV void apply_all(Positions<T, V, Alone<T, V>>& pos, const float4* group_s, const Place& p, const GnShape& g, const float* gamma,
+template <typename T, int V, bool ONE, bool SAVE, bool HELD, bool SUMS>
+ACTNN_DEV void apply_all(Positions<T, V, Alone<T, V>, SUMS>& pos, const float4* group_s, const Place& p, const GnShape& g, const float* gamma,
                          const float* beta, T* y, int8_t* codes, int kind) {
   Row<V> a, b;
   GroupRow<V, ONE> mid, inv;
@@ -619,7 +632,7 @@ gn_stats_kernel(const T* __restrict__ x, Part* __restrict__ out, const GnShape g
   using Stats = ThreadStats<T, V, ONE>;
   extern __shared__ float4 dynamic_s[];                   // scratch, ring
   const Place p = place_of<V>(g);
-  Positions<T, V, Alone<T, V>> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_scratch(g, true), Positions<T, V, Alone<T, V>>::kDepth);
+  Positions<T, V, Alone<T, V>, true> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_scratch(g, true), Positions<T, V, Alone<T, V>, true>::kDepth);
   pos.start();
   float4* cells = dynamic_s + threadIdx.x * Stats::M;
   if (p.count > 0) {
@@ -644,7 +657,7 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
                   int kind, const GnShape g) {
   extern __shared__ float4 dynamic_s[];                   // tables, ring
   const Place p = place_of<V, true>(g);
-  Positions<T, V, Alone<T, V>> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Alone<T, V>>::kDepth);
+  Positions<T, V, Alone<T, V>, false> pos(x, nullptr, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Alone<T, V>, false>::kDepth);
   pos.start();
   const int g0 = p.g0, groups = g.parts == 1 ? (int)fast_div(p.width, g.by_cpg) : 1, count = g.first_chunks * g.first_parts;
   const int L = lanes_for(count, groups), per = blockDim.x / L, member = threadIdx.x & (L - 1);
@@ -659,7 +672,7 @@ gn_forward_kernel(const T* __restrict__ x, const Part* __restrict__ parts, const
     }
   }
   __syncthreads();
-  if (p.count > 0) apply_all<T, V, ONE, SAVE, false>(pos, dynamic_s, p, g, gamma, beta, y, codes, kind);
+  if (p.count > 0) apply_all<T, V, ONE, SAVE, false, false>(pos, dynamic_s, p, g, gamma, beta, y, codes, kind);
 }
 // One launch, a cluster of `chunks` blocks for each sample and run of channels (whole groups).
 template <typename T, int V, bool ONE, bool SAVE>
@@ -671,7 +684,7 @@ gn_forward_held_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
   const int table = gn_groups(g);
   float4 *own_s = dynamic_s, *group_s = dynamic_s + table, *cell_s = group_s + table;
   const Place p = place_of<V>(g);
-  Positions<T, V, Alone<T, V>> pos(x, nullptr, p, smem_addr(cell_s) + gn_scratch(g, true), g.held);
+  Positions<T, V, Alone<T, V>, false> pos(x, nullptr, p, smem_addr(cell_s) + gn_scratch(g, true), g.held);
   pos.start_all();
   float4* cells = cell_s + threadIdx.x * Stats::M;
   if (p.count > 0) {
@@ -700,7 +713,7 @@ gn_forward_held_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
   }
   cluster_arrive();                                       // what was read of the others' tables is read
   __syncthreads();
-  if (p.count > 0) apply_all<T, V, ONE, SAVE, true>(pos, group_s, p, g, gamma, beta, y, codes, kind);
+  if (p.count > 0) apply_all<T, V, ONE, SAVE, true, false>(pos, group_s, p, g, gamma, beta, y, codes, kind);
   cluster_wait();
 }
 
@@ -784,8 +797,8 @@ template <typename T, int V, bool ONE, int KIND, bool CODES> struct Grad {
 
 // The first half: the sums of the block's positions for each channel, over its threads in order: give(channel of the tile, sums of
 // dz and of dz * h).  sum_s: a place for each thread and channel.
-template <typename T, int V, bool ONE, bool CODES, bool HELD, typename Give>
-ACTNN_DEV void sums_all(Positions<T, V, Kept<T, V, CODES>>& pos, const Line<T, V, ONE, CODES>& l, float2* sum_s, const Place& p,
+template <typename T, int V, bool ONE, bool CODES, bool HELD, bool SUMS, typename Give>
+ACTNN_DEV void sums_all(Positions<T, V, Kept<T, V, CODES>, SUMS>& pos, const Line<T, V, ONE, CODES>& l, float2* sum_s, const Place& p,
                         const GnShape& g, const float* stats, int kind, Give give) {
   if (p.r < p.R) {
     Row<V> s1, s2;
@@ -820,8 +833,8 @@ ACTNN_DEV void sums_all(Positions<T, V, Kept<T, V, CODES>>& pos, const Line<T, V
   }
 }
 // The second half: mean_s holds the means over the tile's groups of dz * gamma and of dz * gamma * h.
-template <typename T, int V, bool ONE, bool CODES, bool HELD>
-ACTNN_DEV void grad_all(Positions<T, V, Kept<T, V, CODES>>& pos, const Line<T, V, ONE, CODES>& l, const float4* mean_s, const Place& p,
+template <typename T, int V, bool ONE, bool CODES, bool HELD, bool SUMS>
+ACTNN_DEV void grad_all(Positions<T, V, Kept<T, V, CODES>, SUMS>& pos, const Line<T, V, ONE, CODES>& l, const float4* mean_s, const Place& p,
                         const GnShape& g, const float* stats, const float* gamma, T* dx, int kind) {
   Row<V> k1;
   GroupRow<V, ONE> k2, k3;
@@ -882,12 +895,12 @@ gn_backward_sums_kernel(const T* __restrict__ dy, const void* __restrict__ kept,
                         const GnShape g) {
   extern __shared__ float4 dynamic_s[];                   // scratch, ring
   const Place p = place_of<V>(g);
-  Positions<T, V, Kept<T, V, CODES>> pos(dy, kept, p, smem_addr(dynamic_s) + gn_scratch(g, false), Positions<T, V, Kept<T, V, CODES>>::kDepth);
+  Positions<T, V, Kept<T, V, CODES>, true> pos(dy, kept, p, smem_addr(dynamic_s) + gn_scratch(g, false), Positions<T, V, Kept<T, V, CODES>, true>::kDepth);
   pos.start();
   float2* out = sums + (p.n * g.chunks + p.chunk) * g.C + p.c0;
   Line<T, V, ONE, CODES> l;
   if (p.r < p.R) l.start(p, g, stats, gamma, beta);
-  sums_all<T, V, ONE, CODES, false>(pos, l, reinterpret_cast<float2*>(dynamic_s), p, g, stats, kind,
+  sums_all<T, V, ONE, CODES, false, true>(pos, l, reinterpret_cast<float2*>(dynamic_s), p, g, stats, kind,
                                     [&](int c, float2 s) { out[c] = s; });
 }
 // The second.
@@ -898,14 +911,14 @@ gn_backward_kernel(const T* __restrict__ dy, const void* __restrict__ kept, cons
                    T* __restrict__ dx, int kind, const GnShape g) {
   extern __shared__ float4 dynamic_s[];                   // tables, ring
   const Place p = place_of<V, true>(g);
-  Positions<T, V, Kept<T, V, CODES>> pos(dy, kept, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Kept<T, V, CODES>>::kDepth);
+  Positions<T, V, Kept<T, V, CODES>, false> pos(dy, kept, p, smem_addr(dynamic_s) + gn_tables(g), Positions<T, V, Kept<T, V, CODES>, false>::kDepth);
   pos.start();
   group_means(dynamic_s, p, g, gamma, g.first_chunks, [&](int k, int c) { return sums[(p.n * g.first_chunks + k) * g.C + c]; });
   __syncthreads();
   if (p.count == 0) return;
   Line<T, V, ONE, CODES> l;
   l.start(p, g, stats, gamma, beta);
-  grad_all<T, V, ONE, CODES, false>(pos, l, dynamic_s, p, g, stats, gamma, dx, kind);
+  grad_all<T, V, ONE, CODES, false, false>(pos, l, dynamic_s, p, g, stats, gamma, dx, kind);
 }
 // One launch, a cluster of `chunks` blocks for each sample and run of channels (whole groups); the sums of each block are written
 // for the gradients of the parameters.
@@ -919,12 +932,12 @@ gn_backward_held_kernel(const T* __restrict__ dy, const void* __restrict__ kept,
   float4 *own_s = dynamic_s, *mean_s = dynamic_s + table;
   float2* sum_s = reinterpret_cast<float2*>(mean_s + table);
   const Place p = place_of<V>(g);
-  Positions<T, V, Kept<T, V, CODES>> pos(dy, kept, p, smem_addr(sum_s) + gn_scratch(g, false), g.held);
+  Positions<T, V, Kept<T, V, CODES>, false> pos(dy, kept, p, smem_addr(sum_s) + gn_scratch(g, false), g.held);
   pos.start_all();
   float2* out = sums + (p.n * g.chunks + p.chunk) * g.C + p.c0;
   Line<T, V, ONE, CODES> l;
   if (p.r < p.R) l.start(p, g, stats, gamma, beta);
-  sums_all<T, V, ONE, CODES, true>(pos, l, sum_s, p, g, stats, kind, [&](int c, float2 s) {
+  sums_all<T, V, ONE, CODES, true, false>(pos, l, sum_s, p, g, stats, kind, [&](int c, float2 s) {
     out[c] = s;
     sum_s[c] = s;                                         // its own column alone was read for it
   });
@@ -943,7 +956,7 @@ gn_backward_held_kernel(const T* __restrict__ dy, const void* __restrict__ kept,
   }
   cluster_arrive();
   __syncthreads();
-  if (p.count > 0) grad_all<T, V, ONE, CODES, true>(pos, l, mean_s, p, g, stats, gamma, dx, kind);
+  if (p.count > 0) grad_all<T, V, ONE, CODES, true, false>(pos, l, mean_s, p, g, stats, gamma, dx, kind);
   cluster_wait();
 }
 
@@ -1047,7 +1060,8 @@ template <auto KERNEL> void gn_cut_for(GnShape& g, int64_t N, int smem, int extr
 }
 
 template <typename T, int V, bool ONE, bool SAVE> bool gn_forward(const GnCall& c, const GnShape& g) {
-  using Pos = Positions<T, V, Alone<T, V>>;
+  using Pos = Positions<T, V, Alone<T, V>, false>;
+  using Pos1 = Positions<T, V, Alone<T, V>, true>;
   const T* x = (const T*)c.x;
   Part* parts = (Part*)c.workspace;
   if constexpr (Pos::kAsync) {
@@ -1056,7 +1070,7 @@ template <typename T, int V, bool ONE, bool SAVE> bool gn_forward(const GnCall& 
                                                                (T*)c.out, c.codes, c.stats, c.kind, g);
   }
   GnShape first = g, second = g;
-  const int smem1 = gn_scratch(g, true) + Pos::kDepth * Pos::kPlace, smem2 = gn_tables(g) + Pos::kDepth * Pos::kPlace;
+  const int smem1 = gn_scratch(g, true) + Pos1::kDepth * Pos1::kPlace, smem2 = gn_tables(g) + Pos::kDepth * Pos::kPlace;
   gn_cut_for<gn_stats_kernel<T, V, ONE>>(first, c.N, smem1, kExtraStats);
   gn_cut_for<gn_forward_kernel<T, V, ONE, SAVE>>(second, c.N, smem2, kExtraSecond);
   second.first_chunks = first.first_chunks = first.chunks;
@@ -1076,7 +1090,8 @@ template <typename T, int V, bool ONE, bool SAVE> bool gn_forward(const GnCall& 
                                                       c.kind, second);
 }
 template <typename T, int V, bool ONE, bool CODES> bool gn_backward(const GnCall& c, const GnShape& g) {
-  using Pos = Positions<T, V, Kept<T, V, CODES>>;
+  using Pos = Positions<T, V, Kept<T, V, CODES>, false>;
+  using Pos1 = Positions<T, V, Kept<T, V, CODES>, true>;
   const T* dy = (const T*)c.dy;
   const void* kept = CODES ? (const void*)c.codes : c.x;
   const float* stats = c.stats;
@@ -1090,7 +1105,7 @@ template <typename T, int V, bool ONE, bool CODES> bool gn_backward(const GnCall
     else
       ok = false;
   } else {
-    const int smem1 = gn_scratch(g, false) + Pos::kDepth * Pos::kPlace, smem2 = gn_tables(g) + Pos::kDepth * Pos::kPlace;
+    const int smem1 = gn_scratch(g, false) + Pos1::kDepth * Pos1::kPlace, smem2 = gn_tables(g) + Pos::kDepth * Pos::kPlace;
     gn_cut_for<gn_backward_sums_kernel<T, V, ONE, CODES>>(first, c.N, smem1, kExtraSums);
     gn_cut_for<gn_backward_kernel<T, V, ONE, CODES>>(second, c.N, smem2, kExtraSecond);
     second.first_chunks = first.chunks;
