@@ -1024,16 +1024,19 @@ inline int gn_threads(const GnShape& g) {
   const int vecs = g.tile / g.V, R = kGnThreads / vecs;
   return (vecs * R + 31) / 32 * 32;
 }
-// KERNEL's limit of dynamic shared memory is raised to what any call may ask for, once on a device.
-template <auto KERNEL, typename... Args> bool gn_start(const GnCall& c, const GnShape& g, int smem, Args... args) {
+// KERNEL's limit of dynamic shared memory, raised to what any call may ask for, once on a device.
+template <auto KERNEL> bool gn_raise() {
   static std::atomic<uint64_t> raised{0};
   int dev = 0;
   cudaGetDevice(&dev);
   const uint64_t bit = (uint64_t)1 << (dev & 63);
-  if (!(raised.load(std::memory_order_acquire) & bit)) {
-    if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kGnMostSmem) != cudaSuccess) return false;
-    raised.fetch_or(bit, std::memory_order_release);
-  }
+  if (raised.load(std::memory_order_acquire) & bit) return true;
+  if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kGnMostSmem) != cudaSuccess) return false;
+  raised.fetch_or(bit, std::memory_order_release);
+  return true;
+}
+template <auto KERNEL, typename... Args> bool gn_start(const GnCall& c, const GnShape& g, int smem, Args... args) {
+  if (!gn_raise<KERNEL>()) return false;
   if (c.N * g.chunks * g.tiles > 0x7fffffff) return false;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(c.N * g.chunks * g.tiles));
@@ -1053,7 +1056,7 @@ template <auto KERNEL> void gn_cut_for(GnShape& g, int64_t N, int smem, int extr
   static std::atomic<int> resident{0};
   int n = resident.load(std::memory_order_acquire);
   if (n == 0) {
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kGnThreads, smem) != cudaSuccess || n < 1) n = 1;
+    if (!gn_raise<KERNEL>() || cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kGnThreads, smem) != cudaSuccess || n < 1) n = 1;
     resident.store(n, std::memory_order_release);
   }
   gn_cut_positions(g, N, (int64_t)device_info().sm_count * n, extra);
