@@ -68,8 +68,11 @@ bool hold_positions(GnShape& g, int64_t N, int size, int kept) {
       const int64_t smem = gn_tables(h) + gn_scratch(h, kept == 0) + held * place;
       const int64_t resident = sms * std::min<int64_t>(size == 2 ? 3 : 2, (227 * 1024) / (smem + 1024));
       if (smem > kGnMostSmem || N * h.tiles * k > resident) continue;
-      // more blocks while SMs are without one and a thread keeps kGnFew positions
-      if (k < kGnCluster && N * h.tiles * k < sms && g.S / (2 * k) >= (int64_t)R * kGnFew) continue;
+      // more blocks while SMs are without one and a thread keeps kGnFew positions, while half of them are and it keeps one
+      // (forward / backward, float16: 1 x 64 x 14 x 14 by one block 7.0 / 9.4 us, by four 6.4 / 7.9; 32 x 256 x 14 x 14 by 128 blocks
+      // 7.7 / 10.2, by 256 9.2 / 11.4)
+      const int64_t blocks = N * h.tiles * k, halved = g.S / (2 * k);
+      if (k < kGnCluster && ((blocks < sms && halved >= (int64_t)R * kGnFew) || (2 * blocks < sms && halved >= R))) continue;
       h.chunks = k;
       h.held = (int)held;
       g = h;

@@ -697,7 +697,8 @@ gn_forward_held_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
   }
   __syncthreads();
   join_block<V, Stats::M>(cell_s, p, g, [&](int j, const Part& q) { own_s[j] = make_float4(q.mean, q.m2, q.lo, q.hi); });
-  cluster_sync();
+  if (g.chunks > 1) cluster_sync();
+  else __syncthreads();
   const int g0 = p.g0, groups = (int)fast_div(p.width, g.by_cpg), L = lanes_for(g.chunks, groups), per = blockDim.x / L, member = threadIdx.x & (L - 1);
   for (int j0 = 0; j0 < groups; j0 += per) {
     const int j = j0 + threadIdx.x / L;
@@ -711,10 +712,10 @@ gn_forward_held_kernel(const T* __restrict__ x, const float* __restrict__ gamma,
       keep_stats(stats, p, g, g0 + j, st);
     }
   }
-  cluster_arrive();                                       // what was read of the others' tables is read
+  if (g.chunks > 1) cluster_arrive();                     // what was read of the others' tables is read
   __syncthreads();
   if (p.count > 0) apply_all<T, V, ONE, SAVE, true, false>(pos, group_s, p, g, gamma, beta, y, codes, kind);
-  cluster_wait();
+  if (g.chunks > 1) cluster_wait();
 }
 
 // ------------------------------------------------------------------ backward
@@ -943,7 +944,8 @@ gn_backward_held_kernel(const T* __restrict__ dy, const void* __restrict__ kept,
   });
   __syncthreads();
   group_means(own_s, p, g, gamma, 1, [&](int, int c) { return sum_s[c - p.c0]; });
-  cluster_sync();
+  if (g.chunks > 1) cluster_sync();
+  else __syncthreads();
   const int groups = (int)fast_div(p.width, g.by_cpg);
   for (int j = threadIdx.x; j < groups; j += blockDim.x) {
     float4 m = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -954,10 +956,10 @@ gn_backward_held_kernel(const T* __restrict__ dy, const void* __restrict__ kept,
     }
     mean_s[j] = m;
   }
-  cluster_arrive();
+  if (g.chunks > 1) cluster_arrive();
   __syncthreads();
   if (p.count > 0) grad_all<T, V, ONE, CODES, true, false>(pos, l, mean_s, p, g, stats, gamma, dx, kind);
-  cluster_wait();
+  if (g.chunks > 1) cluster_wait();
 }
 
 // Many runs: partial results joined once, in a launch between the two, instead of by every block of the second.  A warp per group.
