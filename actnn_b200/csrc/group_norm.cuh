@@ -19,6 +19,11 @@
 // read it copies to places of its own in shared memory, so that neither registers nor barriers limit how many bytes are under
 // way.
 //
+// Measured on a B200, float16, 512 x 256 x 28 x 28 (103 M elements), two launches each way: statistics 45 us, output and codes 79, sums 73,
+// gradient 80; their bytes take 31, 79, 47 and 79 at the copy rate.  The sums wait for nothing but instructions: 14 an element, the
+// unit of exponentials and reciprocals 60 - 70 % busy.  Batches of samples small enough for the L2 between the two launches were
+// slower (fills and drains of the GPU), so was one launch in several waves; one reciprocal for a pair of elements changed nothing.
+//
 // The range, and with it the codes, follow from exact minima and maxima by single fp32 operations: reproducible to the bit.
 // The variance is joined from sums about a value of each thread's own (its first one), which loses nothing to cancellation
 // however far the mean is from zero: the sum of squares about one of n values exceeds the one about their mean n-fold at most.

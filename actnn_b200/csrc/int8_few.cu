@@ -6,6 +6,8 @@
 // 16 bytes of a row with the same place of each token by four-way integer dot products, and the 32 partial sums of a
 // (row, token) are one redux instruction.  More tokens are two launches: codes of the rows into the workspace, then the
 // product on the tensor cores.
+//
+// Measured on a B200: 1 x 2048 x 4096 4.0 us of which about 2 are the launch (1.3 for the weight's bytes), 1 x 8192 x 8192 14.2 (10.3).
 #include "activation.cuh"
 
 namespace actnn {

@@ -12,6 +12,14 @@
 // fills.  Where the tiles are too few for the SMs, the reduction is split over the blocks of a cluster, which add their
 // integer sums through distributed shared memory: order does not matter to them.
 //
+// Where the tiles fill the GPU, two blocks compute one of 256 channels together: each loads half of the channels' operand and half
+// of the tokens'.  Outputs are turned into rows of channels in shared memory and leave as boxes of 128 channels, because 32
+// lanes' 64 bytes each took longer than the multiplication (8192 x 2048 x 4096: 87 us with them, 65 with boxes).
+//
+// Measured on a B200, bfloat16 outputs: 16384 x 4096 x 8192 340 - 360 us, 3.1e15 operations a second (twice the measured bfloat16 rate
+// is 3.24e15; the tensor pipe is 82 % busy, the rest is the L2's, 12 TB/s); 8192 x 2048 x 4096 48 - 65; 200 x 4096 x 4096 12.2, where
+// the weight's bytes take 2.6 and the fixed latencies of launch, first copies, sums through the cluster and outputs about 8.
+//
 // Every wait is bounded.  A block whose wait runs out writes nothing more, is counted (the counter of the bulk waits), lets
 // its copies and instructions end and leaves.
 #include <atomic>

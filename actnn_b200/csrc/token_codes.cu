@@ -5,7 +5,8 @@
 // And the column sums that a bias's gradient is.
 //
 // A row is read once where the threads that share it can hold it in registers (up to 32 elements each), else twice, the
-// second time from the L2.  Bound by HBM: 2 + 1 bytes an element of a 16-bit type.
+// second time from the L2.  Bound by HBM: 2 + 1 bytes an element of a 16-bit type; 16384 x 4096 bfloat16 take 30.7 us, the copy
+// rate (one block a row, a quarter of its registers idle: 48), 8192 x 2048 8.6, rows that no vector fits 12.9.
 #include "activation.cuh"
 #include "cluster.cuh"
 
