@@ -121,7 +121,8 @@ def _check_product(x, weight_codes, bias, dtype):
 
 
 def linear(x, weight_codes, weight_scale, bias=None):
-    """A linear layer on a weight kept as codes: the tokens ``x`` ``[.., K]`` are coded row by row, the result has their type."""
+    """A linear layer on a weight kept as codes: the tokens ``x`` ``[.., K]`` are coded row by row, the result has their type.
+    No gradient passes through it: training goes through ``ops.int8_linear``."""
     nat = _lib.native()
     if nat:
         return nat.int8_linear(x, weight_codes, weight_scale, bias)
