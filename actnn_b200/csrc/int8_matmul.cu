@@ -166,6 +166,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       }
     }
   } else if (warp == 9) {                                       // ---------------- matrix instructions
+    if (a.early) grid_wait();                                   // the limit of a wait is for copies, not for the launch before
     if (lane == 0 && (!PAIR || rank == 0)) {
       const uint32_t instruction = int8_instruction(tile_channels, a.tokens);
       int stage = 0, buf = 0;
