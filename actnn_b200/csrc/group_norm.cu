@@ -46,9 +46,6 @@ int64_t most_runs(const GnShape& g, int64_t N) {
 // kept of the input (0 in the forward pass).
 constexpr int kGnSegment = 128, kGnCluster = 8;
 bool hold_positions(GnShape& g, int64_t N, int size, int kept) {
-#ifdef GN_NO_HOLD
-  return false;
-#endif
   const int V = g.V;
   if (V < 2 || V * size < 4 || (kept > 0 && V * kept < 4)) return false;   // what the asynchronous copy does not know
   const int64_t sms = device_info().sm_count, whole = (int64_t)g.cpg / gcd(g.cpg, V) * V;

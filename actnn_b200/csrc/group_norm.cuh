@@ -67,9 +67,9 @@ struct GnCall {
 // One partial result of the statistics.
 struct Part { float mean, m2, lo, hi; };
 
-// group_norm.cu, group_norm_f16.cu, group_norm_bf16.cu
-// Cuts the positions for a launch of which `resident` blocks fit the GPU at a time, and a block spends as long as `extra` positions of
-// a thread take before and after them.
+// group_norm.cu, group_norm_f16.cu, group_norm_bf16.cu: the launches of a type; and, in the first,
+// the cut of the positions for a launch of which `resident` blocks fit the GPU at a time, and a block spends as long as `extra`
+// positions of a thread take before and after them.
 void gn_cut_positions(GnShape& g, int64_t N, int64_t resident, int extra);
 int gn_run_f32(const GnCall& c, const GnShape& g, bool forward);
 int gn_run_f16(const GnCall& c, const GnShape& g, bool forward);
