@@ -18,7 +18,7 @@ constexpr int kFewWarps = kFewThreads / 32;
 constexpr int kFewTokens = 8;
 constexpr int kFewRows = 2;                             // rows of the weight a warp has under way
 constexpr int kFewAhead = 4;                            // pieces of 512 bytes of each that are requested at a time
-constexpr int kFewSmem = 48 * 1024;                     // codes of all tokens
+constexpr int kFewSmem = 48 * 1024 - 512;               // codes of all tokens: what needs no opt-in, less a piece for `most_s` beside them
 
 // 16 bytes of a row at `k`, zeros from K on; nothing behind K is read.
 ACTNN_DEV uint4 weight_piece(const int8_t* row, int k, int K) {

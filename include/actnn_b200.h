@@ -456,9 +456,9 @@ int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8
 
 /* ------------------------------------------------------------------------------------
  * A linear layer on a weight kept as codes: x [T, K] of `dtype`, rows `ld_x` elements apart, is coded as by
- * actnn_row_codes and multiplied as by actnn_int8_matmul, with the same result.  Up to eight tokens (whose codes
- * fit 48 KB) in one launch; otherwise `workspace`, 16-byte aligned, takes the codes:
- * actnn_int8_linear_workspace bytes (0: may be NULL).  The reference has no counterpart
+ * actnn_row_codes and multiplied as by actnn_int8_matmul, with the same result.  One launch for one token of up to
+ * 48640 values and for up to eight with K <= 4096 and T * K <= 16384; otherwise `workspace`, 16-byte aligned, takes
+ * the codes: actnn_int8_linear_workspace bytes (0: may be NULL).  The reference has no counterpart
  * (actnn/actnn/ops.py:408-428 computes in the activation's type). */
 int actnn_int8_linear_workspace(int64_t T, int64_t K, int64_t* bytes);
 int actnn_int8_linear(const void* x, const int8_t* weights, const float* channel_scale, const void* bias, void* out,
