@@ -21,7 +21,7 @@
 // the weight's bytes take 2.6 and the fixed latencies of launch, first copies, sums through the cluster and outputs about 8.
 //
 // Every wait is bounded.  A block whose wait runs out writes nothing more, is counted (the counter of the bulk waits), lets
-// its copies and instructions end and leaves.
+// its copies and instructions end and leaves.  The epilogue's warps leave together: its barriers count all of them.
 #include <atomic>
 
 #include "activation.cuh"
@@ -76,6 +76,15 @@ ACTNN_DEV bool mm_wait(uint32_t bar, uint32_t parity, MmShared& s, unsigned* gav
   *dead = 1;
   if (gave_up) atomicAdd(gave_up, 1u);
   return false;
+}
+
+// Of the epilogue's eight warps: whether the waits of all of them came to their end.  A warp that left alone, because another
+// wait had run out just before its own phase was complete, would leave those whose phase was to barriers it never comes to.
+ACTNN_DEV bool epilogue_agrees(bool ok) {
+  uint32_t all;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+               "barrier.cta.red.and.pred q, 1, 256, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(all) : "r"((uint32_t)ok) : "memory");
+  return all != 0;
 }
 
 // SPLIT: the reduction is split over a cluster.  PAIR: a cluster of two blocks computes a tile of 256 channels, half of the channels
@@ -205,12 +214,12 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * tile_channels + rank * kMmChannels * PAIR + quarter * 32 + lane;
       if constexpr (!SPLIT) {
         if ((int)threadIdx.x < a.tokens) s.scale[buf][threadIdx.x] = t0 + threadIdx.x < a.T ? __ldg(a.token_scale + t0 + threadIdx.x) : 0.f;
-        asm volatile("bar.sync 1, 256;" ::: "memory");
       }
       const float w = n < a.N ? __ldg(a.channel_scale + n) : 0.f;
       const float b = n < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
       const bool ok = mm_wait(smem_addr(&s.sum_full[buf]), buf_phase, s, lane == 0 ? gave_up : nullptr);
-      if (__any_sync(kFull, !ok)) break;
+      __syncwarp();
+      if (!epilogue_agrees(ok)) break;                          // and the scales are there for all
       tmem_fence_after_sync();
       const uint32_t d = tmem + buf * a.columns + ((uint32_t)(quarter * 32) << 16);
       if (!SPLIT && a.boxes) {

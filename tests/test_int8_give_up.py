@@ -1,0 +1,68 @@
+"""What the integer product does when one of its waits runs out, shown on the CPU: every order in which its warps can take their
+steps is followed, and none may end with some of them waiting for others that have left."""
+import os
+import re
+
+import pytest
+
+from conftest import ROOT
+
+SOURCE = os.path.join(ROOT, "actnn_b200", "csrc", "int8_matmul.cu")
+
+
+def ends(warps, tiles, together):
+    """All ends of an epilogue of `warps` warps over `tiles` tiles, each warp's last place.  A warp waits for its tile (the phase may
+    complete at any time, another wait of the block may run out at any time; a try looks at the phase first, then at the flag)
+    and passes a barrier that counts all warps.  `together`: the barrier also tells whether every wait was good, and all leave
+    where one was not; otherwise a warp whose wait was not good leaves by itself."""
+    start = (tuple(("try", 0) for _ in range(warps)), 0, False)         # places, tiles complete, flag
+    seen, todo, found = {start}, [start], set()
+    while todo:
+        places, complete, dead = todo.pop()
+        after = []
+        if complete < tiles:
+            after.append((places, complete + 1, dead))
+        if not dead:
+            after.append((places, complete, True))
+        for i, (what, tile) in enumerate(places):
+            def to(place):
+                return places[:i] + (place,) + places[i + 1:]
+            if what == "try":                               # the phase
+                after.append((to(("through", tile) if tile < complete else ("flag", tile)), complete, dead))
+            elif what == "flag":                            # then the flag
+                bad = ("bad", tile) if together else ("left", tile)
+                after.append((to(bad if dead else ("try", tile)), complete, dead))
+        at = [w for w, _ in places]
+        if all(w in ("through", "bad") for w in at):        # the barrier is complete
+            on = ("try", places[0][1] + 1) if places[0][1] + 1 < tiles else ("done", tiles)
+            after.append((tuple(("left", t) if "bad" in at else on for _, t in places), complete, dead))
+        moved = [s for s in after if s != (places, complete, dead)]
+        if not moved:
+            found.add(places)
+        for s in moved:
+            if s not in seen:
+                seen.add(s)
+                todo.append(s)
+    return found
+
+
+@pytest.mark.parametrize("warps,tiles", [(2, 1), (2, 3), (3, 2), (4, 2)])
+def test_the_epilogue_leaves_together(warps, tiles):
+    alone = ends(warps, tiles, False)
+    assert any({"left", "through"} <= {w for w, _ in e} for e in alone)         # what leaving one by one can end with
+    for e in ends(warps, tiles, True):
+        assert {w for w, _ in e} in ({"left"}, {"done"})
+
+
+def epilogue():
+    text = open(SOURCE).read()
+    return text[text.index("---------------- epilogue"):text.index("host")]
+
+
+def test_the_kernel_asks_all_warps_before_it_goes_on():
+    """Between the wait for a tile's sums and anything else of the tile stands the vote of all eight warps, and no warp leaves by
+    its own result."""
+    code = epilogue()
+    assert re.search(r"const bool ok = mm_wait\(smem_addr\(&s\.sum_full\[buf\]\)[^;]*;\s*(__syncwarp\(\);\s*)?if \(!epilogue_agrees\(ok\)\) break;", code)
+    assert len(re.findall(r"\bbreak;", code)) == 1 and "bar.sync 1" not in code
+    assert re.search(r"barrier\.cta\.red\.and\.pred q, 1, 256, p", open(SOURCE).read())
