@@ -161,6 +161,13 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
           if (++stage == a.stages) stage = 0, phase ^= 1;
         }
       }
+      // What the matrix instructions arrive at is this block's until they have arrived: the stages' barriers, and of a pair's second
+      // block the one for the end, which is waited for by the first block's thread alone otherwise.
+      for (int i = 0, at = stage; ok && i < a.stages; ++i) {
+        ok = mm_wait(smem_addr(&s.empty[at]), phase ^ (at < stage ? 0 : 1), s, gave_up);
+        if (++at == a.stages) at = 0;
+      }
+      if (PAIR && ok && rank != 0) ok = mm_wait(smem_addr(&s.drained), 0, s, gave_up);
       if (!ok) {
         // What was requested still lands in this block's memory.  Where no barrier of this block tells (a pair's second block; a
         // stage whose tokens were never asked for), the limit of a wait outlasts it: `drained` has no second phase.

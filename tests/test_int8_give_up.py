@@ -66,3 +66,33 @@ def test_the_kernel_asks_all_warps_before_it_goes_on():
     assert re.search(r"const bool ok = mm_wait\(smem_addr\(&s\.sum_full\[buf\]\)[^;]*;\s*(__syncwarp\(\);\s*)?if \(!epilogue_agrees\(ok\)\) break;", code)
     assert len(re.findall(r"\bbreak;", code)) == 1 and "bar.sync 1" not in code
     assert re.search(r"barrier\.cta\.red\.and\.pred q, 1, 256, p", open(SOURCE).read())
+
+
+@pytest.mark.parametrize("stages", [1, 2, 3, 5, 8])
+def test_every_stage_is_waited_for_at_the_end(stages):
+    """The thread that requests copies waits, before its block may leave, for the last arrival at every stage's barrier: the parity it asks
+    for is that of the last phase that the stage's matrix instructions complete, and one that is over where there were none."""
+    for issued in range(4 * stages + 1):
+        stage, phase, rounds = 0, 0, [0] * stages          # rounds: how often a stage was filled, so how many phases will complete
+        for _ in range(issued):
+            rounds[stage] += 1
+            stage += 1
+            if stage == stages:
+                stage, phase = 0, phase ^ 1
+        at, asked = stage, []
+        for _ in range(stages):
+            asked.append((at, phase ^ (0 if at < stage else 1)))
+            at = (at + 1) % stages
+        assert sorted(a for a, _ in asked) == list(range(stages))
+        for a, parity in asked:
+            # a wait for a parity ends when the phase that runs has the other one, and no sooner than after the last arrival
+            assert [done for done in range(rounds[a] + 1) if done % 2 != parity][-1] == rounds[a]
+            assert rounds[a] == 0 or (rounds[a] - 1) % 2 == parity
+
+
+def test_the_kernel_waits_for_what_the_pairs_first_block_sends():
+    text = open(SOURCE).read()
+    copies = text[text.index("---------------- copies"):text.index("---------------- matrix instructions")]
+    assert re.search(r"for \(int i = 0, at = stage; ok && i < a\.stages; \+\+i\) \{\s*"
+                     r"ok = mm_wait\(smem_addr\(&s\.empty\[at\]\), phase \^ \(at < stage \? 0 : 1\), s, gave_up\);", copies)
+    assert re.search(r"if \(PAIR && ok && rank != 0\) ok = mm_wait\(smem_addr\(&s\.drained\), 0", copies)
