@@ -126,11 +126,11 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   tmem_fence_after_sync();
   const uint32_t tmem = s.tmem;
 
+  int copy_stage = 0, issued = 0, ahead = 0;                    // of the copies' thread, to the end
+  uint32_t copy_phase = 0;
+  bool copied = true;
   if (warp == 8) {                                              // ---------------- copies
     if (lane == 0) {
-      int stage = 0, issued = 0, ahead = 0;
-      uint32_t phase = 0;
-      bool ok = true;
       // Requests one operand of a stage; of a pair, the first block's barrier counts.
       auto request = [&](int stage, uint32_t offset, const CUtensorMap* map, int k, int row) {
         const uint32_t dst = stage0 + stage * stage_bytes + offset, bar = smem_addr(&s.full[stage]);
@@ -148,38 +148,26 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
         }
         grid_wait();
       }
-      for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+      for (int tile = first_tile; copied && tile < a.tiles; tile += tile_step) {
         const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
         for (int k = k_first; k < k_end; ++k) {
-          if (!(ok = mm_wait(smem_addr(&s.empty[stage]), phase ^ 1, s, gave_up))) break;
+          if (!(copied = mm_wait(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1, s, gave_up))) break;
           if (issued >= ahead) {
-            expect(stage);
-            request(stage, 0, &weights, k, ct * tile_channels + (int)rank * kMmChannels * PAIR);
+            expect(copy_stage);
+            request(copy_stage, 0, &weights, k, ct * tile_channels + (int)rank * kMmChannels * PAIR);
           }
-          request(stage, a_bytes, &tokens, k, tt * a.tokens + (int)rank * load_tokens * PAIR);
+          request(copy_stage, a_bytes, &tokens, k, tt * a.tokens + (int)rank * load_tokens * PAIR);
           ++issued;
-          if (++stage == a.stages) stage = 0, phase ^= 1;
+          if (++copy_stage == a.stages) copy_stage = 0, copy_phase ^= 1;
         }
       }
-      // What the matrix instructions arrive at is this block's until they have arrived: the stages' barriers, and of a pair's second
-      // block the one for the end, which is waited for by the first block's thread alone otherwise.
-      for (int i = 0, at = stage; ok && i < a.stages; ++i) {
-        ok = mm_wait(smem_addr(&s.empty[at]), phase ^ (at < stage ? 0 : 1), s, gave_up);
+      // A pair's second block is there until what the first one's matrix instructions arrive at has been arrived at: the stages' barriers
+      // and the one for the end.  (In their own block the thread that issues them waits for the end.)
+      for (int i = 0, at = copy_stage; PAIR && copied && i < a.stages; ++i) {
+        copied = mm_wait(smem_addr(&s.empty[at]), copy_phase ^ (at < copy_stage ? 0 : 1), s, gave_up);
         if (++at == a.stages) at = 0;
       }
-      if (PAIR && ok && rank != 0) ok = mm_wait(smem_addr(&s.drained), 0, s, gave_up);
-      if (!ok) {
-        // What was requested still lands in this block's memory.  Where no barrier of this block tells (a pair's second block; a
-        // stage whose tokens were never asked for), the limit of a wait outlasts it: `drained` has no second phase.
-        if (PAIR || ahead > issued) {
-          mbar_wait(smem_addr(&s.drained), 0);
-          mbar_wait(smem_addr(&s.drained), 1);
-        }
-        for (int i = 0; !PAIR && i < a.stages && i < issued; ++i) {
-          if (--stage < 0) stage = a.stages - 1, phase ^= 1;
-          mbar_wait(smem_addr(&s.full[stage]), phase);
-        }
-      }
+      if (PAIR && copied) copied = mm_wait(smem_addr(&s.drained), 0, s, gave_up);
     }
   } else if (warp == 9) {                                       // ---------------- matrix instructions
     if (a.early) grid_wait();                                   // the limit of a wait is for copies, not for the launch before
@@ -329,6 +317,19 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   }
   tmem_fence_before_sync();
   __syncthreads();
+  if (warp == 8 && lane == 0 && s.dead) {
+    // What was requested still lands in this block's memory, whichever wait ran out.  Where no barrier of this block tells (a pair's
+    // second block; a stage whose tokens were never asked for), the limit of a wait outlasts it: `drained` has no second phase.
+    if (PAIR || ahead > issued) {
+      mbar_wait(smem_addr(&s.drained), 0);
+      mbar_wait(smem_addr(&s.drained), 1);
+    }
+    for (int i = 0; !PAIR && i < a.stages && i < issued; ++i) {
+      if (--copy_stage < 0) copy_stage = a.stages - 1, copy_phase ^= 1;
+      mbar_wait(smem_addr(&s.full[copy_stage]), copy_phase);
+    }
+  }
+  __syncwarp();
   if constexpr (PAIR) cluster_sync();                           // neither block's memory or barriers are used by the other any more
   if (warp == 9) tmem_free<PAIR>(tmem, columns);
 }

@@ -93,6 +93,15 @@ def test_every_stage_is_waited_for_at_the_end(stages):
 def test_the_kernel_waits_for_what_the_pairs_first_block_sends():
     text = open(SOURCE).read()
     copies = text[text.index("---------------- copies"):text.index("---------------- matrix instructions")]
-    assert re.search(r"for \(int i = 0, at = stage; ok && i < a\.stages; \+\+i\) \{\s*"
-                     r"ok = mm_wait\(smem_addr\(&s\.empty\[at\]\), phase \^ \(at < stage \? 0 : 1\), s, gave_up\);", copies)
-    assert re.search(r"if \(PAIR && ok && rank != 0\) ok = mm_wait\(smem_addr\(&s\.drained\), 0", copies)
+    stages = re.search(r"for \(int i = 0, at = copy_stage; PAIR && copied && i < a\.stages; \+\+i\) \{\s*"
+                       r"copied = mm_wait\(smem_addr\(&s\.empty\[at\]\), copy_phase \^ \(at < copy_stage \? 0 : 1\), s, gave_up\);", copies)
+    last = re.search(r"if \(PAIR && copied\) copied = mm_wait\(smem_addr\(&s\.drained\), 0", copies)
+    assert stages and last and stages.start() < last.start()
+
+
+def test_copies_under_way_are_waited_for_whichever_wait_ran_out():
+    """Behind the block's last barrier, when every thread's waits are over."""
+    text = open(SOURCE).read()
+    end = text[text.index("nobody leaves while its sums are read"):text.index("host")]
+    drain = re.search(r"__syncthreads\(\);\s*if \(warp == 8 && lane == 0 && s\.dead\) \{", end)
+    assert drain and drain.end() < end.index("mbar_wait(smem_addr(&s.full[copy_stage]), copy_phase);") < end.index("if constexpr (PAIR) cluster_sync();")
