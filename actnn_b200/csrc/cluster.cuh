@@ -26,6 +26,9 @@ ACTNN_DEV uint32_t peer_addr(uint32_t addr, uint32_t rank) {
 ACTNN_DEV void peer_arrive(uint32_t remote) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" :: "r"(remote) : "memory");
 }
+ACTNN_DEV void peer_store1(uint32_t addr, uint32_t rank, int v) {
+  asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(peer_addr(addr, rank)), "r"(v) : "memory");
+}
 ACTNN_DEV int4 peer_load4i(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   int4 v;

@@ -54,7 +54,7 @@ struct MmArgs {
 struct MmShared {
   uint64_t full[kMmStagesMost], empty[kMmStagesMost], sum_full[2], sum_empty[2], drained;
   uint32_t tmem;
-  int dead;
+  int dead, gone;                               // a wait of the block has run out; of one of the blocks that share a reduction
   alignas(16) float scale[2][256];
 };
 
@@ -115,7 +115,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       mbar_init(smem_addr(&s.sum_empty[i]), (PAIR ? 2 : 1) * kMmEpilogue / 32);
     }
     mbar_init(smem_addr(&s.drained), 1);
-    s.dead = 0;
+    s.dead = s.gone = 0;
     mbar_init_fence();
   }
   const uint32_t columns = SPLIT ? a.columns : 2 * a.columns;
@@ -123,6 +123,7 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   tmem_fence_before_sync();
   __syncthreads();
   if constexpr (PAIR) cluster_sync();                           // both blocks have their barriers and their tensor memory
+  if constexpr (SPLIT) cluster_arrive();                        // this block's flags are set
   tmem_fence_after_sync();
   const uint32_t tmem = s.tmem;
 
@@ -279,8 +280,13 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
   if (!SPLIT && a.boxes && warp < 8 && (threadIdx.x & 127) == 0) tile_store_done();
   if constexpr (SPLIT) {
     __syncwarp();
+    cluster_wait();                                             // all have begun, long since
+    // Where a wait of any of the cluster's blocks ran out, its sums are not there, and nothing is written by any of them.  The
+    // thread whose wait it was has seen its block's flag set, and tells the others before it comes to the barrier.
+    if (s.dead)
+      for (int k = 0; k < a.splits; ++k) peer_store1(smem_addr(&s.gone), k, 1);
     cluster_sync();
-    if (warp < 8 && !s.dead) {                                  // a warp takes a column: 4 channels a lane, all blocks' sums at once
+    if (warp < 8 && !s.gone) {                                  // a warp takes a column: 4 channels a lane, all blocks' sums at once
       const int tt = first_tile / a.channel_tiles, ct = first_tile - tt * a.channel_tiles;
       const int64_t t0 = (int64_t)tt * a.tokens, n = (int64_t)ct * kMmChannels + lane * 4;
       float w[4], b[4];

@@ -105,3 +105,15 @@ def test_copies_under_way_are_waited_for_whichever_wait_ran_out():
     end = text[text.index("nobody leaves while its sums are read"):text.index("host")]
     drain = re.search(r"__syncthreads\(\);\s*if \(warp == 8 && lane == 0 && s\.dead\) \{", end)
     assert drain and drain.end() < end.index("mbar_wait(smem_addr(&s.full[copy_stage]), copy_phase);") < end.index("if constexpr (PAIR) cluster_sync();")
+
+
+def test_a_cluster_writes_all_of_a_tile_or_nothing():
+    """A reduction that blocks share: a thread whose wait ran out tells every block of the cluster, between the barrier that says that all have
+    set their flags and the one behind which the sums are read, and nothing is written where one has told.  No wait for a phase
+    stands behind the latter."""
+    text = open(SOURCE).read()
+    assert re.search(r"s\.dead = s\.gone = 0;", text) and text.index("s.gone = 0;") < text.index("if constexpr (SPLIT) cluster_arrive();")
+    shared = text[text.index("if constexpr (SPLIT) {\n    __syncwarp();"):text.index("nobody leaves while its sums are read")]
+    told = re.search(r"cluster_wait\(\);[^;]*\n(\s*//[^\n]*\n)*\s*if \(s\.dead\)\s*for \(int k = 0; k < a\.splits; \+\+k\) "
+                     r"peer_store1\(smem_addr\(&s\.gone\), k, 1\);\s*cluster_sync\(\);\s*if \(warp < 8 && !s\.gone\) \{", shared)
+    assert told and told.end() < shared.index("peer_load4i") and "mm_wait" not in shared
