@@ -360,7 +360,7 @@ class QGroupNorm(nn.GroupNorm):
         self.activation = activation or "none"
 
     def forward(self, input):
-        if not torch.is_grad_enabled() or not (input.requires_grad or (self.weight is not None and self.weight.requires_grad)):
+        if not torch.is_grad_enabled() or not any(p is not None and p.requires_grad for p in (input, self.weight, self.bias)):
             return ext_group_norm.inference(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
         return ops.group_norm.apply(input, self.num_groups, self.weight, self.bias, self.eps, self.activation)
 
