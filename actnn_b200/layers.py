@@ -282,14 +282,15 @@ class QInt8Linear(nn.Linear):
 
     In training the weight is coded in every step and the codes of the input are what the backward pass keeps.  For serving,
     ``freeze()`` codes the weight once: until ``unfreeze()`` (or ``train()``) the forward pass reads those codes alone, whatever
-    happens to ``weight``."""
+    happens to ``weight``.  Under autocast the layer computes in autocast's type, frozen or not; codes that ``freeze()`` makes there
+    are those of the weight in that type, as in training, and elsewhere those of the weight as it is."""
 
     def __init__(self, in_features, out_features, bias=True):
         super().__init__(in_features, out_features, bias)
         self.frozen = None
 
     def freeze(self):
-        self.frozen = ext_int8.quantize_rows(self.weight.detach())
+        self.frozen = ext_int8.quantize_rows(*ops._autocast_inputs(self.weight.detach()))
         return self
 
     def unfreeze(self):
@@ -309,7 +310,8 @@ class QInt8Linear(nn.Linear):
         if self.frozen is not None:
             if torch.is_grad_enabled() and input.requires_grad:
                 raise RuntimeError("QInt8Linear is frozen: no gradient passes through it (call unfreeze() first)")
-            return ext_int8.linear(input, *self.frozen, None if self.bias is None else self.bias.detach())
+            input, bias = ops._autocast_inputs(input, None if self.bias is None else self.bias.detach())
+            return ext_int8.linear(input, *self.frozen, bias)
         return ops.int8_linear.apply(input, self.weight, self.bias)
 
 
