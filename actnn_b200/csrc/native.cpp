@@ -576,7 +576,10 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
       check(actnn_int8_matmul(cx.codes.data_ptr<int8_t>(), cx.scale.data_ptr<float>(), cw.codes.data_ptr<int8_t>(), cw.scale.data_ptr<float>(),
                               with ? b.data_ptr() : nullptr, out.data_ptr(), cx.rows, n, k, cx.ld, cw.ld, dtype_id(x.scalar_type()), stream()),
             "actnn_int8_matmul");
-    ctx->save_for_backward({cx.codes, cx.scale, cw.codes, cw.scale});
+    // the input's codes are what the weight's gradient is made of, and the other way round: what no gradient needs is not kept
+    const bool keep_x = weight.requires_grad(), keep_w = x.requires_grad();
+    ctx->save_for_backward({keep_x ? cx.codes : Tensor(), keep_x ? cx.scale : Tensor(), keep_w ? cw.codes : Tensor(),
+                            keep_w ? cw.scale : Tensor()});
     ctx->saved_data["sizes"] = x.sizes();
     ctx->saved_data["n"] = n;
     ctx->saved_data["x"] = x.scalar_type();
@@ -589,14 +592,16 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
     const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
     const int64_t k = sizes.back(), n = ctx->saved_data["n"].toInt();
     const auto type = ctx->saved_data["x"].toScalarType();
-    const RowCodes cx{saved[0], saved[1], saved[0].size(0), k, saved[0].size(1)}, cw{saved[2], saved[3], n, k, saved[2].size(1)};
-    c10::cuda::CUDAGuard guard(cx.codes.device());
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < sizes.size(); ++i) rows *= sizes[i];
+    c10::cuda::CUDAGuard guard(grads[0].device());
     c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);       // products in the types of the forward pass
-    const Tensor go = grads[0].reshape({n ? grads[0].numel() / n : (k ? cx.rows : 0), n});
+    const Tensor go = grads[0].reshape({rows, n});
     Tensor gx, gw, gb;
-    if (ctx->needs_input_grad(0)) gx = k ? go.mm(row_decode(cw, type)).view(sizes) : at::zeros(sizes, go.options());
+    if (ctx->needs_input_grad(0))
+      gx = k ? go.mm(row_decode({saved[2], saved[3], n, k, row_bytes(k)}, type)).view(sizes) : at::zeros(sizes, go.options());
     if (ctx->needs_input_grad(1))
-      gw = k ? go.t().mm(row_decode(cx, type)).to(ctx->saved_data["w"].toScalarType())
+      gw = k ? go.t().mm(row_decode({saved[0], saved[1], rows, k, row_bytes(k)}, type)).to(ctx->saved_data["w"].toScalarType())
              : at::zeros({n, k}, go.options().dtype(ctx->saved_data["w"].toScalarType()));
     const int64_t bias_type = ctx->saved_data["b"].toInt();
     if (bias_type >= 0 && ctx->needs_input_grad(2)) gb = column_sums(go).to((at::ScalarType)bias_type);
