@@ -663,13 +663,14 @@ class _Int8Linear(Function):
         codes, scale, wcodes, wscale = ctx.saved
         dtype, shape, wdtype, bdtype = ctx.other_args
         with _autocast_off():
-            go = grad_output.reshape(-1, grad_output.shape[-1]) if grad_output.dim() != 2 else grad_output
+            rows = shape[:-1].numel()                    # an empty dimension leaves nothing to infer it from
+            go = grad_output.reshape(rows, grad_output.shape[-1])
             grad_input = grad_weight = grad_bias = None
             if ctx.needs_input_grad[0]:
                 grad_input = go.mm(ext_int8.dequantize_rows(wcodes, wscale, dtype)).view(shape)
             if ctx.needs_input_grad[1]:
                 x = ext_int8.dequantize_rows(_kept(codes), scale, dtype)
-                grad_weight = go.t().mm(x.view(-1, shape[-1])).to(wdtype)
+                grad_weight = go.t().mm(x.view(rows, shape[-1])).to(wdtype)
             if bdtype is not None and ctx.needs_input_grad[2]:
                 grad_bias = ext_int8.column_sums(go).to(bdtype)
         return grad_input, grad_weight, grad_bias
