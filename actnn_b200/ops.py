@@ -693,9 +693,12 @@ class int8_linear:
 class _Activation(Function):
     @staticmethod
     def forward(ctx, input, name, gated):
-        ctx.name, ctx.gated, ctx.codes = name, gated, None
+        ctx.name, ctx.gated, ctx.codes, ctx.parked = name, gated, None, None
         if not config.compress_activation:
-            ctx.save_for_backward(input)
+            if config.swap:
+                ctx.parked = swap_to_cpu(input)
+            else:
+                ctx.save_for_backward(input)
             return ext_checkpoint.activation_forward(input, name, gated, save=False)[0]
         output, codes, scale = ext_checkpoint.activation_forward(input, name, gated)
         ctx.codes = _keep(codes), scale
@@ -704,7 +707,8 @@ class _Activation(Function):
     @staticmethod
     def backward(ctx, grad_output):
         if ctx.codes is None:
-            grad = ext_checkpoint.activation_backward(grad_output, ctx.name, x=ctx.saved_tensors[0], gated=ctx.gated)
+            x = _kept(ctx.parked) if ctx.parked is not None else ctx.saved_tensors[0]
+            grad = ext_checkpoint.activation_backward(grad_output, ctx.name, x=x, gated=ctx.gated)
         else:
             codes, scale = ctx.codes
             grad = ext_checkpoint.activation_backward(grad_output, ctx.name, _kept(codes), scale, gated=ctx.gated)
@@ -739,8 +743,9 @@ class _GroupNorm(Function):
     def forward(ctx, input, num_groups, weight, bias, eps, name):
         compress = config.compress_activation
         output, saved, stats = ext_group_norm.forward(input, num_groups, weight, bias, eps, name, compress)
-        ctx.save_for_backward(weight, bias, None if compress else input)
-        ctx.codes = _keep(saved) if compress else None
+        here = not compress and not config.swap              # the caller's own tensor
+        ctx.save_for_backward(weight, bias, input if here else None)
+        ctx.kept = None if here else _keep(saved)
         ctx.other_args = (num_groups, name, stats)
         return output
 
@@ -748,7 +753,7 @@ class _GroupNorm(Function):
     def backward(ctx, grad_output):
         weight, bias, input = ctx.saved_tensors
         groups, name, stats = ctx.other_args
-        saved = _kept(ctx.codes) if input is None else input.movedim(1, -1).contiguous()
+        saved = _kept(ctx.kept) if input is None else input.movedim(1, -1).contiguous()
         gx, gw, gb = ext_group_norm.backward(grad_output, saved, stats, groups, weight, bias, name,
                                              (ctx.needs_input_grad[2], ctx.needs_input_grad[3]))
         return gx, None, None if gw is None else gw.to(weight.dtype), None if gb is None else gb.to(bias.dtype), None, None
