@@ -266,7 +266,9 @@ template <bool PRECISE, typename F> ACTNN_DEV F logistic(F z, float factor) {
 
 // The normal distribution's function and density at z.  Fast form: 1 - erf(x) = (a1 t + ... + a5 t^5) exp(-x^2) + e,
 // t = 1 / (1 + p x), |e| < 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26), at x = |z| / sqrt(2);
-// half of it is the distribution's tail, and exp(-x^2) is the density's exponential.
+// half of it is the distribution's tail, and exp(-x^2) is the density's exponential.  Far out the tail's own relative error is what
+// counts: 0.0016 of it down to z = -5, 0.0036 to -6, 0.010 to -8.  Precise form: the sum of one and erf, errors of 2^-24 of one; erfc, whose errors are of the tail
+// itself, made 8192 x 4096 float32 elements 72 us forward and 73 back instead of 58 and 62.
 template <bool PRECISE, bool DENSITY, typename F> ACTNN_DEV void normal(F z, F& below, F& density) {
   if constexpr (PRECISE) {
     below = f_each(z, [](float v) { return 0.5f * (1.f + erff(v * 0.70710678118654752f)); });
@@ -280,10 +282,10 @@ template <bool PRECISE, bool DENSITY, typename F> ACTNN_DEV void normal(F z, F& 
     p = f_fma(p, t, f_both<F>(0.5f * -0.284496736f));
     p = f_fma(p, t, f_both<F>(0.5f * 0.254829592f));
     const F tail = f_mul(f_mul(p, t), e);
-    // 1 - tail above zero: half plus or minus (half - tail)
-    const F rest = f_add(f_both<F>(0.5f), f_mul(tail, f_both<F>(-1.f)));
-    if constexpr (sizeof(F) == 8) below = f_add(f_both<F>(0.5f), make_float2(copysignf(rest.x, z.x), copysignf(rest.y, z.y)));
-    else below = 0.5f + copysignf(rest, z);
+    // The tail as it is below zero, 1 - tail above, by the sign m of -z: m * tail + (1 - m) / 2.  (Half plus or minus half less the
+    // tail would be gone at -6.)
+    const F m = f_each(z, [](float v) { return __uint_as_float((~__float_as_uint(v) & 0x80000000u) | 0x3f800000u); });
+    below = f_fma(tail, m, f_fma(m, f_both<F>(-0.5f), f_both<F>(0.5f)));
     if constexpr (DENSITY) density = f_mul(e, f_both<F>(0.3989422804014327f));
   }
 }
