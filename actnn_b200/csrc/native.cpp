@@ -609,19 +609,21 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
   }
 };
 
-// `compress` false: the input itself is kept
+// `compress` false: the input itself is kept.  The identity without a gate keeps nothing.
 struct Activation : torch::autograd::Function<Activation> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, int64_t kind, bool gated, bool compress) {
-    auto [y, codes, scale] = act_forward(x, (int)kind, gated, compress);
+    const bool identity = kind == 0 && !gated;
+    auto [y, codes, scale] = act_forward(x, (int)kind, gated, compress && !identity);
     ctx->saved_data["kind"] = kind;
     ctx->saved_data["gated"] = gated;
     ctx->saved_data["compress"] = compress;
-    if (compress) ctx->save_for_backward({codes, scale});
-    else ctx->save_for_backward({x});
+    if (compress && !identity) ctx->save_for_backward({codes, scale});
+    else if (!identity) ctx->save_for_backward({x});
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
+    if (saved.empty()) return {grads[0], Tensor(), Tensor(), Tensor()};
     const bool compress = ctx->saved_data["compress"].toBool();
     return {act_backward(grads[0], compress ? Tensor() : saved[0], compress ? saved[0] : Tensor(), compress ? saved[1] : Tensor(),
                          (int)ctx->saved_data["kind"].toInt(), ctx->saved_data["gated"].toBool()),

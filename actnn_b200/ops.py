@@ -30,6 +30,7 @@ from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import checkpoint as ext_checkpoint
 from .cpp_extension import group_norm as ext_group_norm
 from .cpp_extension import int8 as ext_int8
+from .cpp_extension._checks import activation_kind
 from .cpp_extension import minimax as ext_minimax  # noqa: F401  (kept under the name the reference imports)
 from .cpp_extension import quantization as ext_quantization
 from .qbnscheme import QBNScheme
@@ -694,6 +695,9 @@ class _Activation(Function):
     @staticmethod
     def forward(ctx, input, name, gated):
         ctx.name, ctx.gated, ctx.codes, ctx.parked = name, gated, None, None
+        ctx.identity = not gated and activation_kind(name) == 0
+        if ctx.identity:                                      # its backward pass needs nothing
+            return ext_checkpoint.activation_forward(input, name, save=False)[0]
         if not config.compress_activation:
             if config.swap:
                 ctx.parked = swap_to_cpu(input)
@@ -706,7 +710,9 @@ class _Activation(Function):
 
     @staticmethod
     def backward(ctx, grad_output):
-        if ctx.codes is None:
+        if ctx.identity:
+            grad = grad_output
+        elif ctx.codes is None:
             x = _kept(ctx.parked) if ctx.parked is not None else ctx.saved_tensors[0]
             grad = ext_checkpoint.activation_backward(grad_output, ctx.name, x=x, gated=ctx.gated)
         else:
@@ -723,7 +729,11 @@ def _activation(input, name, gated):
 
 
 class activation:
-    """An activation function ("none", "relu", "silu", "gelu", "gelu_tanh") that keeps its input in 8 bits."""
+    """An activation function ("none", "relu", "silu", "gelu", "gelu_tanh") that keeps its input in 8 bits ("none" keeps nothing).
+
+    The derivative is taken at what the codes stand for.  That matters for "relu", whose derivative jumps: an input between zero and half
+    a step, its 256 elements' largest magnitude over 254, has the gradient zero.  ``QReLU`` decides on the input itself and
+    keeps one bit; the form here is for where codes of the input are wanted anyway."""
 
     @staticmethod
     def apply(input, name):
