@@ -1058,13 +1058,19 @@ template <auto KERNEL, typename... Args> bool gn_start(const GnCall& c, const Gn
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, KERNEL, args...) == cudaSuccess;
 }
-// The cut of one of two launches of KERNEL, by the blocks of 256 threads that an SM holds of it.
+// The cut of one of two launches of KERNEL, by the blocks of 256 threads that an SM holds of it with `smem` bytes each.  The last
+// answer is kept with its question (bytes in the upper half, blocks in the lower one); one that failed is not.
 template <auto KERNEL> void gn_cut_for(GnShape& g, int64_t N, int smem, int extra) {
-  static std::atomic<int> resident{0};
-  int n = resident.load(std::memory_order_acquire);
-  if (n == 0) {
-    if (!gn_raise<KERNEL>() || cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kGnThreads, smem) != cudaSuccess || n < 1) n = 1;
-    resident.store(n, std::memory_order_release);
+  static std::atomic<uint64_t> answer{0};
+  const uint64_t kept = answer.load(std::memory_order_acquire);
+  int n = (int)(uint32_t)kept;
+  if (n == 0 || (int)(kept >> 32) != smem) {
+    if (gn_raise<KERNEL>() && cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, KERNEL, kGnThreads, smem) == cudaSuccess && n > 0) {
+      answer.store((uint64_t)smem << 32 | (uint32_t)n, std::memory_order_release);
+    } else {
+      cudaGetLastError();
+      n = 1;
+    }
   }
   gn_cut_positions(g, N, (int64_t)device_info().sm_count * n, extra);
 }
