@@ -280,7 +280,6 @@ Tensor relu_backward(const Tensor& grad_in, const Tensor& mask) {
   return out;
 }
 
-// with_minmax: also min and max of every 256 outputs, not differentiable
 // ---------------------------------------------------------------------------------------- token operators
 constexpr const char* kNames[] = {"none", "relu", "silu", "gelu", "gelu_tanh"};
 int activation_kind(const std::string& name) {
@@ -460,6 +459,7 @@ NormForward norm_forward(const Tensor& x, int64_t groups, const OptTensor& weigh
   return r;
 }
 
+// with_minmax: also min and max of every 256 outputs, not differentiable
 struct Relu : torch::autograd::Function<Relu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, bool with_minmax) {
     c10::cuda::CUDAGuard guard(x.device());
@@ -685,9 +685,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("int8_linear_train", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return Int8Linear::apply(x, w, b); });
   m.def("activation", [](const Tensor& x, const std::string& name, bool gated, bool compress) {
     return Activation::apply(x, activation_kind(name), gated, compress);
-  });
-  m.def("activation_value", [](const Tensor& x, const std::string& name, bool gated) {
-    return std::get<0>(act_forward(x, activation_kind(name), gated, false));
   });
   m.def("group_norm", [](const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps, const std::string& name,
                          bool compress) { return GroupNorm::apply(x, groups, w, b, eps, activation_kind(name), compress); });
