@@ -29,6 +29,12 @@ def activation_kind(name):
         raise RuntimeError("activation must be one of %s, got %r" % (", ".join(sorted(ACTIVATIONS)), name)) from None
 
 
+def activation_name(name):
+    """The name that both halves of the binding take for what a caller named, or ``None``."""
+    activation_kind(name)
+    return "none" if name is None else name
+
+
 def check_cuda_values(t, name, device=None):
     """A floating CUDA tensor of a supported type, any strides; on ``device`` when given."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda:

@@ -10,7 +10,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from ._checks import activation_kind, check_cuda_values
+from ._checks import activation_kind, activation_name, check_cuda_values
 
 
 def _positions(x, name, groups):
@@ -57,7 +57,7 @@ def inference(x, groups, weight=None, bias=None, eps=1e-5, activation="none"):
     """The output alone."""
     nat = _lib.native()
     if nat:
-        return nat.group_norm_value(x, groups, weight, bias, eps, "none" if activation is None else activation)
+        return nat.group_norm_value(x, groups, weight, bias, eps, activation_name(activation))
     return _run(x, groups, weight, bias, eps, activation, False, False)[0]
 
 

@@ -20,7 +20,7 @@ from .cpp_extension import checkpoint as ext_checkpoint
 from .cpp_extension import group_norm as ext_group_norm
 from .cpp_extension import int8 as ext_int8
 from .cpp_extension import quantization as ext_quantization
-from .cpp_extension._checks import activation_kind
+from .cpp_extension._checks import activation_name
 from .qbnscheme import QBNScheme
 from .qscheme import QScheme
 
@@ -349,8 +349,7 @@ class QGLU(_QActivation):
 
     def __init__(self, activation: str = "silu"):
         super().__init__()
-        activation_kind(activation)
-        self._name = activation
+        self._name = activation_name(activation)
 
 
 class QGroupNorm(nn.GroupNorm):
@@ -358,8 +357,7 @@ class QGroupNorm(nn.GroupNorm):
 
     def __init__(self, num_groups, num_channels, eps=1e-5, affine=True, activation: Optional[str] = None):
         super().__init__(num_groups, num_channels, eps, affine)
-        activation_kind(activation)
-        self.activation = activation or "none"
+        self.activation = activation_name(activation)
 
     def forward(self, input):
         if not torch.is_grad_enabled() or not any(p is not None and p.requires_grad for p in (input, self.weight, self.bias)):

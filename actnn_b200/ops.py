@@ -30,7 +30,7 @@ from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import checkpoint as ext_checkpoint
 from .cpp_extension import group_norm as ext_group_norm
 from .cpp_extension import int8 as ext_int8
-from .cpp_extension._checks import activation_kind
+from .cpp_extension._checks import activation_kind, activation_name
 from .cpp_extension import minimax as ext_minimax  # noqa: F401  (kept under the name the reference imports)
 from .cpp_extension import quantization as ext_quantization
 from .qbnscheme import QBNScheme
@@ -722,6 +722,7 @@ class _Activation(Function):
 
 
 def _activation(input, name, gated):
+    name = activation_name(name)
     nat = _lib.native()
     if nat and not config.swap:
         return nat.activation(input, name, gated, config.compress_activation)
@@ -774,7 +775,8 @@ class group_norm:
 
     @staticmethod
     def apply(input, num_groups, weight=None, bias=None, eps=1e-5, name="none"):
+        name = activation_name(name)
         nat = _lib.native()
         if nat and not config.swap:
-            return nat.group_norm(input, num_groups, weight, bias, eps, "none" if name is None else name, config.compress_activation)
+            return nat.group_norm(input, num_groups, weight, bias, eps, name, config.compress_activation)
         return _GroupNorm.apply(input, num_groups, weight, bias, eps, name)
