@@ -213,8 +213,10 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
       }
       const float w = n < a.N ? __ldg(a.channel_scale + n) : 0.f;
       const float b = n < a.N && a.bias ? to_float(reinterpret_cast<const T*>(a.bias)[n]) : 0.f;
-      const bool ok = mm_wait(smem_addr(&s.sum_full[buf]), buf_phase, s, lane == 0 ? gave_up : nullptr);
-      __syncwarp();
+      // One warp waits for the sums, the others for its word: sleepers wake up to a microsecond apart.
+      const bool ok = warp != 0 || mm_wait(smem_addr(&s.sum_full[buf]), buf_phase, s, lane == 0 ? gave_up : nullptr);
+      tmem_fence_after_sync();
+      tmem_fence_before_sync();
       if (!epilogue_agrees(ok)) break;                          // and the scales are there for all
       tmem_fence_after_sync();
       const uint32_t d = tmem + buf * a.columns + ((uint32_t)(quarter * 32) << 16);
