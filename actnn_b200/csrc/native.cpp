@@ -598,6 +598,10 @@ struct Int8Linear : torch::autograd::Function<Int8Linear> {
     c10::impl::ExcludeDispatchKeyGuard no_autocast(c10::DispatchKey::AutocastCUDA);       // products in the types of the forward pass
     const Tensor go = grads[0].reshape({rows, n});
     Tensor gx, gw, gb;
+    // The decoded operand of each product is rounded to the activation's type, as the operands of any layer in that type are; the
+    // products' sums are float32.  bfloat16, 8192 x 2048 x 4096: the gradients are 0.0024 of their norm from the exact ones, of which
+    // 0.0017 is their own rounding.  Products of the upper and of the lower half of each decoded value, added in float32,
+    // leave 0.0017 and take 380 us instead of 190.
     if (ctx->needs_input_grad(0))
       gx = k ? go.mm(row_decode({saved[2], saved[3], n, k, row_bytes(k)}, type)).view(sizes) : at::zeros(sizes, go.options());
     if (ctx->needs_input_grad(1))

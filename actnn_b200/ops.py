@@ -680,7 +680,10 @@ class _Int8Linear(Function):
 class int8_linear:
     """``x @ weight.T + bias`` in 8-bit integers: rows of ``x`` and of ``weight`` are coded on the way (scale per token, scale per
     output channel), and the codes are all that is kept.  The gradients are those of the product of the decoded matrices, passed
-    straight through the rounding; like those of ``linear`` they are dense products in the activation's type."""
+    straight through the rounding; like those of ``linear`` they are dense products in the activation's type.
+
+    In 16 bits that rounds the decoded operands once more: bfloat16 gradients are off by 0.0024 of their norm, where the rounding of
+    the result alone is 0.0017 (8192 x 2048 x 4096).  With float32 activations nothing is rounded but the results."""
 
     @staticmethod
     def apply(input, weight, bias=None):
