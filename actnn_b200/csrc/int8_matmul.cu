@@ -17,7 +17,7 @@
 // lanes' 64 bytes each took longer than the multiplication (8192 x 2048 x 4096: 87 us with them, 65 with boxes).
 //
 // Measured on a B200, bfloat16 outputs: 16384 x 4096 x 8192 340 - 360 us, 3.1e15 operations a second (twice the measured bfloat16 rate
-// is 3.24e15; the tensor pipe is 82 % busy, the rest is the L2's, 12 TB/s); 8192 x 2048 x 4096 48 - 65; 200 x 4096 x 4096 12.2, where
+// is 3.24e15; the tensor pipe is 79 - 82 % busy, the rest is the L2's, 12 TB/s); 8192 x 2048 x 4096 48 - 61; 200 x 4096 x 4096 12.5, where
 // the weight's bytes take 2.6 and the fixed latencies of launch, first copies, sums through the cluster and outputs about 8.
 //
 // Every wait is bounded.  A block whose wait runs out writes nothing more, is counted (the counter of the bulk waits), lets

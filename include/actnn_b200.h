@@ -447,8 +447,8 @@ int actnn_column_sums(const void* x, void* out, int64_t rows, int64_t cols, int 
  * on the integer tensor cores; the sum is exact (int32), out is [T, N] contiguous of `dtype`, rounded
  * once.  `bias` (of `dtype`) may be NULL.  Rows of codes start on 16 bytes: pointers and ld_* (bytes)
  * are multiples of 16, and what lies between K and ld is not read as data.  1 <= K <= 131072.
- * A block whose bounded wait runs out leaves its outputs unwritten and counts the event
- * (actnn_bulk_wait_failures).  The reference has no counterpart (its layers compute in the
+ * A block whose bounded wait runs out leaves its outputs unwritten, as do those that share its reduction, and counts
+ * the event (actnn_bulk_wait_failures).  The reference has no counterpart (its layers compute in the
  * activation's type, actnn/actnn/ops.py:408-428). */
 int actnn_int8_matmul(const int8_t* tokens, const float* token_scale, const int8_t* weights,
                       const float* channel_scale, const void* bias, void* out, int64_t T, int64_t N, int64_t K,
