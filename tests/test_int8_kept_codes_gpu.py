@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from test_int8_linear_gpu import tokens
+from test_swap_token_inputs_gpu import held
 
 pytestmark = pytest.mark.gpu
 
@@ -19,9 +20,6 @@ def test_bytes(cuda_device, monkeypatch, flags, half):
     every = [v.clone().requires_grad_() for v in (x, w, b)]
     ops.int8_linear.apply(*every).backward(dy)
     mine = [v.requires_grad_(f) for v, f in zip((x, w, b), flags)]
-
-    def held():
-        return torch.cuda.memory_stats()["requested_bytes.all.current"]
 
     before = held()
     y = ops.int8_linear.apply(*mine)

@@ -2,6 +2,8 @@
 import pytest
 import torch
 
+from test_swap_token_inputs_gpu import held
+
 pytestmark = pytest.mark.gpu
 
 
@@ -14,12 +16,12 @@ def test_bytes_and_gradient(cuda_device, monkeypatch, level, half):
         monkeypatch.setattr(_lib, "_native", False)
     actnn.set_optimization_level(level)
     leaf = torch.randn(512, 1000, device="cuda", requires_grad=True)
-    before = torch.cuda.memory_stats()["requested_bytes.all.current"]
+    before = held()
     h = leaf * 1
     y = ops.activation.apply(h, "none")
     assert torch.equal(y, h)
     del h
-    assert torch.cuda.memory_stats()["requested_bytes.all.current"] - before == y.numel() * 4
+    assert held() - before == y.numel() * 4
     dy = torch.randn_like(y)
     y.backward(dy)
     assert torch.equal(leaf.grad, dy)
