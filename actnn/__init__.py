@@ -19,7 +19,8 @@ from actnn_b200 import __all__      # noqa: F401
 
 _SUBMODULES = ("ops", "conf", "layers", "module", "qscheme", "qbnscheme", "utils", "cpp_extension",
                "cpp_extension.minimax", "cpp_extension.quantization", "cpp_extension.calc_precision",
-               "cpp_extension.backward_func", "cpp_extension.int8", "cpp_extension.checkpoint", "cpp_extension.group_norm")
+               "cpp_extension.backward_func", "cpp_extension.int8", "cpp_extension.checkpoint", "cpp_extension.group_norm",
+               "cpp_extension.fp8", "cpp_extension.residual_norm", "cpp_extension.seeded_dropout")
 for _name in _SUBMODULES:
     _mod = importlib.import_module("actnn_b200." + _name)
     sys.modules[__name__ + "." + _name] = _mod

@@ -10,8 +10,8 @@ _lib.load()
 from . import ops                                                         # noqa: E402
 from .conf import config, set_optimization_level                          # noqa: E402
 from .layers import (QAvgPool2d, QBatchNorm1d, QBatchNorm2d, QBatchNorm3d, QConv1d, QConv2d, QConv3d,   # noqa: E402
-                     QConvTranspose1d, QConvTranspose2d, QConvTranspose3d, QDropout, QGELU, QGLU, QGroupNorm, QInt8Linear,
-                     QLinear, QMaxPool2d, QReLU, QSiLU, QSyncBatchNorm)
+                     QConvTranspose1d, QConvTranspose2d, QConvTranspose3d, QDropout, QFp8Linear, QGELU, QGLU, QGroupNorm,
+                     QInt8Linear, QLinear, QMaxPool2d, QReLU, QResidualNorm, QSeededDropout, QSiLU, QSyncBatchNorm)
 from .module import QModule                                               # noqa: E402
 from .qbnscheme import QBNScheme                                          # noqa: E402
 from .qscheme import QScheme                                              # noqa: E402
@@ -20,4 +20,5 @@ from .utils import compute_tensor_bytes, exp_recorder, get_memory_usage   # noqa
 __all__ = ["config", "set_optimization_level", "QModule", "QScheme", "QBNScheme", "ops",
            "QConv1d", "QConv2d", "QConv3d", "QConvTranspose1d", "QConvTranspose2d", "QConvTranspose3d",
            "QBatchNorm1d", "QBatchNorm2d", "QBatchNorm3d", "QSyncBatchNorm", "QLinear", "QReLU", "QDropout",
-           "QMaxPool2d", "QAvgPool2d", "QInt8Linear", "QSiLU", "QGELU", "QGLU", "QGroupNorm", "get_memory_usage", "compute_tensor_bytes", "exp_recorder"]
+           "QMaxPool2d", "QAvgPool2d", "QInt8Linear", "QSiLU", "QGELU", "QGLU", "QGroupNorm", "QFp8Linear", "QSeededDropout",
+           "QResidualNorm", "get_memory_usage", "compute_tensor_bytes", "exp_recorder"]

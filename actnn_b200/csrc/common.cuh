@@ -335,6 +335,11 @@ int int8_matmul_impl(const int8_t* tokens, const float* token_scale, const int8_
                      const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens, int64_t ld_weights,
                      int dtype, bool early, actnn_stream_t stream);
 
+// fp8_matmul.cu: actnn_fp8_matmul, `early` as above.
+int fp8_matmul_impl(const uint8_t* tokens, const uint8_t* token_scales, const uint8_t* weights, const uint8_t* weight_scales,
+                    const void* bias, void* out, int64_t T, int64_t N, int64_t K, int64_t ld_tokens, int64_t ld_weights, int dtype,
+                    bool early, actnn_stream_t stream);
+
 static inline bool aligned(const void* p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
 
 #ifdef __CUDACC__

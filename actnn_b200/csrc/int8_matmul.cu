@@ -26,6 +26,7 @@
 
 #include "activation.cuh"
 #include "tcgen05.cuh"
+#include "tensor_map.cuh"
 
 namespace actnn {
 namespace {
@@ -343,46 +344,6 @@ int8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_con
 }
 
 // ------------------------------------------------------------------ host
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-EncodeTiled encode_tiled() {
-  static std::atomic<EncodeTiled> fn{nullptr};
-  EncodeTiled f = fn.load(std::memory_order_acquire);
-  if (!f) {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult found;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) != cudaSuccess ||
-        found != cudaDriverEntryPointSuccess) {
-      cudaGetLastError();
-      return nullptr;
-    }
-    f = (EncodeTiled)p;
-    fn.store(f, std::memory_order_release);
-  }
-  return f;
-}
-// Rows of K bytes, `ld` bytes apart, in boxes of 128 bytes by `box` rows; zeros where a box reaches past the matrix.
-bool map_rows(CUtensorMap* m, const void* p, int64_t K, int64_t rows, int64_t ld, int box) {
-  const cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)ld};
-  const cuuint32_t boxes[2] = {(cuuint32_t)kMmStageK, (cuuint32_t)box}, ones[2] = {1, 1};
-  const EncodeTiled f = encode_tiled();
-  return f && f(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(p), dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-// Outputs [T, N] in boxes of 128 channels by the tokens of a box.
-bool map_outputs(CUtensorMap* m, void* p, int64_t N, int64_t T, int dtype, int box) {
-  const int size = dtype_size(dtype);
-  const cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)T}, strides[1] = {(cuuint64_t)(N * size)};
-  const cuuint32_t boxes[2] = {(cuuint32_t)kMmChannels, (cuuint32_t)box}, ones[2] = {1, 1};
-  const CUtensorMapDataType type = dtype == ACTNN_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                   : dtype == ACTNN_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const EncodeTiled f = encode_tiled();
-  return f && f(m, type, 2, p, dims, strides, boxes, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
-                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 // The cut: tokens of a tile, blocks that share a reduction, pairs or single blocks, by what they are expected to take (us): a
 // stage's bytes at what an SM gets from the L2 or its matrix instructions, the epilogue, and what a wave spends besides.  The
 // constants are fitted to times of all cuts for 16 to 16384 tokens, 500 to 16384 channels and reductions over 1000 to 8192, e.g.
@@ -488,8 +449,9 @@ int actnn::int8_matmul_impl(const int8_t* tokens, const float* token_scale, cons
   if ((N + kMmChannels - 1) / kMmChannels * ((T + 15) / 16) > 0x7fffffff) return ACTNN_ERR_SHAPE;
   plan(a);
   CUtensorMap w, x, y{};
-  if (a.boxes && !map_outputs(&y, out, N, T, dtype, kMmStaging / 4 / (kMmChannels * size))) return ACTNN_ERR_LAUNCH;
-  if (!map_rows(&w, weights, K, N, ld_weights, kMmChannels) || !map_rows(&x, tokens, K, T, ld_tokens, a.pair ? a.tokens / 2 : a.tokens)) return ACTNN_ERR_LAUNCH;
+  if (a.boxes && !map_values(&y, out, N, T, dtype, kMmChannels, kMmStaging / 4 / (kMmChannels * size))) return ACTNN_ERR_LAUNCH;
+  if (!map_bytes(&w, weights, K, N, ld_weights, kMmStageK, kMmChannels, true) ||
+      !map_bytes(&x, tokens, K, T, ld_tokens, kMmStageK, a.pair ? a.tokens / 2 : a.tokens, true)) return ACTNN_ERR_LAUNCH;
   switch (dtype) {
     case ACTNN_F32: return launch_typed<float>(w, x, y, a, (cudaStream_t)stream);
     case ACTNN_F16: return launch_typed<__half>(w, x, y, a, (cudaStream_t)stream);

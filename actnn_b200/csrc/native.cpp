@@ -459,6 +459,190 @@ NormForward norm_forward(const Tensor& x, int64_t groups, const OptTensor& weigh
   return r;
 }
 
+// ---------------------------------------------------------------------------------------- 8-bit floating point
+struct FpCodes { Tensor codes, scales; };                             // [rows, row_bytes(k)]; [ceil(k / 512), ceil(rows / 128), 512]
+FpCodes fp8_room(int64_t rows, int64_t k, const Tensor& like) {
+  return {make({rows, row_bytes(k)}, at::kByte, like), make({(k + 511) / 512, (rows + 127) / 128, 512}, at::kByte, like)};
+}
+uint8_t* bytes_of(const Tensor& t) { return t.defined() ? t.data_ptr<uint8_t>() : nullptr; }
+FpCodes fp8_row_codes(const Tensor& flat, int64_t rows, int64_t k, int64_t ldx) {
+  FpCodes r = fp8_room(rows, k, flat);
+  check(actnn_fp8_row_codes(flat.data_ptr(), bytes_of(r.codes), bytes_of(r.scales), rows, k, ldx, row_bytes(k), dtype_id(flat.scalar_type()),
+                            stream()),
+        "actnn_fp8_row_codes");
+  return r;
+}
+struct FpTiles { FpCodes here, there; Tensor parts; };
+FpTiles fp8_tile_codes(const Tensor& flat, int64_t rows, int64_t k, int64_t ldx, bool here, bool there, bool sums, bool square) {
+  FpTiles r;
+  if (here) r.here = fp8_room(rows, k, flat);
+  if (there) r.there = fp8_room(k, rows, flat);
+  if (sums) r.parts = make({(rows + 127) / 128, k}, at::kFloat, flat);
+  if (here || there || sums)
+    check(actnn_fp8_tile_codes(flat.data_ptr(), bytes_of(r.here.codes), bytes_of(r.here.scales), bytes_of(r.there.codes), bytes_of(r.there.scales),
+                               sums ? r.parts.data_ptr<float>() : nullptr, rows, k, ldx, row_bytes(k), row_bytes(rows), square,
+                               dtype_id(flat.scalar_type()), stream()),
+          "actnn_fp8_tile_codes");
+  return r;
+}
+Tensor fp8_join_sums(const Tensor& parts, at::ScalarType t) {
+  Tensor out = make({parts.size(1)}, t, parts);
+  check(actnn_fp8_join_sums(parts.data_ptr<float>(), out.data_ptr(), parts.size(0), parts.size(1), dtype_id(t), stream()), "actnn_fp8_join_sums");
+  return out;
+}
+// Of [rows, k] codes by [n, k] ones.
+void fp8_product(const FpCodes& x, const FpCodes& w, const Tensor& bias, Tensor& out, int64_t rows, int64_t n, int64_t k) {
+  check(actnn_fp8_matmul(bytes_of(x.codes), bytes_of(x.scales), bytes_of(w.codes), bytes_of(w.scales), bias.defined() ? bias.data_ptr() : nullptr,
+                         out.data_ptr(), rows, n, k, row_bytes(k), row_bytes(k), dtype_id(out.scalar_type()), stream()),
+        "actnn_fp8_matmul");
+}
+Tensor on16_bytes_of(const Tensor& t) {
+  Tensor c = t.contiguous();
+  return on16(c) ? c : c.clone();
+}
+
+Tensor fp8_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, const OptTensor& bias) {
+  check_values(x, "x");
+  TORCH_CHECK(codes.is_cuda(), "weight_codes must be a CUDA tensor!");
+  TORCH_CHECK(codes.scalar_type() == at::kFloat8_e4m3fn && scales.scalar_type() == at::kByte,
+              "The type of weight_codes is not correct! (float8_e4m3fn codes, uint8 scales)");
+  TORCH_CHECK(codes.dim() == 2 && scales.dim() == 3 && scales.size(0) == (codes.size(1) + 511) / 512 &&
+                  scales.size(1) == (codes.size(0) + 127) / 128 && scales.size(2) == 512, "The dimension of weight_codes is not correct!");
+  TORCH_CHECK(x.dim() >= 1 && x.size(-1) == codes.size(1), "shapes ", x.sizes(), " and ", codes.sizes(), " cannot be multiplied");
+  const int64_t n = codes.size(0), k = codes.size(1);
+  TORCH_CHECK(codes.device() == x.device() && scales.device() == x.device(), "the weight is on ", codes.device(), ", the tokens on ", x.device());
+  check_bias(bias, x, n);
+  c10::cuda::CUDAGuard guard(x.device());
+  Tensor out = make(with_last(x, n), x.scalar_type(), x);
+  const bool with = bias.has_value() && bias->defined();
+  const Tensor b = with ? bias->detach().to(x.scalar_type()).contiguous() : Tensor();
+  if (k == 0) return with ? out.copy_(b) : out.zero_();
+  const auto [flat, ldx] = as_rows(x);
+  const auto [w, ldw] = code_rows(codes.view(at::kByte));
+  const Tensor s = on16_bytes_of(scales);
+  const int64_t rows = x.numel() / k;
+  int64_t bytes = 0;
+  check(actnn_fp8_linear_workspace(rows, k, &bytes), "actnn_fp8_linear_workspace");
+  Tensor ws;
+  if (bytes) ws = make({bytes}, at::kByte, x);
+  check(actnn_fp8_linear(flat.data_ptr(), w.data_ptr<uint8_t>(), s.data_ptr<uint8_t>(), with ? b.data_ptr() : nullptr, out.data_ptr(), rows, n, k,
+                         ldx, ldw, dtype_id(x.scalar_type()), bytes ? ws.data_ptr() : nullptr, bytes, stream()),
+        "actnn_fp8_linear");
+  return out;
+}
+
+// ---------------------------------------------------------------------------------------- seeded dropout
+// A key as the kernels take it: numbers, or, while a stream is captured, two numbers on the device that every replay writes anew.
+struct Key { uint64_t seed = 0, offset = 0; Tensor state; };
+using OptKey = std::optional<std::pair<uint64_t, uint64_t>>;
+Key make_key(const OptKey& given, const Tensor& like) {
+  if (given.has_value()) return {given->first, given->second, Tensor()};
+  auto* gen = at::get_generator_or_default<at::CUDAGeneratorImpl>(std::nullopt, at::cuda::detail::getDefaultCUDAGenerator());
+  at::PhiloxCudaState st;
+  {
+    std::lock_guard<std::mutex> lock(gen->mutex_);
+    st = gen->philox_cuda_state(4);
+  }
+  if (!st.captured_) return {st.seed_.val, st.offset_.val, Tensor()};
+  Key k;
+  k.state = make({2}, at::kLong, like);
+  check(actnn_philox_state(st.seed_.ptr, st.offset_.ptr, st.offset_intragraph_, k.state.data_ptr<int64_t>(), stream()), "actnn_philox_state");
+  return k;
+}
+int64_t* state_of(const Key& k) { return k.state.defined() ? k.state.data_ptr<int64_t>() : nullptr; }
+void check_probability(double p) { TORCH_CHECK(p >= 0 && p < 1, "the dropout probability must be at least 0 and below 1, got ", p); }
+Tensor drop(const Tensor& x_in, double p, const Key& k) {
+  const Tensor x = on_16_bytes(x_in);
+  Tensor y = make(x.sizes(), x.scalar_type(), x);
+  check(actnn_seeded_dropout(x.data_ptr(), y.data_ptr(), x.numel(), (float)p, dtype_id(x.scalar_type()), k.seed, k.offset, state_of(k), stream()),
+        "actnn_seeded_dropout");
+  return y;
+}
+
+// ---------------------------------------------------------------------------------------- norms around a residual branch
+constexpr int64_t kMostChannels = 32768;
+Tensor given(const OptTensor& t) { return t.has_value() ? *t : Tensor(); }
+// What a call is about, its tensors contiguous.
+struct Residual {
+  Tensor weight, bias, post_weight, post_bias, gate;
+  int64_t rows, c, gate_rows;
+  double scale, p, eps;
+  int layer;
+  bool post;
+  at::ScalarType ptype, gtype;
+};
+Residual residual_of(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& post_weight, const Tensor& post_bias,
+                     const Tensor& gate, double scale, double p, double eps, int layer, bool post) {
+  check_probability(p);
+  const int64_t c = x.size(-1);
+  int64_t rows = 1;
+  for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+  TORCH_CHECK(c >= 1 && c <= kMostChannels, "a row has ", c, " channels; 1 to ", kMostChannels, " are accepted");
+  TORCH_CHECK(rows <= INT_MAX, rows, " rows are more than 2^31 - 1");
+  Residual r{weight, bias, post_weight, post_bias, gate, rows, c, std::max<int64_t>(rows, 1), scale, p, eps, layer, post, at::kFloat, x.scalar_type()};
+  Tensor* const params[] = {&r.weight, &r.bias, &r.post_weight, &r.post_bias};
+  constexpr const char* names[] = {"weight", "bias", "post_weight", "post_bias"};
+  bool mixed = false;
+  at::ScalarType type = at::kFloat;
+  bool any = false;
+  for (int i = 0; i < 4; ++i) {
+    const Tensor& q = *params[i];
+    if (!q.defined()) continue;
+    TORCH_CHECK(post || i < 2, names[i], " without the norm that it belongs to");
+    check_values(q, names[i]);
+    TORCH_CHECK(q.device() == x.device(), names[i], " is on ", q.device(), ", expected ", x.device());
+    TORCH_CHECK(q.dim() == 1 && q.size(0) == c, names[i], " must have one value for each of the ", c, " channels");
+    mixed = mixed || (any && q.scalar_type() != type);
+    type = q.scalar_type();
+    any = true;
+  }
+  r.ptype = mixed ? at::kFloat : type;
+  for (Tensor* q : params)
+    if (q->defined()) *q = q->detach().to(r.ptype).contiguous();
+  if (gate.defined()) {
+    check_values(gate, "gate");
+    TORCH_CHECK(gate.device() == x.device(), "gate is on ", gate.device(), ", expected ", x.device());
+    const int64_t lead = x.dim() - 1, missing = lead - (gate.dim() - 1);
+    bool ok = gate.dim() >= 1 && gate.size(-1) == c && missing >= 0;
+    int64_t j = 0, each = 1;
+    auto own = [&](int64_t i) { return i < missing ? 1 : gate.size(i - missing); };
+    while (ok && j < lead && own(j) == x.size(j)) ++j;
+    for (int64_t i = j; ok && i < lead; ++i) ok = own(i) == 1, each *= x.size(i);
+    TORCH_CHECK(ok, "a gate of shape ", gate.sizes(), " does not belong to rows of shape ", x.sizes(), ": it has the channels and before them "
+                "the leading dimensions up to some place");
+    r.gate_rows = std::max<int64_t>(each, 1);
+    r.gtype = gate.scalar_type();
+    r.gate = gate.detach().contiguous();
+  }
+  return r;
+}
+struct ResidualOut { Tensor r, h, cx, sx, cf, sf, stats; };
+ResidualOut residual_forward(const Tensor& x_in, const Tensor& f_in, const Residual& q, const Key& k, bool codes, bool stats) {
+  const Tensor x = x_in.contiguous(), f = f_in.contiguous();
+  ResidualOut o;
+  o.r = make(x.sizes(), x.scalar_type(), x);
+  o.h = make(x.sizes(), x.scalar_type(), x);
+  if (codes) {
+    const int64_t blocks = (q.c + 255) / 256;
+    o.cx = make({q.rows, q.c}, at::kChar, x), o.sx = make({q.rows, blocks}, at::kFloat, x);
+    o.cf = make({q.rows, q.c}, at::kChar, x), o.sf = make({q.rows, blocks}, at::kFloat, x);
+  }
+  if (stats) o.stats = make({q.rows, 4}, at::kFloat, x);
+  auto data = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+  check(actnn_residual_norm_forward(x.data_ptr(), f.data_ptr(), data(q.weight), data(q.bias), data(q.post_weight), data(q.post_bias), data(q.gate),
+                                    o.r.data_ptr(), o.h.data_ptr(), (int8_t*)data(o.cx), (int8_t*)data(o.cf), (float*)data(o.sx), (float*)data(o.sf),
+                                    (float*)data(o.stats), q.rows, q.c, q.gate_rows, q.scale, q.eps, q.layer, q.post, (float)q.p,
+                                    dtype_id(x.scalar_type()), dtype_id(q.ptype), dtype_id(q.gtype), k.seed, k.offset, state_of(k), stream()),
+        "actnn_residual_norm_forward");
+  return o;
+}
+void check_pair(const Tensor& x, const Tensor& f) {
+  check_values(x, "x");
+  check_values(f, "branch");
+  TORCH_CHECK(f.device() == x.device(), "branch is on ", f.device(), ", expected ", x.device());
+  TORCH_CHECK(x.dim() >= 1 && x.sizes() == f.sizes(), "x and branch must have the same shape of at least one dimension, got ", x.sizes(), " and ", f.sizes());
+}
+
 // with_minmax: also min and max of every 256 outputs, not differentiable
 struct Relu : torch::autograd::Function<Relu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, bool with_minmax) {
@@ -672,6 +856,155 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
   }
 };
 
+// x, weight, bias -> x weight^T + bias in 8-bit floating point.  Kept are the codes that the gradients multiply: those of x along the
+// tokens, those of the weight along the output channels, and of these only what a gradient asked for needs.
+struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+    check_values(x, "x");
+    check_values(weight, "weight");
+    TORCH_CHECK(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "shapes ", x.sizes(), " and ", weight.sizes(),
+                " cannot be multiplied");
+    TORCH_CHECK(weight.device() == x.device(), "the weight is on ", weight.device(), ", the tokens on ", x.device());
+    const int64_t n = weight.size(0), k = weight.size(1);
+    check_bias(bias, x, n);
+    const bool with = bias.has_value() && bias->defined();
+    c10::cuda::CUDAGuard guard(x.device());
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+    const bool keep_x = weight.requires_grad(), keep_w = x.requires_grad();
+    Tensor out = make(with_last(x, n), x.scalar_type(), x);
+    const Tensor b = with ? bias->to(x.scalar_type()).contiguous() : Tensor();
+    FpTiles cx, cw;
+    if (k == 0 || rows == 0 || n == 0) {
+      with ? out.copy_(b) : out.zero_();
+    } else {
+      const auto [fx, ldx] = as_rows(x);
+      const auto [fw, ldw] = as_rows(weight);
+      if (keep_x) cx = fp8_tile_codes(fx, rows, k, ldx, true, true, false, false);
+      else cx.here = fp8_row_codes(fx, rows, k, ldx);
+      cw = fp8_tile_codes(fw, n, k, ldw, true, keep_w, false, true);
+      fp8_product(cx.here, cw.here, b, out, rows, n, k);
+    }
+    ctx->save_for_backward({cx.there.codes, cx.there.scales, cw.there.codes, cw.there.scales});
+    ctx->saved_data["sizes"] = x.sizes();
+    ctx->saved_data["n"] = n;
+    ctx->saved_data["x"] = x.scalar_type();
+    ctx->saved_data["w"] = weight.scalar_type();
+    ctx->saved_data["b"] = with ? (int64_t)bias->scalar_type() : (int64_t)-1;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const std::vector<int64_t> sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t k = sizes.back(), n = ctx->saved_data["n"].toInt();
+    int64_t rows = 1;
+    for (size_t i = 0; i + 1 < sizes.size(); ++i) rows *= sizes[i];
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    const Tensor go = grads[0].reshape({rows, n});
+    const int64_t bias_type = ctx->saved_data["b"].toInt();
+    const bool want_x = ctx->needs_input_grad(0), want_w = ctx->needs_input_grad(1), want_b = bias_type >= 0 && ctx->needs_input_grad(2);
+    Tensor gx, gw, gb;
+    if (want_x) gx = make(sizes, ctx->saved_data["x"].toScalarType(), go);
+    if (want_w) gw = make({n, k}, ctx->saved_data["w"].toScalarType(), go);
+    if (k == 0 || rows == 0 || n == 0) {
+      if (want_x) gx.zero_();
+      if (want_w) gw.zero_();
+      if (want_b) gb = go.sum(0).to((at::ScalarType)bias_type);
+      return {gx, gw, gb};
+    }
+    const auto [flat, ld] = as_rows(go);
+    const FpTiles c = fp8_tile_codes(flat, rows, n, ld, want_x, want_w, want_b, false);
+    if (want_x) fp8_product(c.here, {saved[2], saved[3]}, Tensor(), gx, rows, k, n);
+    if (want_w) fp8_product(c.there, {saved[0], saved[1]}, Tensor(), gw, n, k, rows);
+    if (want_b) gb = fp8_join_sums(c.parts, (at::ScalarType)bias_type);
+    return {gx, gw, gb};
+  }
+};
+
+void save_key(AutogradContext* ctx, const Key& k) {
+  ctx->saved_data["seed"] = (int64_t)k.seed;
+  ctx->saved_data["offset"] = (int64_t)k.offset;
+}
+Key saved_key(AutogradContext* ctx, const Tensor& state) {
+  return {(uint64_t)ctx->saved_data["seed"].toInt(), (uint64_t)ctx->saved_data["offset"].toInt(), state};
+}
+
+// Nothing of an element is kept.
+struct SeededDropout : torch::autograd::Function<SeededDropout> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, double p, const OptKey& key) {
+    check_values(x, "x");
+    check_probability(p);
+    c10::cuda::CUDAGuard guard(x.device());
+    const Key k = make_key(key, x);
+    save_key(ctx, k);
+    ctx->saved_data["p"] = p;
+    ctx->save_for_backward({k.state});
+    return drop(x, p, k);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    c10::cuda::CUDAGuard guard(grads[0].device());
+    return {drop(grads[0], ctx->saved_data["p"].toDouble(), saved_key(ctx, ctx->get_saved_variables()[0])), Tensor(), Tensor()};
+  }
+};
+
+// (r, h) of the residual stream x and a block's output; `compress` false: both are kept as they are.
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& f, const OptTensor& weight, const OptTensor& bias,
+                               const OptTensor& post_weight, const OptTensor& post_bias, const OptTensor& gate, double scale, double p, double eps,
+                               int64_t layer, bool post, const OptKey& key, bool compress) {
+    c10::cuda::CUDAGuard guard(x.device());
+    const Residual q = residual_of(x, given(weight), given(bias), given(post_weight), given(post_bias), given(gate), scale, p, eps, (int)layer, post);
+    const Key k = p > 0 ? make_key(key, x) : Key{};
+    const ResidualOut o = residual_forward(x, f, q, k, compress, true);
+    ctx->set_materialize_grads(false);
+    save_key(ctx, k);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["layer"] = layer;
+    ctx->saved_data["post"] = post;
+    ctx->saved_data["compress"] = compress;
+    ctx->save_for_backward({compress ? o.cx : x, compress ? o.cf : f, o.sx, o.sf, o.stats, k.state, given(weight), given(bias), given(post_weight),
+                            given(post_bias), given(gate)});
+    return {o.r, o.h};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    variable_list out(14);
+    if (!grads[0].defined() && !grads[1].defined()) return out;
+    const auto s = ctx->get_saved_variables();
+    const Tensor& any = grads[0].defined() ? grads[0] : grads[1];
+    c10::cuda::CUDAGuard guard(any.device());
+    const bool compress = ctx->saved_data["compress"].toBool();
+    const Residual q = residual_of(any, s[6], s[7], s[8], s[9], s[10], ctx->saved_data["scale"].toDouble(), ctx->saved_data["p"].toDouble(), 0.,
+                                   (int)ctx->saved_data["layer"].toInt(), ctx->saved_data["post"].toBool());
+    const Key k = saved_key(ctx, s[5]);
+    const Tensor dr = grads[0].defined() ? grads[0].contiguous() : Tensor(), dh = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    const Tensor x = compress ? Tensor() : s[0].contiguous(), f = compress ? Tensor() : s[1].contiguous();
+    size_t at = 2;                                                     // of needs_input_grad, which counts tensors that are there
+    if (ctx->needs_input_grad(0)) out[0] = make(any.sizes(), any.scalar_type(), any);
+    if (ctx->needs_input_grad(1)) out[1] = make(any.sizes(), any.scalar_type(), any);
+    for (int i = 0; i < 5; ++i)
+      if (s[6 + i].defined() && ctx->needs_input_grad(at++)) out[2 + i] = make(s[6 + i].sizes(), i < 4 ? q.ptype : q.gtype, any);
+    if (q.rows == 0) {
+      for (Tensor& g : out) if (g.defined()) g.zero_();
+    } else {
+      int64_t bytes = 0;
+      check(actnn_residual_norm_workspace(q.rows, q.c, q.gate_rows, out[6].defined(), &bytes), "actnn_residual_norm_workspace");
+      const Tensor ws = make({bytes}, at::kByte, any);
+      auto data = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      check(actnn_residual_norm_backward(data(dr), data(dh), data(x), data(f), compress ? (int8_t*)data(s[0]) : nullptr,
+                                         compress ? (int8_t*)data(s[1]) : nullptr, (float*)data(s[2]), (float*)data(s[3]), (float*)data(s[4]),
+                                         data(q.weight), data(q.post_weight), data(q.post_bias), data(q.gate), data(out[0]), data(out[1]), data(out[2]),
+                                         data(out[3]), data(out[4]), data(out[5]), data(out[6]), q.rows, q.c, q.gate_rows, q.scale, q.layer, q.post,
+                                         (float)q.p, dtype_id(any.scalar_type()), dtype_id(q.ptype), dtype_id(q.gtype), k.seed, k.offset, state_of(k),
+                                         ws.data_ptr(), bytes, stream()),
+            "actnn_residual_norm_backward");
+    }
+    for (int i = 0; i < 4; ++i)
+      if (out[2 + i].defined()) out[2 + i] = out[2 + i].to(s[6 + i].scalar_type());
+    return out;
+  }
+};
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -695,6 +1028,27 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("group_norm_value", [](const Tensor& x, int64_t groups, const OptTensor& w, const OptTensor& b, double eps,
                                const std::string& name) {
     return norm_forward(x, groups, w, b, eps, activation_kind(name), false, false).y;
+  });
+  m.def("fp8_linear", &fp8_linear);
+  m.def("fp8_linear_train", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return Fp8Linear::apply(x, w, b); });
+  m.def("seeded_dropout", [](const Tensor& x, double p, const OptKey& key) { return SeededDropout::apply(x, p, key); });
+  m.def("residual_norm", [](const Tensor& x, const Tensor& f, const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
+                            const OptTensor& post_bias, const OptTensor& gate, double scale, double p, double eps, int64_t layer, bool post,
+                            const OptKey& key, bool compress) {
+    check_pair(x, f);
+    TORCH_CHECK(x.scalar_type() == f.scalar_type(), "x and branch must have the same type");
+    const variable_list o = ResidualNorm::apply(x, f, weight, bias, post_weight, post_bias, gate, scale, p, eps, layer, post, key, compress);
+    return py::make_tuple(o[0], o[1]);
+  });
+  m.def("residual_norm_value", [](const Tensor& x, const Tensor& f, const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
+                                  const OptTensor& post_bias, const OptTensor& gate, double scale, double p, double eps, int64_t layer, bool post,
+                                  const OptKey& key) {
+    check_pair(x, f);
+    TORCH_CHECK(x.scalar_type() == f.scalar_type(), "x and branch must have the same type");
+    c10::cuda::CUDAGuard guard(x.device());
+    const Residual q = residual_of(x, given(weight), given(bias), given(post_weight), given(post_bias), given(gate), scale, p, eps, (int)layer, post);
+    const ResidualOut o = residual_forward(x.detach(), f.detach(), q, p > 0 ? make_key(key, x) : Key{}, false, false);
+    return py::make_tuple(o.r, o.h);
   });
   m.def("relu", [](const Tensor& x) { return Relu::apply(x, false)[0]; });
   m.def("relu_minmax", [](const Tensor& x) { return Relu::apply(x, true); });

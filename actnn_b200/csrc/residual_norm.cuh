@@ -1,0 +1,627 @@
+// The norms before and after a block with its gate and residual scale, on rows of C channels:
+//
+//   u = (f - m1) p1 w1 + b1        the block's output f, normalised (or as it is)
+//   d = keep u / (1 - p)           dropout (dropout.cuh)
+//   r = s x + g d                  the residual stream x, scaled, and what passes the gate
+//   h = (r - m2) p2 w2 + b2        what the next block reads
+//
+// m, p: mean and reciprocal deviation of the row, sqrt(mean((v - m)^2) + eps); the rms kind has m = 0.  What the backward pass
+// keeps are the inputs x and f in 8 bits, a scale for 256 channels of a row, and the four statistics: codes of inputs follow from
+// exact numbers, those of r would move with the last bit of a sum.  With n1, n2 the normalised values made of the decoded inputs:
+//
+//   dn2 = dh w2      c = dr + p2 dn2      t = c - p2 (mean dn2 + n2 mean(dn2 n2))      dx = s t      dg = sum t d
+//   du = keep g t / (1 - p)      dn1 = du w1      df = p1 (dn1 - mean dn1 - n1 mean(dn1 n1))
+//   dw2 = sum dh n2, db2 = sum dh, dw1 = sum du n1, db1 = sum du   over the rows
+//
+// With a = keep g w1 / (1 - p), dn1 is a t, so that the means of the second norm's gradient follow from sums that do not wait for
+// those of the first: mean(dn1 n1) = (sum a c n1 - p2 mean dn2 sum a n1 - p2 mean(dn2 n2) sum a n1 n2) / C.  A row takes one
+// joint reduction, not two.
+#pragma once
+
+#include "cluster.cuh"
+#include "dropout.cuh"
+
+namespace actnn {
+
+constexpr int kRnBlock = 256;                          // channels that share a scale
+constexpr int kRnMostC = 32768;
+constexpr int kRnThreads = 256;                        // of the kernels that give a warp a row
+constexpr int kRnMostThreads = 512, kRnMostCluster = 8;          // of the backward pass: eight channels a thread
+
+struct RnArgs {
+  const void *x, *f;                                   // forward; backward where no codes were kept
+  const void *dr, *dh;                                 // gradients, NULL: zero
+  const void *w1, *b1, *w2, *b2, *gate;                // NULL: ones, zeros
+  void *r, *h, *dx, *df;                               // dx, df NULL: not wanted
+  int8_t *cx, *cf;                                     // codes [rows, C], NULL: none
+  float *sx, *sf;                                      // their scales [rows, ceil(C / 256)]
+  float4* stats;                                       // [rows]: m1, p1, m2, p2
+  float* parts;                                        // [runs][slots][C], backward: partial sums of the parameters' gradients
+  void *dw2, *db2, *dw1, *db1, *dgate;                 // the parameters' gradients
+  uint32_t rows;
+  int C, blocks;                                       // blocks: scales a row
+  float scale, eps, inv_c;
+  int pdtype, gdtype;                                  // types of the parameters and of the gate
+  bool pvec;                                           // vectors of both are aligned
+  bool layer, post, dropped;
+  FastDiv by_gate;                                     // rows of a gate
+  DropKey drop;
+  // the runs of rows of the backward pass
+  int cluster;                                                  // blocks that share a row
+  int slots, slot_w2, slot_b2, slot_w1, slot_b1, slot_gate;     // -1: not wanted
+  uint32_t unit_rows, units;                                    // rows whose sums belong together: those of a gate where its gradient is wanted, else all
+  uint32_t runs_of_unit, units_of_run, runs;                    // units_of_run > 0: a run is so many whole units, else a part of one
+  bool coded;                                                   // backward: of codes, else of x and f
+  cudaStream_t stream;
+};
+enum RnWhat { kRnForward, kRnBackward };
+int rn_run_f32(const RnArgs& a, RnWhat what, bool vec);
+int rn_run_f16(const RnArgs& a, RnWhat what, bool vec);
+int rn_run_bf16(const RnArgs& a, RnWhat what, bool vec);
+
+#ifdef __CUDACC__
+// Loads that happen where they stand: of pointers that may be NULL, and of rows that a loop may not reach.
+ACTNN_DEV float rn_ld(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+ACTNN_DEV float2 rn_ld(const float2* p) {
+  float2 v;
+  asm volatile("ld.global.nc.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+  return v;
+}
+ACTNN_DEV float4 rn_ld(const float4* p) {
+  float4 v;
+  asm volatile("ld.global.nc.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p));
+  return v;
+}
+ACTNN_DEV uint4 rn_ld(const uint4* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+// ------------------------------------------------------------------ eight channels of a thread
+// Elements from `c` on, zero behind C.
+template <typename T, bool VEC> ACTNN_DEV Vec<T, 8> rn_load(const T* row, int c, int C) {
+  Vec<T, 8> v;
+  if (VEC && c < C) return load_vec<T, 8>(row + c);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && c + i < C ? __ldg(row + c + i) : from_float<T>(0.f);
+  return v;
+}
+template <typename T, bool VEC> ACTNN_DEV void rn_store(T* row, int c, int C, const float2 (&f)[4]) {
+  if constexpr (VEC) {
+    if (c < C) store_vec<T, 8>(row + c, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < C) row[c + i] = from_float<T>(i & 1 ? f[i / 2].y : f[i / 2].x);
+  }
+}
+template <bool VEC> ACTNN_DEV Codes<8> rn_load_codes(const int8_t* row, int c, int C) {
+  Codes<8> r;
+  r.w[0] = r.w[1] = 0;
+  if constexpr (VEC) {
+    if (c < C) r = load_codes<8>(row + c);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < C) r.w[i / 4] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(row) + c + i) << (8 * (i % 4));
+  }
+  return r;
+}
+template <bool VEC> ACTNN_DEV void rn_store_codes(int8_t* row, int c, int C, const float2 (&f)[4]) {
+  if constexpr (VEC) {
+    if (c < C) store_codes<8>(row + c, f);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < C) row[c + i] = (int8_t)__float_as_uint(i & 1 ? f[i / 2].y : f[i / 2].x);
+  }
+}
+// A parameter's values, of any of the three types; through the L1, every row reads them again.
+template <typename P> ACTNN_DEV void rn_parameter(const P* p, int c, int C, bool vec, float2 (&f)[4]) {
+  if (vec) {
+    Vec<P, 8> v;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(P) / 2; ++i) {
+      const uint4 q = c < C ? rn_ld(reinterpret_cast<const uint4*>(p + c) + i) : make_uint4(0, 0, 0, 0);
+      v.w[4 * i] = q.x, v.w[4 * i + 1] = q.y, v.w[4 * i + 2] = q.z, v.w[4 * i + 3] = q.w;
+    }
+    unpack_vec(v, f);
+  } else {
+    float e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = c + i < C ? to_float(__ldg(p + c + i)) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(e[2 * i], e[2 * i + 1]);
+  }
+}
+ACTNN_DEV void rn_parameter(const void* p, int dtype, int c, int C, bool vec, float none, float2 (&f)[4]) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = make_float2(none, none);
+  } else if (dtype == ACTNN_F32) {
+    rn_parameter((const float*)p, c, C, vec, f);
+  } else if (dtype == ACTNN_F16) {
+    rn_parameter((const __half*)p, c, C, vec, f);
+  } else {
+    rn_parameter((const __nv_bfloat16*)p, c, C, vec, f);
+  }
+}
+ACTNN_DEV const void* rn_gate_row(const RnArgs& a, uint32_t row) {
+  if (!a.gate) return nullptr;
+  return (const char*)a.gate + (size_t)fast_div(row, a.by_gate) * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
+}
+// What dropout multiplies the eight channels from `c` of a row by.  Where C is no multiple of eight they belong to two calls.
+template <bool VEC> ACTNN_DEV void rn_factors(const RnArgs& a, const NoiseKey& key, uint32_t row, int c, float2 (&m)[4]) {
+  const uint64_t e = (uint64_t)row * a.C + c;
+  const Philox4 r = noise_call(key, e >> 3);
+  if (VEC) return drop_factors(r, a.drop.least, a.drop.inv, m);
+  const Philox4 q = noise_call(key, (e >> 3) + 1);
+  float k[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t at = (uint32_t)(e & 7) + i, j = at & 7;
+    const uint32_t lo = j & 4 ? (j & 2 ? r.v[3] : r.v[2]) : (j & 2 ? r.v[1] : r.v[0]);
+    const uint32_t hi = j & 4 ? (j & 2 ? q.v[3] : q.v[2]) : (j & 2 ? q.v[1] : q.v[0]);
+    const uint32_t word = at < 8 ? lo : hi;
+    k[i] = (j & 1 ? word : word << 16) >= a.drop.least ? a.drop.inv : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = make_float2(k[2 * i], k[2 * i + 1]);
+}
+// m times v; a dropped element is zero whatever it was.
+ACTNN_DEV float2 rn_drop(float2 v, float2 m) {
+  const float2 y = f_mul(v, m);
+  return make_float2(m.x != 0.f ? y.x : 0.f, m.y != 0.f ? y.y : 0.f);
+}
+
+// ------------------------------------------------------------------ sums over the threads of a row
+template <int N> struct Sums { float v[N]; };
+// WARP: a warp has the row.  Otherwise the block has it, and `place` counts its reductions: two are never under way at a time, so two
+// places suffice.
+template <int N, bool WARP> ACTNN_DEV Sums<N> rn_sum(Sums<N> s, int place) {
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s.v[i] += __shfl_xor_sync(kFull, s.v[i], o);
+  if constexpr (!WARP) {
+    __shared__ Sums<N> part_s[2][16];
+    const int warps = blockDim.x >> 5;
+    if ((threadIdx.x & 31) == 0) part_s[place & 1][threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = part_s[place & 1][0];
+    for (int w = 1; w < warps; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) s.v[i] += part_s[place & 1][w].v[i];
+    }
+  }
+  return s;
+}
+// Mean (of the layer kind) and reciprocal deviation of a row.
+template <int V, bool WARP> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int lane, int lanes, const RnArgs& a, int& place) {
+  float mean = 0.f;
+  if (a.layer) {
+    float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = f_add(s, v[k][i]);      // zero behind C
+    mean = rn_sum<1, WARP>({{f_sum(s)}}, place++).v[0] * a.inv_c;
+  }
+  float2 s = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * lanes + lane) * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 e = make_float2(c + 2 * i < a.C ? v[k][i].x - mean : 0.f, c + 2 * i + 1 < a.C ? v[k][i].y - mean : 0.f);
+      s = f_fma(e, e, s);
+    }
+  }
+  return make_float2(mean, rsqrtf(rn_sum<1, WARP>({{f_sum(s)}}, place++).v[0] * a.inv_c + a.eps));
+}
+
+// ------------------------------------------------------------------ forward
+template <typename T, int V, bool WARP, bool VEC>
+__global__ void __launch_bounds__(WARP ? kRnThreads : 512) rn_forward_kernel(const __grid_constant__ RnArgs a) {
+  const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
+  const uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  if (WARP && row >= a.rows) return;
+  const size_t at = (size_t)row * a.C;
+  Vec<T, 8> xv[V], fv[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) fv[k] = rn_load<T, VEC>((const T*)a.f + at, (k * lanes + lane) * 8, a.C);
+#pragma unroll
+  for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>((const T*)a.x + at, (k * lanes + lane) * 8, a.C);
+  if (a.cx) {
+    // a warp's vectors are 256 channels that share a scale
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * lanes + lane) * 8, first = (k * lanes + (lane & ~31)) * 8;
+      if (first >= a.C) continue;
+      auto code = [&](const Vec<T, 8>& v, int8_t* codes, float* scales) {
+        const float most = largest(__reduce_max_sync(kFull, most_of(v))), factor = code_factor(most);
+        float2 q[4];
+        unpack_vec(v, q);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) q[i] = code_bits(q[i], make_float2(factor, factor));
+        rn_store_codes<VEC>(codes + at, c, a.C, q);
+        if ((threadIdx.x & 31) == 0) scales[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
+      };
+      code(fv[k], a.cf, a.sf);
+      code(xv[k], a.cx, a.sx);
+    }
+  }
+  float2 u[V][4];
+#pragma unroll
+  for (int k = 0; k < V; ++k) unpack_vec(fv[k], u[k]);
+  int place = 0;
+  const float2 one = a.post ? rn_statistics<V, WARP>(u, lane, lanes, a, place) : make_float2(0.f, 1.f);
+  NoiseKey key;
+  if (a.dropped) key = drop_key(a.drop);
+  const void* gate = rn_gate_row(a, row);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * lanes + lane) * 8;
+    float2 w[4], b[4], g[4], x[4];
+    unpack_vec(xv[k], x);
+    if (c < a.C) {
+      if (a.post) {
+        rn_parameter(a.w1, a.pdtype, c, a.C, a.pvec, 1.f, w);
+        rn_parameter(a.b1, a.pdtype, c, a.C, a.pvec, 0.f, b);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          u[k][i] = f_fma(f_mul(f_add(u[k][i], make_float2(-one.x, -one.x)), make_float2(one.y, one.y)), w[i], b[i]);
+      }
+      if (a.dropped) {
+        float2 m[4];
+        rn_factors<VEC>(a, key, row, c, m);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[k][i] = rn_drop(u[k][i], m[i]);
+      }
+      rn_parameter(gate, a.gdtype, c, a.C, a.pvec, 1.f, g);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[k][i] = f_fma(u[k][i], g[i], f_mul(x[i], make_float2(a.scale, a.scale)));
+      rn_store<T, VEC>((T*)a.r + at, c, a.C, u[k]);
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
+      }
+    }
+  }
+  const float2 two = rn_statistics<V, WARP>(u, lane, lanes, a, place);
+  if (a.stats && lane == 0) a.stats[row] = make_float4(one.x, one.y, two.x, two.y);
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    const int c = (k * lanes + lane) * 8;
+    if (c >= a.C) continue;
+    float2 w[4], b[4];
+    rn_parameter(a.w2, a.pdtype, c, a.C, a.pvec, 1.f, w);
+    rn_parameter(a.b2, a.pdtype, c, a.C, a.pvec, 0.f, b);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) u[k][i] = f_fma(f_mul(f_add(u[k][i], make_float2(-two.x, -two.x)), make_float2(two.y, two.y)), w[i], b[i]);
+    rn_store<T, VEC>((T*)a.h + at, c, a.C, u[k]);
+  }
+}
+
+// ------------------------------------------------------------------ backward
+// What the backward pass reads of eight channels of a row, as it lies in memory.
+template <typename T, bool CODED> struct RnRaw {
+  Vec<T, 8> dr, dh, x, f;
+};
+template <typename T> struct RnRaw<T, true> {
+  Vec<T, 8> dr, dh;
+  Codes<8> x, f;
+  float sx, sf;
+};
+template <typename T, bool CODED, bool VEC> ACTNN_DEV void rn_load_raw(RnRaw<T, CODED>& v, const RnArgs& a, uint32_t row, int c) {
+  const size_t at = (size_t)row * a.C;
+  const int C = a.C;
+  v.dr = rn_load<T, VEC>((const T*)a.dr + at, a.dr ? c : C, C);
+  v.dh = rn_load<T, VEC>((const T*)a.dh + at, a.dh ? c : C, C);
+  if constexpr (CODED) {
+    v.x = rn_load_codes<VEC>(a.cx + at, c, C);
+    v.f = rn_load_codes<VEC>(a.cf + at, c, C);
+    v.sx = v.sf = 0.f;
+    if (c < C) {
+      const size_t s = (size_t)row * a.blocks + c / kRnBlock;
+      v.sx = rn_ld(a.sx + s);
+      v.sf = rn_ld(a.sf + s);
+    }
+  } else {
+    v.x = rn_load<T, VEC>((const T*)a.x + at, c, C);
+    v.f = rn_load<T, VEC>((const T*)a.f + at, c, C);
+  }
+}
+template <typename T, bool CODED> ACTNN_DEV void rn_inputs(const RnRaw<T, CODED>& v, float2 (&x)[4], float2 (&f)[4]) {
+  if constexpr (CODED) {
+    unpack_codes(v.x, x);
+    unpack_codes(v.f, f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] = f_mul(x[i], make_float2(v.sx, v.sx)), f[i] = f_mul(f[i], make_float2(v.sf, v.sf));
+  } else {
+    unpack_vec(v.x, x);
+    unpack_vec(v.f, f);
+  }
+}
+ACTNN_DEV void rn_store_any(void* p, int dtype, size_t at, float v) {
+  if (dtype == ACTNN_F32) ((float*)p)[at] = v;
+  else if (dtype == ACTNN_F16) ((__half*)p)[at] = __float2half_rn(v);
+  else ((__nv_bfloat16*)p)[at] = __float2bfloat16_rn(v);
+}
+ACTNN_DEV void rn_store_eight(void* p, int dtype, size_t row, int c, int C, const float2 (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (c + 2 * i < C) rn_store_any(p, dtype, row + c + 2 * i, v[i].x);
+    if (c + 2 * i + 1 < C) rn_store_any(p, dtype, row + c + 2 * i + 1, v[i].y);
+  }
+}
+
+// N sums (4 or 8) over the lanes of a warp: halves of the sums are exchanged with halves of the lanes, so that 4 take 6 shuffles and
+// 8 take 9.  Returned is the sum whose number the lane's upper bits are.
+template <int N> ACTNN_DEV float rn_warp_sums(float (&v)[N]) {
+  const int lane = threadIdx.x & 31;
+  int o = 16;
+#pragma unroll
+  for (int n = N / 2; n >= 1; n /= 2, o /= 2) {
+    const bool upper = lane & o;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      const float give = upper ? v[i] : v[n + i], keep = upper ? v[n + i] : v[i];
+      v[i] = keep + __shfl_xor_sync(kFull, give, o);
+    }
+  }
+  float s = v[0];
+#pragma unroll
+  for (; o >= 1; o /= 2) s += __shfl_xor_sync(kFull, s, o);
+  return s;
+}
+
+// A run of rows by a block, or by a cluster of blocks of 4096 channels each.  A thread has eight channels of every row and keeps the sums of
+// their parameters' gradients; the next row's values are requested as soon as this row's are unpacked.  The warps' sums of a row go to
+// shared memory (of every block of the cluster), a barrier, and each warp joins them for itself: two places in turn, so that
+// one barrier a row is enough.  Parameters lie in shared memory as float32, a thread's own.
+template <typename T, bool VEC, bool CODED, bool LAYER>
+__global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a) {
+  constexpr int N = LAYER ? 8 : 4, kWarps = kRnMostThreads / 32;
+  extern __shared__ float4 parameters_s[];              // [w1, w2, gate, b1][half][thread]
+  __shared__ float part_s[2][kRnMostCluster * kWarps][N];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
+  const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0, run = blockIdx.x / a.cluster;
+  const int c = ((int)rank * threads + (int)threadIdx.x) * 8, C = a.C, entries = a.cluster * warps;
+  uint32_t row, end, unit = 0, left = 0;                // left: rows of the unit, where the run has whole ones
+  if (a.units_of_run) {
+    unit = run * a.units_of_run;
+    row = unit * a.unit_rows;
+    end = min(a.units, unit + a.units_of_run) * a.unit_rows;
+    left = a.unit_rows;
+  } else {
+    const uint32_t u = run / a.runs_of_unit, k = run - u * a.runs_of_unit;
+    row = u * a.unit_rows + (uint32_t)((uint64_t)k * a.unit_rows / a.runs_of_unit);
+    end = u * a.unit_rows + (uint32_t)((uint64_t)(k + 1) * a.unit_rows / a.runs_of_unit);
+  }
+  auto put = [&](int set, const float2 (&v)[4]) {
+    parameters_s[(2 * set) * threads + threadIdx.x] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+    parameters_s[(2 * set + 1) * threads + threadIdx.x] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+  };
+  auto get = [&](int set, float2 (&v)[4]) {
+    const float4 p = parameters_s[(2 * set) * threads + threadIdx.x], q = parameters_s[(2 * set + 1) * threads + threadIdx.x];
+    v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
+  };
+  {
+    float2 v[4];
+    rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, v), put(0, v);
+    rn_parameter(a.w2, a.pdtype, c, C, a.pvec, 1.f, v), put(1, v);
+    if (LAYER) rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, v), put(3, v);
+  }
+  if (a.cluster > 1) cluster_sync();                    // the others' shared memory is there
+  uint32_t gate_of = 0xffffffffu;
+  NoiseKey key;
+  if (a.dropped) key = drop_key(a.drop);
+  float2 dw2[4] = {}, dw1[4] = {}, dg[4] = {}, db2[4] = {}, db1[4] = {};
+  RnRaw<T, CODED> raw;
+  float4 st = make_float4(0.f, 0.f, 0.f, 0.f), next_st = st;
+  if (row < end) {
+    rn_load_raw<T, CODED, VEC>(raw, a, row, c);
+    next_st = rn_ld(a.stats + row);
+  }
+  for (int place = 0; row < end; ++row, place ^= 1) {
+    st = next_st;
+    if (const uint32_t g = fast_div(row, a.by_gate); g != gate_of) {
+      float2 v[4];
+      rn_parameter(rn_gate_row(a, row), a.gdtype, c, C, a.pvec, 1.f, v), put(2, v);
+      gate_of = g;
+    }
+    float2 n1[4], n2[4], x[4], dn[4], cc[4];            // dn: dh, then d;  cc: dr + p2 dn2
+    rn_inputs<T, CODED>(raw, x, n1);
+    unpack_vec(raw.dr, cc);
+    unpack_vec(raw.dh, dn);
+    if (row + 1 < end) {
+      rn_load_raw<T, CODED, VEC>(raw, a, row + 1, c);
+      next_st = rn_ld(a.stats + row + 1);
+    }
+    float2 q[4], w1[4];
+    get(2, q);
+    get(0, w1);
+    float2 s0{}, s1{}, s2{}, s3{}, s4{}, s5{}, s6{}, s7{};
+    {
+      float2 w2[4], b1[4], m[4];
+      get(1, w2);
+      if (LAYER) get(3, b1);
+      if (a.dropped) rn_factors<VEC>(a, key, row, c, m);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (LAYER) n1[i] = f_add(n1[i], make_float2(-st.x, -st.x));
+        n1[i] = f_mul(n1[i], make_float2(st.y, st.y));
+        float2 d = a.post ? (LAYER ? f_fma(n1[i], w1[i], b1[i]) : f_mul(n1[i], w1[i])) : n1[i];
+        if (a.dropped) d = rn_drop(d, m[i]);
+        n2[i] = f_fma(d, q[i], f_mul(x[i], make_float2(a.scale, a.scale)));
+        if (LAYER) n2[i] = f_add(n2[i], make_float2(-st.z, -st.z));
+        n2[i] = f_mul(n2[i], make_float2(st.w, st.w));
+        if (a.dropped) q[i] = rn_drop(q[i], m[i]);
+        if constexpr (!VEC) {                            // nothing behind C
+          const bool in0 = c + 2 * i < C, in1 = c + 2 * i + 1 < C;
+          auto only = [&](float2& p) { p = make_float2(in0 ? p.x : 0.f, in1 ? p.y : 0.f); };
+          only(n1[i]), only(n2[i]), only(d), only(q[i]);
+        } else if (c >= C) {
+          n1[i] = n2[i] = d = q[i] = make_float2(0.f, 0.f);
+        }
+        const float2 dn2 = f_mul(dn[i], w2[i]);
+        cc[i] = f_fma(make_float2(st.w, st.w), dn2, cc[i]);
+        dw2[i] = f_fma(dn[i], n2[i], dw2[i]);
+        if (LAYER) db2[i] = f_add(db2[i], dn[i]);
+        dn[i] = d;
+        s0 = f_fma(dn2, n2[i], s0);
+        const float2 g = f_mul(q[i], w1[i]), gn = f_mul(g, n1[i]);
+        s1 = f_fma(gn, cc[i], s1);
+        s2 = f_fma(gn, n2[i], s2);
+        if (LAYER) s3 = f_add(s3, dn2), s4 = f_add(s4, gn), s5 = f_fma(g, cc[i], s5), s6 = f_add(s6, g), s7 = f_fma(g, n2[i], s7);
+      }
+    }
+    float v[N];
+    v[0] = f_sum(s0), v[1] = f_sum(s1), v[2] = f_sum(s2), v[3] = f_sum(s3);
+    if constexpr (LAYER) v[4] = f_sum(s4), v[5] = f_sum(s5), v[6] = f_sum(s6), v[7] = f_sum(s7);
+    const float mine = rn_warp_sums<N>(v);
+    if (lane % (32 / N) == 0) {
+      float* at = &part_s[place][rank * warps + warp][lane / (32 / N)];
+      if (a.cluster > 1) {
+        for (int k = 0; k < a.cluster; ++k) peer_store1(smem_addr(at), k, __float_as_int(mine));
+      } else {
+        *at = mine;
+      }
+    }
+    if (a.cluster > 1) cluster_sync();
+    else if (warps > 1) __syncthreads();
+    else __syncwarp();
+    float total[N] = {};
+    for (int e = lane; e < entries; e += 32) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) total[i] += part_s[place][e][i];
+    }
+    const float joined = rn_warp_sums<N>(total);
+#pragma unroll
+    for (int i = 0; i < N; ++i) total[i] = __shfl_sync(kFull, joined, i * (32 / N)) * a.inv_c;
+    float M = 0.f, mean1 = 0.f;                          // p2 mean dn2; mean of dn1
+    const float m2 = st.w * total[0];                    // p2 mean(dn2 n2)
+    float dot1 = total[1] - m2 * total[2];               // mean(dn1 n1)
+    if constexpr (LAYER) {
+      M = st.w * total[3];
+      dot1 -= M * total[4];
+      mean1 = total[5] - M * total[6] - m2 * total[7];
+    }
+    float2 dx[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float2 t = f_fma(n2[i], make_float2(-m2, -m2), cc[i]);
+      if (LAYER) t = f_add(t, make_float2(-M, -M));
+      dg[i] = f_fma(t, dn[i], dg[i]);
+      float2 du = f_mul(q[i], t);
+      dw1[i] = f_fma(du, n1[i], dw1[i]);
+      if (LAYER) db1[i] = f_add(db1[i], du);
+      dx[i] = f_mul(t, make_float2(a.scale, a.scale));
+      if (a.post) {
+        du = f_fma(n1[i], make_float2(-dot1, -dot1), f_mul(du, w1[i]));
+        if (LAYER) du = f_add(du, make_float2(-mean1, -mean1));
+        du = f_mul(du, make_float2(st.y, st.y));
+      }
+      n1[i] = du;
+    }
+    if (a.dx) rn_store<T, VEC>((T*)a.dx + (size_t)row * C, c, C, dx);
+    if (a.df) rn_store<T, VEC>((T*)a.df + (size_t)row * C, c, C, n1);
+    if (a.units_of_run && --left == 0) {
+      rn_store_eight(a.dgate, a.gdtype, (size_t)unit * C, c, C, dg);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) dg[i] = make_float2(0.f, 0.f);
+      ++unit;
+      left = a.unit_rows;
+    }
+  }
+  auto leave = [&](const float2 (&sum)[4], int slot) {
+    if (slot >= 0) rn_store_eight(a.parts, ACTNN_F32, ((size_t)run * a.slots + slot) * C, c, C, sum);
+  };
+  leave(dw2, a.slot_w2);
+  leave(dw1, a.slot_w1);
+  leave(dg, a.slot_gate);
+  if (LAYER) leave(db2, a.slot_b2), leave(db1, a.slot_b1);
+}
+
+// The partial sums of the runs, added in order: a block has 32 columns of one sum, eight threads a column.
+template <typename T>
+__global__ void __launch_bounds__(kRnThreads) rn_join_kernel(const __grid_constant__ RnArgs a) {
+  constexpr int kWays = kRnThreads / 32;
+  __shared__ float part_s[kWays][32];
+  const uint32_t blocks = (a.C + 31) / 32, which = blockIdx.x / blocks;
+  const int way = threadIdx.x >> 5, column = (blockIdx.x - which * blocks) * 32 + (threadIdx.x & 31);
+  // slots in their order, the gate's last, which has a sum for each unit
+  const bool gate = a.slot_gate >= 0 && which >= (uint32_t)a.slot_gate;
+  const uint32_t slot = gate ? a.slot_gate : which, unit = which - slot;
+  const uint32_t first = gate ? unit * a.runs_of_unit : 0, count = gate ? a.runs_of_unit : a.runs;
+  float s = 0.f;
+  if (column < a.C) {
+#pragma unroll 4
+    for (uint32_t k = way; k < count; k += kWays) s += rn_ld(a.parts + ((size_t)(first + k) * a.slots + slot) * a.C + column);
+  }
+  part_s[way][threadIdx.x & 31] = s;
+  __syncthreads();
+  if (way == 0 && column < a.C) {
+#pragma unroll
+    for (int w = 1; w < kWays; ++w) s += part_s[w][threadIdx.x];
+    void* to = gate ? a.dgate : (int)slot == a.slot_w2 ? a.dw2 : (int)slot == a.slot_b2 ? a.db2 : (int)slot == a.slot_w1 ? a.dw1 : a.db1;
+    rn_store_any(to, gate ? a.gdtype : a.pdtype, (size_t)unit * a.C + column, s);
+  }
+}
+
+// ------------------------------------------------------------------ host
+// A warp has rows of up to 1024 channels, a block longer ones; as few vectors a thread as 512 threads need.
+template <typename T, bool VEC> int rn_forward(const RnArgs& a) {
+  auto run = [&](auto kernel, bool warp, int V) {
+    const unsigned grid = warp ? (a.rows + kRnThreads / 32 - 1) / (kRnThreads / 32) : a.rows;
+    const int threads = warp ? kRnThreads : (a.C + V * 256 - 1) / (V * 256) * 32;
+    kernel<<<grid, threads, 0, a.stream>>>(a);
+    return check_launch();
+  };
+  if (a.C <= 256) return run(rn_forward_kernel<T, 1, true, VEC>, true, 1);
+  if (a.C <= 1024) return run(rn_forward_kernel<T, 4, true, VEC>, true, 4);
+  if (a.C <= 8192) return run(rn_forward_kernel<T, 2, false, VEC>, false, 2);
+  if (a.C <= 16384) return run(rn_forward_kernel<T, 4, false, VEC>, false, 4);
+  return run(rn_forward_kernel<T, 8, false, VEC>, false, 8);
+}
+template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const RnArgs& a) {
+  auto* kernel = rn_backward_kernel<T, VEC, CODED, LAYER>;
+  const int threads = a.cluster > 1 ? kRnMostThreads : (a.C + 255) / 256 * 32;
+  const int smem = (LAYER ? 4 : 3) * 2 * threads * (int)sizeof(float4);
+  // The limit of dynamic shared memory is raised once for the most that any size takes.
+  cached_blocks_per_sm((const void*)kernel, kRnMostThreads, (LAYER ? 4 : 3) * 2 * kRnMostThreads * (int)sizeof(float4));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(a.runs * a.cluster);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = a.stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return cudaGetLastError(), ACTNN_ERR_LAUNCH;
+  if (int st = check_launch()) return st;
+  if (a.slots == 0) return ACTNN_OK;
+  const int sums = a.slot_gate >= 0 ? a.slots - 1 + (int)a.units : a.slots;
+  rn_join_kernel<T><<<(unsigned)((a.C + 31) / 32 * sums), kRnThreads, 0, a.stream>>>(a);
+  return check_launch();
+}
+template <typename T, bool VEC> int rn_run_typed(const RnArgs& a, RnWhat what) {
+  if (what == kRnForward) return rn_forward<T, VEC>(a);
+  if (a.coded) return a.layer ? rn_backward<T, VEC, true, true>(a) : rn_backward<T, VEC, true, false>(a);
+  return a.layer ? rn_backward<T, VEC, false, true>(a) : rn_backward<T, VEC, false, false>(a);
+}
+template <typename T> int rn_run(const RnArgs& a, RnWhat what, bool vec) {
+  return vec ? rn_run_typed<T, true>(a, what) : rn_run_typed<T, false>(a, what);
+}
+#endif
+
+}  // namespace actnn

@@ -86,6 +86,31 @@ template <bool PAIR> ACTNN_DEV void mma_int8(uint32_t d, uint64_t a, uint64_t b,
                  "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}"
                  :: "r"(d), "l"(a), "l"(b), "r"(instruction), "r"((uint32_t)add) : "memory");
 }
+// E4M3 operands with a power-of-two scale for 32 values of the reduction, 32-bit floating-point sums.  `byte`: which of the four bytes of
+// a column of scales counts.
+ACTNN_DEV uint32_t fp8_instruction(int m, int n, int byte) {
+  return ((uint32_t)byte << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 7) << 27) | ((uint32_t)byte << 29);
+}
+// D[m, n] (+)= (A scales_a)[m, 32] (B scales_b)[n, 32]^T.  Scales of 32 rows are a column of tensor memory, in every quarter of its lanes;
+// of a PAIR those of A are a block's own, those of B all of them in both.
+template <bool PAIR>
+ACTNN_DEV void mma_fp8(uint32_t d, uint64_t a, uint64_t b, uint32_t instruction, uint32_t scales_a, uint32_t scales_b, bool add) {
+  if constexpr (PAIR)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(instruction), "r"(scales_a), "r"(scales_b), "r"((uint32_t)add) : "memory");
+  else
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %6, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(instruction), "r"(scales_a), "r"(scales_b), "r"((uint32_t)add) : "memory");
+}
+// 512 bytes of shared memory, 32 rows of 16, to four columns of tensor memory, once for every 32 lanes.  Done before the matrix
+// instructions that the thread issues after it; of a PAIR in both blocks, each from its own memory.
+template <bool PAIR> ACTNN_DEV void scales_to_tmem(uint32_t tmem, uint32_t addr) {
+  const uint64_t rows = (uint64_t)((addr & 0x3ffff) >> 4) | ((uint64_t)(128 >> 4) << 32) | ((uint64_t)1 << 46);      // eight rows are 128 bytes
+  if constexpr (PAIR) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(rows) : "memory");
+  else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" :: "r"(tmem), "l"(rows) : "memory");
+}
 // The barrier (of a PAIR that of both blocks) is arrived at once all matrix instructions that this thread issued before are done.
 template <bool PAIR> ACTNN_DEV void mma_commit(uint32_t bar) {
   if constexpr (PAIR)

@@ -17,9 +17,12 @@ from torch.nn.modules.utils import _pair, _single, _triple
 from . import ops
 from .conf import config
 from .cpp_extension import checkpoint as ext_checkpoint
+from .cpp_extension import fp8 as ext_fp8
 from .cpp_extension import group_norm as ext_group_norm
 from .cpp_extension import int8 as ext_int8
 from .cpp_extension import quantization as ext_quantization
+from .cpp_extension import residual_norm as ext_residual_norm
+from .cpp_extension import seeded_dropout as ext_seeded_dropout
 from .cpp_extension._checks import activation_name
 from .qbnscheme import QBNScheme
 from .qscheme import QScheme
@@ -366,3 +369,83 @@ class QGroupNorm(nn.GroupNorm):
 
     def extra_repr(self):
         return super().extra_repr() + ", activation=" + self.activation
+
+
+# ------------------------------------------------------------------------- operators of a residual branch (no counterpart in the reference)
+class QFp8Linear(nn.Linear):
+    """A linear layer whose products, forward and backward, run in 8-bit floating point with a power-of-two scale for each block of 128.
+
+    In training the weight is coded in every step and the codes of the input are what the backward pass keeps.  For serving,
+    ``freeze()`` codes the weight once: until ``unfreeze()`` (or ``train()``) the forward pass reads those codes alone.  Under
+    autocast the layer computes in autocast's type, frozen or not."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        super().__init__(in_features, out_features, bias)
+        self.frozen = None
+
+    def freeze(self):
+        self.frozen = ext_fp8.quantize_weight(*ops._autocast_inputs(self.weight.detach()))
+        return self
+
+    def unfreeze(self):
+        self.frozen = None
+        return self
+
+    def train(self, mode: bool = True):
+        if mode:
+            self.unfreeze()
+        return super().train(mode)
+
+    def _apply(self, fn, recurse=True):
+        self.frozen = None                    # the weight moves or changes its type: freeze again
+        return super()._apply(fn, recurse)
+
+    def forward(self, input):
+        if self.frozen is not None:
+            if torch.is_grad_enabled() and input.requires_grad:
+                raise RuntimeError("QFp8Linear is frozen: no gradient passes through it (call unfreeze() first)")
+            input, bias = ops._autocast_inputs(input, None if self.bias is None else self.bias.detach())
+            return ext_fp8.linear(input, *self.frozen, bias)
+        return ops.fp8_linear.apply(input, self.weight, self.bias)
+
+
+class QSeededDropout(nn.Dropout):
+    """Dropout that keeps no mask: the backward pass draws it again.  ``QDropout`` keeps a bit an element."""
+
+    def __init__(self, p=0.5):
+        super().__init__(ext_seeded_dropout.check_probability(p))
+
+    def forward(self, input):
+        return ops.seeded_dropout.apply(input, self.p) if self.training else input
+
+
+class QResidualNorm(nn.Module):
+    """The end of one block and the beginning of the next, ``(r, h)`` of the residual stream and the block's output:
+
+        r = scale * x + gate * drop(norm(branch) * post_weight + post_bias)        h = norm(r) * weight + bias
+
+    ``kind``: "rms" (no biases) or "layer"; ``post`` false: no norm of the branch; ``gate``: a number with which a learned gate for
+    each channel begins, or ``None``; ``forward`` takes a gate of its own too (``[B, 1, C]``, ...), for layers without a learned one.
+    The inputs are kept in 8 bits for the backward pass, the dropout's mask not at all."""
+
+    def __init__(self, channels, eps=1e-5, kind="rms", post=True, gate: Optional[float] = None, scale=1.0, p=0.0):
+        super().__init__()
+        self.layer = ext_residual_norm.norm_kind(kind) == 1
+        self.channels, self.eps, self.kind, self.post, self.scale, self.p = channels, eps, kind, post, scale, ext_seeded_dropout.check_probability(p)
+
+        def parameter(value, there=True):
+            return nn.Parameter(torch.full((channels,), float(value))) if there else None
+
+        self.weight, self.bias = parameter(1), parameter(0, self.layer)
+        self.post_weight, self.post_bias = parameter(1, post), parameter(0, post and self.layer)
+        self.gate = parameter(gate or 0, gate is not None)
+
+    def forward(self, input, branch, gate=None):
+        if gate is not None and self.gate is not None:
+            raise RuntimeError("QResidualNorm has a learned gate: it takes no other")
+        return ops.residual_norm.apply(input, branch, self.weight, self.bias, self.post_weight, self.post_bias,
+                                       self.gate if gate is None else gate, self.scale, self.p if self.training else 0.0, self.eps,
+                                       self.kind, self.post)
+
+    def extra_repr(self):
+        return "%d, eps=%g, kind=%s, post=%s, scale=%g, p=%g" % (self.channels, self.eps, self.kind, self.post, self.scale, self.p)

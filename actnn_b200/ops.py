@@ -28,11 +28,14 @@ from . import _lib
 from .conf import config
 from .cpp_extension import backward_func as ext_backward_func
 from .cpp_extension import checkpoint as ext_checkpoint
+from .cpp_extension import fp8 as ext_fp8
 from .cpp_extension import group_norm as ext_group_norm
 from .cpp_extension import int8 as ext_int8
 from .cpp_extension._checks import activation_kind, activation_name
 from .cpp_extension import minimax as ext_minimax  # noqa: F401  (kept under the name the reference imports)
 from .cpp_extension import quantization as ext_quantization
+from .cpp_extension import residual_norm as ext_residual_norm
+from .cpp_extension import seeded_dropout as ext_seeded_dropout
 from .qbnscheme import QBNScheme
 from .qscheme import group_minimax, to_groups
 from .utils import compute_tensor_bytes, empty_cache, get_memory_usage, swap_to_cpu, swap_to_gpu
@@ -783,3 +786,133 @@ class group_norm:
         if nat and not config.swap:
             return nat.group_norm(input, num_groups, weight, bias, eps, name, config.compress_activation)
         return _GroupNorm.apply(input, num_groups, weight, bias, eps, name)
+
+
+# ---------------------------------------------------------------------------------------
+# operators of a residual branch (the reference has no counterpart)
+# ---------------------------------------------------------------------------------------
+class _Fp8Linear(Function):
+    @staticmethod
+    def forward(ctx, input, weight, bias=None):
+        with _autocast_off():
+            if weight.dim() != 2 or input.dim() < 1 or input.shape[-1] != weight.shape[1]:
+                raise RuntimeError("shapes %s and %s cannot be multiplied" % (tuple(input.shape), tuple(weight.shape)))
+            x = input.reshape(input.shape[:-1].numel(), input.shape[-1])
+            need_x, need_w = ctx.needs_input_grad[:2]
+            here, there, _ = ext_fp8.tile_codes(x, True, True) if need_w else (ext_fp8.quantize(x), None, None)
+            whole = ext_fp8.quantize_weight(weight, both=need_x)
+            output = ext_fp8.matmul(*here, *whole[:2], bias, input.dtype).view(input.shape[:-1] + weight.shape[:1])
+            ctx.saved = (None if there is None else (_keep(there[0].view(torch.uint8)), there[1])), whole[2:]
+            ctx.other_args = (input.dtype, input.shape, weight.dtype, None if bias is None else bias.dtype)
+            return output
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        tokens, weight = ctx.saved
+        dtype, shape, wdtype, bdtype = ctx.other_args
+        need_x, need_w, need_b = ctx.needs_input_grad[0], ctx.needs_input_grad[1], bdtype is not None and ctx.needs_input_grad[2]
+        with _autocast_off():
+            go = grad_output.reshape(shape[:-1].numel(), grad_output.shape[-1])
+            here, there, parts = ext_fp8.tile_codes(go, need_x, need_w, need_b)
+            grad_input = ext_fp8.matmul(*here, *weight, None, dtype).view(shape) if need_x else None
+            grad_weight = ext_fp8.matmul(*there, _kept(tokens[0]).view(ext_fp8.CODES), tokens[1], None, wdtype) if need_w else None
+            grad_bias = ext_fp8.join_sums(parts, bdtype) if need_b else None
+        return grad_input, grad_weight, grad_bias
+
+
+class fp8_linear:
+    """``x @ weight.T + bias`` in 8-bit floating point with a power-of-two scale for each block of 128, forward and backward.
+
+    Each of the three products takes operands coded along its own reduction: the forward product tokens in blocks of 128 channels and
+    the weight in squares of 128 x 128, the gradient of the input the output's gradient in blocks of 128 output channels and the same
+    squares, the gradient of the weight both in blocks of 128 tokens.  Sums are float32; the gradients pass straight through
+    the rounding.  Kept is the input's code for the gradient of the weight, a byte a value, and the weight's."""
+
+    @staticmethod
+    def apply(input, weight, bias=None):
+        input, weight, bias = _autocast_inputs(input, weight, bias)
+        nat = _lib.native()
+        if nat and not config.swap:
+            return nat.fp8_linear_train(input, weight, bias)
+        return _Fp8Linear.apply(input, weight, bias)
+
+
+class _SeededDropout(Function):
+    @staticmethod
+    def forward(ctx, input, p, key):
+        ctx.other_args = p, key
+        return ext_seeded_dropout.apply_mask(input, p, key)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        return ext_seeded_dropout.apply_mask(grad_output, *ctx.other_args), None, None
+
+
+class seeded_dropout:
+    """Dropout whose mask is drawn again in the backward pass: nothing of an element is kept.
+
+    ``key``: the pair (seed, offset) that says which elements go; without one it comes from the device's generator, as everywhere
+    else.  In a captured graph the key is read on the device, so every replay drops other elements."""
+
+    @staticmethod
+    def apply(input, p=0.5, key=None):
+        p = ext_seeded_dropout.check_probability(p)
+        key = None if key is None else ext_seeded_dropout.check_key(key)
+        nat = _lib.native()
+        if nat:
+            return nat.seeded_dropout(input, p, key)
+        return _SeededDropout.apply(input, p, _lib.next_philox(input.device) if key is None else key)
+
+
+class _ResidualNorm(Function):
+    @staticmethod
+    def forward(ctx, input, branch, weight, bias, post_weight, post_bias, gate, scale, p, eps, kind, post, key):
+        compress = config.compress_activation
+        r, h, codes, stats = ext_residual_norm.run(input, branch, weight, bias, post_weight, post_bias, gate, scale, p, eps, kind, post, key,
+                                                   codes=compress, stats=True)
+        ctx.set_materialize_grads(False)
+        here = not compress and not config.swap              # the caller's own tensors
+        ctx.save_for_backward(weight, bias, post_weight, post_bias, gate, *((input, branch) if here else ()))
+        kept = codes if compress else (input.contiguous(), branch.contiguous())
+        ctx.kept = None if here else tuple(_keep(t) if i % 2 == 0 or not compress else t for i, t in enumerate(kept))
+        ctx.other_args = (scale, p, kind, post, key, stats)
+        return r, h
+
+    @staticmethod
+    def backward(ctx, grad_r, grad_h):
+        if grad_r is None and grad_h is None:
+            return (None,) * 13
+        parameters, here = ctx.saved_tensors[:5], ctx.saved_tensors[5:]
+        scale, p, kind, post, key, stats = ctx.other_args
+        kept = tuple(t.contiguous() for t in here) if here else tuple(_kept(t) for t in ctx.kept)
+        grads = ext_residual_norm.backward(grad_r, grad_h, kept, stats, *parameters, scale, p, kind, post, key, ctx.needs_input_grad[:7])
+        return grads + (None,) * 6
+
+
+class residual_norm:
+    """The end of one block and the beginning of the next: ``r = scale * x + gate * drop(norm(branch) * post_weight + post_bias)`` and
+    ``h = norm(r) * weight + bias``; returns ``(r, h)``.  ``kind``: "rms" or "layer"; ``post`` false leaves the first norm out.  The inputs
+    are kept in 8 bits, the dropout's mask (``p``, ``key`` as in ``seeded_dropout``) not at all.  An input or branch in a narrower
+    type than the other is taken in that one's."""
+
+    @staticmethod
+    def apply(input, branch, weight=None, bias=None, post_weight=None, post_bias=None, gate=None, scale=1.0, p=0.0, eps=1e-5, kind="rms",
+              post=True, key=None):
+        layer, p = ext_residual_norm.norm_kind(kind), ext_seeded_dropout.check_probability(p)
+        key = None if key is None else ext_seeded_dropout.check_key(key)
+        if isinstance(input, torch.Tensor) and isinstance(branch, torch.Tensor) and input.dtype != branch.dtype:
+            wide = torch.promote_types(input.dtype, branch.dtype)
+            input, branch = input.to(wide), branch.to(wide)
+        parameters = weight, bias, post_weight, post_bias, gate
+        training = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (input, branch) + parameters)
+        nat = _lib.native()
+        if nat and not training:
+            return nat.residual_norm_value(input, branch, *parameters, float(scale), p, float(eps), layer, bool(post), key)
+        if nat and not config.swap:
+            return nat.residual_norm(input, branch, *parameters, float(scale), p, float(eps), layer, bool(post), key, config.compress_activation)
+        if key is None:
+            key = _lib.next_philox(input.device) if p > 0 else (0, 0)
+        if not training:
+            return ext_residual_norm.run(input, branch, *parameters, scale, p, eps, kind, post, key)[:2]
+        ext_residual_norm._inputs(input, branch)
+        return _ResidualNorm.apply(input, branch, *parameters, scale, p, eps, kind, post, key)

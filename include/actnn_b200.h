@@ -498,6 +498,93 @@ int actnn_group_norm_backward(const void* grad_y, const void* x, const int8_t* c
                               void* workspace, int64_t workspace_bytes, actnn_stream_t stream);
 
 /* ------------------------------------------------------------------------------------
+ * Codes in 8-bit floating point (e4m3) with a power-of-two scale for each block of 128.  Of a block, e is the least
+ * integer, at least -126, with max |x| <= 448 * 2^e; a code is x * 2^-e rounded to e4m3, half to even.  What is not
+ * finite takes no part in the maximum and is coded as NaN.  `scales` are bytes e + 127 in the order
+ * [ceil(cols / 512)][ceil(rows / 128)][512]: of 128 rows and four blocks, that of row r and block j at
+ * (r % 32) * 16 + (r / 32) * 4 + j; bytes of rows behind the last are not written.  Rows of codes are ld_codes bytes
+ * apart, the least multiple of 16 that holds them, zero behind the end; rows of x ld_x elements.
+ * actnn_fp8_row_codes: blocks of 128 consecutive elements of a row.
+ * actnn_fp8_tile_codes: the same to `codes`, and to `codes_t` [cols, ld_codes_t] the transposed matrix in blocks of
+ * 128 consecutive rows of x; with `square` both in blocks of 128 x 128.  Either may be NULL.  parts (NULL: not wanted)
+ * [ceil(rows / 128), cols]: sums of the columns of 128 rows, which actnn_fp8_join_sums adds in a fixed order.
+ * actnn_fp8_decode: code * 2^e, [rows, cols] contiguous.
+ * Code and scale pointers are on 16 bytes.  The reference has no counterpart (its codes are per group of 256 with a
+ * minimum, actnn/actnn/cpp_extension/quantization_cuda_kernel.cu:86-142). */
+int actnn_fp8_row_codes(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, int64_t ld_x,
+                        int64_t ld_codes, int dtype, actnn_stream_t stream);
+int actnn_fp8_tile_codes(const void* x, uint8_t* codes, uint8_t* scales, uint8_t* codes_t, uint8_t* scales_t,
+                         float* parts, int64_t rows, int64_t cols, int64_t ld_x, int64_t ld_codes, int64_t ld_codes_t,
+                         int square, int dtype, actnn_stream_t stream);
+int actnn_fp8_join_sums(const float* parts, void* out, int64_t runs, int64_t cols, int dtype, actnn_stream_t stream);
+int actnn_fp8_decode(const uint8_t* codes, const uint8_t* scales, void* out, int64_t rows, int64_t cols,
+                     int64_t ld_codes, int dtype, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * out[t, n] = sum_k tokens[t, k] * weights[n, k] + bias[n] of what the codes above stand for, summed in fp32 on the
+ * tensor cores; out is [T, N] contiguous of `dtype`, rounded once.  `bias` (of `dtype`) may be NULL.  What lies between
+ * K and ld is not read as data.  Reproducible for given sizes.  A block whose bounded wait runs out leaves its
+ * outputs unwritten, as do those that share its reduction, and counts the event (actnn_bulk_wait_failures).
+ * The reference has no counterpart (its layers compute in the activation's type, actnn/actnn/ops.py:408-428). */
+int actnn_fp8_matmul(const uint8_t* tokens, const uint8_t* token_scales, const uint8_t* weights,
+                     const uint8_t* weight_scales, const void* bias, void* out, int64_t T, int64_t N, int64_t K,
+                     int64_t ld_tokens, int64_t ld_weights, int dtype, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * A linear layer on a weight kept as codes: x [T, K] of `dtype`, rows `ld_x` elements apart, is coded as by
+ * actnn_fp8_row_codes and multiplied.  One launch for up to eight tokens whose codes fit a block's shared memory;
+ * otherwise `workspace`, 16-byte aligned, takes the codes: actnn_fp8_linear_workspace bytes (0: may be NULL).  The sums of
+ * the one launch are added in another order than those of the other.  The reference has no counterpart
+ * (actnn/actnn/ops.py:408-428 computes in the activation's type). */
+int actnn_fp8_linear_workspace(int64_t T, int64_t K, int64_t* bytes);
+int actnn_fp8_linear(const void* x, const uint8_t* weights, const uint8_t* weight_scales, const void* bias, void* out,
+                     int64_t T, int64_t N, int64_t K, int64_t ld_x, int64_t ld_weights, int dtype, void* workspace,
+                     int64_t workspace_bytes, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * Dropout whose mask is never stored.  Element e has the 16-bit field e % 8 (words and halves upwards) of the
+ * Philox4x32-10 output for counter e / 8 and key (seed, offset), as actnn_dropout_forward; it is kept where
+ * field + 1 > 65536 p, and multiplied by 1 / (1 - p).  y = x after it; the gradient is the same call on grad_y.
+ * `state` (device, on 16 bytes; NULL: the key of the arguments): seed and offset, read by the kernel, for
+ * launches that are replayed.  x and y contiguous, on 16 bytes.  0 <= p < 1.
+ * actnn_philox_state writes such a state, (*seed, *offset + more), all on the device.
+ * The reference keeps a bit an element (actnn/actnn/cpp_extension/quantization.cc:128-148). */
+int actnn_seeded_dropout(const void* x, void* y, int64_t numel, float p, int dtype, uint64_t seed, uint64_t offset,
+                         const int64_t* state, actnn_stream_t stream);
+int actnn_philox_state(const int64_t* seed, const int64_t* offset, uint64_t more, int64_t* state,
+                       actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
+ * The norms before and after a block with its gate and residual scale, on rows of C channels (1 to 32768):
+ *   r = scale * x + gate * drop(norm(f) * post_weight + post_bias),   h = norm(r) * weight + bias
+ * `layer` 0: norm(v) = v / sqrt(mean(v^2) + eps); 1: of v less its mean.  `post` 0: f is taken as it is.
+ * `gate` [rows / gate_rows, C]; it and the parameters [C], of param_dtype and gate_dtype, may be NULL (ones,
+ * zeros).  Dropout as above, of element row * C + channel; p = 0: none.  x, f, r, h [rows, C] of `dtype`.
+ * codes_x, codes_f [rows, C] with scales [rows, ceil(C / 256)] (all four NULL: not saved): the inputs in 8 bits
+ * as in actnn_row_codes, 256 channels of a row to a scale.  stats [rows, 4] on 16 bytes: mean and reciprocal
+ * deviation of f, of r (NULL only without codes).
+ * Backward: of the codes, or of x and f where those are NULL.  grad_r or grad_h may be NULL (zeros); gradients
+ * that are not wanted are NULL.  Those of parameters and gate are sums over rows in a fixed order, float32,
+ * rounded once.  Workspace: 16-byte aligned, actnn_residual_norm_workspace bytes.
+ * The reference has no counterpart (its norms are batch norms, actnn/actnn/ops.py:444-500). */
+int actnn_residual_norm_forward(const void* x, const void* f, const void* weight, const void* bias,
+                                const void* post_weight, const void* post_bias, const void* gate, void* r, void* h,
+                                int8_t* codes_x, int8_t* codes_f, float* scale_x, float* scale_f, float* stats,
+                                int64_t rows, int64_t C, int64_t gate_rows, double scale, double eps, int layer,
+                                int post, float p, int dtype, int param_dtype, int gate_dtype, uint64_t seed,
+                                uint64_t offset, const int64_t* state, actnn_stream_t stream);
+int actnn_residual_norm_workspace(int64_t rows, int64_t C, int64_t gate_rows, int gate_grad, int64_t* bytes);
+int actnn_residual_norm_backward(const void* grad_r, const void* grad_h, const void* x, const void* f,
+                                 const int8_t* codes_x, const int8_t* codes_f, const float* scale_x,
+                                 const float* scale_f, const float* stats, const void* weight,
+                                 const void* post_weight, const void* post_bias, const void* gate, void* grad_x,
+                                 void* grad_f, void* grad_weight, void* grad_bias, void* grad_post_weight,
+                                 void* grad_post_bias, void* grad_gate, int64_t rows, int64_t C, int64_t gate_rows,
+                                 double scale, int layer, int post, float p, int dtype, int param_dtype,
+                                 int gate_dtype, uint64_t seed, uint64_t offset, const int64_t* state,
+                                 void* workspace, int64_t workspace_bytes, actnn_stream_t stream);
+
+/* ------------------------------------------------------------------------------------
  * How many bulk-copy waits gave up on the current device since the library was loaded.
  * The opt-in staged pack kernels (environment ACTNN_STAGED_PACK=1) copy their inputs into
  * shared memory with the bulk-copy engine and bound every wait on the completion barrier;
