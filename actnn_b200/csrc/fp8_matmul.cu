@@ -75,6 +75,14 @@ ACTNN_DEV bool fp_wait(uint32_t bar, uint32_t parity, FpShared& s, unsigned* gav
   return false;
 }
 
+// Whether a phase is complete: asked for the next stage before this one's work is issued, so that the answer's latency passes beside it.
+ACTNN_DEV bool fp_test(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
+  return ok != 0;
+}
+
 // Of the epilogue's eight warps: whether the waits of all of them came to their end.  A warp that left alone, because another
 // wait had run out just before its own phase was complete, would leave those whose phase was to barriers it never comes to.
 ACTNN_DEV bool epilogue_agrees(bool ok) {
@@ -126,100 +134,119 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
   tmem_fence_after_sync();
   const uint32_t tmem = s.tmem;
 
-  int copy_stage = 0, issued = 0, ahead = 0;                    // of the copies' thread, to the end
+  // The copies' and the matrix instructions' warps go through their loops with all lanes, of which the first one issues: what a loop
+  // counts is then uniform, and its addresses are where the instructions want them.  (A loop of one lane alone took 650 cycles a
+  // stage, whatever it issued, 0.39 us where the matrix instructions of 192 tokens take 0.22.)
+  const bool issues = lane == 0;
+  int copy_stage = 0, issued = 0, ahead = 0;                    // of the copies, to the end
   uint32_t copy_phase = 0;
   bool copied = true;
   if (warp == 8) {                                              // ---------------- copies
-    if (lane == 0) {
-      // Requests a box of a stage; of a pair, the first block's barrier counts.
-      auto request = [&](int stage, uint32_t dst, const CUtensorMap* map, int x, int row) {
-        const uint32_t bar = smem_addr(&s.full[stage]);
-        if constexpr (PAIR) tile_load_pair(dst, map, x, row, peer_addr(bar, 0));
-        else tile_load(dst, map, x, row, bar);
-      };
-      // The scales of four blocks come with the first of them that is multiplied.
-      auto begins = [&](int k) { return k == k_first || k % 4 == 0; };
-      auto expect = [&](int stage, int k) {
-        const uint32_t bytes = stage_bytes + (begins(k) ? scale_bytes : 0);
-        if (!PAIR || rank == 0) mbar_expect_tx(smem_addr(&s.full[stage]), PAIR ? 2 * bytes : bytes);
-      };
-      auto request_weights = [&](int stage, int k, int ct) {
-        const int row = ct * tile_channels + (int)rank * kFpChannels * PAIR;
-        request(stage, stage0 + stage * stage_bytes, &weights, k * kFpStageK, row);
-        if (begins(k)) request(stage, scales0 + stage * kFpScales, &weight_scales, 0, 2 * (k / 4 * a.scale_rows_w + row / 128));
-      };
-      auto request_tokens = [&](int stage, int k, int tt) {
-        request(stage, stage0 + stage * stage_bytes + a_bytes, &tokens, k * kFpStageK, tt * a.tokens + (int)rank * load_tokens * PAIR);
-        if (begins(k)) request(stage, scales0 + stage * kFpScales + 512, &token_scales, 0, 2 * (k / 4 * a.scale_rows_x + tt * a.tokens / 128));
-      };
-      if (a.early) {                                            // weights of the first stages before the tokens are there
-        const int ct = first_tile % a.channel_tiles;
-        for (ahead = 0; first_tile < a.tiles && ahead < a.stages && ahead < k_end - k_first; ++ahead) {
-          expect(ahead, k_first + ahead);
-          request_weights(ahead, k_first + ahead, ct);
-        }
-        grid_wait();
-      }
-      for (int tile = first_tile; copied && tile < a.tiles; tile += tile_step) {
-        const int tt = tile / a.channel_tiles, ct = tile - tt * a.channel_tiles;
-        for (int k = k_first; k < k_end; ++k) {
-          if (!(copied = fp_wait(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1, s, gave_up))) break;
-          if (issued >= ahead) {
-            expect(copy_stage, k);
-            request_weights(copy_stage, k, ct);
-          }
-          request_tokens(copy_stage, k, tt);
-          ++issued;
-          if (++copy_stage == a.stages) copy_stage = 0, copy_phase ^= 1;
+    const int channel_step = (int)rank * kFpChannels * PAIR, token_step = (int)rank * load_tokens * PAIR;
+    // Requests a box of a stage; of a pair, the first block's barrier counts.
+    auto request = [&](uint32_t bar, uint32_t dst, const CUtensorMap* map, int x, int row) {
+      if constexpr (PAIR) tile_load_pair(dst, map, x, row, peer_addr(bar, 0));
+      else tile_load(dst, map, x, row, bar);
+    };
+    // The scales of four blocks come with the first of them that is multiplied.
+    auto expect = [&](uint32_t bar, bool begins) {
+      const uint32_t bytes = stage_bytes + (begins ? scale_bytes : 0);
+      if (!PAIR || rank == 0) mbar_expect_tx(bar, PAIR ? 2 * bytes : bytes);
+    };
+    auto request_weights = [&](uint32_t bar, int stage, int k, bool begins, int row) {
+      request(bar, stage0 + stage * stage_bytes, &weights, k * kFpStageK, row);
+      if (begins) request(bar, scales0 + stage * kFpScales, &weight_scales, 0, 2 * ((k >> 2) * a.scale_rows_w + (row >> 7)));
+    };
+    if (a.early) {                                              // weights of the first stages before the tokens are there
+      const int row = first_tile % a.channel_tiles * tile_channels + channel_step;
+      for (ahead = 0; first_tile < a.tiles && ahead < a.stages && ahead < k_end - k_first; ++ahead) {
+        const int k = k_first + ahead;
+        const bool begins = ahead == 0 || (k & 3) == 0;
+        const uint32_t bar = smem_addr(&s.full[ahead]);
+        if (elect_one()) {
+          expect(bar, begins);
+          request_weights(bar, ahead, k, begins, row);
         }
       }
-      // A pair's second block is there until what the first one's matrix instructions arrive at has been arrived at: the stages' barriers
-      // and the one for the end.  (In their own block the thread that issues them waits for the end.)
-      for (int i = 0, at = copy_stage; PAIR && copied && i < a.stages; ++i) {
-        copied = fp_wait(smem_addr(&s.empty[at]), copy_phase ^ (at < copy_stage ? 0 : 1), s, gave_up);
-        if (++at == a.stages) at = 0;
-      }
-      if (PAIR && copied) copied = fp_wait(smem_addr(&s.drained), 0, s, gave_up);
+      grid_wait();
     }
+    bool free = false;
+    for (int tile = first_tile; copied && tile < a.tiles; tile += tile_step) {
+      const int tt = tile / a.channel_tiles, row = (tile - tt * a.channel_tiles) * tile_channels + channel_step, t0 = tt * a.tokens;
+      for (int k = k_first; k < k_end; ++k) {
+        if (!free && !(copied = fp_wait(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+        const int now = copy_stage;
+        if (++copy_stage == a.stages) copy_stage = 0, copy_phase ^= 1;
+        free = fp_test(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1);
+        const bool begins = k == k_first || (k & 3) == 0;
+        const uint32_t bar = smem_addr(&s.full[now]);
+        if (elect_one()) {
+          if (issued >= ahead) {
+            expect(bar, begins);
+            request_weights(bar, now, k, begins, row);
+          }
+          request(bar, stage0 + now * stage_bytes + a_bytes, &tokens, k * kFpStageK, t0 + token_step);
+          if (begins) request(bar, scales0 + now * kFpScales + 512, &token_scales, 0, 2 * ((k >> 2) * a.scale_rows_x + (t0 >> 7)));
+        }
+        ++issued;
+      }
+    }
+    // A pair's second block is there until what the first one's matrix instructions arrive at has been arrived at: the stages' barriers
+    // and the one for the end.  (In their own block the warp that issues them waits for the end.)
+    for (int i = 0, at = copy_stage; PAIR && copied && i < a.stages; ++i) {
+      copied = fp_wait(smem_addr(&s.empty[at]), copy_phase ^ (at < copy_stage ? 0 : 1), s, issues ? gave_up : nullptr);
+      if (++at == a.stages) at = 0;
+    }
+    if (PAIR && copied) copied = fp_wait(smem_addr(&s.drained), 0, s, issues ? gave_up : nullptr);
+    __syncwarp();
   } else if (warp == 9) {                                       // ---------------- matrix instructions
     if (a.early) grid_wait();                                   // the limit of a wait is for copies, not for the launch before
-    if (lane == 0 && (!PAIR || rank == 0)) {
-      uint32_t instruction[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) instruction[i] = fp8_instruction(tile_channels, a.tokens, i);
+    if (!PAIR || rank == 0) {
+      const uint32_t instruction = fp8_instruction(tile_channels, a.tokens, 0), one_byte = fp8_instruction(tile_channels, a.tokens, 1) - instruction;
       const uint32_t sets = tmem + (SPLIT ? 1 : 2) * a.tokens;
       int stage = 0, buf = 0, set = 0;
       uint32_t phase = 0, buf_phase = 0;
       bool ok = true;
       for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
-        if (!(ok = fp_wait(smem_addr(&s.sum_empty[buf]), buf_phase ^ 1, s, gave_up))) break;
+        if (!(ok = fp_wait(smem_addr(&s.sum_empty[buf]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
         tmem_fence_after_sync();
         const uint32_t d = tmem + buf * a.tokens, shift = (tile / a.channel_tiles * a.tokens & 127) / 32;   // columns from a set of 128 tokens
         uint32_t at_w = 0;
+        bool ready = false;
         for (int k = k_first; k < k_end; ++k) {
-          if (!(ok = fp_wait(smem_addr(&s.full[stage]), phase, s, gave_up))) break;
-          tmem_fence_after_sync();
-          if (k == k_first || k % 4 == 0) {
+          if (!ready && !(ok = fp_wait(smem_addr(&s.full[stage]), phase, s, issues ? gave_up : nullptr))) break;
+          const int now = stage;
+          if (++stage == a.stages) stage = 0, phase ^= 1;
+          ready = fp_test(smem_addr(&s.full[stage]), phase);
+          const bool begins = k == k_first || (k & 3) == 0;
+          if (begins) {
             at_w = sets + set * kFpScaleColumns;
             set = (set + 1) % kFpScaleSets;
-            const uint32_t from = scales0 + stage * kFpScales;
-            for (int i = 0; i <= a.atoms; ++i) scales_to_tmem<PAIR>(at_w + 4 * i, from + 512 * i);
           }
-          const uint32_t at = stage0 + stage * stage_bytes, which = k % 4;
-          const uint32_t instr = which == 0 ? instruction[0] : which == 1 ? instruction[1] : which == 2 ? instruction[2] : instruction[3];
+          const uint32_t at = stage0 + now * stage_bytes, from = scales0 + now * kFpScales, instr = instruction + (k & 3) * one_byte;
           const uint64_t da = rows128_descriptor(at), db = rows128_descriptor(at + a_bytes);
+          if (elect_one()) {
+            if (begins) {
+              scales_to_tmem<PAIR>(at_w, from);
+              scales_to_tmem<PAIR>(at_w + 4, from + 512);
+              if (a.atoms > 1) scales_to_tmem<PAIR>(at_w + 8, from + 1024);
+              if (a.atoms > 2) scales_to_tmem<PAIR>(at_w + 12, from + 1536);
+            }
 #pragma unroll
-          for (int i = 0; i < kFpStageK / 32; ++i)              // 32 bytes further along the rows: 2 in units of 16 bytes
-            mma_fp8<PAIR>(d, da + 2 * i, db + 2 * i, instr, at_w, at_w + 4 + shift, k > k_first || i > 0);
-          mma_commit<PAIR>(smem_addr(&s.empty[stage]));
-          if (++stage == a.stages) stage = 0, phase ^= 1;
+            for (int i = 0; i < kFpStageK / 32; ++i)            // 32 bytes further along the rows: 2 in units of 16 bytes
+              mma_fp8<PAIR>(d, da + 2 * i, db + 2 * i, instr, at_w, at_w + 4 + shift, k > k_first || i > 0);
+            mma_commit<PAIR>(smem_addr(&s.empty[now]));
+          }
         }
         if (!ok) break;
-        mma_commit<PAIR>(smem_addr(&s.sum_full[buf]));
+        if (elect_one()) mma_commit<PAIR>(smem_addr(&s.sum_full[buf]));
         if (++buf == 2) buf = 0, buf_phase ^= 1;
       }
-      mma_commit<PAIR>(smem_addr(&s.drained));
-      mbar_wait(smem_addr(&s.drained), 0);
+      __syncwarp();
+      if (elect_one()) {
+        mma_commit<PAIR>(smem_addr(&s.drained));
+        mbar_wait(smem_addr(&s.drained), 0);
+      }
     }
     __syncwarp();
   } else {                                                      // ---------------- epilogue

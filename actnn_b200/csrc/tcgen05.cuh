@@ -11,6 +11,14 @@ namespace actnn {
 // ------------------------------------------------------------------ barriers
 ACTNN_DEV void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
 
+// One lane of a warp that is together, always the same.  A branch on it the compiler knows to be of one lane, and keeps what is uniform
+// in the registers that copies and matrix instructions take their operands from.
+ACTNN_DEV bool elect_one() {
+  uint32_t mine;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(mine));
+  return mine != 0;
+}
+
 // ------------------------------------------------------------------ tiled copies
 // A box of a rank-2 tensor to shared memory; x (elements of the contiguous dimension) starts on 16 bytes.
 ACTNN_DEV void tile_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
