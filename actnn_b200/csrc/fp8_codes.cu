@@ -4,6 +4,7 @@
 // its own reduction.  What is read once is coded both ways: tokens along their channels for the product they enter, and along the
 // tokens, transposed, for the gradient of the weight.  A weight is coded in squares, whose codes are the same either way.
 // Bound by HBM: 2 + 1 bytes an element one way, 2 + 2 both ways.
+#include "cluster.cuh"
 #include "fp8.cuh"
 
 namespace actnn {
@@ -11,39 +12,72 @@ namespace {
 
 constexpr int kCodeThreads = 256;
 
-// A warp has 512 elements of a row, two vectors a lane; half a warp and a vector are a block.
-template <typename T, bool VEC>
+// A warp has 512 elements of a row, two vectors a lane, TASKS times; half a warp and a vector are a block.
+template <typename T, bool VEC, int TASKS>
 __global__ void __launch_bounds__(kCodeThreads)
 fp8_row_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
                      int64_t ldx, int64_t ldc, int groups) {
-  const int64_t task = (int64_t)blockIdx.x * (kCodeThreads / 32) + (threadIdx.x >> 5), row = task / groups;
-  if (row >= rows) return;
-  const int lane = threadIdx.x & 31, g = (int)(task - row * groups);
-  const T* p = x + row * ldx;
-  Vec<T, 8> v[2];
-  uint32_t byte[2];
+  const int lane = threadIdx.x & 31;
+  const int64_t first = ((int64_t)blockIdx.x * (kCodeThreads / 32) + (threadIdx.x >> 5)) * TASKS;
+  grid_release();                                      // of the product that may follow: it waits for the end of this launch itself
+  int64_t row[TASKS];
+  int g[TASKS];
+  Vec<T, 8> v[TASKS][2];
 #pragma unroll
-  for (int k = 0; k < 2; ++k) v[k] = fp8_load<T, VEC>(p, g * 512 + k * 256 + lane * 8, cols);
+  for (int i = 0; i < TASKS; ++i) {
+    row[i] = (first + i) / groups;
+    g[i] = (int)(first + i - row[i] * groups);
 #pragma unroll
-  for (int k = 0; k < 2; ++k) {
-    const int64_t e = g * 512 + k * 256 + lane * 8;
-    bool bad;
-    byte[k] = fp8_scale_byte(half_warp_max(fp8_most(v[k], bad)));
-    if (e < ldc) *reinterpret_cast<uint2*>(codes + row * ldc + e) = fp8_codes8(v[k], fp8_factor(byte[k]), bad);
+    for (int k = 0; k < 2; ++k) v[i][k] = fp8_load<T, VEC>(x + row[i] * ldx, g[i] * 512 + k * 256 + lane * 8, row[i] < rows ? cols : 0);
   }
-  const uint32_t mine = byte[0] | byte[1] << 16, other = __shfl_xor_sync(kFull, mine, 16);
-  if (lane == 0) *reinterpret_cast<uint32_t*>(scales + fp8_scale_at(row, g * 4, (rows + 127) / 128)) = mine | other << 8;
+#pragma unroll
+  for (int i = 0; i < TASKS; ++i) {
+    if (row[i] >= rows) return;
+    uint32_t byte[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int64_t e = g[i] * 512 + k * 256 + lane * 8;
+      bool bad;
+      byte[k] = fp8_scale_byte(half_warp_max(fp8_most(v[i][k], bad)));
+      if (e < ldc) *reinterpret_cast<uint2*>(codes + row[i] * ldc + e) = fp8_codes8(v[i][k], fp8_factor(byte[k]), bad);
+    }
+    const uint32_t mine = byte[0] | byte[1] << 16, other = __shfl_xor_sync(kFull, mine, 16);
+    if (lane == 0) *reinterpret_cast<uint32_t*>(scales + fp8_scale_at(row[i], g[i] * 4, (rows + 127) / 128)) = mine | other << 8;
+  }
+}
+
+// The magnitudes of a vector's elements as words that can be compared: one of float32, two of a 16-bit type side by side.
+template <typename T> constexpr int word_columns() { return 4 / (int)sizeof(T); }
+template <typename T> ACTNN_DEV uint32_t word_max(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
+template <typename T> ACTNN_DEV uint32_t word_abs(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
+// Zero in the place of what is not finite.
+template <typename T> ACTNN_DEV uint32_t word_finite(uint32_t w) {
+  if (sizeof(T) == 4) return not_finite(w) ? 0u : w;
+  const float2 f = pair_to_float(w, T());
+  return (not_finite(__float_as_uint(f.x)) ? 0u : w & 0xffffu) | (not_finite(__float_as_uint(f.y)) ? 0u : w & 0xffff0000u);
+}
+template <> ACTNN_DEV uint32_t word_finite<float>(uint32_t w) { return not_finite(w) ? 0u : w; }
+// The bits of float32 of one of a word's magnitudes.
+template <typename T> ACTNN_DEV uint32_t word_bits(uint32_t w, int which) { return abs_bits(pair_to_float(which ? w >> 16 : w & 0xffffu, T()).x); }
+template <> ACTNN_DEV uint32_t word_bits<float>(uint32_t w, int) { return w; }
+// Columns 2 j and 2 j + 1 of a vector.
+template <typename T> ACTNN_DEV float2 column_pair(const Vec<T, 8>& v, int j) { return pair_to_float(v.w[j], T()); }
+template <> ACTNN_DEV float2 column_pair<float>(const Vec<float, 8>& v, int j) {
+  return make_float2(__uint_as_float(v.w[2 * j]), __uint_as_float(v.w[2 * j + 1]));
 }
 
 // A tile of 128 x 128: a thread has eight neighbouring columns of eight neighbouring rows.  SQUARE: one scale for the tile.
-// codes, codes_t and parts may be NULL; parts [tiles of rows][cols] are the sums of the tile's columns.
+// codes, codes_t and parts may be NULL; parts [tiles of rows][cols] are the sums of the tile's columns.  Registers are what bounds the
+// loads under way: three blocks an SM hold 96 KB of a 16-bit type (one block, with maxima kept as float32: 8192 x 4096 and 8192 x 2048
+// both ways 71 us together; the floor is 31).
 template <typename T, bool VEC, bool SQUARE>
-__global__ void __launch_bounds__(kCodeThreads)
+__global__ void __launch_bounds__(kCodeThreads, sizeof(T) == 4 ? 2 : 3)
 fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales, uint8_t* __restrict__ codes_t,
                       uint8_t* __restrict__ scales_t, float* __restrict__ parts, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc,
                       int64_t ldt, int column_tiles) {
+  constexpr int kWords = 8 / word_columns<T>();
   __shared__ uint4 turned_s[128 * 8];                  // [column][128 rows], chunks of eight rows in the order rotated by column / 8
-  __shared__ uint32_t most_s[16][128];
+  __shared__ uint32_t most_s[16][128];                 // [team][word of columns]; later float sums of columns
   __shared__ float factor_s[128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c8 = lane & 15, team = warp * 2 + (lane >> 4);
   const int64_t tr = blockIdx.x / column_tiles, tc = blockIdx.x - tr * column_tiles, r0 = tr * 128 + team * 8, c = tc * 128 + c8 * 8;
@@ -51,22 +85,14 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = fp8_load<T, VEC>(x + (r0 + i) * ldx, c, r0 + i < rows ? cols : 0);
 
-  // ---- the largest of rows, of columns or of all
-  uint32_t bad = 0, row_most[8], column_most[8] = {};
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    bool b;
-    row_most[i] = fp8_most(v[i], b);
-    bad |= (uint32_t)b << i;
-  }
-  if (!SQUARE) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) row_most[i] = half_warp_max(row_most[i]);
-  }
-  uint32_t square = 0;
+  uint32_t bad = 0, square = 0;                         // bad: rows with elements that are not finite
   if (SQUARE) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) square = max(square, row_most[i]);
+    for (int i = 0; i < 8; ++i) {
+      bool b;
+      square = max(square, fp8_most(v[i], b));
+      bad |= (uint32_t)b << i;
+    }
     square = __reduce_max_sync(kFull, square);
     if (lane == 0) most_s[0][warp] = square;
     __syncthreads();
@@ -74,44 +100,41 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
 #pragma unroll
     for (int w = 1; w < kCodeThreads / 32; ++w) square = max(square, most_s[0][w]);
     square = fp8_scale_byte(square);
-  } else if (codes_t) {
+  }
+  // ---- rows, and the largest of the thread's columns
+  uint32_t most[kWords] = {};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float2 f[4];
-      unpack_vec(v[i], f);
+  for (int i = 0; i < 8; ++i) {
+    uint32_t byte = square;
+    if (!SQUARE) {
+      bool b;
+      byte = fp8_most(v[i], b);
+      bad |= (uint32_t)b << i;
+      if (codes) byte = fp8_scale_byte(half_warp_max(byte));
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        uint32_t a = abs_bits(f[j].x), b = abs_bits(f[j].y);
-        if (bad >> i & 1) a = not_finite(a) ? 0 : a, b = not_finite(b) ? 0 : b;
-        column_most[2 * j] = max(column_most[2 * j], a);
-        column_most[2 * j + 1] = max(column_most[2 * j + 1], b);
+      for (int j = 0; j < kWords; ++j) {
+        const uint32_t w = word_abs<T>(v[i].w[j]);
+        most[j] = word_max<T>(most[j], b ? word_finite<T>(w) : w);
       }
     }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) most_s[team][c8 * 8 + j] = column_most[j];
-  }
-
-  // ---- rows
-  if (codes) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t byte = SQUARE ? square : fp8_scale_byte(row_most[i]);
-      if (r0 + i < rows) {
-        if (c < ldc) *reinterpret_cast<uint2*>(codes + (r0 + i) * ldc + c) = fp8_codes8(v[i], fp8_factor(byte), bad >> i & 1);
-        if (c8 == 0) scales[fp8_scale_at(r0 + i, tc, (rows + 127) / 128)] = (uint8_t)byte;
-      }
+    if (codes && r0 + i < rows) {
+      if (c < ldc) *reinterpret_cast<uint2*>(codes + (r0 + i) * ldc + c) = fp8_codes8(v[i], fp8_factor(byte), bad >> i & 1);
+      if (c8 == 0) scales[fp8_scale_at(r0 + i, tc, (rows + 127) / 128)] = (uint8_t)byte;
     }
   }
 
   // ---- columns
   if (codes_t) {
     if (!SQUARE) {
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) most_s[team][c8 * kWords + j] = most[j];
       __syncthreads();
       if (threadIdx.x < 128) {
-        uint32_t most = most_s[0][threadIdx.x];
+        const int word = threadIdx.x / word_columns<T>();
+        uint32_t all = most_s[0][word];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) most = max(most, most_s[k][threadIdx.x]);
-        const uint32_t byte = fp8_scale_byte(most);
+        for (int k = 1; k < 16; ++k) all = word_max<T>(all, most_s[k][word]);
+        const uint32_t byte = fp8_scale_byte(word_bits<T>(all, threadIdx.x % word_columns<T>()));
         factor_s[threadIdx.x] = fp8_factor(byte);
         if (tc * 128 + threadIdx.x < cols) scales_t[fp8_scale_at(tc * 128 + threadIdx.x, tr, column_tiles)] = (uint8_t)byte;
       }
@@ -125,12 +148,10 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
       uint32_t px[4], py[4];                           // two rows each
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        float2 a[4], b[4];
-        unpack_vec(v[i], a);
-        unpack_vec(v[i + 1], b);
-        if (bad) a[j] = make_float2(finite_or_nan(a[j].x), finite_or_nan(a[j].y)), b[j] = make_float2(finite_or_nan(b[j].x), finite_or_nan(b[j].y));
-        px[i / 2] = fp8_pair(a[j].x * fx, b[j].x * fx);
-        py[i / 2] = fp8_pair(a[j].y * fy, b[j].y * fy);
+        float2 a = column_pair(v[i], j), b = column_pair(v[i + 1], j);
+        if (bad) a = make_float2(finite_or_nan(a.x), finite_or_nan(a.y)), b = make_float2(finite_or_nan(b.x), finite_or_nan(b.y));
+        px[i / 2] = fp8_pair(a.x * fx, b.x * fx);
+        py[i / 2] = fp8_pair(a.y * fy, b.y * fy);
       }
       uint2* at = reinterpret_cast<uint2*>(turned_s) + (c8 * 8 + 2 * j) * 16 + (team ^ c8);
       at[0] = make_uint2(px[0] | px[1] << 16, px[2] | px[3] << 16);
@@ -155,11 +176,7 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
     for (int j = 0; j < 4; ++j) {
       float2 s = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float2 f[4];
-        unpack_vec(v[i], f);
-        s = f_add(s, f[j]);
-      }
+      for (int i = 0; i < 8; ++i) s = f_add(s, column_pair(v[i], j));
       sum_s[team * 128 + c8 * 8 + 2 * j] = s.x;
       sum_s[team * 128 + c8 * 8 + 2 * j + 1] = s.y;
     }
@@ -216,9 +233,14 @@ fp8_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
 
 template <typename T>
 int row_codes(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc, cudaStream_t s) {
-  const int64_t groups = (cols + 511) / 512, grid = (rows * groups + kCodeThreads / 32 - 1) / (kCodeThreads / 32);
+  // two tasks a warp keep more loads under way, where there are warps enough (16384 x 4096 bfloat16: 40 us with one)
+  const int64_t groups = (cols + 511) / 512, tasks = rows * groups;
+  const int each = tasks >= (int64_t)device_info().sm_count * 256 ? 2 : 1;
+  const int64_t grid = (tasks + kCodeThreads / 32 * each - 1) / (kCodeThreads / 32 * each);
   if (grid > 0x7fffffff) return ACTNN_ERR_SHAPE;
-  auto* kernel = cols % 8 == 0 && (ldx % 8 == 0 || rows == 1) && aligned(x, 16) ? fp8_row_codes_kernel<T, true> : fp8_row_codes_kernel<T, false>;
+  const bool vec = cols % 8 == 0 && (ldx % 8 == 0 || rows == 1) && aligned(x, 16);
+  auto* kernel = vec ? (each == 2 ? fp8_row_codes_kernel<T, true, 2> : fp8_row_codes_kernel<T, true, 1>)
+                     : (each == 2 ? fp8_row_codes_kernel<T, false, 2> : fp8_row_codes_kernel<T, false, 1>);
   kernel<<<(unsigned)grid, kCodeThreads, 0, s>>>((const T*)x, codes, scales, rows, cols, ldx, ldc, (int)groups);
   return check_launch();
 }

@@ -179,7 +179,7 @@ extern "C" int actnn_fp8_linear(const void* x, const uint8_t* weights, const uin
     if (workspace_bytes < codes + fp8_scale_bytes(T, K)) return ACTNN_ERR_CAPACITY;
     uint8_t *c = (uint8_t*)workspace, *s = c + codes;
     if (int st = actnn_fp8_row_codes(x, c, s, T, K, ldx, fp8_row_bytes(K), dtype, stream)) return st;
-    return fp8_matmul_impl(c, s, weights, weight_scales, bias, out, T, N, K, fp8_row_bytes(K), ldw, dtype, false, stream);
+    return fp8_matmul_impl(c, s, weights, weight_scales, bias, out, T, N, K, fp8_row_bytes(K), ldw, dtype, true, stream);
   }
   const cudaStream_t s = (cudaStream_t)stream;
   switch (dtype) {

@@ -16,6 +16,7 @@
 //
 // Every wait is bounded, with the integer product's rules: a block whose wait runs out writes nothing more, is counted, lets its copies
 // and instructions end and leaves; the epilogue's warps leave together; of blocks that share a reduction none writes.
+#include <algorithm>
 #include <atomic>
 
 #include "fp8.cuh"
@@ -32,9 +33,9 @@ constexpr int kFpStageK = 128;                  // bytes of the reduction in a s
 constexpr int kFpChannels = 128;
 constexpr int kFpStaging = 32 * 1024;           // outputs on their way: two buffers for each half of the epilogue's warps
 constexpr int kFpSmem = 216 * 1024;             // of the SM's 227 KB: stages with their scales, and 1 KB to align them
-constexpr int kFpScales = 2048;                 // of a stage: 512 bytes for the channels, up to three times that for the tokens
 constexpr int kFpTokens = 224;                  // of an accumulator that has a twin
-constexpr int kFpScaleSets = 4, kFpScaleColumns = 16;
+constexpr int kFpWide = 448;                    // of one that has none
+constexpr int kFpScaleSets = 4;                 // at most, of columns of tensor memory
 
 struct FpArgs {
   const void* bias;
@@ -43,7 +44,10 @@ struct FpArgs {
   int K, tokens, stages, k_blocks, splits;      // tokens: columns of a tile
   int channel_tiles, tiles, columns;            // columns: of tensor memory, all
   int atoms, scale_rows_w, scale_rows_x;        // sets of 128 rows that a tile's tokens lie in; that the operands have
+  int stage_scales, sets, set_columns;          // bytes of a stage's scales; sets of columns for them
+  int first;                                    // of a wide tile: the tokens of its first half
   bool pair;                                    // tiles of 256 channels by pairs of blocks
+  bool wide;                                    // one accumulator of two halves
   bool boxes;                                   // outputs leave as boxes of 128 channels
   bool vectors;                                 // four outputs of a token at a time are aligned
   bool early;                                   // the launch before this one makes the tokens' codes, and is not waited for sooner than they are read
@@ -94,10 +98,13 @@ ACTNN_DEV bool epilogue_agrees(bool ok) {
 
 // SPLIT: the reduction is split over a cluster.  PAIR: a cluster of two blocks computes a tile of 256 channels, half of the channels
 // and half of the tokens' operand in each; the first one issues the matrix instructions, its barriers count the copies of both.
-template <typename T, bool SPLIT, bool PAIR>
+// WIDE (of a pair): one accumulator of up to 448 columns instead of two, since what an SM gets from the L2 limits the tiles of
+// 192.  Its columns are two halves: while the epilogue has the second one, the matrix instructions begin the next tile with the first,
+// for as many stages as there are, and then catch up.
+template <typename T, bool SPLIT, bool PAIR, bool WIDE>
 __global__ void __launch_bounds__(kFpThreads, 1)
 fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_constant__ CUtensorMap tokens,
-                  const __grid_constant__ CUtensorMap weight_scales, const __grid_constant__ CUtensorMap token_scales,
+                  const __grid_constant__ CUtensorMap more_tokens, const __grid_constant__ CUtensorMap weight_scales, const __grid_constant__ CUtensorMap token_scales,
                   const __grid_constant__ CUtensorMap outputs, const FpArgs a, unsigned* gave_up) {
   extern __shared__ uint8_t dynamic_s[];
   __shared__ FpShared s;
@@ -155,7 +162,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
     };
     auto request_weights = [&](uint32_t bar, int stage, int k, bool begins, int row) {
       request(bar, stage0 + stage * stage_bytes, &weights, k * kFpStageK, row);
-      if (begins) request(bar, scales0 + stage * kFpScales, &weight_scales, 0, 2 * ((k >> 2) * a.scale_rows_w + (row >> 7)));
+      if (begins) request(bar, scales0 + stage * a.stage_scales, &weight_scales, 0, 2 * ((k >> 2) * a.scale_rows_w + (row >> 7)));
     };
     if (a.early) {                                              // weights of the first stages before the tokens are there
       const int row = first_tile % a.channel_tiles * tile_channels + channel_step;
@@ -185,8 +192,14 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
             expect(bar, begins);
             request_weights(bar, now, k, begins, row);
           }
-          request(bar, stage0 + now * stage_bytes + a_bytes, &tokens, k * kFpStageK, t0 + token_step);
-          if (begins) request(bar, scales0 + now * kFpScales + 512, &token_scales, 0, 2 * ((k >> 2) * a.scale_rows_x + (t0 >> 7)));
+          if constexpr (WIDE) {                                 // half of each half
+            request(bar, stage0 + now * stage_bytes + a_bytes, &tokens, k * kFpStageK, t0 + (int)rank * (a.first / 2));
+            request(bar, stage0 + now * stage_bytes + a_bytes + a.first / 2 * kFpStageK, &more_tokens, k * kFpStageK,
+                    t0 + a.first + (int)rank * ((a.tokens - a.first) / 2));
+          } else {
+            request(bar, stage0 + now * stage_bytes + a_bytes, &tokens, k * kFpStageK, t0 + token_step);
+          }
+          if (begins) request(bar, scales0 + now * a.stage_scales + 512, &token_scales, 0, 2 * ((k >> 2) * a.scale_rows_x + (t0 >> 7)));
         }
         ++issued;
       }
@@ -202,45 +215,82 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
   } else if (warp == 9) {                                       // ---------------- matrix instructions
     if (a.early) grid_wait();                                   // the limit of a wait is for copies, not for the launch before
     if (!PAIR || rank == 0) {
-      const uint32_t instruction = fp8_instruction(tile_channels, a.tokens, 0), one_byte = fp8_instruction(tile_channels, a.tokens, 1) - instruction;
-      const uint32_t sets = tmem + (SPLIT ? 1 : 2) * a.tokens;
+      const int first = WIDE ? a.first : a.tokens;
+      const uint32_t instruction = fp8_instruction(tile_channels, first, 0), second = fp8_instruction(tile_channels, a.tokens - first, 0);
+      const uint32_t one_byte = fp8_instruction(tile_channels, first, 1) - instruction, sets = tmem + (SPLIT || WIDE ? 1 : 2) * a.tokens;
       int stage = 0, buf = 0, set = 0;
-      uint32_t phase = 0, buf_phase = 0;
+      uint32_t phase = 0, buf_phase = 0, d = tmem, at_w = 0, shift = 0;
       bool ok = true;
+      auto next = [&](int& at, uint32_t& at_phase) { if (++at == a.stages) at = 0, at_phase ^= 1; };
+      // One lane: the scales of a stage that begins a set; the products of a stage, `half` of a wide tile.
+      auto scales = [&](int at) {
+        const uint32_t from = scales0 + at * a.stage_scales;
+        scales_to_tmem<PAIR>(at_w, from);
+        scales_to_tmem<PAIR>(at_w + 4, from + 512);
+        if (a.atoms > 1) scales_to_tmem<PAIR>(at_w + 8, from + 1024);
+        if (a.atoms > 2) scales_to_tmem<PAIR>(at_w + 12, from + 1536);
+        if (WIDE && a.atoms > 3) scales_to_tmem<PAIR>(at_w + 16, from + 2048);
+      };
+      auto multiply = [&](int at, int k, int half) {
+        const uint32_t from = stage0 + at * stage_bytes;
+        const uint64_t da = rows128_descriptor(from), db = rows128_descriptor(from + a_bytes + (half ? first / 2 * kFpStageK : 0));
+        const uint32_t instr = (half ? second : instruction) + (k & 3) * one_byte, to = d + (half ? first : 0);
+        const uint32_t at_x = at_w + 4 + shift + (half ? first / 32 : 0);
+#pragma unroll
+        for (int i = 0; i < kFpStageK / 32; ++i)                // 32 bytes further along the rows: 2 in units of 16 bytes
+          mma_fp8<PAIR>(to, da + 2 * i, db + 2 * i, instr, at_w, at_x, k > k_first || i > 0);
+      };
       for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
-        if (!(ok = fp_wait(smem_addr(&s.sum_empty[buf]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+        if (!(ok = fp_wait(smem_addr(&s.sum_empty[WIDE ? 0 : buf]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
         tmem_fence_after_sync();
-        const uint32_t d = tmem + buf * a.tokens, shift = (tile / a.channel_tiles * a.tokens & 127) / 32;   // columns from a set of 128 tokens
-        uint32_t at_w = 0;
+        d = tmem + (WIDE ? 0 : buf * a.tokens);
+        shift = (tile / a.channel_tiles * a.tokens & 127) / 32;                     // columns from a set of 128 tokens
+        int k = k_first;
+        if constexpr (WIDE) {                                   // a set of scales covers the stages that are caught up on
+          const int head = min(min(a.stages, 4), k_end - k_first);
+          int at = stage;
+          uint32_t at_phase = phase;
+          at_w = sets + set * a.set_columns;
+          if (++set == a.sets) set = 0;
+          for (int i = 0; ok && i < head; ++i) {
+            if (!(ok = fp_wait(smem_addr(&s.full[at]), at_phase, s, issues ? gave_up : nullptr))) break;
+            if (elect_one()) {
+              if (i == 0) scales(at);
+              multiply(at, k_first + i, 0);
+            }
+            next(at, at_phase);
+          }
+          if (!ok || !(ok = fp_wait(smem_addr(&s.sum_empty[1]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+          tmem_fence_after_sync();
+          for (; k < k_first + head; ++k) {
+            if (elect_one()) {
+              multiply(stage, k, 1);
+              mma_commit<PAIR>(smem_addr(&s.empty[stage]));
+            }
+            next(stage, phase);
+          }
+        }
         bool ready = false;
-        for (int k = k_first; k < k_end; ++k) {
+        for (; k < k_end; ++k) {
           if (!ready && !(ok = fp_wait(smem_addr(&s.full[stage]), phase, s, issues ? gave_up : nullptr))) break;
           const int now = stage;
-          if (++stage == a.stages) stage = 0, phase ^= 1;
+          next(stage, phase);
           ready = fp_test(smem_addr(&s.full[stage]), phase);
           const bool begins = k == k_first || (k & 3) == 0;
           if (begins) {
-            at_w = sets + set * kFpScaleColumns;
-            set = (set + 1) % kFpScaleSets;
+            at_w = sets + set * a.set_columns;
+            if (++set == a.sets) set = 0;
           }
-          const uint32_t at = stage0 + now * stage_bytes, from = scales0 + now * kFpScales, instr = instruction + (k & 3) * one_byte;
-          const uint64_t da = rows128_descriptor(at), db = rows128_descriptor(at + a_bytes);
           if (elect_one()) {
-            if (begins) {
-              scales_to_tmem<PAIR>(at_w, from);
-              scales_to_tmem<PAIR>(at_w + 4, from + 512);
-              if (a.atoms > 1) scales_to_tmem<PAIR>(at_w + 8, from + 1024);
-              if (a.atoms > 2) scales_to_tmem<PAIR>(at_w + 12, from + 1536);
-            }
-#pragma unroll
-            for (int i = 0; i < kFpStageK / 32; ++i)            // 32 bytes further along the rows: 2 in units of 16 bytes
-              mma_fp8<PAIR>(d, da + 2 * i, db + 2 * i, instr, at_w, at_w + 4 + shift, k > k_first || i > 0);
+            if (begins) scales(now);
+            multiply(now, k, 0);
+            if constexpr (WIDE) multiply(now, k, 1);
             mma_commit<PAIR>(smem_addr(&s.empty[now]));
           }
         }
         if (!ok) break;
-        if (elect_one()) mma_commit<PAIR>(smem_addr(&s.sum_full[buf]));
-        if (++buf == 2) buf = 0, buf_phase ^= 1;
+        if (elect_one()) mma_commit<PAIR>(smem_addr(&s.sum_full[WIDE ? 0 : buf]));
+        if (WIDE || ++buf == 2) buf = 0, buf_phase ^= 1;
       }
       __syncwarp();
       if (elect_one()) {
@@ -265,11 +315,14 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
       if (!epilogue_agrees(ok)) break;
       tmem_fence_after_sync();
       const uint32_t d = tmem + buf * a.tokens + ((uint32_t)(quarter * 32) << 16);
+#pragma unroll
+      for (int part = 0; part < (WIDE ? 2 : 1); ++part) {
+      const int begin = part ? a.first : 0, end = WIDE && !part ? a.first : a.tokens;
       if (!SPLIT && a.boxes) {
         // The warps of a half turn kBoxTokens columns into rows of 128 channels in shared memory, which one thread sends off as a
         // box while the next ones are made.
         constexpr int kBoxTokens = box_tokens<T>();
-        for (int c = half * kBoxTokens; c < a.tokens; c += 2 * kBoxTokens) {
+        for (int c = begin + half * kBoxTokens; c < end; c += 2 * kBoxTokens) {
           const uint32_t box = stage0 + a.stages * stage_bytes + (half * 2 + box_buf) * (kFpStaging / 4);
           if ((threadIdx.x & 127) == 0) tile_store_read<1>();                       // the buffer's last box has been read
           asm volatile("bar.sync %0, 128;" :: "r"(2 + half) : "memory");
@@ -288,7 +341,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
           box_buf ^= 1;
         }
       } else
-      for (int c = half * 16; c < a.tokens; c += 32) {
+      for (int c = begin + half * 16; c < end; c += 32) {
         uint32_t r[16];
         tmem_load16(d + c, r);
         tmem_load_wait();
@@ -311,11 +364,12 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
         tmem_fence_before_sync();
         __syncwarp();
         if (lane == 0) {
-          if constexpr (PAIR) peer_arrive(peer_addr(smem_addr(&s.sum_empty[buf]), 0));
+          if constexpr (PAIR) peer_arrive(peer_addr(smem_addr(&s.sum_empty[WIDE ? part : buf]), 0));
           else mbar_arrive(smem_addr(&s.sum_empty[buf]));
         }
-        if (++buf == 2) buf = 0, buf_phase ^= 1;
       }
+      }
+      if (!SPLIT && (WIDE || ++buf == 2)) buf = 0, buf_phase ^= 1;
     }
   }
   if (!SPLIT && a.boxes && warp < 8 && (threadIdx.x & 127) == 0) tile_store_done();
@@ -377,61 +431,69 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
 }
 
 // ------------------------------------------------------------------ host
-// The cut: tokens of a tile, blocks that share a reduction, pairs or single blocks, by what they are expected to take (us): a
-// stage's bytes at what an SM gets from the L2 or its matrix instructions, the epilogue, and what a wave spends besides.  The
-// constants are fitted to times of all cuts for 16 to 16384 tokens, 500 to 16384 channels and reductions over 1000 to 8192, e.g.
-// 200 x 4096 x 4096: 208 tokens shared by four 12.4, by two 15.5, 64 tokens alone 14.2; 512 x 4096 x 4096: 128 tokens alone 15.1,
-// 256 shared by two 17.2; pairs or single blocks, 16384 x 4096 x 8192 360 / 390, 16384 x 1024 x 1024 23.0 / 21.5.
+// The cut: tokens of a tile, blocks that share a reduction, pairs or single blocks, two accumulators or a wide one, by what they are
+// expected to take (us): a stage, which is no shorter than its instructions take to issue, and what a tile takes besides.  Fitted to
+// times of all cuts in long runs, where the power cap sets the clock: 16384 x 4096 x 8192, 448 tokens wide 462, 192 by pairs 484, by single
+// blocks 546; 8192 x 2048 x 4096, 192 by pairs 72, 384 wide 74, 192 by single blocks 78; 4096 x 512 x 16384, 192 by single blocks 51, by
+// pairs 65, 448 wide 68; 1024 x 4096 x 4096, 256 wide 20.5, 128 by pairs 24.3; 100 x 8192 x 2048, 64 shared by four 10.5, by two 14.6, alone
+// 19.9.  Eight blocks that share a reduction find room for few such clusters at a time: 100 x 8192 x 2048 18.2 in two rounds.
 void plan(FpArgs& a) {
-  constexpr double kBytes = 100e3, kColumns = 950.;            // a microsecond: bytes of an SM, columns of a stage
   const int sms = device_info().sm_count;
   const int64_t least = a.T <= kFpTokens ? 1 : (a.T + kFpTokens / 64 * 64 - 1) / (kFpTokens / 64 * 64);
   const bool boxes = a.boxes;
   a.k_blocks = (a.K + kFpStageK - 1) / kFpStageK;
   double best = -1.;
-  auto offer = [&](int tokens, int splits, bool pair) {
+  auto offer = [&](int tokens, int splits, bool pair, bool wide) {
     // Scales of 32 tokens are a column, and the instructions want theirs to begin at an even one: where there are several tiles, they begin
-    // at multiples of 64 tokens.
-    const int step = a.T <= 16 && !boxes ? 16 : 32;
+    // at multiples of 64 tokens, and so does the second half of a wide one.
+    const int step = wide ? 64 : a.T <= 16 && !boxes ? 16 : 32;
     tokens = (tokens + step - 1) / step * step;
     if (tokens < a.T) tokens = (tokens + 63) / 64 * 64;
-    if (tokens > (splits > 1 ? 256 : kFpTokens)) return;
+    if (tokens > (wide ? kFpWide : splits > 1 ? 256 : kFpTokens) || (wide && tokens < 256)) return;
     const int channels = pair ? 2 * kFpChannels : kFpChannels;
     const int64_t channel_tiles = (a.N + channels - 1) / channels, tiles = channel_tiles * ((a.T + tokens - 1) / tokens);
     const int64_t blocks = tiles * splits * (pair ? 2 : 1), waves = (blocks + sms - 1) / sms;
-    if (splits > 1 && blocks > sms) return;
-    const double load = (kFpChannels + (pair ? tokens / 2 : tokens)) * kFpStageK / kBytes, multiply = tokens / kColumns;
-    const double stages = (a.k_blocks + splits - 1) / splits * (load > multiply ? load : multiply);
-    const double time = (double)waves * (stages + (splits > 1 ? 1.7 + tokens * 0.0075 : tokens * 0.006) + (pair ? 2. : 0.5));
+    if (splits > 1 && blocks > (splits > 4 ? 64 : sms)) return;
+    const double stage = wide ? tokens * 0.0017 : pair ? std::max(0.23, 0.15 + tokens * 0.00105) : std::max(splits > 1 ? 0.3 : 0.27, 0.2 + tokens * 0.0011);
+    const double besides = wide ? 3.8 : pair ? 0.8 + tokens * 0.004 : splits > 1 ? 3. + tokens * 0.0135 : 0.4 + tokens * 0.004;
+    const double time = (double)waves * ((a.k_blocks + splits - 1) / splits * stage + besides) + (pair ? 1. : 0.);
     if (best >= 0. && time >= best) return;
     best = time;
     a.tokens = tokens;
     a.splits = splits;
     a.pair = pair;
+    a.wide = wide;
     a.channel_tiles = (int)channel_tiles;
     a.tiles = (int)tiles;
   };
   for (const int64_t more : {1, 2, 3, 4, 6, 8}) {
     const int tokens = (int)((a.T + least * more - 1) / (least * more));
     if (more > 1 && tokens < 16) break;
-    for (int splits = 1; splits <= kFpSplitsMost && a.k_blocks >= 2 * splits; splits *= 2) offer(tokens, splits, false);
-    if (a.k_blocks < 2) offer(tokens, 1, false);
-    if (tokens > 64) offer(tokens, 1, true);
+    for (int splits = 1; splits <= kFpSplitsMost && a.k_blocks >= 2 * splits; splits *= 2) offer(tokens, splits, false, false);
+    if (a.k_blocks < 2) offer(tokens, 1, false, false);
+    if (tokens > 64) offer(tokens, 1, true, false);
   }
+  for (int tokens = 256; tokens <= kFpWide && tokens - 64 < a.T; tokens += 64) offer(tokens, 1, true, true);
   a.boxes = boxes && a.splits == 1;
+  a.first = a.wide ? (a.tokens / 2 + 63) / 64 * 64 : a.tokens;
   int common = 128;
   while (a.tokens % common) common /= 2;
   a.atoms = (128 - common + a.tokens + 127) / 128;
   if (a.T <= a.tokens) a.atoms = (a.tokens + 127) / 128;
+  a.set_columns = 4 + 4 * a.atoms;
+  a.stage_scales = 512 * (1 + a.atoms);
+  const int sums = (a.splits > 1 || a.wide ? 1 : 2) * a.tokens;
+  a.sets = (512 - sums) / a.set_columns;
+  if (a.sets > kFpScaleSets) a.sets = kFpScaleSets;
   a.columns = 32;
-  while (a.columns < (a.splits > 1 ? 1 : 2) * a.tokens + kFpScaleSets * kFpScaleColumns) a.columns *= 2;
-  a.stages = (kFpSmem - 1024 - (a.boxes ? kFpStaging : 0)) / ((kFpChannels + (a.pair ? a.tokens / 2 : a.tokens)) * kFpStageK + kFpScales);
+  while (a.columns < sums + a.sets * a.set_columns) a.columns *= 2;
+  a.stages = (kFpSmem - 1024 - (a.boxes ? kFpStaging : 0)) / ((kFpChannels + (a.pair ? a.tokens / 2 : a.tokens)) * kFpStageK + a.stage_scales);
   if (a.stages > kFpStagesMost) a.stages = kFpStagesMost;
 }
 
-struct FpMaps { CUtensorMap w, x, sw, sx, y; };
-template <typename T, bool SPLIT, bool PAIR> int launch(const FpMaps& m, const FpArgs& a, cudaStream_t stream) {
-  auto* kernel = fp8_matmul_kernel<T, SPLIT, PAIR>;
+struct FpMaps { CUtensorMap w, x, x2, sw, sx, y; };
+template <typename T, bool SPLIT, bool PAIR, bool WIDE> int launch(const FpMaps& m, const FpArgs& a, cudaStream_t stream) {
+  auto* kernel = fp8_matmul_kernel<T, SPLIT, PAIR, WIDE>;
   static std::atomic<uint64_t> raised{0};                       // devices whose limit of dynamic shared memory is raised
   int dev = 0;
   cudaGetDevice(&dev);
@@ -455,14 +517,17 @@ template <typename T, bool SPLIT, bool PAIR> int launch(const FpMaps& m, const F
   cfg.attrs = at;
   cfg.numAttrs = a.early ? 2 : 1;
   unsigned* gave_up = bulk_wait_counter();
-  if (cudaLaunchKernelEx(&cfg, kernel, m.w, m.x, m.sw, m.sx, m.y, a, gave_up) != cudaSuccess) {
+  if (cudaLaunchKernelEx(&cfg, kernel, m.w, m.x, m.x2, m.sw, m.sx, m.y, a, gave_up) != cudaSuccess) {
     cudaGetLastError();
     return ACTNN_ERR_LAUNCH;
   }
   return check_launch();
 }
 template <typename T> int launch_typed(const FpMaps& m, const FpArgs& a, cudaStream_t stream) {
-  return a.pair ? launch<T, false, true>(m, a, stream) : a.splits > 1 ? launch<T, true, false>(m, a, stream) : launch<T, false, false>(m, a, stream);
+  return a.wide        ? launch<T, false, true, true>(m, a, stream)
+         : a.pair      ? launch<T, false, true, false>(m, a, stream)
+         : a.splits > 1 ? launch<T, true, false, false>(m, a, stream)
+                       : launch<T, false, false, false>(m, a, stream);
 }
 
 }  // namespace
@@ -496,7 +561,8 @@ int actnn::fp8_matmul_impl(const uint8_t* tokens, const uint8_t* token_scales, c
   FpMaps m{};
   if (a.boxes && !map_values(&m.y, out, N, T, dtype, kFpChannels, kFpStaging / 4 / (kFpChannels * size))) return ACTNN_ERR_LAUNCH;
   if (!map_bytes(&m.w, weights, K, N, ld_weights, kFpStageK, kFpChannels, true) ||
-      !map_bytes(&m.x, tokens, K, T, ld_tokens, kFpStageK, a.pair ? a.tokens / 2 : a.tokens, true) ||
+      !map_bytes(&m.x, tokens, K, T, ld_tokens, kFpStageK, a.wide ? a.first / 2 : a.pair ? a.tokens / 2 : a.tokens, true) ||
+      (a.wide && !map_bytes(&m.x2, tokens, K, T, ld_tokens, kFpStageK, (a.tokens - a.first) / 2, true)) ||
       !map_bytes(&m.sw, weight_scales, 256, 2 * rows_w * groups, 256, 256, 2, false) ||
       !map_bytes(&m.sx, token_scales, 256, 2 * rows_x * groups, 256, 256, 2 * a.atoms, false)) return ACTNN_ERR_LAUNCH;
   switch (dtype) {

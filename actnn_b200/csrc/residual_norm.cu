@@ -1,5 +1,6 @@
 // The norms around a residual branch: arguments, and the cut of the kernels of residual_norm.cuh.
 #include <algorithm>
+#include <mutex>
 
 #include "residual_norm.cuh"
 
@@ -44,6 +45,22 @@ int rn_dispatch(const RnArgs& a, int dtype, RnWhat what, bool vec) {
 bool rn_dtype(int d) { return d >= ACTNN_F32 && d <= ACTNN_BF16; }
 
 }  // namespace
+
+// Asked of the occupancy calculator once for each kernel, number of threads and device.
+int rn_blocks_per_sm(const void* kernel, int threads) {
+  struct Entry { const void* kernel; int threads, device, blocks; };
+  static Entry table[1024];
+  static int used = 0;
+  static std::mutex lock;
+  int device = 0, blocks = 0;
+  cudaGetDevice(&device);
+  std::lock_guard<std::mutex> guard(lock);
+  for (int i = 0; i < used; ++i)
+    if (table[i].kernel == kernel && table[i].threads == threads && table[i].device == device) return table[i].blocks;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0) != cudaSuccess || blocks < 1) cudaGetLastError(), blocks = 1;
+  if (used < 1024) table[used++] = Entry{kernel, threads, device, blocks};
+  return blocks;
+}
 }  // namespace actnn
 
 using namespace actnn;

@@ -18,6 +18,8 @@
 // joint reduction, not two.
 #pragma once
 
+#include <algorithm>
+
 #include "cluster.cuh"
 #include "dropout.cuh"
 
@@ -54,6 +56,7 @@ struct RnArgs {
   bool coded;                                                   // backward: of codes, else of x and f
   cudaStream_t stream;
 };
+int rn_blocks_per_sm(const void* kernel, int threads);           // of this many threads, resident at a time
 enum RnWhat { kRnForward, kRnBackward };
 int rn_run_f32(const RnArgs& a, RnWhat what, bool vec);
 int rn_run_f16(const RnArgs& a, RnWhat what, bool vec);
@@ -179,132 +182,154 @@ ACTNN_DEV float2 rn_drop(float2 v, float2 m) {
   return make_float2(m.x != 0.f ? y.x : 0.f, m.y != 0.f ? y.y : 0.f);
 }
 
-// ------------------------------------------------------------------ sums over the threads of a row
-template <int N> struct Sums { float v[N]; };
-// WARP: a warp has the row.  Otherwise the block has it, and `place` counts its reductions: two are never under way at a time, so two
-// places suffice.
-template <int N, bool WARP> ACTNN_DEV Sums<N> rn_sum(Sums<N> s, int place) {
+// ------------------------------------------------------------------ forward
+// The sum over the threads of a row: a warp's, or a block's, whose reductions take two places in turn (two are never under way at a time).
+template <bool WARP> ACTNN_DEV float rn_sum(float v, int& place) {
 #pragma unroll
-  for (int i = 0; i < N; ++i)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s.v[i] += __shfl_xor_sync(kFull, s.v[i], o);
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   if constexpr (!WARP) {
-    __shared__ Sums<N> part_s[2][16];
-    const int warps = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) part_s[place & 1][threadIdx.x >> 5] = s;
+    __shared__ float part_s[2][kRnMostThreads / 32];
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) part_s[place][threadIdx.x >> 5] = v;
     __syncthreads();
-    s = part_s[place & 1][0];
-    for (int w = 1; w < warps; ++w) {
+    v = lane < (int)(blockDim.x >> 5) ? part_s[place][lane] : 0.f;
 #pragma unroll
-      for (int i = 0; i < N; ++i) s.v[i] += part_s[place & 1][w].v[i];
-    }
+    for (int o = kRnMostThreads / 64; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
+    v = __shfl_sync(kFull, v, 0);
+    place ^= 1;
   }
-  return s;
+  return v;
 }
-// Mean (of the layer kind) and reciprocal deviation of a row.
+// Mean (of the layer kind) and reciprocal deviation of a row.  Values behind C are zero.
 template <int V, bool WARP> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int lane, int lanes, const RnArgs& a, int& place) {
   float mean = 0.f;
+  float2 s = make_float2(0.f, 0.f);
   if (a.layer) {
-    float2 s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = f_add(s, v[k][i]);      // zero behind C
-    mean = rn_sum<1, WARP>({{f_sum(s)}}, place++).v[0] * a.inv_c;
-  }
-  float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * lanes + lane) * 8;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 e = make_float2(c + 2 * i < a.C ? v[k][i].x - mean : 0.f, c + 2 * i + 1 < a.C ? v[k][i].y - mean : 0.f);
-      s = f_fma(e, e, s);
-    }
-  }
-  return make_float2(mean, rsqrtf(rn_sum<1, WARP>({{f_sum(s)}}, place++).v[0] * a.inv_c + a.eps));
-}
-
-// ------------------------------------------------------------------ forward
-template <typename T, int V, bool WARP, bool VEC>
-__global__ void __launch_bounds__(WARP ? kRnThreads : 512) rn_forward_kernel(const __grid_constant__ RnArgs a) {
-  const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  const uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  if (WARP && row >= a.rows) return;
-  const size_t at = (size_t)row * a.C;
-  Vec<T, 8> xv[V], fv[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) fv[k] = rn_load<T, VEC>((const T*)a.f + at, (k * lanes + lane) * 8, a.C);
-#pragma unroll
-  for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>((const T*)a.x + at, (k * lanes + lane) * 8, a.C);
-  if (a.cx) {
-    // a warp's vectors are 256 channels that share a scale
+      for (int i = 0; i < 4; ++i) s = f_add(s, v[k][i]);
+    mean = rn_sum<WARP>(f_sum(s), place) * a.inv_c;
+    s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * lanes + lane) * 8, first = (k * lanes + (lane & ~31)) * 8;
-      if (first >= a.C) continue;
-      auto code = [&](const Vec<T, 8>& v, int8_t* codes, float* scales) {
-        const float most = largest(__reduce_max_sync(kFull, most_of(v))), factor = code_factor(most);
-        float2 q[4];
-        unpack_vec(v, q);
+      const int c = (k * lanes + lane) * 8;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) q[i] = code_bits(q[i], make_float2(factor, factor));
-        rn_store_codes<VEC>(codes + at, c, a.C, q);
-        if ((threadIdx.x & 31) == 0) scales[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
-      };
-      code(fv[k], a.cf, a.sf);
-      code(xv[k], a.cx, a.sx);
+      for (int i = 0; i < 4; ++i) {
+        const float2 e = make_float2(c + 2 * i < a.C ? v[k][i].x - mean : 0.f, c + 2 * i + 1 < a.C ? v[k][i].y - mean : 0.f);
+        s = f_fma(e, e, s);
+      }
     }
-  }
-  float2 u[V][4];
+  } else {
 #pragma unroll
-  for (int k = 0; k < V; ++k) unpack_vec(fv[k], u[k]);
-  int place = 0;
-  const float2 one = a.post ? rn_statistics<V, WARP>(u, lane, lanes, a, place) : make_float2(0.f, 1.f);
+    for (int k = 0; k < V; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s = f_fma(v[k][i], v[k][i], s);
+  }
+  return make_float2(mean, rsqrtf(rn_sum<WARP>(f_sum(s), place) * a.inv_c + a.eps));
+}
+
+// A warp, or a block, goes through rows; a thread has V vectors of eight channels of each.  The next row's inputs are requested as soon
+// as this row's are unpacked (unless V is so large that registers are short), so that the two or four reductions of a row do
+// not wait for memory.
+template <typename T, int V, bool WARP, bool VEC>
+__global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && !WARP ? 2 : 1) rn_forward_kernel(const __grid_constant__ RnArgs a) {
+  constexpr bool kAhead = V <= 4;
+  const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
+  uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
+  const uint32_t step = WARP ? gridDim.x * (kRnThreads / 32) : gridDim.x;
+  Vec<T, 8> xv[V], fv[V];
+  auto load = [&](uint32_t r) {
+    const size_t at = (size_t)r * a.C;
+#pragma unroll
+    for (int k = 0; k < V; ++k) fv[k] = rn_load<T, VEC>((const T*)a.f + at, (k * lanes + lane) * 8, a.C);
+#pragma unroll
+    for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>((const T*)a.x + at, (k * lanes + lane) * 8, a.C);
+  };
   NoiseKey key;
   if (a.dropped) key = drop_key(a.drop);
-  const void* gate = rn_gate_row(a, row);
+  if (kAhead && row < a.rows) load(row);
+  for (int place = 0; row < a.rows; row += step) {
+    const size_t at = (size_t)row * a.C;
+    if (!kAhead) load(row);
+    if (a.cx) {
+      // a warp's vectors are 256 channels that share a scale
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * lanes + lane) * 8;
-    float2 w[4], b[4], g[4], x[4];
-    unpack_vec(xv[k], x);
-    if (c < a.C) {
+      for (int k = 0; k < V; ++k) {
+        const int c = (k * lanes + lane) * 8, first = (k * lanes + (lane & ~31)) * 8;
+        if (first >= a.C) continue;
+        auto code = [&](const Vec<T, 8>& v, int8_t* codes, float* scales) {
+          const float most = largest(__reduce_max_sync(kFull, most_of(v))), factor = code_factor(most);
+          float2 q[4];
+          unpack_vec(v, q);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) q[i] = code_bits(q[i], make_float2(factor, factor));
+          rn_store_codes<VEC>(codes + at, c, a.C, q);
+          if ((threadIdx.x & 31) == 0) scales[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
+        };
+        code(fv[k], a.cf, a.sf);
+        code(xv[k], a.cx, a.sx);
+      }
+    }
+    float2 u[V][4], x[V][4];
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      unpack_vec(fv[k], u[k]);
+      unpack_vec(xv[k], x[k]);
+    }
+    if (kAhead && row + step < a.rows) load(row + step);
+    const float2 one = a.post ? rn_statistics<V, WARP>(u, lane, lanes, a, place) : make_float2(0.f, 1.f);
+    const void* gate = rn_gate_row(a, row);
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * lanes + lane) * 8;
+      if (c >= a.C) continue;
+      float2 p[4];
       if (a.post) {
-        rn_parameter(a.w1, a.pdtype, c, a.C, a.pvec, 1.f, w);
-        rn_parameter(a.b1, a.pdtype, c, a.C, a.pvec, 0.f, b);
+        rn_parameter(a.w1, a.pdtype, c, a.C, a.pvec, 1.f, p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          u[k][i] = f_fma(f_mul(f_add(u[k][i], make_float2(-one.x, -one.x)), make_float2(one.y, one.y)), w[i], b[i]);
+        for (int i = 0; i < 4; ++i) u[k][i] = f_mul(f_mul(f_add(u[k][i], make_float2(-one.x, -one.x)), make_float2(one.y, one.y)), p[i]);
+        if (a.b1) {
+          rn_parameter(a.b1, a.pdtype, c, a.C, a.pvec, 0.f, p);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
+        }
       }
       if (a.dropped) {
-        float2 m[4];
-        rn_factors<VEC>(a, key, row, c, m);
+        rn_factors<VEC>(a, key, row, c, p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[k][i] = rn_drop(u[k][i], m[i]);
+        for (int i = 0; i < 4; ++i) u[k][i] = rn_drop(u[k][i], p[i]);
       }
-      rn_parameter(gate, a.gdtype, c, a.C, a.pvec, 1.f, g);
+      if (gate) {
+        rn_parameter(gate, a.gdtype, c, a.C, a.pvec, 1.f, p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[k][i] = f_fma(u[k][i], g[i], f_mul(x[i], make_float2(a.scale, a.scale)));
+        for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[k][i] = f_fma(x[k][i], make_float2(a.scale, a.scale), u[k][i]);
       rn_store<T, VEC>((T*)a.r + at, c, a.C, u[k]);
       if constexpr (!VEC) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
       }
     }
-  }
-  const float2 two = rn_statistics<V, WARP>(u, lane, lanes, a, place);
-  if (a.stats && lane == 0) a.stats[row] = make_float4(one.x, one.y, two.x, two.y);
+    const float2 two = rn_statistics<V, WARP>(u, lane, lanes, a, place);
+    if (a.stats && lane == 0) a.stats[row] = make_float4(one.x, one.y, two.x, two.y);
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    const int c = (k * lanes + lane) * 8;
-    if (c >= a.C) continue;
-    float2 w[4], b[4];
-    rn_parameter(a.w2, a.pdtype, c, a.C, a.pvec, 1.f, w);
-    rn_parameter(a.b2, a.pdtype, c, a.C, a.pvec, 0.f, b);
+    for (int k = 0; k < V; ++k) {
+      const int c = (k * lanes + lane) * 8;
+      if (c >= a.C) continue;
+      float2 p[4];
+      rn_parameter(a.w2, a.pdtype, c, a.C, a.pvec, 1.f, p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) u[k][i] = f_fma(f_mul(f_add(u[k][i], make_float2(-two.x, -two.x)), make_float2(two.y, two.y)), w[i], b[i]);
-    rn_store<T, VEC>((T*)a.h + at, c, a.C, u[k]);
+      for (int i = 0; i < 4; ++i) u[k][i] = f_mul(f_mul(f_add(u[k][i], make_float2(-two.x, -two.x)), make_float2(two.y, two.y)), p[i]);
+      if (a.b2) {
+        rn_parameter(a.b2, a.pdtype, c, a.C, a.pvec, 0.f, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
+      }
+      rn_store<T, VEC>((T*)a.h + at, c, a.C, u[k]);
+    }
   }
 }
 
@@ -549,10 +574,10 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   if (LAYER) leave(db2, a.slot_b2), leave(db1, a.slot_b1);
 }
 
-// The partial sums of the runs, added in order: a block has 32 columns of one sum, eight threads a column.
+// The partial sums of the runs, added in order: a block has 32 columns of one sum, 32 threads a column.
 template <typename T>
-__global__ void __launch_bounds__(kRnThreads) rn_join_kernel(const __grid_constant__ RnArgs a) {
-  constexpr int kWays = kRnThreads / 32;
+__global__ void __launch_bounds__(1024) rn_join_kernel(const __grid_constant__ RnArgs a) {
+  constexpr int kWays = 32;
   __shared__ float part_s[kWays][32];
   const uint32_t blocks = (a.C + 31) / 32, which = blockIdx.x / blocks;
   const int way = threadIdx.x >> 5, column = (blockIdx.x - which * blocks) * 32 + (threadIdx.x & 31);
@@ -576,16 +601,17 @@ __global__ void __launch_bounds__(kRnThreads) rn_join_kernel(const __grid_consta
 }
 
 // ------------------------------------------------------------------ host
-// A warp has rows of up to 1024 channels, a block longer ones; as few vectors a thread as 512 threads need.
+// A warp has rows of up to 256 channels, a block longer ones; as few vectors a thread as 512 threads need.  As many blocks as are resident.
 template <typename T, bool VEC> int rn_forward(const RnArgs& a) {
   auto run = [&](auto kernel, bool warp, int V) {
-    const unsigned grid = warp ? (a.rows + kRnThreads / 32 - 1) / (kRnThreads / 32) : a.rows;
     const int threads = warp ? kRnThreads : (a.C + V * 256 - 1) / (V * 256) * 32;
-    kernel<<<grid, threads, 0, a.stream>>>(a);
+    const int64_t wanted = warp ? ((int64_t)a.rows + kRnThreads / 32 - 1) / (kRnThreads / 32) : a.rows;
+    const int64_t resident = (int64_t)device_info().sm_count * rn_blocks_per_sm((const void*)kernel, threads);
+    kernel<<<(unsigned)std::min(wanted, resident), threads, 0, a.stream>>>(a);
     return check_launch();
   };
   if (a.C <= 256) return run(rn_forward_kernel<T, 1, true, VEC>, true, 1);
-  if (a.C <= 1024) return run(rn_forward_kernel<T, 4, true, VEC>, true, 4);
+  if (a.C <= 4096) return run(rn_forward_kernel<T, 1, false, VEC>, false, 1);
   if (a.C <= 8192) return run(rn_forward_kernel<T, 2, false, VEC>, false, 2);
   if (a.C <= 16384) return run(rn_forward_kernel<T, 4, false, VEC>, false, 4);
   return run(rn_forward_kernel<T, 8, false, VEC>, false, 8);
@@ -611,7 +637,7 @@ template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const Rn
   if (int st = check_launch()) return st;
   if (a.slots == 0) return ACTNN_OK;
   const int sums = a.slot_gate >= 0 ? a.slots - 1 + (int)a.units : a.slots;
-  rn_join_kernel<T><<<(unsigned)((a.C + 31) / 32 * sums), kRnThreads, 0, a.stream>>>(a);
+  rn_join_kernel<T><<<(unsigned)((a.C + 31) / 32 * sums), 1024, 0, a.stream>>>(a);
   return check_launch();
 }
 template <typename T, bool VEC> int rn_run_typed(const RnArgs& a, RnWhat what) {

@@ -46,10 +46,12 @@ __global__ void philox_state_kernel(const int64_t* seed, const int64_t* offset, 
 }
 
 template <typename T> int seeded_dropout(const void* x, void* y, int64_t numel, const DropKey& drop, cudaStream_t s) {
+  constexpr int kMany = sizeof(T) == 4 ? 2 : 4;
   const int64_t octs = (numel + 7) / 8;
-  const int64_t grid = (octs + kDropThreads - 1) / kDropThreads;
+  const int each = octs >= (int64_t)device_info().sm_count * 2048 * kMany ? kMany : 1;
+  const int64_t grid = (octs + kDropThreads * each - 1) / (kDropThreads * each);
   if (grid > 0x7fffffff) return ACTNN_ERR_SHAPE;
-  seeded_dropout_kernel<T, 1><<<(unsigned)grid, kDropThreads, 0, s>>>((const T*)x, (T*)y, numel, drop);
+  (each > 1 ? seeded_dropout_kernel<T, kMany> : seeded_dropout_kernel<T, 1>)<<<(unsigned)grid, kDropThreads, 0, s>>>((const T*)x, (T*)y, numel, drop);
   return check_launch();
 }
 
