@@ -46,10 +46,10 @@ bool rn_dtype(int d) { return d >= ACTNN_F32 && d <= ACTNN_BF16; }
 
 }  // namespace
 
-// Asked of the occupancy calculator once for each kernel, number of threads and device.
-int rn_blocks_per_sm(const void* kernel, int threads) {
+// Asked of the occupancy calculator once for each kernel, number of threads and device (the shared memory follows from these).
+int rn_blocks_per_sm(const void* kernel, int threads, int smem) {
   struct Entry { const void* kernel; int threads, device, blocks; };
-  static Entry table[1024];
+  static Entry table[2048];
   static int used = 0;
   static std::mutex lock;
   int device = 0, blocks = 0;
@@ -57,8 +57,13 @@ int rn_blocks_per_sm(const void* kernel, int threads) {
   std::lock_guard<std::mutex> guard(lock);
   for (int i = 0; i < used; ++i)
     if (table[i].kernel == kernel && table[i].threads == threads && table[i].device == device) return table[i].blocks;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, 0) != cudaSuccess || blocks < 1) cudaGetLastError(), blocks = 1;
-  if (used < 1024) table[used++] = Entry{kernel, threads, device, blocks};
+  // one limit for all sizes: what is left of an SM's 227 KB besides the kernel's own
+  cudaFuncAttributes own{};
+  if (cudaFuncGetAttributes(&own, kernel) == cudaSuccess)
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024 - (int)own.sharedSizeBytes);
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, smem) != cudaSuccess || blocks < 1) blocks = 1;
+  cudaGetLastError();
+  if (used < 2048) table[used++] = Entry{kernel, threads, device, blocks};
   return blocks;
 }
 }  // namespace actnn

@@ -56,7 +56,7 @@ struct RnArgs {
   bool coded;                                                   // backward: of codes, else of x and f
   cudaStream_t stream;
 };
-int rn_blocks_per_sm(const void* kernel, int threads);           // of this many threads, resident at a time
+int rn_blocks_per_sm(const void* kernel, int threads, int smem);           // resident at a time; raises the kernel's limit of shared memory
 enum RnWhat { kRnForward, kRnBackward };
 int rn_run_f32(const RnArgs& a, RnWhat what, bool vec);
 int rn_run_f16(const RnArgs& a, RnWhat what, bool vec);
@@ -201,10 +201,10 @@ template <bool WARP> ACTNN_DEV float rn_sum(float v, int& place) {
   return v;
 }
 // Mean (of the layer kind) and reciprocal deviation of a row.  Values behind C are zero.
-template <int V, bool WARP> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int lane, int lanes, const RnArgs& a, int& place) {
+template <int V, bool WARP, bool LAYER> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int c0, int step, const RnArgs& a, int& place) {
   float mean = 0.f;
   float2 s = make_float2(0.f, 0.f);
-  if (a.layer) {
+  if constexpr (LAYER) {
 #pragma unroll
     for (int k = 0; k < V; ++k)
 #pragma unroll
@@ -213,11 +213,19 @@ template <int V, bool WARP> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][
     s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * lanes + lane) * 8;
+      const int c = c0 + k * step;
+      if (c + 8 <= a.C) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 e = make_float2(c + 2 * i < a.C ? v[k][i].x - mean : 0.f, c + 2 * i + 1 < a.C ? v[k][i].y - mean : 0.f);
-        s = f_fma(e, e, s);
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = f_add(v[k][i], make_float2(-mean, -mean));
+          s = f_fma(e, e, s);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 e = make_float2(c + 2 * i < a.C ? v[k][i].x - mean : 0.f, c + 2 * i + 1 < a.C ? v[k][i].y - mean : 0.f);
+          s = f_fma(e, e, s);
+        }
       }
     }
   } else {
@@ -229,46 +237,84 @@ template <int V, bool WARP> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][
   return make_float2(mean, rsqrtf(rn_sum<WARP>(f_sum(s), place) * a.inv_c + a.eps));
 }
 
+// The parameters of a thread's channels in shared memory, as float32: what every row reads again takes two loads and no conversion.
+// Sets of two halves, [set][half][vector * threads + thread].
+ACTNN_DEV void rn_put(float4* at, int width, const float2 (&v)[4]) {
+  at[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+  at[width] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+}
+ACTNN_DEV void rn_get(const float4* at, int width, float2 (&v)[4]) {
+  const float4 p = at[0], q = at[width];
+  v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
+}
+enum RnSet { kRnW1, kRnW2, kRnGate, kRnB1, kRnB2 };
+template <bool LAYER> constexpr int rn_sets() { return LAYER ? 5 : 3; }
+
 // A warp, or a block, goes through rows; a thread has V vectors of eight channels of each.  The next row's inputs are requested as soon
 // as this row's are unpacked (unless V is so large that registers are short), so that the two or four reductions of a row do
 // not wait for memory.
-template <typename T, int V, bool WARP, bool VEC>
+template <typename T, int V, bool WARP, bool VEC, bool LAYER>
 __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && !WARP ? 2 : 1) rn_forward_kernel(const __grid_constant__ RnArgs a) {
-  constexpr bool kAhead = V <= 4;
-  const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x;
-  uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x;
-  const uint32_t step = WARP ? gridDim.x * (kRnThreads / 32) : gridDim.x;
+  constexpr bool kAhead = V <= 4, kShared = V <= 2;     // parameters in shared memory, or read from the L1
+  extern __shared__ float4 parameters_s[];
+  const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, c0 = lane * 8, step = lanes * 8;
+  const int width = V * blockDim.x;
+  const uint32_t rows_step = WARP ? gridDim.x * (kRnThreads / 32) : gridDim.x;
+  uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x, gate_of = 0xffffffffu;
   Vec<T, 8> xv[V], fv[V];
   auto load = [&](uint32_t r) {
     const size_t at = (size_t)r * a.C;
+    const T *f = (const T*)a.f + at, *x = (const T*)a.x + at;
 #pragma unroll
-    for (int k = 0; k < V; ++k) fv[k] = rn_load<T, VEC>((const T*)a.f + at, (k * lanes + lane) * 8, a.C);
+    for (int k = 0; k < V; ++k) fv[k] = rn_load<T, VEC>(f, c0 + k * step, a.C);
 #pragma unroll
-    for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>((const T*)a.x + at, (k * lanes + lane) * 8, a.C);
+    for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>(x, c0 + k * step, a.C);
   };
+  if (kAhead && row < a.rows) load(row);
+  auto put = [&](int set, const void* p, int dtype, float none) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float2 v[4];
+      rn_parameter(p, dtype, c0 + k * step, a.C, a.pvec, none, v);
+      rn_put(parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x, width, v);
+    }
+  };
+  auto get = [&](int set, int k, const void* p, int dtype, float none, float2 (&v)[4]) {
+    if constexpr (kShared) rn_get(parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x, width, v);
+    else rn_parameter(p, dtype, c0 + k * step, a.C, a.pvec, none, v);
+  };
+  if constexpr (kShared) {
+    if (a.post) put(kRnW1, a.w1, a.pdtype, 1.f);
+    put(kRnW2, a.w2, a.pdtype, 1.f);
+    if (LAYER) {
+      if (a.post) put(kRnB1, a.b1, a.pdtype, 0.f);
+      put(kRnB2, a.b2, a.pdtype, 0.f);
+    }
+  }
   NoiseKey key;
   if (a.dropped) key = drop_key(a.drop);
-  if (kAhead && row < a.rows) load(row);
-  for (int place = 0; row < a.rows; row += step) {
+  for (int place = 0; row < a.rows; row += rows_step) {
     const size_t at = (size_t)row * a.C;
     if (!kAhead) load(row);
     if (a.cx) {
-      // a warp's vectors are 256 channels that share a scale
+      // A warp's vectors are 256 channels that share a scale; the factors of both inputs are made at once, one in each half of the warp.
 #pragma unroll
       for (int k = 0; k < V; ++k) {
-        const int c = (k * lanes + lane) * 8, first = (k * lanes + (lane & ~31)) * 8;
+        const int c = c0 + k * step, first = c & ~(kRnBlock - 1);
         if (first >= a.C) continue;
-        auto code = [&](const Vec<T, 8>& v, int8_t* codes, float* scales) {
-          const float most = largest(__reduce_max_sync(kFull, most_of(v))), factor = code_factor(most);
+        const uint32_t mf = __reduce_max_sync(kFull, most_of(fv[k])), mx = __reduce_max_sync(kFull, most_of(xv[k]));
+        const bool upper = threadIdx.x & 16;
+        const float most = largest(upper ? mx : mf), factor = code_factor(most);
+        auto code = [&](const Vec<T, 8>& v, int8_t* codes, float by) {
           float2 q[4];
           unpack_vec(v, q);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) q[i] = code_bits(q[i], make_float2(factor, factor));
+          for (int i = 0; i < 4; ++i) q[i] = code_bits(q[i], make_float2(by, by));
           rn_store_codes<VEC>(codes + at, c, a.C, q);
-          if ((threadIdx.x & 31) == 0) scales[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
         };
-        code(fv[k], a.cf, a.sf);
-        code(xv[k], a.cx, a.sx);
+        code(fv[k], a.cf, __shfl_sync(kFull, factor, 0));
+        code(xv[k], a.cx, __shfl_sync(kFull, factor, 16));
+        if ((threadIdx.x & 15) == 0) (upper ? a.sx : a.sf)[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
       }
     }
     float2 u[V][4], x[V][4];
@@ -277,20 +323,31 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
       unpack_vec(fv[k], u[k]);
       unpack_vec(xv[k], x[k]);
     }
-    if (kAhead && row + step < a.rows) load(row + step);
-    const float2 one = a.post ? rn_statistics<V, WARP>(u, lane, lanes, a, place) : make_float2(0.f, 1.f);
-    const void* gate = rn_gate_row(a, row);
+    if (kAhead && row + rows_step < a.rows) load(row + rows_step);
+    const float2 one = a.post ? rn_statistics<V, WARP, LAYER>(u, c0, step, a, place) : make_float2(0.f, 1.f);
+    const void* gate = nullptr;
+    if (a.gate) {
+      const uint32_t g = fast_div(row, a.by_gate);
+      gate = (const char*)a.gate + (size_t)g * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
+      if (kShared && g != gate_of) {
+        put(kRnGate, gate, a.gdtype, 1.f);
+        gate_of = g;
+      }
+    }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * lanes + lane) * 8;
+      const int c = c0 + k * step;
       if (c >= a.C) continue;
       float2 p[4];
       if (a.post) {
-        rn_parameter(a.w1, a.pdtype, c, a.C, a.pvec, 1.f, p);
+        get(kRnW1, k, a.w1, a.pdtype, 1.f, p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[k][i] = f_mul(f_mul(f_add(u[k][i], make_float2(-one.x, -one.x)), make_float2(one.y, one.y)), p[i]);
-        if (a.b1) {
-          rn_parameter(a.b1, a.pdtype, c, a.C, a.pvec, 0.f, p);
+        for (int i = 0; i < 4; ++i) {
+          if (LAYER) u[k][i] = f_add(u[k][i], make_float2(-one.x, -one.x));
+          u[k][i] = f_mul(f_mul(u[k][i], make_float2(one.y, one.y)), p[i]);
+        }
+        if (LAYER) {
+          get(kRnB1, k, a.b1, a.pdtype, 0.f, p);
 #pragma unroll
           for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
         }
@@ -301,7 +358,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
         for (int i = 0; i < 4; ++i) u[k][i] = rn_drop(u[k][i], p[i]);
       }
       if (gate) {
-        rn_parameter(gate, a.gdtype, c, a.C, a.pvec, 1.f, p);
+        get(kRnGate, k, gate, a.gdtype, 1.f, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
       }
@@ -309,22 +366,27 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
       for (int i = 0; i < 4; ++i) u[k][i] = f_fma(x[k][i], make_float2(a.scale, a.scale), u[k][i]);
       rn_store<T, VEC>((T*)a.r + at, c, a.C, u[k]);
       if constexpr (!VEC) {
+        if (c + 8 > a.C) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
+          for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
+        }
       }
     }
-    const float2 two = rn_statistics<V, WARP>(u, lane, lanes, a, place);
+    const float2 two = rn_statistics<V, WARP, LAYER>(u, c0, step, a, place);
     if (a.stats && lane == 0) a.stats[row] = make_float4(one.x, one.y, two.x, two.y);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int c = (k * lanes + lane) * 8;
+      const int c = c0 + k * step;
       if (c >= a.C) continue;
       float2 p[4];
-      rn_parameter(a.w2, a.pdtype, c, a.C, a.pvec, 1.f, p);
+      get(kRnW2, k, a.w2, a.pdtype, 1.f, p);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) u[k][i] = f_mul(f_mul(f_add(u[k][i], make_float2(-two.x, -two.x)), make_float2(two.y, two.y)), p[i]);
-      if (a.b2) {
-        rn_parameter(a.b2, a.pdtype, c, a.C, a.pvec, 0.f, p);
+      for (int i = 0; i < 4; ++i) {
+        if (LAYER) u[k][i] = f_add(u[k][i], make_float2(-two.x, -two.x));
+        u[k][i] = f_mul(f_mul(u[k][i], make_float2(two.y, two.y)), p[i]);
+      }
+      if (LAYER) {
+        get(kRnB2, k, a.b2, a.pdtype, 0.f, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
       }
@@ -362,16 +424,29 @@ template <typename T, bool CODED, bool VEC> ACTNN_DEV void rn_load_raw(RnRaw<T, 
     v.f = rn_load<T, VEC>((const T*)a.f + at, c, C);
   }
 }
-template <typename T, bool CODED> ACTNN_DEV void rn_inputs(const RnRaw<T, CODED>& v, float2 (&x)[4], float2 (&f)[4]) {
+// scale x, and n1 = (f - m1) p1.
+template <typename T, bool CODED, bool LAYER>
+ACTNN_DEV void rn_inputs(const RnRaw<T, CODED>& v, const RnArgs& a, const float4& st, float2 (&x)[4], float2 (&n1)[4]) {
+  float by_x = a.scale, by_f = st.y;
   if constexpr (CODED) {
     unpack_codes(v.x, x);
-    unpack_codes(v.f, f);
+    unpack_codes(v.f, n1);
+    by_x *= v.sx;
+    if (!LAYER) by_f *= v.sf;
+    if (LAYER) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = f_mul(x[i], make_float2(v.sx, v.sx)), f[i] = f_mul(f[i], make_float2(v.sf, v.sf));
+      for (int i = 0; i < 4; ++i) n1[i] = f_fma(n1[i], make_float2(v.sf, v.sf), make_float2(-st.x, -st.x));
+    }
   } else {
     unpack_vec(v.x, x);
-    unpack_vec(v.f, f);
+    unpack_vec(v.f, n1);
+    if (LAYER) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) n1[i] = f_add(n1[i], make_float2(-st.x, -st.x));
+    }
   }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = f_mul(x[i], make_float2(by_x, by_x)), n1[i] = f_mul(n1[i], make_float2(by_f, by_f));
 }
 ACTNN_DEV void rn_store_any(void* p, int dtype, size_t at, float v) {
   if (dtype == ACTNN_F32) ((float*)p)[at] = v;
@@ -413,8 +488,8 @@ template <int N> ACTNN_DEV float rn_warp_sums(float (&v)[N]) {
 template <typename T, bool VEC, bool CODED, bool LAYER>
 __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a) {
   constexpr int N = LAYER ? 8 : 4, kWarps = kRnMostThreads / 32;
-  extern __shared__ float4 parameters_s[];              // [w1, w2, gate, b1][half][thread]
-  __shared__ float part_s[2][kRnMostCluster * kWarps][N];
+  extern __shared__ float4 parameters_s[];
+  __shared__ __align__(16) float part_s[2][kRnMostCluster * kWarps][N];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
   const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0, run = blockIdx.x / a.cluster;
   const int c = ((int)rank * threads + (int)threadIdx.x) * 8, C = a.C, entries = a.cluster * warps;
@@ -429,20 +504,20 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
     row = u * a.unit_rows + (uint32_t)((uint64_t)k * a.unit_rows / a.runs_of_unit);
     end = u * a.unit_rows + (uint32_t)((uint64_t)(k + 1) * a.unit_rows / a.runs_of_unit);
   }
-  auto put = [&](int set, const float2 (&v)[4]) {
-    parameters_s[(2 * set) * threads + threadIdx.x] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-    parameters_s[(2 * set + 1) * threads + threadIdx.x] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
-  };
-  auto get = [&](int set, float2 (&v)[4]) {
-    const float4 p = parameters_s[(2 * set) * threads + threadIdx.x], q = parameters_s[(2 * set + 1) * threads + threadIdx.x];
-    v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
-  };
-  {
+  // Behind C they are zero: with the gate and w2 so, nothing there enters a sum.
+  auto put = [&](int set, const void* p, int dtype, float none) {
     float2 v[4];
-    rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, v), put(0, v);
-    rn_parameter(a.w2, a.pdtype, c, C, a.pvec, 1.f, v), put(1, v);
-    if (LAYER) rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, v), put(3, v);
-  }
+    rn_parameter(p, dtype, c, C, a.pvec, none, v);
+    if (c + 8 > C) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = make_float2(c + 2 * i < C ? v[i].x : 0.f, c + 2 * i + 1 < C ? v[i].y : 0.f);
+    }
+    rn_put(parameters_s + 2 * set * threads + threadIdx.x, threads, v);
+  };
+  auto get = [&](int set, float2 (&v)[4]) { rn_get(parameters_s + 2 * set * threads + threadIdx.x, threads, v); };
+  put(kRnW1, a.w1, a.pdtype, 1.f);
+  put(kRnW2, a.w2, a.pdtype, 1.f);
+  if (LAYER) put(kRnB1, a.b1, a.pdtype, 0.f);
   if (a.cluster > 1) cluster_sync();                    // the others' shared memory is there
   uint32_t gate_of = 0xffffffffu;
   NoiseKey key;
@@ -457,12 +532,11 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   for (int place = 0; row < end; ++row, place ^= 1) {
     st = next_st;
     if (const uint32_t g = fast_div(row, a.by_gate); g != gate_of) {
-      float2 v[4];
-      rn_parameter(rn_gate_row(a, row), a.gdtype, c, C, a.pvec, 1.f, v), put(2, v);
+      put(kRnGate, rn_gate_row(a, row), a.gdtype, 1.f);
       gate_of = g;
     }
-    float2 n1[4], n2[4], x[4], dn[4], cc[4];            // dn: dh, then d;  cc: dr + p2 dn2
-    rn_inputs<T, CODED>(raw, x, n1);
+    float2 n1[4], n2[4], dn[4], cc[4];                  // n2: scale x until the norm is known; dn: dh, then d;  cc: dr + p2 dn2
+    rn_inputs<T, CODED, LAYER>(raw, a, st, n2, n1);
     unpack_vec(raw.dr, cc);
     unpack_vec(raw.dh, dn);
     if (row + 1 < end) {
@@ -470,31 +544,22 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
       next_st = rn_ld(a.stats + row + 1);
     }
     float2 q[4], w1[4];
-    get(2, q);
-    get(0, w1);
+    get(kRnGate, q);
+    get(kRnW1, w1);
     float2 s0{}, s1{}, s2{}, s3{}, s4{}, s5{}, s6{}, s7{};
     {
       float2 w2[4], b1[4], m[4];
-      get(1, w2);
-      if (LAYER) get(3, b1);
+      get(kRnW2, w2);
+      if (LAYER) get(kRnB1, b1);
       if (a.dropped) rn_factors<VEC>(a, key, row, c, m);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if (LAYER) n1[i] = f_add(n1[i], make_float2(-st.x, -st.x));
-        n1[i] = f_mul(n1[i], make_float2(st.y, st.y));
         float2 d = a.post ? (LAYER ? f_fma(n1[i], w1[i], b1[i]) : f_mul(n1[i], w1[i])) : n1[i];
         if (a.dropped) d = rn_drop(d, m[i]);
-        n2[i] = f_fma(d, q[i], f_mul(x[i], make_float2(a.scale, a.scale)));
+        n2[i] = f_fma(d, q[i], n2[i]);
         if (LAYER) n2[i] = f_add(n2[i], make_float2(-st.z, -st.z));
         n2[i] = f_mul(n2[i], make_float2(st.w, st.w));
         if (a.dropped) q[i] = rn_drop(q[i], m[i]);
-        if constexpr (!VEC) {                            // nothing behind C
-          const bool in0 = c + 2 * i < C, in1 = c + 2 * i + 1 < C;
-          auto only = [&](float2& p) { p = make_float2(in0 ? p.x : 0.f, in1 ? p.y : 0.f); };
-          only(n1[i]), only(n2[i]), only(d), only(q[i]);
-        } else if (c >= C) {
-          n1[i] = n2[i] = d = q[i] = make_float2(0.f, 0.f);
-        }
         const float2 dn2 = f_mul(dn[i], w2[i]);
         cc[i] = f_fma(make_float2(st.w, st.w), dn2, cc[i]);
         dw2[i] = f_fma(dn[i], n2[i], dw2[i]);
@@ -522,8 +587,13 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
     if (a.cluster > 1) cluster_sync();
     else if (warps > 1) __syncthreads();
     else __syncwarp();
-    float total[N] = {};
-    for (int e = lane; e < entries; e += 32) {
+    float total[N];
+#pragma unroll
+    for (int i = 0; i < N; i += 4) {
+      const float4 q = lane < entries ? *reinterpret_cast<const float4*>(&part_s[place][lane][i]) : make_float4(0.f, 0.f, 0.f, 0.f);
+      total[i] = q.x, total[i + 1] = q.y, total[i + 2] = q.z, total[i + 3] = q.w;
+    }
+    for (int e = lane + 32; e < entries; e += 32) {
 #pragma unroll
       for (int i = 0; i < N; ++i) total[i] += part_s[place][e][i];
     }
@@ -602,26 +672,26 @@ __global__ void __launch_bounds__(1024) rn_join_kernel(const __grid_constant__ R
 
 // ------------------------------------------------------------------ host
 // A warp has rows of up to 256 channels, a block longer ones; as few vectors a thread as 512 threads need.  As many blocks as are resident.
-template <typename T, bool VEC> int rn_forward(const RnArgs& a) {
+template <typename T, bool VEC, bool LAYER> int rn_forward(const RnArgs& a) {
   auto run = [&](auto kernel, bool warp, int V) {
     const int threads = warp ? kRnThreads : (a.C + V * 256 - 1) / (V * 256) * 32;
+    const int smem = V <= 2 ? rn_sets<LAYER>() * 2 * V * threads * (int)sizeof(float4) : 0;
     const int64_t wanted = warp ? ((int64_t)a.rows + kRnThreads / 32 - 1) / (kRnThreads / 32) : a.rows;
-    const int64_t resident = (int64_t)device_info().sm_count * rn_blocks_per_sm((const void*)kernel, threads);
-    kernel<<<(unsigned)std::min(wanted, resident), threads, 0, a.stream>>>(a);
+    const int64_t resident = (int64_t)device_info().sm_count * rn_blocks_per_sm((const void*)kernel, threads, smem);
+    kernel<<<(unsigned)std::min(wanted, resident), threads, smem, a.stream>>>(a);
     return check_launch();
   };
-  if (a.C <= 256) return run(rn_forward_kernel<T, 1, true, VEC>, true, 1);
-  if (a.C <= 4096) return run(rn_forward_kernel<T, 1, false, VEC>, false, 1);
-  if (a.C <= 8192) return run(rn_forward_kernel<T, 2, false, VEC>, false, 2);
-  if (a.C <= 16384) return run(rn_forward_kernel<T, 4, false, VEC>, false, 4);
-  return run(rn_forward_kernel<T, 8, false, VEC>, false, 8);
+  if (a.C <= 256) return run(rn_forward_kernel<T, 1, true, VEC, LAYER>, true, 1);
+  if (a.C <= 4096) return run(rn_forward_kernel<T, 1, false, VEC, LAYER>, false, 1);
+  if (a.C <= 8192) return run(rn_forward_kernel<T, 2, false, VEC, LAYER>, false, 2);
+  if (a.C <= 16384) return run(rn_forward_kernel<T, 4, false, VEC, LAYER>, false, 4);
+  return run(rn_forward_kernel<T, 8, false, VEC, LAYER>, false, 8);
 }
 template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const RnArgs& a) {
   auto* kernel = rn_backward_kernel<T, VEC, CODED, LAYER>;
   const int threads = a.cluster > 1 ? kRnMostThreads : (a.C + 255) / 256 * 32;
   const int smem = (LAYER ? 4 : 3) * 2 * threads * (int)sizeof(float4);
-  // The limit of dynamic shared memory is raised once for the most that any size takes.
-  cached_blocks_per_sm((const void*)kernel, kRnMostThreads, (LAYER ? 4 : 3) * 2 * kRnMostThreads * (int)sizeof(float4));
+  rn_blocks_per_sm((const void*)kernel, threads, smem);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.runs * a.cluster);
   cfg.blockDim = dim3(threads);
@@ -641,7 +711,7 @@ template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const Rn
   return check_launch();
 }
 template <typename T, bool VEC> int rn_run_typed(const RnArgs& a, RnWhat what) {
-  if (what == kRnForward) return rn_forward<T, VEC>(a);
+  if (what == kRnForward) return a.layer ? rn_forward<T, VEC, true>(a) : rn_forward<T, VEC, false>(a);
   if (a.coded) return a.layer ? rn_backward<T, VEC, true, true>(a) : rn_backward<T, VEC, true, false>(a);
   return a.layer ? rn_backward<T, VEC, false, true>(a) : rn_backward<T, VEC, false, false>(a);
 }
