@@ -34,12 +34,13 @@ fp8_row_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8
   for (int i = 0; i < TASKS; ++i) {
     if (row[i] >= rows) return;
     uint32_t byte[2];
+    bool bad[2];
+    fp8_block_bits(v[i][0], v[i][1], byte, bad);
+    uint8_t* to = codes + row[i] * ldc + g[i] * 512 + lane * 8;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      const int64_t e = g[i] * 512 + k * 256 + lane * 8;
-      bool bad;
-      byte[k] = fp8_scale_byte(half_warp_max(fp8_most(v[i][k], bad)));
-      if (e < ldc) *reinterpret_cast<uint2*>(codes + row[i] * ldc + e) = fp8_codes8(v[i][k], fp8_factor(byte[k]), bad);
+      byte[k] = fp8_scale_byte(byte[k]);
+      if (g[i] * 512 + k * 256 + lane * 8 < ldc) *reinterpret_cast<uint2*>(to + k * 256) = fp8_codes8(v[i][k], fp8_factor(byte[k]), bad[k]);
     }
     const uint32_t mine = byte[0] | byte[1] << 16, other = __shfl_xor_sync(kFull, mine, 16);
     if (lane == 0) *reinterpret_cast<uint32_t*>(scales + fp8_scale_at(row[i], g[i] * 4, (rows + 127) / 128)) = mine | other << 8;
@@ -76,6 +77,7 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
                       uint8_t* __restrict__ scales_t, float* __restrict__ parts, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc,
                       int64_t ldt, int column_tiles) {
   constexpr int kWords = 8 / word_columns<T>();
+  const int64_t row_tiles = (rows + 127) / 128;
   __shared__ uint4 turned_s[128 * 8];                  // [column][128 rows], chunks of eight rows in the order rotated by column / 8
   __shared__ uint32_t most_s[16][128];                 // [team][word of columns]; later float sums of columns
   __shared__ float factor_s[128];
@@ -101,25 +103,29 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
     for (int w = 1; w < kCodeThreads / 32; ++w) square = max(square, most_s[0][w]);
     square = fp8_scale_byte(square);
   }
-  // ---- rows, and the largest of the thread's columns
+  // ---- rows, two at a time, and the largest of the thread's columns
   uint32_t most[kWords] = {};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    uint32_t byte = square;
+  for (int i = 0; i < 8; i += 2) {
+    uint32_t byte[2] = {square, square};
     if (!SQUARE) {
-      bool b;
-      byte = fp8_most(v[i], b);
-      bad |= (uint32_t)b << i;
-      if (codes) byte = fp8_scale_byte(half_warp_max(byte));
+      bool b[2];
+      fp8_block_bits(v[i], v[i + 1], byte, b);
+      byte[0] = fp8_scale_byte(byte[0]), byte[1] = fp8_scale_byte(byte[1]);
+      bad |= (uint32_t)b[0] << i | (uint32_t)b[1] << (i + 1);
 #pragma unroll
       for (int j = 0; j < kWords; ++j) {
-        const uint32_t w = word_abs<T>(v[i].w[j]);
-        most[j] = word_max<T>(most[j], b ? word_finite<T>(w) : w);
+        const uint32_t w = word_abs<T>(v[i].w[j]), x = word_abs<T>(v[i + 1].w[j]);
+        most[j] = word_max<T>(word_max<T>(most[j], b[0] ? word_finite<T>(w) : w), b[1] ? word_finite<T>(x) : x);
       }
     }
-    if (codes && r0 + i < rows) {
-      if (c < ldc) *reinterpret_cast<uint2*>(codes + (r0 + i) * ldc + c) = fp8_codes8(v[i], fp8_factor(byte), bad >> i & 1);
-      if (c8 == 0) scales[fp8_scale_at(r0 + i, tc, (rows + 127) / 128)] = (uint8_t)byte;
+    if (codes) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        if (r0 + i + k >= rows) continue;
+        if (c < ldc) *reinterpret_cast<uint2*>(codes + (r0 + i + k) * ldc + c) = fp8_codes8(v[i + k], fp8_factor(byte[k]), bad >> (i + k) & 1);
+        if (c8 == 0) scales[fp8_scale_at(r0 + i + k, tc, row_tiles)] = (uint8_t)byte[k];
+      }
     }
   }
 
@@ -233,7 +239,6 @@ fp8_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
 
 template <typename T>
 int row_codes(const void* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, int64_t ldx, int64_t ldc, cudaStream_t s) {
-  // two tasks a warp keep more loads under way, where there are warps enough (16384 x 4096 bfloat16: 40 us with one)
   const int64_t groups = (cols + 511) / 512, tasks = rows * groups;
   const int each = tasks >= (int64_t)device_info().sm_count * 256 ? 2 : 1;
   const int64_t grid = (tasks + kCodeThreads / 32 * each - 1) / (kCodeThreads / 32 * each);

@@ -158,7 +158,7 @@ ACTNN_DEV const void* rn_gate_row(const RnArgs& a, uint32_t row) {
   if (!a.gate) return nullptr;
   return (const char*)a.gate + (size_t)fast_div(row, a.by_gate) * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
 }
-// What dropout multiplies the eight channels from `c` of a row by.  Where C is no multiple of eight they belong to two calls.
+// What dropout multiplies the eight channels from `c` of a row by (a value that is not finite makes its row NaN, dropped or not).  Where C is no multiple of eight they belong to two calls.
 template <bool VEC> ACTNN_DEV void rn_factors(const RnArgs& a, const NoiseKey& key, uint32_t row, int c, float2 (&m)[4]) {
   const uint64_t e = (uint64_t)row * a.C + c;
   const Philox4 r = noise_call(key, e >> 3);
@@ -176,12 +176,6 @@ template <bool VEC> ACTNN_DEV void rn_factors(const RnArgs& a, const NoiseKey& k
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = make_float2(k[2 * i], k[2 * i + 1]);
 }
-// m times v; a dropped element is zero whatever it was.
-ACTNN_DEV float2 rn_drop(float2 v, float2 m) {
-  const float2 y = f_mul(v, m);
-  return make_float2(m.x != 0.f ? y.x : 0.f, m.y != 0.f ? y.y : 0.f);
-}
-
 // ------------------------------------------------------------------ forward
 // The sum over the threads of a row: a warp's, or a block's, whose reductions take two places in turn (two are never under way at a time).
 template <bool WARP> ACTNN_DEV float rn_sum(float v, int& place) {
@@ -355,7 +349,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
       if (a.dropped) {
         rn_factors<VEC>(a, key, row, c, p);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[k][i] = rn_drop(u[k][i], p[i]);
+        for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
       }
       if (gate) {
         get(kRnGate, k, gate, a.gdtype, 1.f, p);
@@ -555,11 +549,11 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float2 d = a.post ? (LAYER ? f_fma(n1[i], w1[i], b1[i]) : f_mul(n1[i], w1[i])) : n1[i];
-        if (a.dropped) d = rn_drop(d, m[i]);
+        if (a.dropped) d = f_mul(d, m[i]);
         n2[i] = f_fma(d, q[i], n2[i]);
         if (LAYER) n2[i] = f_add(n2[i], make_float2(-st.z, -st.z));
         n2[i] = f_mul(n2[i], make_float2(st.w, st.w));
-        if (a.dropped) q[i] = rn_drop(q[i], m[i]);
+        if (a.dropped) q[i] = f_mul(q[i], m[i]);
         const float2 dn2 = f_mul(dn[i], w2[i]);
         cc[i] = f_fma(make_float2(st.w, st.w), dn2, cc[i]);
         dw2[i] = f_fma(dn[i], n2[i], dw2[i]);
