@@ -87,6 +87,12 @@ ACTNN_DEV bool fp_test(uint32_t bar, uint32_t parity) {
   return ok != 0;
 }
 
+// Of a warp that issues by an elected lane: all of its lanes go on, or none.  A lane that left alone, because its own last try came a
+// moment before the phase, would be missing where the others elect one.
+ACTNN_DEV bool fp_warp_waits(bool ready, uint32_t bar, uint32_t parity, FpShared& s, unsigned* gave_up) {
+  return __all_sync(kFull, ready || fp_wait(bar, parity, s, gave_up));
+}
+
 // Of the epilogue's eight warps: whether the waits of all of them came to their end.  A warp that left alone, because another
 // wait had run out just before its own phase was complete, would leave those whose phase was to barriers it never comes to.
 ACTNN_DEV bool epilogue_agrees(bool ok) {
@@ -181,7 +187,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
     for (int tile = first_tile; copied && tile < a.tiles; tile += tile_step) {
       const int tt = tile / a.channel_tiles, row = (tile - tt * a.channel_tiles) * tile_channels + channel_step, t0 = tt * a.tokens;
       for (int k = k_first; k < k_end; ++k) {
-        if (!free && !(copied = fp_wait(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+        if (!(copied = fp_warp_waits(free, smem_addr(&s.empty[copy_stage]), copy_phase ^ 1, s, issues ? gave_up : nullptr))) break;
         const int now = copy_stage;
         if (++copy_stage == a.stages) copy_stage = 0, copy_phase ^= 1;
         free = fp_test(smem_addr(&s.empty[copy_stage]), copy_phase ^ 1);
@@ -207,10 +213,10 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
     // A pair's second block is there until what the first one's matrix instructions arrive at has been arrived at: the stages' barriers
     // and the one for the end.  (In their own block the warp that issues them waits for the end.)
     for (int i = 0, at = copy_stage; PAIR && copied && i < a.stages; ++i) {
-      copied = fp_wait(smem_addr(&s.empty[at]), copy_phase ^ (at < copy_stage ? 0 : 1), s, issues ? gave_up : nullptr);
+      copied = fp_warp_waits(false, smem_addr(&s.empty[at]), copy_phase ^ (at < copy_stage ? 0 : 1), s, issues ? gave_up : nullptr);
       if (++at == a.stages) at = 0;
     }
-    if (PAIR && copied) copied = fp_wait(smem_addr(&s.drained), 0, s, issues ? gave_up : nullptr);
+    if (PAIR && copied) copied = fp_warp_waits(false, smem_addr(&s.drained), 0, s, issues ? gave_up : nullptr);
     __syncwarp();
   } else if (warp == 9) {                                       // ---------------- matrix instructions
     if (a.early) grid_wait();                                   // the limit of a wait is for copies, not for the launch before
@@ -241,7 +247,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
           mma_fp8<PAIR>(to, da + 2 * i, db + 2 * i, instr, at_w, at_x, k > k_first || i > 0);
       };
       for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
-        if (!(ok = fp_wait(smem_addr(&s.sum_empty[WIDE ? 0 : buf]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+        if (!(ok = fp_warp_waits(false, smem_addr(&s.sum_empty[WIDE ? 0 : buf]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
         tmem_fence_after_sync();
         d = tmem + (WIDE ? 0 : buf * a.tokens);
         shift = (tile / a.channel_tiles * a.tokens & 127) / 32;                     // columns from a set of 128 tokens
@@ -253,14 +259,14 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
           at_w = sets + set * a.set_columns;
           if (++set == a.sets) set = 0;
           for (int i = 0; ok && i < head; ++i) {
-            if (!(ok = fp_wait(smem_addr(&s.full[at]), at_phase, s, issues ? gave_up : nullptr))) break;
+            if (!(ok = fp_warp_waits(false, smem_addr(&s.full[at]), at_phase, s, issues ? gave_up : nullptr))) break;
             if (elect_one()) {
               if (i == 0) scales(at);
               multiply(at, k_first + i, 0);
             }
             next(at, at_phase);
           }
-          if (!ok || !(ok = fp_wait(smem_addr(&s.sum_empty[1]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
+          if (!ok || !(ok = fp_warp_waits(false, smem_addr(&s.sum_empty[1]), buf_phase ^ 1, s, issues ? gave_up : nullptr))) break;
           tmem_fence_after_sync();
           for (; k < k_first + head; ++k) {
             if (elect_one()) {
@@ -272,7 +278,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
         }
         bool ready = false;
         for (; k < k_end; ++k) {
-          if (!ready && !(ok = fp_wait(smem_addr(&s.full[stage]), phase, s, issues ? gave_up : nullptr))) break;
+          if (!(ok = fp_warp_waits(ready, smem_addr(&s.full[stage]), phase, s, issues ? gave_up : nullptr))) break;
           const int now = stage;
           next(stage, phase);
           ready = fp_test(smem_addr(&s.full[stage]), phase);
@@ -455,7 +461,7 @@ void plan(FpArgs& a) {
     const int64_t blocks = tiles * splits * (pair ? 2 : 1), waves = (blocks + sms - 1) / sms;
     if (splits > 1 && blocks > (splits > 4 ? 64 : sms)) return;
     const double stage = wide ? tokens * 0.0017 : pair ? std::max(0.23, 0.15 + tokens * 0.00105) : std::max(splits > 1 ? 0.3 : 0.27, 0.2 + tokens * 0.0011);
-    const double besides = wide ? 3.8 : pair ? 0.8 + tokens * 0.004 : splits > 1 ? 3. + tokens * 0.0135 : 0.4 + tokens * 0.004;
+    const double besides = wide ? 4.3 : pair ? 0.8 + tokens * 0.004 : splits > 1 ? 3. + tokens * 0.0135 : 0.4 + tokens * 0.004;
     const double time = (double)waves * ((a.k_blocks + splits - 1) / splits * stage + besides) + (pair ? 1. : 0.);
     if (best >= 0. && time >= best) return;
     best = time;
