@@ -2,8 +2,8 @@
 
     r = scale * x + gate * drop(norm(branch) * post_weight + post_bias)        h = norm(r) * weight + bias
 
-``x`` is the residual stream, ``branch`` the block's output, ``h`` what the next block reads.  ``kind``: "rms" or "layer"; ``post``
-false leaves the first norm out.  Parameters are ``[C]`` or ``None``; a gate has the last dimension C and before it the leading
+``x`` is the residual stream, ``branch`` the block's output, ``h`` what the next block reads.  ``kind``: "rms" (without biases) or
+"layer"; ``post`` false leaves the first norm out.  Parameters are ``[C]`` or ``None``; a gate has the last dimension C and before it the leading
 dimensions of ``x`` up to some place, ones behind it (``[C]``, ``[B, 1, C]``, ``[B, S, C]``).
 
 For the backward pass ``x`` and ``branch`` are kept in 8 bits: 256 consecutive channels of a row share a float32 scale, their largest
@@ -41,12 +41,14 @@ def _inputs(x, branch):
         raise RuntimeError("%d rows are more than 2^31 - 1" % x.shape[:-1].numel())
 
 
-def _parameters(x, weight, bias, post_weight, post_bias, post):
+def _parameters(x, weight, bias, post_weight, post_bias, post, layer):
     """The four as contiguous tensors of one type, and that type."""
     given = {"weight": weight, "bias": bias, "post_weight": post_weight, "post_bias": post_bias}
     for name, p in given.items():
         if p is None:
             continue
+        if not layer and name.endswith("bias"):
+            raise RuntimeError("%s belongs to the kind \"layer\"" % name)
         if not post and name.startswith("post"):
             raise RuntimeError("%s without the norm that it belongs to" % name)
         check_cuda_values(p, name, x.device)
@@ -81,7 +83,7 @@ def run(x, branch, weight=None, bias=None, post_weight=None, post_bias=None, gat
     _inputs(x, branch)
     if branch.dtype != x.dtype:
         raise RuntimeError("x and branch must have the same type")
-    params, pdtype = _parameters(x, weight, bias, post_weight, post_bias, post)
+    params, pdtype = _parameters(x, weight, bias, post_weight, post_bias, post, layer)
     each = gate_rows(x, gate)
     gate = None if gate is None else gate.detach().contiguous()
     x, branch = x.contiguous(), branch.contiguous()
@@ -121,7 +123,7 @@ def backward(grad_r, grad_h, saved, stats, weight=None, bias=None, post_weight=N
             if g.shape != like.shape or g.dtype != like.dtype:
                 raise RuntimeError("grad_r and grad_h must have the same shape and type")
     c, rows = like.shape[-1], like.shape[:-1].numel()
-    params, pdtype = _parameters(like, weight, bias, post_weight, post_bias, post)
+    params, pdtype = _parameters(like, weight, bias, post_weight, post_bias, post, layer)
     each = gate_rows(like, gate)
     flat = None if gate is None else gate.detach().contiguous()
     gdtype = like.dtype if gate is None else gate.dtype

@@ -588,6 +588,7 @@ Residual residual_of(const Tensor& x, const Tensor& weight, const Tensor& bias, 
   for (int i = 0; i < 4; ++i) {
     const Tensor& q = *params[i];
     if (!q.defined()) continue;
+    TORCH_CHECK(layer || i % 2 == 0, names[i], " belongs to the kind \"layer\"");
     TORCH_CHECK(post || i < 2, names[i], " without the norm that it belongs to");
     check_values(q, names[i]);
     TORCH_CHECK(q.device() == x.device(), names[i], " is on ", q.device(), ", expected ", x.device());
