@@ -29,6 +29,11 @@ ACTNN_DEV void peer_arrive(uint32_t remote) {
 ACTNN_DEV void peer_store1(uint32_t addr, uint32_t rank, int v) {
   asm volatile("st.shared::cluster.s32 [%0], %1;" :: "r"(peer_addr(addr, rank)), "r"(v) : "memory");
 }
+// Sends 16 bytes to block `rank`, whose barrier counts them as they arrive.
+ACTNN_DEV void peer_send4(uint32_t addr, uint32_t bar, uint32_t rank, const float4& v) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1,%2,%3,%4}, [%5];"
+               :: "r"(peer_addr(addr, rank)), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(peer_addr(bar, rank)) : "memory");
+}
 ACTNN_DEV int4 peer_load4i(uint32_t addr, uint32_t rank) {
   uint32_t remote;
   int4 v;

@@ -19,6 +19,7 @@
 #pragma once
 
 #include <algorithm>
+#include <type_traits>
 
 #include "cluster.cuh"
 #include "dropout.cuh"
@@ -86,17 +87,21 @@ ACTNN_DEV uint4 rn_ld(const uint4* p) {
 }
 
 // ------------------------------------------------------------------ eight channels of a thread
+// Element `c` of a row that all threads have in common, by a 32-bit offset.
+template <typename T> ACTNN_DEV T* rn_at(T* row, int c) {
+  return (T*)((std::conditional_t<std::is_const_v<T>, const char, char>*)row + (uint32_t)c * (uint32_t)sizeof(T));
+}
 // Elements from `c` on, zero behind C.
 template <typename T, bool VEC> ACTNN_DEV Vec<T, 8> rn_load(const T* row, int c, int C) {
   Vec<T, 8> v;
-  if (VEC && c < C) return load_vec<T, 8>(row + c);
+  if (VEC && c < C) return load_vec<T, 8>(rn_at(row, c));
 #pragma unroll
   for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && c + i < C ? __ldg(row + c + i) : from_float<T>(0.f);
   return v;
 }
 template <typename T, bool VEC> ACTNN_DEV void rn_store(T* row, int c, int C, const float2 (&f)[4]) {
   if constexpr (VEC) {
-    if (c < C) store_vec<T, 8>(row + c, f);
+    if (c < C) store_vec<T, 8>(rn_at(row, c), f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -107,7 +112,7 @@ template <bool VEC> ACTNN_DEV Codes<8> rn_load_codes(const int8_t* row, int c, i
   Codes<8> r;
   r.w[0] = r.w[1] = 0;
   if constexpr (VEC) {
-    if (c < C) r = load_codes<8>(row + c);
+    if (c < C) r = load_codes<8>(rn_at(row, c));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -117,7 +122,7 @@ template <bool VEC> ACTNN_DEV Codes<8> rn_load_codes(const int8_t* row, int c, i
 }
 template <bool VEC> ACTNN_DEV void rn_store_codes(int8_t* row, int c, int C, const float2 (&f)[4]) {
   if constexpr (VEC) {
-    if (c < C) store_codes<8>(row + c, f);
+    if (c < C) store_codes<8>(rn_at(row, c), f);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -158,23 +163,22 @@ ACTNN_DEV const void* rn_gate_row(const RnArgs& a, uint32_t row) {
   if (!a.gate) return nullptr;
   return (const char*)a.gate + (size_t)fast_div(row, a.by_gate) * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
 }
-// What dropout multiplies the eight channels from `c` of a row by (a value that is not finite makes its row NaN, dropped or not).  Where C is no multiple of eight they belong to two calls.
-template <bool VEC> ACTNN_DEV void rn_factors(const RnArgs& a, const NoiseKey& key, uint32_t row, int c, float2 (&m)[4]) {
+// The fields that decide over the eight channels from `c` of a row, two a word.  Where C is no multiple of eight they belong to two calls.
+// (Both directions multiply by factors: a value that is not finite makes its row NaN, dropped or not.)
+template <bool VEC> ACTNN_DEV Philox4 rn_fields(const RnArgs& a, const NoiseKey& key, uint32_t row, int c) {
   const uint64_t e = (uint64_t)row * a.C + c;
-  const Philox4 r = noise_call(key, e >> 3);
-  if (VEC) return drop_factors(r, a.drop.least, a.drop.inv, m);
+  Philox4 r = noise_call(key, e >> 3);
+  if (VEC) return r;
   const Philox4 q = noise_call(key, (e >> 3) + 1);
-  float k[8];
+  const uint32_t at = (uint32_t)e & 7;                  // fields to leave out: four, two and one
+  uint32_t w[8] = {r.v[0], r.v[1], r.v[2], r.v[3], q.v[0], q.v[1], q.v[2], q.v[3]};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t at = (uint32_t)(e & 7) + i, j = at & 7;
-    const uint32_t lo = j & 4 ? (j & 2 ? r.v[3] : r.v[2]) : (j & 2 ? r.v[1] : r.v[0]);
-    const uint32_t hi = j & 4 ? (j & 2 ? q.v[3] : q.v[2]) : (j & 2 ? q.v[1] : q.v[0]);
-    const uint32_t word = at < 8 ? lo : hi;
-    k[i] = (j & 1 ? word : word << 16) >= a.drop.least ? a.drop.inv : 0.f;
-  }
+  for (int i = 0; i < 6; ++i) w[i] = at & 4 ? w[i + 2] : w[i];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) m[i] = make_float2(k[2 * i], k[2 * i + 1]);
+  for (int i = 0; i < 5; ++i) w[i] = at & 2 ? w[i + 1] : w[i];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = __funnelshift_r(w[i], w[i + 1], at & 1 ? 16 : 0);
+  return r;
 }
 // ------------------------------------------------------------------ forward
 // The sum over the threads of a row: a warp's, or a block's, whose reductions take two places in turn (two are never under way at a time).
@@ -347,7 +351,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
         }
       }
       if (a.dropped) {
-        rn_factors<VEC>(a, key, row, c, p);
+        drop_factors(rn_fields<VEC>(a, key, row, c), a.drop.least, a.drop.inv, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
       }
@@ -409,19 +413,19 @@ template <typename T, bool CODED, bool VEC> ACTNN_DEV void rn_load_raw(RnRaw<T, 
     v.f = rn_load_codes<VEC>(a.cf + at, c, C);
     v.sx = v.sf = 0.f;
     if (c < C) {
-      const size_t s = (size_t)row * a.blocks + c / kRnBlock;
-      v.sx = rn_ld(a.sx + s);
-      v.sf = rn_ld(a.sf + s);
+      const size_t s = (size_t)row * a.blocks;
+      v.sx = rn_ld(rn_at((const float*)a.sx + s, c / kRnBlock));
+      v.sf = rn_ld(rn_at((const float*)a.sf + s, c / kRnBlock));
     }
   } else {
     v.x = rn_load<T, VEC>((const T*)a.x + at, c, C);
     v.f = rn_load<T, VEC>((const T*)a.f + at, c, C);
   }
 }
-// scale x, and n1 = (f - m1) p1.
+// p2 (scale x - m2), and n1 = (f - m1) p1.
 template <typename T, bool CODED, bool LAYER>
 ACTNN_DEV void rn_inputs(const RnRaw<T, CODED>& v, const RnArgs& a, const float4& st, float2 (&x)[4], float2 (&n1)[4]) {
-  float by_x = a.scale, by_f = st.y;
+  float by_x = a.scale * st.w, by_f = st.y;
   if constexpr (CODED) {
     unpack_codes(v.x, x);
     unpack_codes(v.f, n1);
@@ -439,8 +443,12 @@ ACTNN_DEV void rn_inputs(const RnRaw<T, CODED>& v, const RnArgs& a, const float4
       for (int i = 0; i < 4; ++i) n1[i] = f_add(n1[i], make_float2(-st.x, -st.x));
     }
   }
+  const float m = -st.z * st.w;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) x[i] = f_mul(x[i], make_float2(by_x, by_x)), n1[i] = f_mul(n1[i], make_float2(by_f, by_f));
+  for (int i = 0; i < 4; ++i) {
+    x[i] = LAYER ? f_fma(x[i], make_float2(by_x, by_x), make_float2(m, m)) : f_mul(x[i], make_float2(by_x, by_x));
+    n1[i] = f_mul(n1[i], make_float2(by_f, by_f));
+  }
 }
 ACTNN_DEV void rn_store_any(void* p, int dtype, size_t at, float v) {
   if (dtype == ACTNN_F32) ((float*)p)[at] = v;
@@ -477,31 +485,39 @@ template <int N> ACTNN_DEV float rn_warp_sums(float (&v)[N]) {
 
 // A run of rows by a block, or by a cluster of blocks of 4096 channels each.  A thread has eight channels of every row and keeps the sums of
 // their parameters' gradients; the next row's values are requested as soon as this row's are unpacked.  The warps' sums of a row go to
-// shared memory (of every block of the cluster), a barrier, and each warp joins them for itself: two places in turn, so that
-// one barrier a row is enough.  Parameters lie in shared memory as float32, a thread's own.
+// shared memory in two places in turn, so that one barrier a row is enough, and each warp joins them for itself.  The blocks of a
+// cluster send theirs to one another, counted as they arrive by a barrier in memory: a barrier of the cluster would wait for
+// the results of the row before to reach the L2 as well.  A wait that runs out is counted, and the rows from there on get NaN.
+//
+// What bounds it are instructions (16 warps an SM is what registers allow), so the gate g and w1 enter as their product, and what
+// depends on the rows of one gate alone is summed once: with S = sum m t n1 and S' = sum m t, dw1 = g S, db1 = g S', dg = w1 S + b1 S'.
+// These products, in shared memory as float32, are a thread's own: g w1, g b1 and w2, and dw1 and db1 over the gates.
 template <typename T, bool VEC, bool CODED, bool LAYER>
-__global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a) {
+__global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a, unsigned* gave_up) {
   constexpr int N = LAYER ? 8 : 4, kWarps = kRnMostThreads / 32;
+  enum { kW2, kDw1, kGw, kGb, kDb1 };
   extern __shared__ float4 parameters_s[];
   __shared__ __align__(16) float part_s[2][kRnMostCluster * kWarps][N];
+  __shared__ uint64_t there_s[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, threads = blockDim.x, warps = threads >> 5;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < 2; ++i) mbar_init(smem_addr(&there_s[i]), 1);
+    mbar_init_fence();
+  }
   const uint32_t rank = a.cluster > 1 ? cluster_rank() : 0, run = blockIdx.x / a.cluster;
   const int c = ((int)rank * threads + (int)threadIdx.x) * 8, C = a.C, entries = a.cluster * warps;
-  uint32_t row, end, unit = 0, left = 0;                // left: rows of the unit, where the run has whole ones
+  uint32_t first, end;
   if (a.units_of_run) {
-    unit = run * a.units_of_run;
-    row = unit * a.unit_rows;
+    const uint32_t unit = run * a.units_of_run;
+    first = unit * a.unit_rows;
     end = min(a.units, unit + a.units_of_run) * a.unit_rows;
-    left = a.unit_rows;
   } else {
     const uint32_t u = run / a.runs_of_unit, k = run - u * a.runs_of_unit;
-    row = u * a.unit_rows + (uint32_t)((uint64_t)k * a.unit_rows / a.runs_of_unit);
+    first = u * a.unit_rows + (uint32_t)((uint64_t)k * a.unit_rows / a.runs_of_unit);
     end = u * a.unit_rows + (uint32_t)((uint64_t)(k + 1) * a.unit_rows / a.runs_of_unit);
   }
-  // Behind C they are zero: with the gate and w2 so, nothing there enters a sum.
-  auto put = [&](int set, const void* p, int dtype, float none) {
-    float2 v[4];
-    rn_parameter(p, dtype, c, C, a.pvec, none, v);
+  // Behind C they are zero: with w2 and the gate's products so, nothing there enters a sum.
+  auto put = [&](int set, float2 (&v)[4]) {
     if (c + 8 > C) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = make_float2(c + 2 * i < C ? v[i].x : 0.f, c + 2 * i + 1 < C ? v[i].y : 0.f);
@@ -509,78 +525,133 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
     rn_put(parameters_s + 2 * set * threads + threadIdx.x, threads, v);
   };
   auto get = [&](int set, float2 (&v)[4]) { rn_get(parameters_s + 2 * set * threads + threadIdx.x, threads, v); };
-  put(kRnW1, a.w1, a.pdtype, 1.f);
-  put(kRnW2, a.w2, a.pdtype, 1.f);
-  if (LAYER) put(kRnB1, a.b1, a.pdtype, 0.f);
-  if (a.cluster > 1) cluster_sync();                    // the others' shared memory is there
-  uint32_t gate_of = 0xffffffffu;
+  float2 none[4] = {}, w2[4];
+  rn_parameter(a.w2, a.pdtype, c, C, a.pvec, 1.f, w2);
+  put(kW2, w2);
+  put(kDw1, none);
+  if (LAYER) put(kDb1, none);
+  if (a.cluster > 1) cluster_sync();                    // the others' barriers are there
   NoiseKey key;
   if (a.dropped) key = drop_key(a.drop);
-  float2 dw2[4] = {}, dw1[4] = {}, dg[4] = {}, db2[4] = {}, db1[4] = {};
+  float2 dw2[4] = {}, sum[4] = {}, db2[4] = {}, sum_b[4] = {};
   RnRaw<T, CODED> raw;
-  float4 st = make_float4(0.f, 0.f, 0.f, 0.f), next_st = st;
-  if (row < end) {
-    rn_load_raw<T, CODED, VEC>(raw, a, row, c);
-    next_st = rn_ld(a.stats + row);
+  float4 next_st = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (first < end) {
+    rn_load_raw<T, CODED, VEC>(raw, a, first, c);
+    next_st = rn_ld(a.stats + first);
   }
-  for (int place = 0; row < end; ++row, place ^= 1) {
-    st = next_st;
-    if (const uint32_t g = fast_div(row, a.by_gate); g != gate_of) {
-      put(kRnGate, rn_gate_row(a, row), a.gdtype, 1.f);
-      gate_of = g;
+  uint32_t gate = fast_div(first, a.by_gate), gate_left = (gate + 1) * a.by_gate.d - first;        // rows that the gate still has
+  bool ok = true, other = true;                         // other: the next row has another gate
+  // dw1, db1 and what the gate's gradient is, of the rows of a gate that are over.
+  auto turn = [&](uint32_t row) {
+    const uint32_t g = fast_div(row, a.by_gate);
+    float2 q[4], v[4], d[4];
+    rn_parameter(rn_gate_row(a, row), a.gdtype, c, C, a.pvec, 1.f, q);
+    get(kDw1, d);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) d[i] = f_fma(q[i], sum[i], d[i]);
+    put(kDw1, d);
+    if (LAYER) {
+      get(kDb1, d);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = f_fma(q[i], sum_b[i], d[i]);
+      put(kDb1, d);
     }
-    float2 n1[4], n2[4], dn[4], cc[4];                  // n2: scale x until the norm is known; dn: dh, then d;  cc: dr + p2 dn2
-    rn_inputs<T, CODED, LAYER>(raw, a, st, n2, n1);
-    unpack_vec(raw.dr, cc);
-    unpack_vec(raw.dh, dn);
-    if (row + 1 < end) {
-      rn_load_raw<T, CODED, VEC>(raw, a, row + 1, c);
-      next_st = rn_ld(a.stats + row + 1);
+    if (a.dgate) {
+      rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = f_mul(v[i], sum[i]);
+      if (LAYER) {
+        rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = f_fma(d[i], sum_b[i], v[i]);
+      }
+      if (a.units_of_run) rn_store_eight(a.dgate, a.gdtype, (size_t)g * C, c, C, v);
+      else rn_store_eight(a.parts, ACTNN_F32, ((size_t)run * a.slots + a.slot_gate) * C, c, C, v);
     }
-    float2 q[4], w1[4];
-    get(kRnGate, q);
-    get(kRnW1, w1);
-    float2 s0{}, s1{}, s2{}, s3{}, s4{}, s5{}, s6{}, s7{};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum[i] = sum_b[i] = make_float2(0.f, 0.f);
+  };
+  uint32_t phase = 0;
+  for (int place = 0; first < end; ++first, place ^= 1) {
+    if (other) {
+      float2 q[4], w[4];
+      rn_parameter(rn_gate_row(a, first), a.gdtype, c, C, a.pvec, 1.f, q);
+      rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, w);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
+      put(kGw, w);
+      if (LAYER) {
+        rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, w);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
+        put(kGb, w);
+      }
+    }
+    other = --gate_left == 0;
+    if (other) gate_left = a.by_gate.d;
+    const float4 st = next_st;
+    float2 n1[4], n2[4], cc[4], m[4];                   // m: the dropout's factors
     {
-      float2 w2[4], b1[4], m[4];
-      get(kRnW2, w2);
-      if (LAYER) get(kRnB1, b1);
-      if (a.dropped) rn_factors<VEC>(a, key, row, c, m);
+      float2 dh[4], p[4];
+      rn_inputs<T, CODED, LAYER>(raw, a, st, n2, n1);
+      unpack_vec(raw.dr, cc);
+      unpack_vec(raw.dh, dh);
+      if (first + 1 < end) {
+        rn_load_raw<T, CODED, VEC>(raw, a, first + 1, c);
+        next_st = rn_ld(a.stats + first + 1);
+      }
+      if (a.dropped) drop_factors(rn_fields<VEC>(a, key, first, c), a.drop.least, a.drop.inv, m);
+      const float2 p2 = make_float2(st.w, st.w);
+      if constexpr (LAYER) {
+        get(kGb, p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (a.dropped) p[i] = f_mul(p[i], m[i]);
+          n2[i] = f_fma(p[i], p2, n2[i]);
+        }
+      }
+      float2 s0{}, s1{}, s2{}, s3{}, s4{}, s5{}, s6{}, s7{};
+      get(kGw, p);
+      get(kW2, w2);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float2 d = a.post ? (LAYER ? f_fma(n1[i], w1[i], b1[i]) : f_mul(n1[i], w1[i])) : n1[i];
-        if (a.dropped) d = f_mul(d, m[i]);
-        n2[i] = f_fma(d, q[i], n2[i]);
-        if (LAYER) n2[i] = f_add(n2[i], make_float2(-st.z, -st.z));
-        n2[i] = f_mul(n2[i], make_float2(st.w, st.w));
-        if (a.dropped) q[i] = f_mul(q[i], m[i]);
-        const float2 dn2 = f_mul(dn[i], w2[i]);
-        cc[i] = f_fma(make_float2(st.w, st.w), dn2, cc[i]);
-        dw2[i] = f_fma(dn[i], n2[i], dw2[i]);
-        if (LAYER) db2[i] = f_add(db2[i], dn[i]);
-        dn[i] = d;
+        if (a.dropped) p[i] = f_mul(p[i], m[i]);
+        const float2 gn = f_mul(p[i], n1[i]);
+        n2[i] = f_fma(gn, p2, n2[i]);
+        const float2 dn2 = f_mul(dh[i], w2[i]);
+        cc[i] = f_fma(p2, dn2, cc[i]);
+        dw2[i] = f_fma(dh[i], n2[i], dw2[i]);
+        if (LAYER) db2[i] = f_add(db2[i], dh[i]);
         s0 = f_fma(dn2, n2[i], s0);
-        const float2 g = f_mul(q[i], w1[i]), gn = f_mul(g, n1[i]);
         s1 = f_fma(gn, cc[i], s1);
         s2 = f_fma(gn, n2[i], s2);
-        if (LAYER) s3 = f_add(s3, dn2), s4 = f_add(s4, gn), s5 = f_fma(g, cc[i], s5), s6 = f_add(s6, g), s7 = f_fma(g, n2[i], s7);
+        if (LAYER) s3 = f_add(s3, dn2), s4 = f_add(s4, gn), s5 = f_fma(p[i], cc[i], s5), s6 = f_add(s6, p[i]), s7 = f_fma(p[i], n2[i], s7);
       }
-    }
-    float v[N];
-    v[0] = f_sum(s0), v[1] = f_sum(s1), v[2] = f_sum(s2), v[3] = f_sum(s3);
-    if constexpr (LAYER) v[4] = f_sum(s4), v[5] = f_sum(s5), v[6] = f_sum(s6), v[7] = f_sum(s7);
-    const float mine = rn_warp_sums<N>(v);
-    if (lane % (32 / N) == 0) {
-      float* at = &part_s[place][rank * warps + warp][lane / (32 / N)];
-      if (a.cluster > 1) {
-        for (int k = 0; k < a.cluster; ++k) peer_store1(smem_addr(at), k, __float_as_int(mine));
+      float v[N];
+      v[0] = f_sum(s0), v[1] = f_sum(s1), v[2] = f_sum(s2), v[3] = f_sum(s3);
+      if constexpr (LAYER) v[4] = f_sum(s4), v[5] = f_sum(s5), v[6] = f_sum(s6), v[7] = f_sum(s7);
+      const float mine = rn_warp_sums<N>(v);
+      if (a.cluster > 1) {                              // all have read the place's sums of two rows ago: they have sent those of the last one since
+        const uint32_t bar = smem_addr(&there_s[place]), at = smem_addr(part_s[place][rank * warps + warp]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kFull, mine, i * (32 / N));
+        if (threadIdx.x == 0) mbar_expect_tx(bar, entries * N * (int)sizeof(float));
+        if (lane < a.cluster) {
+#pragma unroll
+          for (int i = 0; i < N; i += 4) peer_send4(at + 4 * i, bar, lane, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+        }
+        if (ok) {
+          ok = __all_sync(kFull, mbar_wait(bar, phase >> place & 1));
+          if (!ok && lane == 0) atomicAdd(gave_up, 1u);
+        }
+        phase ^= 1u << place;
       } else {
-        *at = mine;
+        if (lane % (32 / N) == 0) part_s[place][warp][lane / (32 / N)] = mine;
+        if (warps > 1) __syncthreads();
+        else __syncwarp();
       }
     }
-    if (a.cluster > 1) cluster_sync();
-    else if (warps > 1) __syncthreads();
-    else __syncwarp();
     float total[N];
 #pragma unroll
     for (int i = 0; i < N; i += 4) {
@@ -591,51 +662,52 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
 #pragma unroll
       for (int i = 0; i < N; ++i) total[i] += part_s[place][e][i];
     }
-    const float joined = rn_warp_sums<N>(total);
+    float joined = rn_warp_sums<N>(total);
+    if (!ok) joined = __int_as_float(0x7fffffff);
 #pragma unroll
     for (int i = 0; i < N; ++i) total[i] = __shfl_sync(kFull, joined, i * (32 / N)) * a.inv_c;
-    float M = 0.f, mean1 = 0.f;                          // p2 mean dn2; mean of dn1
-    const float m2 = st.w * total[0];                    // p2 mean(dn2 n2)
-    float dot1 = total[1] - m2 * total[2];               // mean(dn1 n1)
+    float M = 0.f, mean1 = 0.f;                         // p2 mean dn2; p1 times the mean of dn1
+    const float m2 = st.w * total[0];                   // p2 mean(dn2 n2)
+    float dot1 = total[1] - m2 * total[2];              // mean(dn1 n1)
     if constexpr (LAYER) {
       M = st.w * total[3];
       dot1 -= M * total[4];
-      mean1 = total[5] - M * total[6] - m2 * total[7];
+      mean1 = (total[5] - M * total[6] - m2 * total[7]) * st.y;
     }
-    float2 dx[4];
+    dot1 *= st.y;
+    float2 p[4], dx[4];
+    get(kGw, p);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       float2 t = f_fma(n2[i], make_float2(-m2, -m2), cc[i]);
       if (LAYER) t = f_add(t, make_float2(-M, -M));
-      dg[i] = f_fma(t, dn[i], dg[i]);
-      float2 du = f_mul(q[i], t);
-      dw1[i] = f_fma(du, n1[i], dw1[i]);
-      if (LAYER) db1[i] = f_add(db1[i], du);
       dx[i] = f_mul(t, make_float2(a.scale, a.scale));
+      if (a.dropped) t = f_mul(t, m[i]);                // what passes the dropout
+      sum[i] = f_fma(t, n1[i], sum[i]);
+      if (LAYER) sum_b[i] = f_add(sum_b[i], t);
+      t = f_mul(t, p[i]);
       if (a.post) {
-        du = f_fma(n1[i], make_float2(-dot1, -dot1), f_mul(du, w1[i]));
-        if (LAYER) du = f_add(du, make_float2(-mean1, -mean1));
-        du = f_mul(du, make_float2(st.y, st.y));
+        n1[i] = LAYER ? f_fma(n1[i], make_float2(-dot1, -dot1), make_float2(-mean1, -mean1)) : f_mul(n1[i], make_float2(-dot1, -dot1));
+        t = f_fma(t, make_float2(st.y, st.y), n1[i]);
       }
-      n1[i] = du;
+      n1[i] = t;
     }
-    if (a.dx) rn_store<T, VEC>((T*)a.dx + (size_t)row * C, c, C, dx);
-    if (a.df) rn_store<T, VEC>((T*)a.df + (size_t)row * C, c, C, n1);
-    if (a.units_of_run && --left == 0) {
-      rn_store_eight(a.dgate, a.gdtype, (size_t)unit * C, c, C, dg);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) dg[i] = make_float2(0.f, 0.f);
-      ++unit;
-      left = a.unit_rows;
-    }
+    if (a.dx) rn_store<T, VEC>((T*)a.dx + (size_t)first * C, c, C, dx);
+    if (a.df) rn_store<T, VEC>((T*)a.df + (size_t)first * C, c, C, n1);
+    if (other || first + 1 == end) turn(first);
   }
-  auto leave = [&](const float2 (&sum)[4], int slot) {
-    if (slot >= 0) rn_store_eight(a.parts, ACTNN_F32, ((size_t)run * a.slots + slot) * C, c, C, sum);
+  if (a.cluster > 1) cluster_sync();                    // nobody leaves while sums are on their way to it
+  auto leave = [&](const float2 (&v)[4], int slot) {
+    if (slot >= 0) rn_store_eight(a.parts, ACTNN_F32, ((size_t)run * a.slots + slot) * C, c, C, v);
   };
   leave(dw2, a.slot_w2);
-  leave(dw1, a.slot_w1);
-  leave(dg, a.slot_gate);
-  if (LAYER) leave(db2, a.slot_b2), leave(db1, a.slot_b1);
+  get(kDw1, w2);
+  leave(w2, a.slot_w1);
+  if (LAYER) {
+    leave(db2, a.slot_b2);
+    get(kDb1, w2);
+    leave(w2, a.slot_b1);
+  }
 }
 
 // The partial sums of the runs, added in order: a block has 32 columns of one sum, 32 threads a column.
@@ -683,8 +755,10 @@ template <typename T, bool VEC, bool LAYER> int rn_forward(const RnArgs& a) {
 }
 template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const RnArgs& a) {
   auto* kernel = rn_backward_kernel<T, VEC, CODED, LAYER>;
+  unsigned* gave_up = bulk_wait_counter();
+  if (!gave_up) return ACTNN_ERR_LAUNCH;
   const int threads = a.cluster > 1 ? kRnMostThreads : (a.C + 255) / 256 * 32;
-  const int smem = (LAYER ? 4 : 3) * 2 * threads * (int)sizeof(float4);
+  const int smem = (LAYER ? 5 : 3) * 2 * threads * (int)sizeof(float4);
   rn_blocks_per_sm((const void*)kernel, threads, smem);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(a.runs * a.cluster);
@@ -697,7 +771,7 @@ template <typename T, bool VEC, bool CODED, bool LAYER> int rn_backward(const Rn
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = a.cluster > 1 ? 1 : 0;
-  if (cudaLaunchKernelEx(&cfg, kernel, a) != cudaSuccess) return cudaGetLastError(), ACTNN_ERR_LAUNCH;
+  if (cudaLaunchKernelEx(&cfg, kernel, a, gave_up) != cudaSuccess) return cudaGetLastError(), ACTNN_ERR_LAUNCH;
   if (int st = check_launch()) return st;
   if (a.slots == 0) return ACTNN_OK;
   const int sums = a.slot_gate >= 0 ? a.slots - 1 + (int)a.units : a.slots;

@@ -9,7 +9,6 @@ namespace actnn {
 #ifdef __CUDACC__
 
 // ------------------------------------------------------------------ barriers
-ACTNN_DEV void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" :: "r"(bar) : "memory"); }
 
 // One lane of a warp that is together, always the same.  A branch on it the compiler knows to be of one lane, and keeps what is uniform
 // in the registers that copies and matrix instructions take their operands from.
