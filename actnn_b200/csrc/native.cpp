@@ -515,7 +515,8 @@ Tensor fp8_linear(const Tensor& x, const Tensor& codes, const Tensor& scales, co
   c10::cuda::CUDAGuard guard(x.device());
   Tensor out = make(with_last(x, n), x.scalar_type(), x);
   const bool with = bias.has_value() && bias->defined();
-  const Tensor b = with ? bias->detach().to(x.scalar_type()).contiguous() : Tensor();
+  const bool as_it_is = with && bias->scalar_type() == x.scalar_type() && bias->is_contiguous();
+  const Tensor b = as_it_is ? *bias : with ? bias->detach().to(x.scalar_type()).contiguous() : Tensor();
   if (k == 0) return with ? out.copy_(b) : out.zero_();
   const auto [flat, ldx] = as_rows(x);
   const auto [w, ldw] = code_rows(codes.view(at::kByte));
@@ -598,8 +599,11 @@ Residual residual_of(const Tensor& x, const Tensor& weight, const Tensor& bias, 
     any = true;
   }
   r.ptype = mixed ? at::kFloat : type;
-  for (Tensor* q : params)
-    if (q->defined()) *q = q->detach().to(r.ptype).contiguous();
+  for (Tensor* q : params) {
+    if (!q->defined()) continue;
+    if (q->scalar_type() != r.ptype) *q = q->detach().to(r.ptype);
+    if (!q->is_contiguous()) *q = q->detach().contiguous();
+  }
   if (gate.defined()) {
     check_values(gate, "gate");
     TORCH_CHECK(gate.device() == x.device(), "gate is on ", gate.device(), ", expected ", x.device());
@@ -613,7 +617,7 @@ Residual residual_of(const Tensor& x, const Tensor& weight, const Tensor& bias, 
                 "the leading dimensions up to some place");
     r.gate_rows = std::max<int64_t>(each, 1);
     r.gtype = gate.scalar_type();
-    r.gate = gate.detach().contiguous();
+    if (!gate.is_contiguous()) r.gate = gate.detach().contiguous();
   }
   return r;
 }
