@@ -40,62 +40,67 @@ ACTNN_DEV float2 fp8_unpack(uint32_t pair) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 ACTNN_DEV bool not_finite(uint32_t bits) { return (bits & 0x7fffffffu) >= 0x7f800000u; }
-ACTNN_DEV float finite_or_nan(float v) { return not_finite(__float_as_uint(v)) ? __uint_as_float(0x7fffffffu) : v; }
-
-// The largest magnitude of the finite elements, as bits; `bad`: whether there are others.
-template <typename T> ACTNN_DEV uint32_t fp8_most(const Vec<T, 8>& v, bool& bad) {
-  uint32_t most = most_of(v);
-  bad = not_finite(most);
-  if (bad) {
-    most = 0;
-    float2 f[4];
-    unpack_vec(v, f);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint32_t x = abs_bits(f[i].x), y = abs_bits(f[i].y);
-      most = max(most, max(not_finite(x) ? 0u : x, not_finite(y) ? 0u : y));
-    }
-  }
-  return most;
+// A word of elements (one of float32, two of a 16-bit type): zero, or NaN, in the place of what is not finite.
+template <typename T> ACTNN_DEV uint32_t fp8_word(uint32_t w, uint32_t instead) {
+  const float2 f = pair_to_float(w, T());
+  return (not_finite(__float_as_uint(f.x)) ? instead & 0xffffu : w & 0xffffu) | (not_finite(__float_as_uint(f.y)) ? instead & 0xffff0000u : w & 0xffff0000u);
 }
-// The codes of eight elements.
-template <typename T> ACTNN_DEV uint2 fp8_codes8(const Vec<T, 8>& v, float factor, bool bad) {
+template <> ACTNN_DEV uint32_t fp8_word<float>(uint32_t w, uint32_t instead) { return not_finite(w) ? instead : w; }
+template <typename T> ACTNN_DEV uint32_t fp8_word_finite(uint32_t w) { return fp8_word<T>(w, 0u); }
+template <typename T> ACTNN_DEV uint32_t fp8_word_nan(uint32_t w) { return fp8_word<T>(w, sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
+// Their magnitudes, which compare as unsigned numbers do; whether one of them is not finite; the larger ones.
+template <typename T> ACTNN_DEV uint32_t fp8_word_abs(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
+template <typename T> ACTNN_DEV uint32_t fp8_word_max(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
+template <typename T> ACTNN_DEV bool fp8_word_bad(uint32_t magnitudes) {
+  const float2 f = pair_to_float(magnitudes, T());
+  return not_finite(__float_as_uint(f.x)) || not_finite(__float_as_uint(f.y));
+}
+template <> ACTNN_DEV bool fp8_word_bad<float>(uint32_t magnitudes) { return not_finite(magnitudes); }
+
+// The codes of eight elements, which are finite or NaN.
+template <typename T> ACTNN_DEV uint2 fp8_codes8(const Vec<T, 8>& v, float factor) {
   float2 f[4];
   unpack_vec(v, f);
-  if (bad) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) f[i] = make_float2(finite_or_nan(f[i].x), finite_or_nan(f[i].y));
-  }
 #pragma unroll
   for (int i = 0; i < 4; ++i) f[i] = f_mul(f[i], make_float2(factor, factor));
   return make_uint2(fp8_pair(f[0].x, f[0].y) | fp8_pair(f[1].x, f[1].y) << 16, fp8_pair(f[2].x, f[2].y) | fp8_pair(f[3].x, f[3].y) << 16);
 }
-// The largest magnitudes, as bits of float32, of two vectors over the half of the warp that the lane is in, which with a vector is a
-// block; `bad`: whether the block holds what is not finite, which does not count.  16-bit types go through the lanes side by side.
-template <typename T> ACTNN_DEV void fp8_block_bits(const Vec<T, 8>& a, const Vec<T, 8>& b, uint32_t (&bits)[2], bool (&bad)[2]) {
+// The largest magnitudes, as bits of float32, of two vectors over the half of the warp that the lane is in, given the largest of the words
+// of each.  16-bit types go through the lanes side by side.
+template <typename T> ACTNN_DEV void fp8_half_warp(uint32_t m, uint32_t n, uint32_t (&bits)[2]) {
   if constexpr (sizeof(T) == 2) {
-    uint32_t m = a.w[0] & 0x7fff7fffu, n = b.w[0] & 0x7fff7fffu;
-#pragma unroll
-    for (int i = 1; i < 4; ++i) m = __vmaxu2(m, a.w[i] & 0x7fff7fffu), n = __vmaxu2(n, b.w[i] & 0x7fff7fffu);
     uint32_t w = __vmaxu2(__byte_perm(m, n, 0x5410), __byte_perm(m, n, 0x7632));
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) w = __vmaxu2(w, __shfl_xor_sync(kFull, w, o));
-    bits[0] = __float_as_uint(pair_to_float(w, T()).x);
-    bits[1] = __float_as_uint(pair_to_float(w, T()).y);
+    const float2 f = pair_to_float(w, T());
+    bits[0] = __float_as_uint(f.x), bits[1] = __float_as_uint(f.y);
   } else {
-    bits[0] = most_of(a), bits[1] = most_of(b);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1)
-      bits[0] = max(bits[0], __shfl_xor_sync(kFull, bits[0], o)), bits[1] = max(bits[1], __shfl_xor_sync(kFull, bits[1], o));
+    for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFull, m, o)), n = max(n, __shfl_xor_sync(kFull, n, o));
+    bits[0] = m, bits[1] = n;
   }
-  bad[0] = not_finite(bits[0]), bad[1] = not_finite(bits[1]);
-  if (__any_sync(kFull, bad[0] || bad[1])) {
-    bool mine;
-    uint32_t x = fp8_most(a, mine), y = fp8_most(b, mine);
+}
+template <typename T> ACTNN_DEV uint32_t fp8_words_most(const Vec<T, 8>& v) {
+  uint32_t m = fp8_word_abs<T>(v.w[0]);
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) x = max(x, __shfl_xor_sync(kFull, x, o)), y = max(y, __shfl_xor_sync(kFull, y, o));
-    bits[0] = x, bits[1] = y;
+  for (int i = 1; i < (int)(sizeof(v.w) / 4); ++i) m = fp8_word_max<T>(m, fp8_word_abs<T>(v.w[i]));
+  return m;
+}
+// The largest magnitudes of two vectors' blocks, which with a vector are half a warp.  What is not finite does not count, and is
+// made NaN.
+template <typename T> ACTNN_DEV void fp8_block_bits(Vec<T, 8>& a, Vec<T, 8>& b, uint32_t (&bits)[2]) {
+  uint32_t m = fp8_words_most(a), n = fp8_words_most(b);
+  if (__any_sync(kFull, fp8_word_bad<T>(fp8_word_max<T>(m, n)))) {
+    m = n = 0;
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(a.w) / 4); ++i) {
+      m = fp8_word_max<T>(m, fp8_word_abs<T>(fp8_word_finite<T>(a.w[i])));
+      n = fp8_word_max<T>(n, fp8_word_abs<T>(fp8_word_finite<T>(b.w[i])));
+      a.w[i] = fp8_word_nan<T>(a.w[i]);
+      b.w[i] = fp8_word_nan<T>(b.w[i]);
+    }
   }
+  fp8_half_warp<T>(m, n, bits);
 }
 // Eight elements from e on, zeros from `end` on.  VEC: whole aligned vectors.
 template <typename T, bool VEC> ACTNN_DEV Vec<T, 8> fp8_load(const T* p, int64_t e, int64_t end) {

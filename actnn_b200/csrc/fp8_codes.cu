@@ -34,32 +34,24 @@ fp8_row_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint8
   for (int i = 0; i < TASKS; ++i) {
     if (row[i] >= rows) return;
     uint32_t byte[2];
-    bool bad[2];
-    fp8_block_bits(v[i][0], v[i][1], byte, bad);
+    fp8_block_bits(v[i][0], v[i][1], byte);
     uint8_t* to = codes + row[i] * ldc + g[i] * 512 + lane * 8;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       byte[k] = fp8_scale_byte(byte[k]);
-      if (g[i] * 512 + k * 256 + lane * 8 < ldc) *reinterpret_cast<uint2*>(to + k * 256) = fp8_codes8(v[i][k], fp8_factor(byte[k]), bad[k]);
+      if (g[i] * 512 + k * 256 + lane * 8 < ldc) *reinterpret_cast<uint2*>(to + k * 256) = fp8_codes8(v[i][k], fp8_factor(byte[k]));
     }
     const uint32_t mine = byte[0] | byte[1] << 16, other = __shfl_xor_sync(kFull, mine, 16);
     if (lane == 0) *reinterpret_cast<uint32_t*>(scales + fp8_scale_at(row[i], g[i] * 4, (rows + 127) / 128)) = mine | other << 8;
   }
 }
 
-// The magnitudes of a vector's elements as words that can be compared: one of float32, two of a 16-bit type side by side.
+// Elements of a word of columns, and the bits of float32 of one of its magnitudes.
 template <typename T> constexpr int word_columns() { return 4 / (int)sizeof(T); }
-template <typename T> ACTNN_DEV uint32_t word_max(uint32_t a, uint32_t b) { return sizeof(T) == 4 ? max(a, b) : __vmaxu2(a, b); }
-template <typename T> ACTNN_DEV uint32_t word_abs(uint32_t w) { return w & (sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu); }
-// Zero in the place of what is not finite.
-template <typename T> ACTNN_DEV uint32_t word_finite(uint32_t w) {
-  if (sizeof(T) == 4) return not_finite(w) ? 0u : w;
+template <typename T> ACTNN_DEV uint32_t word_bits(uint32_t w, int which) {
   const float2 f = pair_to_float(w, T());
-  return (not_finite(__float_as_uint(f.x)) ? 0u : w & 0xffffu) | (not_finite(__float_as_uint(f.y)) ? 0u : w & 0xffff0000u);
+  return __float_as_uint(which ? f.y : f.x);
 }
-template <> ACTNN_DEV uint32_t word_finite<float>(uint32_t w) { return not_finite(w) ? 0u : w; }
-// The bits of float32 of one of a word's magnitudes.
-template <typename T> ACTNN_DEV uint32_t word_bits(uint32_t w, int which) { return abs_bits(pair_to_float(which ? w >> 16 : w & 0xffffu, T()).x); }
 template <> ACTNN_DEV uint32_t word_bits<float>(uint32_t w, int) { return w; }
 // Columns 2 j and 2 j + 1 of a vector.
 template <typename T> ACTNN_DEV float2 column_pair(const Vec<T, 8>& v, int j) { return pair_to_float(v.w[j], T()); }
@@ -79,23 +71,52 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
   constexpr int kWords = 8 / word_columns<T>();
   const int64_t row_tiles = (rows + 127) / 128;
   __shared__ uint4 turned_s[128 * 8];                  // [column][128 rows], chunks of eight rows in the order rotated by column / 8
-  __shared__ uint32_t most_s[16][128];                 // [team][word of columns]; later float sums of columns
-  __shared__ float factor_s[128];
+  __shared__ __align__(16) uint32_t most_s[16][128];                 // [team][word of columns]; later float sums of columns
+  __shared__ __align__(16) float factor_s[128];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c8 = lane & 15, team = warp * 2 + (lane >> 4);
   const int64_t tr = blockIdx.x / column_tiles, tc = blockIdx.x - tr * column_tiles, r0 = tr * 128 + team * 8, c = tc * 128 + c8 * 8;
   Vec<T, 8> v[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) v[i] = fp8_load<T, VEC>(x + (r0 + i) * ldx, c, r0 + i < rows ? cols : 0);
 
-  uint32_t bad = 0, square = 0;                         // bad: rows with elements that are not finite
-  if (SQUARE) {
+  // ---- sums of columns
+  float2 sum[4] = {};
+  if (parts) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sum[j] = f_add(sum[j], column_pair(v[i], j));
+  }
+
+  // ---- the largest magnitudes of the thread's rows and columns, as words; what is not finite does not count, and is made NaN
+  uint32_t of_row[8], most[kWords] = {}, any = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    of_row[i] = fp8_words_most(v[i]);
+    any = fp8_word_max<T>(any, of_row[i]);
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) most[j] = fp8_word_max<T>(most[j], fp8_word_abs<T>(v[i].w[j]));
+  }
+  if (__any_sync(kFull, fp8_word_bad<T>(any))) {
+    any = 0;
+#pragma unroll
+    for (int j = 0; j < kWords; ++j) most[j] = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      bool b;
-      square = max(square, fp8_most(v[i], b));
-      bad |= (uint32_t)b << i;
+      of_row[i] = 0;
+#pragma unroll
+      for (int j = 0; j < kWords; ++j) {
+        const uint32_t w = fp8_word_abs<T>(fp8_word_finite<T>(v[i].w[j]));
+        of_row[i] = fp8_word_max<T>(of_row[i], w);
+        most[j] = fp8_word_max<T>(most[j], w);
+        v[i].w[j] = fp8_word_nan<T>(v[i].w[j]);
+      }
+      any = fp8_word_max<T>(any, of_row[i]);
     }
-    square = __reduce_max_sync(kFull, square);
+  }
+  uint32_t square = 0;
+  if (SQUARE) {
+    square = __reduce_max_sync(kFull, max(word_bits<T>(any, 0), word_bits<T>(any, 1)));
     if (lane == 0) most_s[0][warp] = square;
     __syncthreads();
     square = most_s[0][0];
@@ -103,28 +124,23 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
     for (int w = 1; w < kCodeThreads / 32; ++w) square = max(square, most_s[0][w]);
     square = fp8_scale_byte(square);
   }
-  // ---- rows, two at a time, and the largest of the thread's columns
-  uint32_t most[kWords] = {};
+
+  // ---- rows, two at a time
+  if (codes) {
+    const int left = (int)min((int64_t)8, rows - r0);   // rows that there are
+    uint8_t *to = codes + r0 * ldc + c, *to_s = scales + fp8_scale_at(r0, tc, row_tiles);          // eight rows lie 16 bytes apart
 #pragma unroll
-  for (int i = 0; i < 8; i += 2) {
-    uint32_t byte[2] = {square, square};
-    if (!SQUARE) {
-      bool b[2];
-      fp8_block_bits(v[i], v[i + 1], byte, b);
-      byte[0] = fp8_scale_byte(byte[0]), byte[1] = fp8_scale_byte(byte[1]);
-      bad |= (uint32_t)b[0] << i | (uint32_t)b[1] << (i + 1);
-#pragma unroll
-      for (int j = 0; j < kWords; ++j) {
-        const uint32_t w = word_abs<T>(v[i].w[j]), x = word_abs<T>(v[i + 1].w[j]);
-        most[j] = word_max<T>(word_max<T>(most[j], b[0] ? word_finite<T>(w) : w), b[1] ? word_finite<T>(x) : x);
+    for (int i = 0; i < 8; i += 2) {
+      uint32_t byte[2] = {square, square};
+      if (!SQUARE) {
+        fp8_half_warp<T>(of_row[i], of_row[i + 1], byte);
+        byte[0] = fp8_scale_byte(byte[0]), byte[1] = fp8_scale_byte(byte[1]);
       }
-    }
-    if (codes) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        if (r0 + i + k >= rows) continue;
-        if (c < ldc) *reinterpret_cast<uint2*>(codes + (r0 + i + k) * ldc + c) = fp8_codes8(v[i + k], fp8_factor(byte[k]), bad >> (i + k) & 1);
-        if (c8 == 0) scales[fp8_scale_at(r0 + i + k, tc, row_tiles)] = (uint8_t)byte[k];
+        const uint2 q = fp8_codes8(v[i + k], fp8_factor(byte[k]));
+        if (i + k < left && c < ldc) *reinterpret_cast<uint2*>(to + (i + k) * ldc) = q;
+        if (i + k < left && c8 == 0) to_s[16 * (i + k)] = (uint8_t)byte[k];
       }
     }
   }
@@ -139,7 +155,7 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
         const int word = threadIdx.x / word_columns<T>();
         uint32_t all = most_s[0][word];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) all = word_max<T>(all, most_s[k][word]);
+        for (int k = 1; k < 16; ++k) all = fp8_word_max<T>(all, most_s[k][word]);
         const uint32_t byte = fp8_scale_byte(word_bits<T>(all, threadIdx.x % word_columns<T>()));
         factor_s[threadIdx.x] = fp8_factor(byte);
         if (tc * 128 + threadIdx.x < cols) scales_t[fp8_scale_at(tc * 128 + threadIdx.x, tr, column_tiles)] = (uint8_t)byte;
@@ -150,14 +166,13 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const float fx = SQUARE ? fp8_factor(square) : factor_s[c8 * 8 + 2 * j], fy = SQUARE ? fx : factor_s[c8 * 8 + 2 * j + 1];
+      const float2 by = SQUARE ? make_float2(fp8_factor(square), fp8_factor(square)) : *reinterpret_cast<const float2*>(&factor_s[c8 * 8 + 2 * j]);
       uint32_t px[4], py[4];                           // two rows each
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
-        float2 a = column_pair(v[i], j), b = column_pair(v[i + 1], j);
-        if (bad) a = make_float2(finite_or_nan(a.x), finite_or_nan(a.y)), b = make_float2(finite_or_nan(b.x), finite_or_nan(b.y));
-        px[i / 2] = fp8_pair(a.x * fx, b.x * fx);
-        py[i / 2] = fp8_pair(a.y * fy, b.y * fy);
+        const float2 a = f_mul(column_pair(v[i], j), by), b = f_mul(column_pair(v[i + 1], j), by);
+        px[i / 2] = fp8_pair(a.x, b.x);
+        py[i / 2] = fp8_pair(a.y, b.y);
       }
       uint2* at = reinterpret_cast<uint2*>(turned_s) + (c8 * 8 + 2 * j) * 16 + (team ^ c8);
       at[0] = make_uint2(px[0] | px[1] << 16, px[2] | px[3] << 16);
@@ -174,18 +189,11 @@ fp8_tile_codes_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes, uint
     }
   }
 
-  // ---- sums of columns
   if (parts) {
     __syncthreads();
     float* sum_s = reinterpret_cast<float*>(most_s);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float2 s = make_float2(0.f, 0.f);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s = f_add(s, column_pair(v[i], j));
-      sum_s[team * 128 + c8 * 8 + 2 * j] = s.x;
-      sum_s[team * 128 + c8 * 8 + 2 * j + 1] = s.y;
-    }
+    for (int j = 0; j < 4; ++j) *reinterpret_cast<float2*>(&sum_s[team * 128 + c8 * 8 + 2 * j]) = sum[j];
     __syncthreads();
     if (threadIdx.x < 128 && tc * 128 + threadIdx.x < cols) {
       float s = sum_s[threadIdx.x];

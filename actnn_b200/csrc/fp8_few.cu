@@ -79,15 +79,14 @@ fp8_few_kernel(const T* __restrict__ x, const uint8_t* __restrict__ weights, con
     const T* p = x + t * ldx;
     Vec<T, 8> v[2];
     uint32_t byte[2];
-    bool bad[2];
 #pragma unroll
     for (int k = 0; k < 2; ++k) v[k] = vec ? fp8_load<T, true>(p, j * 512 + k * 256 + lane * 8, K) : fp8_load<T, false>(p, j * 512 + k * 256 + lane * 8, K);
-    fp8_block_bits(v[0], v[1], byte, bad);
+    fp8_block_bits(v[0], v[1], byte);
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
       const int e = j * 512 + k * 256 + lane * 8;
       byte[k] = fp8_scale_byte(byte[k]);
-      if (e < stride - 64) *reinterpret_cast<uint2*>(codes_s + t * stride + e) = fp8_codes8(v[k], fp8_factor(byte[k]), bad[k]);
+      if (e < stride - 64) *reinterpret_cast<uint2*>(codes_s + t * stride + e) = fp8_codes8(v[k], fp8_factor(byte[k]));
     }
     const uint32_t mine = byte[0] | byte[1] << 16, other = __shfl_xor_sync(kFull, mine, 16);
     if (lane == 0) scale_s[t * groups + j] = mine | other << 8;

@@ -384,3 +384,14 @@ def test_swapped_codes_give_the_same_gradients(cuda_device):
     want = grads(ops.fp8_linear.apply, (x, w, b))
     actnn.set_optimization_level("L4")
     assert all(torch.equal(a, v) for a, v in zip(grads(ops.fp8_linear.apply, (x, w, b)), want))
+
+
+def test_sums_of_columns_that_are_not_finite(cuda_device):
+    from actnn_b200.cpp_extension import fp8
+    x = tokens(300, 200, torch.bfloat16)
+    x[5, 3], x[130, 4], x[131, 4], x[7, 5] = float("inf"), float("inf"), -float("inf"), float("nan")
+    sums = fp8.join_sums(fp8.tile_codes(x, True, True, True)[2], torch.float32).double().cpu()
+    want = x.double().sum(0).cpu()
+    assert sums[3] == float("inf") and sums[4].isnan() and sums[5].isnan()
+    keep = want.isfinite()
+    assert int(keep.sum()) == 197 and bool(((sums - want)[keep].abs() <= 301 * 2.0 ** -24 * x.double().abs().sum(0).cpu()[keep]).all())
