@@ -20,7 +20,7 @@ SOURCES = ["api.cu", "codec_mixed.cu", "codec_single.cu", "codec_generic.cu", "c
            "group_norm.cu", "group_norm_f16.cu", "group_norm_bf16.cu",
            "fp8_codes.cu", "fp8_matmul.cu", "fp8_few.cu", "seeded_dropout.cu", "residual_norm.cu", "residual_norm_f32.cu", "residual_norm_f16.cu", "residual_norm_bf16.cu"]
 HEADERS = ["common.cuh", "quant_math.cuh", "mixed_bundle.cuh", "column.cuh", "flat_runs.cuh", "activation.cuh", "cluster.cuh", "tcgen05.cuh", "group_norm.cuh",
-           "dropout.cuh", "residual_norm.cuh", "fp8.cuh", "tensor_map.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
+           "dropout.cuh", "load_one.cuh", "residual_norm.cuh", "fp8.cuh", "tensor_map.cuh", os.path.join("..", "..", "include", "actnn_b200.h")]
 LIB = os.path.join(HERE, "libactnn_b200.so")
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

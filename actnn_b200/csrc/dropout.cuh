@@ -6,6 +6,7 @@
 #pragma once
 
 #include "activation.cuh"
+#include "load_one.cuh"
 
 namespace actnn {
 

@@ -9,6 +9,7 @@
 #pragma once
 
 #include "activation.cuh"
+#include "load_one.cuh"
 
 namespace actnn {
 
@@ -107,7 +108,7 @@ template <typename T, bool VEC> ACTNN_DEV Vec<T, 8> fp8_load(const T* p, int64_t
   if (VEC && e < end) return load_vec<T, 8>(p + e);
   Vec<T, 8> v;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && e + i < end ? __ldg(p + e + i) : from_float<T>(0.f);
+  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && e + i < end ? load_one(p + e + i) : from_float<T>(0.f);
   return v;
 }
 #endif

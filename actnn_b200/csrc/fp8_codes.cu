@@ -241,7 +241,7 @@ fp8_decode_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__
     for (int j = 0; j < 4; ++j) f[j] = f_mul(f[j], make_float2(s, s));
     store_vec<T, 8>(out + row * cols + e, f);
   } else {
-    for (int j = 0; j < 8 && e + j < cols; ++j) out[row * cols + e + j] = from_float<T>(fp8_unpack(__ldg(p + j)).x * s);
+    for (int j = 0; j < 8 && e + j < cols; ++j) out[row * cols + e + j] = from_float<T>(fp8_unpack(load_one(p + j)).x * s);
   }
 }
 

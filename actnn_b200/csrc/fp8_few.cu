@@ -31,7 +31,7 @@ ACTNN_DEV uint4 weight_bytes(const uint8_t* row, int k, int K) {
     uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (k + i < K) w[i / 4] |= (uint32_t)__ldg(row + k + i) << (8 * (i % 4));
+      if (k + i < K) w[i / 4] |= load_one(row + k + i) << (8 * (i % 4));
     v = make_uint4(w[0], w[1], w[2], w[3]);
   }
   return v;

@@ -42,6 +42,16 @@ int64_t rn_workspace_bytes(const RnArgs& a) { return (int64_t)a.runs * 5 * a.C *
 int rn_dispatch(const RnArgs& a, int dtype, RnWhat what, bool vec) {
   return dtype == ACTNN_F32 ? rn_run_f32(a, what, vec) : dtype == ACTNN_F16 ? rn_run_f16(a, what, vec) : rn_run_bf16(a, what, vec);
 }
+// Parameters and gate.  What is not given gets the address of a tensor that is: C values of its own type, should a load come before the
+// branch that it stands under.
+void rn_parameters(RnArgs& a, const void* w1, const void* b1, const void* w2, const void* b2, const void* gate, int pdtype, int gdtype, const void* readable) {
+  for (const void* p : {w1, b1, w2, b2}) if (p) readable = p;
+  auto one = [&](const void* p, int dtype) { return p ? RnParameter{p, dtype} : RnParameter{readable, -1}; };
+  a.w1 = one(w1, pdtype), a.b1 = one(b1, pdtype), a.w2 = one(w2, pdtype), a.b2 = one(b2, pdtype), a.gate = one(gate, gdtype);
+  a.pdtype = pdtype, a.gdtype = gdtype;
+  a.pvec = a.C % 8 == 0;
+  for (const void* p : {w1, b1, w2, b2, gate}) a.pvec = a.pvec && aligned(p, 16);
+}
 bool rn_dtype(int d) { return d >= ACTNN_F32 && d <= ACTNN_BF16; }
 
 }  // namespace
@@ -86,16 +96,14 @@ extern "C" int actnn_residual_norm_forward(const void* x, const void* f, const v
   for (const void* q : {x, f, (const void*)r, (const void*)h}) if (!aligned(q, size)) return ACTNN_ERR_ALIGN;
   for (const void* q : {weight, bias, post_weight, post_bias}) if (!aligned(q, psize)) return ACTNN_ERR_ALIGN;
   if (!aligned(gate, dtype_size(gate_dtype)) || !aligned(stats, 16) || !aligned(scale_x, 4) || !aligned(scale_f, 4) || !aligned(state, 16)) return ACTNN_ERR_ALIGN;
-  a.x = x; a.f = f; a.w2 = weight; a.b2 = bias; a.w1 = post_weight; a.b1 = post_bias; a.gate = gate; a.r = r; a.h = h;
+  a.x = x; a.f = f; a.r = r; a.h = h;
+  rn_parameters(a, post_weight, post_bias, weight, bias, gate, param_dtype, gate_dtype, x);
   a.cx = codes_x; a.cf = codes_f; a.sx = scale_x; a.sf = scale_f; a.stats = (float4*)stats;
   a.scale = (float)scale; a.eps = (float)eps; a.layer = layer; a.post = post; a.dropped = p > 0.f;
-  a.pdtype = param_dtype; a.gdtype = gate_dtype;
   a.drop = make_drop_key(p, seed, offset, state);
   a.stream = (cudaStream_t)stream;
   bool vec = C % 8 == 0 && aligned(codes_x, 8) && aligned(codes_f, 8);
   for (const void* q : {x, f, (const void*)r, (const void*)h}) vec = vec && aligned(q, 16);
-  a.pvec = C % 8 == 0;
-  for (const void* q : {weight, bias, post_weight, post_bias, gate}) a.pvec = a.pvec && aligned(q, 16);
   return rn_dispatch(a, dtype, kRnForward, vec);
 }
 
@@ -137,8 +145,9 @@ extern "C" int actnn_residual_norm_backward(const void* grad_r, const void* grad
   for (const void* q : {weight, post_weight, post_bias}) if (!aligned(q, psize)) return ACTNN_ERR_ALIGN;
   if (!aligned(gate, gsize) || !aligned(stats, 16) || !aligned(scale_x, 4) || !aligned(scale_f, 4) || !aligned(state, 16) || !aligned(workspace, 16)) return ACTNN_ERR_ALIGN;
   a.dr = grad_r; a.dh = grad_h; a.x = x; a.f = f; a.cx = (int8_t*)codes_x; a.cf = (int8_t*)codes_f; a.sx = (float*)scale_x; a.sf = (float*)scale_f;
-  a.stats = (float4*)stats; a.w2 = weight; a.w1 = post_weight; a.b1 = post_bias; a.gate = gate; a.dx = grad_x; a.df = grad_f;
-  a.scale = (float)scale; a.layer = layer; a.post = post; a.dropped = p > 0.f; a.pdtype = param_dtype; a.gdtype = gate_dtype;
+  rn_parameters(a, post_weight, post_bias, weight, nullptr, gate, param_dtype, gate_dtype, workspace);
+  a.stats = (float4*)stats; a.dx = grad_x; a.df = grad_f;
+  a.scale = (float)scale; a.layer = layer; a.post = post; a.dropped = p > 0.f;
   a.drop = make_drop_key(p, seed, offset, state);
   a.coded = codes_x != nullptr;
   a.stream = (cudaStream_t)stream;
@@ -150,7 +159,5 @@ extern "C" int actnn_residual_norm_backward(const void* grad_r, const void* grad
   a.parts = (float*)workspace;
   bool vec = C % 8 == 0 && aligned(codes_x, 8) && aligned(codes_f, 8);
   for (const void* q : io) vec = vec && aligned(q, 16);
-  a.pvec = C % 8 == 0;
-  for (const void* q : {weight, post_weight, post_bias, gate}) a.pvec = a.pvec && aligned(q, 16);
   return rn_dispatch(a, dtype, kRnBackward, vec);
 }

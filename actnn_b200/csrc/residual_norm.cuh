@@ -31,10 +31,18 @@ constexpr int kRnMostC = 32768;
 constexpr int kRnThreads = 256;                        // of the kernels that give a warp a row
 constexpr int kRnMostThreads = 512, kRnMostCluster = 8;          // of the backward pass: eight channels a thread
 
+// A tensor of one of the three types, that of `dtype`; -1: not given, ones or zeros (then `p` can be read all the same).
+struct RnParameter {
+  const void* p;
+  int dtype;
+#ifdef __CUDACC__
+  ACTNN_DEV bool given() const { return dtype >= 0; }
+#endif
+};
 struct RnArgs {
   const void *x, *f;                                   // forward; backward where no codes were kept
   const void *dr, *dh;                                 // gradients, NULL: zero
-  const void *w1, *b1, *w2, *b2, *gate;                // NULL: ones, zeros
+  RnParameter w1, b1, w2, b2, gate;
   void *r, *h, *dx, *df;                               // dx, df NULL: not wanted
   int8_t *cx, *cf;                                     // codes [rows, C], NULL: none
   float *sx, *sf;                                      // their scales [rows, ceil(C / 256)]
@@ -44,7 +52,7 @@ struct RnArgs {
   uint32_t rows;
   int C, blocks;                                       // blocks: scales a row
   float scale, eps, inv_c;
-  int pdtype, gdtype;                                  // types of the parameters and of the gate
+  int pdtype, gdtype;                                  // types of their gradients
   bool pvec;                                           // vectors of both are aligned
   bool layer, post, dropped;
   FastDiv by_gate;                                     // rows of a gate
@@ -64,12 +72,8 @@ int rn_run_f16(const RnArgs& a, RnWhat what, bool vec);
 int rn_run_bf16(const RnArgs& a, RnWhat what, bool vec);
 
 #ifdef __CUDACC__
-// Loads that happen where they stand: of pointers that may be NULL, and of rows that a loop may not reach.
-ACTNN_DEV float rn_ld(const float* p) {
-  float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
-}
+// Loads that stay where they stand (load_one.cuh).
+ACTNN_DEV float rn_ld(const float* p) { return load_one(p); }
 ACTNN_DEV float2 rn_ld(const float2* p) {
   float2 v;
   asm volatile("ld.global.nc.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
@@ -96,7 +100,7 @@ template <typename T, bool VEC> ACTNN_DEV Vec<T, 8> rn_load(const T* row, int c,
   Vec<T, 8> v;
   if (VEC && c < C) return load_vec<T, 8>(rn_at(row, c));
 #pragma unroll
-  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && c + i < C ? __ldg(row + c + i) : from_float<T>(0.f);
+  for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && c + i < C ? load_one(row + c + i) : from_float<T>(0.f);
   return v;
 }
 template <typename T, bool VEC> ACTNN_DEV void rn_store(T* row, int c, int C, const float2 (&f)[4]) {
@@ -116,7 +120,7 @@ template <bool VEC> ACTNN_DEV Codes<8> rn_load_codes(const int8_t* row, int c, i
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
-      if (c + i < C) r.w[i / 4] |= (uint32_t)__ldg(reinterpret_cast<const uint8_t*>(row) + c + i) << (8 * (i % 4));
+      if (c + i < C) r.w[i / 4] |= load_one(reinterpret_cast<const uint8_t*>(row) + c + i) << (8 * (i % 4));
   }
   return r;
 }
@@ -142,26 +146,26 @@ template <typename P> ACTNN_DEV void rn_parameter(const P* p, int c, int C, bool
   } else {
     float e[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = c + i < C ? to_float(__ldg(p + c + i)) : 0.f;
+    for (int i = 0; i < 8; ++i) e[i] = c + i < C ? to_float(load_one(p + c + i)) : 0.f;
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = make_float2(e[2 * i], e[2 * i + 1]);
   }
 }
-ACTNN_DEV void rn_parameter(const void* p, int dtype, int c, int C, bool vec, float none, float2 (&f)[4]) {
-  if (!p) {
+ACTNN_DEV void rn_parameter(const RnParameter& q, int c, int C, bool vec, float none, float2 (&f)[4]) {
+  if (!q.given()) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = make_float2(none, none);
-  } else if (dtype == ACTNN_F32) {
-    rn_parameter((const float*)p, c, C, vec, f);
-  } else if (dtype == ACTNN_F16) {
-    rn_parameter((const __half*)p, c, C, vec, f);
+  } else if (q.dtype == ACTNN_F32) {
+    rn_parameter((const float*)q.p, c, C, vec, f);
+  } else if (q.dtype == ACTNN_F16) {
+    rn_parameter((const __half*)q.p, c, C, vec, f);
   } else {
-    rn_parameter((const __nv_bfloat16*)p, c, C, vec, f);
+    rn_parameter((const __nv_bfloat16*)q.p, c, C, vec, f);
   }
 }
-ACTNN_DEV const void* rn_gate_row(const RnArgs& a, uint32_t row) {
-  if (!a.gate) return nullptr;
-  return (const char*)a.gate + (size_t)fast_div(row, a.by_gate) * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
+ACTNN_DEV RnParameter rn_gate_row(const RnArgs& a, uint32_t row) {
+  if (!a.gate.given()) return a.gate;
+  return RnParameter{(const char*)a.gate.p + (size_t)fast_div(row, a.by_gate) * a.C * (a.gate.dtype == ACTNN_F32 ? 4 : 2), a.gate.dtype};
 }
 // The fields that decide over the eight channels from `c` of a row, two a word.  Where C is no multiple of eight they belong to two calls.
 // (Both directions multiply by factors: a value that is not finite makes its row NaN, dropped or not.)
@@ -182,24 +186,25 @@ template <bool VEC> ACTNN_DEV Philox4 rn_fields(const RnArgs& a, const NoiseKey&
 }
 // ------------------------------------------------------------------ forward
 // The sum over the threads of a row: a warp's, or a block's, whose reductions take two places in turn (two are never under way at a time).
-template <bool WARP> ACTNN_DEV float rn_sum(float v, int& place) {
+// Places of warps that are not there hold zero.
+struct RnPlaces { float part[2][kRnMostThreads / 32]; };
+template <bool WARP> ACTNN_DEV float rn_sum(float v, RnPlaces& s, int& place) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
   if constexpr (!WARP) {
-    __shared__ float part_s[2][kRnMostThreads / 32];
+    constexpr int kWarps = kRnMostThreads / 32;
     const int lane = threadIdx.x & 31;
-    if (lane == 0) part_s[place][threadIdx.x >> 5] = v;
+    if (lane == 0) s.part[place][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = lane < (int)(blockDim.x >> 5) ? part_s[place][lane] : 0.f;
+    v = s.part[place][lane & (kWarps - 1)];
 #pragma unroll
-    for (int o = kRnMostThreads / 64; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
-    v = __shfl_sync(kFull, v, 0);
+    for (int o = kWarps / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFull, v, o);
     place ^= 1;
   }
   return v;
 }
 // Mean (of the layer kind) and reciprocal deviation of a row.  Values behind C are zero.
-template <int V, bool WARP, bool LAYER> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int c0, int step, const RnArgs& a, int& place) {
+template <int V, bool WARP, bool LAYER> ACTNN_DEV float2 rn_statistics(const float2 (&v)[V][4], int c0, int step, const RnArgs& a, RnPlaces& places, int& place) {
   float mean = 0.f;
   float2 s = make_float2(0.f, 0.f);
   if constexpr (LAYER) {
@@ -207,7 +212,7 @@ template <int V, bool WARP, bool LAYER> ACTNN_DEV float2 rn_statistics(const flo
     for (int k = 0; k < V; ++k)
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = f_add(s, v[k][i]);
-    mean = rn_sum<WARP>(f_sum(s), place) * a.inv_c;
+    mean = rn_sum<WARP>(f_sum(s), places, place) * a.inv_c;
     s = make_float2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
@@ -232,7 +237,7 @@ template <int V, bool WARP, bool LAYER> ACTNN_DEV float2 rn_statistics(const flo
 #pragma unroll
       for (int i = 0; i < 4; ++i) s = f_fma(v[k][i], v[k][i], s);
   }
-  return make_float2(mean, rsqrtf(rn_sum<WARP>(f_sum(s), place) * a.inv_c + a.eps));
+  return make_float2(mean, rsqrtf(rn_sum<WARP>(f_sum(s), places, place) * a.inv_c + a.eps));
 }
 
 // The parameters of a thread's channels in shared memory, as float32: what every row reads again takes two loads and no conversion.
@@ -245,8 +250,8 @@ ACTNN_DEV void rn_get(const float4* at, int width, float2 (&v)[4]) {
   const float4 p = at[0], q = at[width];
   v[0] = make_float2(p.x, p.y), v[1] = make_float2(p.z, p.w), v[2] = make_float2(q.x, q.y), v[3] = make_float2(q.z, q.w);
 }
-enum RnSet { kRnW1, kRnW2, kRnGate, kRnB1, kRnB2 };
-template <bool LAYER> constexpr int rn_sets() { return LAYER ? 5 : 3; }
+enum RnSet { kRnGw, kRnW2, kRnGb, kRnB2 };             // w1 and b1 times the gate
+template <bool LAYER> constexpr int rn_sets() { return LAYER ? 4 : 2; }
 
 // A warp, or a block, goes through rows; a thread has V vectors of eight channels of each.  The next row's inputs are requested as soon
 // as this row's are unpacked (unless V is so large that registers are short), so that the two or four reductions of a row do
@@ -255,10 +260,11 @@ template <typename T, int V, bool WARP, bool VEC, bool LAYER>
 __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && !WARP ? 2 : 1) rn_forward_kernel(const __grid_constant__ RnArgs a) {
   constexpr bool kAhead = V <= 4, kShared = V <= 2;     // parameters in shared memory, or read from the L1
   extern __shared__ float4 parameters_s[];
+  __shared__ RnPlaces places;
   const int lanes = WARP ? 32 : blockDim.x, lane = WARP ? threadIdx.x & 31 : threadIdx.x, c0 = lane * 8, step = lanes * 8;
   const int width = V * blockDim.x;
   const uint32_t rows_step = WARP ? gridDim.x * (kRnThreads / 32) : gridDim.x;
-  uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x, gate_of = 0xffffffffu;
+  uint32_t row = WARP ? blockIdx.x * (kRnThreads / 32) + (threadIdx.x >> 5) : blockIdx.x, gate_of = 0;
   Vec<T, 8> xv[V], fv[V];
   auto load = [&](uint32_t r) {
     const size_t at = (size_t)r * a.C;
@@ -269,26 +275,46 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
     for (int k = 0; k < V; ++k) xv[k] = rn_load<T, VEC>(x, c0 + k * step, a.C);
   };
   if (kAhead && row < a.rows) load(row);
-  auto put = [&](int set, const void* p, int dtype, float none) {
+  auto slot = [&](int set, int k) { return parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x; };
+  auto read = [&](const RnParameter& p, float none, int k, float2 (&v)[4]) { rn_parameter(p, c0 + k * step, a.C, a.pvec, none, v); };
+  // w1 or b1 times the gate of a row.
+  auto product = [&](const RnParameter& p, float none, const RnParameter& gate, int k, float2 (&v)[4]) {
+    read(p, none, k, v);
+    if (!gate.given()) return;
+    float2 q[4];
+    read(gate, 1.f, k, q);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = f_mul(v[i], q[i]);
+  };
+  auto put_products = [&](const RnParameter& gate) {
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       float2 v[4];
-      rn_parameter(p, dtype, c0 + k * step, a.C, a.pvec, none, v);
-      rn_put(parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x, width, v);
+      product(a.w1, 1.f, gate, k, v);
+      rn_put(slot(kRnGw, k), width, v);
+      if (LAYER) {
+        product(a.b1, 0.f, gate, k, v);
+        rn_put(slot(kRnGb, k), width, v);
+      }
     }
   };
-  auto get = [&](int set, int k, const void* p, int dtype, float none, float2 (&v)[4]) {
-    if constexpr (kShared) rn_get(parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x, width, v);
-    else rn_parameter(p, dtype, c0 + k * step, a.C, a.pvec, none, v);
-  };
+  if (!WARP && threadIdx.x < sizeof(places) / 4) (&places.part[0][0])[threadIdx.x] = 0.f;
   if constexpr (kShared) {
-    if (a.post) put(kRnW1, a.w1, a.pdtype, 1.f);
-    put(kRnW2, a.w2, a.pdtype, 1.f);
-    if (LAYER) {
-      if (a.post) put(kRnB1, a.b1, a.pdtype, 0.f);
-      put(kRnB2, a.b2, a.pdtype, 0.f);
+    if (a.gate.given()) gate_of = fast_div(row, a.by_gate);
+    if (row < a.rows) put_products(rn_gate_row(a, row));
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float2 v[4];
+      read(a.w2, 1.f, k, v);
+      rn_put(slot(kRnW2, k), width, v);
+      if (LAYER) {
+        read(a.b2, 0.f, k, v);
+        rn_put(slot(kRnB2, k), width, v);
+      }
     }
   }
+  if (!WARP) __syncthreads();
+  const bool scaled = a.post || a.gate.given();
   NoiseKey key;
   if (a.dropped) key = drop_key(a.drop);
   for (int place = 0; row < a.rows; row += rows_step) {
@@ -299,7 +325,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
 #pragma unroll
       for (int k = 0; k < V; ++k) {
         const int c = c0 + k * step, first = c & ~(kRnBlock - 1);
-        if (first >= a.C) continue;
+        if (V > 1 && first >= a.C) continue;
         const uint32_t mf = __reduce_max_sync(kFull, most_of(fv[k])), mx = __reduce_max_sync(kFull, most_of(xv[k]));
         const bool upper = threadIdx.x & 16;
         const float most = largest(upper ? mx : mf), factor = code_factor(most);
@@ -312,7 +338,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
         };
         code(fv[k], a.cf, __shfl_sync(kFull, factor, 0));
         code(xv[k], a.cx, __shfl_sync(kFull, factor, 16));
-        if ((threadIdx.x & 15) == 0) (upper ? a.sx : a.sf)[(size_t)row * a.blocks + first / kRnBlock] = code_step(most);
+        if ((threadIdx.x & 15) == 0) *rn_at((upper ? a.sx : a.sf) + (size_t)row * a.blocks, first / kRnBlock) = code_step(most);
       }
     }
     float2 u[V][4], x[V][4];
@@ -322,32 +348,38 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
       unpack_vec(xv[k], x[k]);
     }
     if (kAhead && row + rows_step < a.rows) load(row + rows_step);
-    const float2 one = a.post ? rn_statistics<V, WARP, LAYER>(u, c0, step, a, place) : make_float2(0.f, 1.f);
-    const void* gate = nullptr;
-    if (a.gate) {
-      const uint32_t g = fast_div(row, a.by_gate);
-      gate = (const char*)a.gate + (size_t)g * a.C * (a.gdtype == ACTNN_F32 ? 4 : 2);
-      if (kShared && g != gate_of) {
-        put(kRnGate, gate, a.gdtype, 1.f);
+    const float2 one = a.post ? rn_statistics<V, WARP, LAYER>(u, c0, step, a, places, place) : make_float2(0.f, 1.f);
+    RnParameter gate = a.gate;
+    if (a.gate.given()) {
+      if (const uint32_t g = fast_div(row, a.by_gate); !kShared || g != gate_of) {
+        gate = rn_gate_row(a, row);
+        if (kShared) put_products(gate);
         gate_of = g;
       }
     }
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int c = c0 + k * step;
-      if (c >= a.C) continue;
       float2 p[4];
       if (a.post) {
-        get(kRnW1, k, a.w1, a.pdtype, 1.f, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (LAYER) u[k][i] = f_add(u[k][i], make_float2(-one.x, -one.x));
-          u[k][i] = f_mul(f_mul(u[k][i], make_float2(one.y, one.y)), p[i]);
+          u[k][i] = f_mul(u[k][i], make_float2(one.y, one.y));
         }
-        if (LAYER) {
-          get(kRnB1, k, a.b1, a.pdtype, 0.f, p);
+      }
+      if (scaled) {
+        if constexpr (kShared) rn_get(slot(kRnGw, k), width, p);
+        else product(a.w1, 1.f, gate, k, p);
+        if constexpr (LAYER) {
+          float2 b[4];
+          if constexpr (kShared) rn_get(slot(kRnGb, k), width, b);
+          else product(a.b1, 0.f, gate, k, b);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
+          for (int i = 0; i < 4; ++i) u[k][i] = f_fma(u[k][i], p[i], b[i]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
         }
       }
       if (a.dropped) {
@@ -355,36 +387,30 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
       }
-      if (gate) {
-        get(kRnGate, k, gate, a.gdtype, 1.f, p);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[k][i] = f_mul(u[k][i], p[i]);
-      }
 #pragma unroll
       for (int i = 0; i < 4; ++i) u[k][i] = f_fma(x[k][i], make_float2(a.scale, a.scale), u[k][i]);
       rn_store<T, VEC>((T*)a.r + at, c, a.C, u[k]);
-      if constexpr (!VEC) {
-        if (c + 8 > a.C) {
+      if ((LAYER || !VEC) && c + 8 > a.C) {             // nothing behind C enters the sums
 #pragma unroll
-          for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
-        }
+        for (int i = 0; i < 4; ++i) u[k][i] = make_float2(c + 2 * i < a.C ? u[k][i].x : 0.f, c + 2 * i + 1 < a.C ? u[k][i].y : 0.f);
       }
     }
-    const float2 two = rn_statistics<V, WARP, LAYER>(u, c0, step, a, place);
+    const float2 two = rn_statistics<V, WARP, LAYER>(u, c0, step, a, places, place);
     if (a.stats && lane == 0) a.stats[row] = make_float4(one.x, one.y, two.x, two.y);
 #pragma unroll
     for (int k = 0; k < V; ++k) {
       const int c = c0 + k * step;
-      if (c >= a.C) continue;
       float2 p[4];
-      get(kRnW2, k, a.w2, a.pdtype, 1.f, p);
+      if constexpr (kShared) rn_get(slot(kRnW2, k), width, p);
+      else read(a.w2, 1.f, k, p);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (LAYER) u[k][i] = f_add(u[k][i], make_float2(-two.x, -two.x));
         u[k][i] = f_mul(f_mul(u[k][i], make_float2(two.y, two.y)), p[i]);
       }
-      if (LAYER) {
-        get(kRnB2, k, a.b2, a.pdtype, 0.f, p);
+      if constexpr (LAYER) {
+        if constexpr (kShared) rn_get(slot(kRnB2, k), width, p);
+        else read(a.b2, 0.f, k, p);
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[k][i] = f_add(u[k][i], p[i]);
       }
@@ -526,7 +552,7 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   };
   auto get = [&](int set, float2 (&v)[4]) { rn_get(parameters_s + 2 * set * threads + threadIdx.x, threads, v); };
   float2 none[4] = {}, w2[4];
-  rn_parameter(a.w2, a.pdtype, c, C, a.pvec, 1.f, w2);
+  rn_parameter(a.w2, c, C, a.pvec, 1.f, w2);
   put(kW2, w2);
   put(kDw1, none);
   if (LAYER) put(kDb1, none);
@@ -546,7 +572,7 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   auto turn = [&](uint32_t row) {
     const uint32_t g = fast_div(row, a.by_gate);
     float2 q[4], v[4], d[4];
-    rn_parameter(rn_gate_row(a, row), a.gdtype, c, C, a.pvec, 1.f, q);
+    rn_parameter(rn_gate_row(a, row), c, C, a.pvec, 1.f, q);
     get(kDw1, d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i] = f_fma(q[i], sum[i], d[i]);
@@ -558,11 +584,11 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
       put(kDb1, d);
     }
     if (a.dgate) {
-      rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, v);
+      rn_parameter(a.w1, c, C, a.pvec, 1.f, v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = f_mul(v[i], sum[i]);
       if (LAYER) {
-        rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, d);
+        rn_parameter(a.b1, c, C, a.pvec, 0.f, d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = f_fma(d[i], sum_b[i], v[i]);
       }
@@ -576,13 +602,13 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   for (int place = 0; first < end; ++first, place ^= 1) {
     if (other) {
       float2 q[4], w[4];
-      rn_parameter(rn_gate_row(a, first), a.gdtype, c, C, a.pvec, 1.f, q);
-      rn_parameter(a.w1, a.pdtype, c, C, a.pvec, 1.f, w);
+      rn_parameter(rn_gate_row(a, first), c, C, a.pvec, 1.f, q);
+      rn_parameter(a.w1, c, C, a.pvec, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
       put(kGw, w);
       if (LAYER) {
-        rn_parameter(a.b1, a.pdtype, c, C, a.pvec, 0.f, w);
+        rn_parameter(a.b1, c, C, a.pvec, 0.f, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
         put(kGb, w);

@@ -20,7 +20,7 @@ seeded_dropout_kernel(const T* __restrict__ x, T* __restrict__ y, int64_t numel,
       v[k] = load_vec<T, 8>(x + e);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v[k].w)[i] = e + i < numel ? __ldg(x + e + i) : from_float<T>(0.f);
+      for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v[k].w)[i] = e + i < numel ? load_one(x + e + i) : from_float<T>(0.f);
     }
   }
   const NoiseKey key = drop_key(drop);
