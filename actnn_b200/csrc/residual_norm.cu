@@ -49,8 +49,6 @@ void rn_parameters(RnArgs& a, const void* w1, const void* b1, const void* w2, co
   auto one = [&](const void* p, int dtype) { return p ? RnParameter{p, dtype} : RnParameter{readable, -1}; };
   a.w1 = one(w1, pdtype), a.b1 = one(b1, pdtype), a.w2 = one(w2, pdtype), a.b2 = one(b2, pdtype), a.gate = one(gate, gdtype);
   a.pdtype = pdtype, a.gdtype = gdtype;
-  a.pvec = a.C % 8 == 0;
-  for (const void* p : {w1, b1, w2, b2, gate}) a.pvec = a.pvec && aligned(p, 16);
 }
 bool rn_dtype(int d) { return d >= ACTNN_F32 && d <= ACTNN_BF16; }
 
@@ -103,7 +101,7 @@ extern "C" int actnn_residual_norm_forward(const void* x, const void* f, const v
   a.drop = make_drop_key(p, seed, offset, state);
   a.stream = (cudaStream_t)stream;
   bool vec = C % 8 == 0 && aligned(codes_x, 8) && aligned(codes_f, 8);
-  for (const void* q : {x, f, (const void*)r, (const void*)h}) vec = vec && aligned(q, 16);
+  for (const void* q : {x, f, (const void*)r, (const void*)h, weight, bias, post_weight, post_bias, gate}) vec = vec && aligned(q, 16);
   return rn_dispatch(a, dtype, kRnForward, vec);
 }
 
@@ -159,5 +157,6 @@ extern "C" int actnn_residual_norm_backward(const void* grad_r, const void* grad
   a.parts = (float*)workspace;
   bool vec = C % 8 == 0 && aligned(codes_x, 8) && aligned(codes_f, 8);
   for (const void* q : io) vec = vec && aligned(q, 16);
+  for (const void* q : {weight, post_weight, post_bias, gate}) vec = vec && aligned(q, 16);
   return rn_dispatch(a, dtype, kRnBackward, vec);
 }

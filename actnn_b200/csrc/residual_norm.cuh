@@ -53,7 +53,6 @@ struct RnArgs {
   int C, blocks;                                       // blocks: scales a row
   float scale, eps, inv_c;
   int pdtype, gdtype;                                  // types of their gradients
-  bool pvec;                                           // vectors of both are aligned
   bool layer, post, dropped;
   FastDiv by_gate;                                     // rows of a gate
   DropKey drop;
@@ -134,8 +133,8 @@ template <bool VEC> ACTNN_DEV void rn_store_codes(int8_t* row, int c, int C, con
   }
 }
 // A parameter's values, of any of the three types; through the L1, every row reads them again.
-template <typename P> ACTNN_DEV void rn_parameter(const P* p, int c, int C, bool vec, float2 (&f)[4]) {
-  if (vec) {
+template <bool VEC, typename P> ACTNN_DEV void rn_values(const P* p, int c, int C, float2 (&f)[4]) {
+  if constexpr (VEC) {
     Vec<P, 8> v;
 #pragma unroll
     for (int i = 0; i < (int)sizeof(P) / 2; ++i) {
@@ -151,16 +150,16 @@ template <typename P> ACTNN_DEV void rn_parameter(const P* p, int c, int C, bool
     for (int i = 0; i < 4; ++i) f[i] = make_float2(e[2 * i], e[2 * i + 1]);
   }
 }
-ACTNN_DEV void rn_parameter(const RnParameter& q, int c, int C, bool vec, float none, float2 (&f)[4]) {
+template <bool VEC> ACTNN_DEV void rn_parameter(const RnParameter& q, int c, int C, float none, float2 (&f)[4]) {
   if (!q.given()) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) f[i] = make_float2(none, none);
   } else if (q.dtype == ACTNN_F32) {
-    rn_parameter((const float*)q.p, c, C, vec, f);
+    rn_values<VEC>((const float*)q.p, c, C, f);
   } else if (q.dtype == ACTNN_F16) {
-    rn_parameter((const __half*)q.p, c, C, vec, f);
+    rn_values<VEC>((const __half*)q.p, c, C, f);
   } else {
-    rn_parameter((const __nv_bfloat16*)q.p, c, C, vec, f);
+    rn_values<VEC>((const __nv_bfloat16*)q.p, c, C, f);
   }
 }
 ACTNN_DEV RnParameter rn_gate_row(const RnArgs& a, uint32_t row) {
@@ -276,7 +275,7 @@ __global__ void __launch_bounds__(WARP ? kRnThreads : kRnMostThreads, V == 1 && 
   };
   if (kAhead && row < a.rows) load(row);
   auto slot = [&](int set, int k) { return parameters_s + 2 * set * width + k * blockDim.x + threadIdx.x; };
-  auto read = [&](const RnParameter& p, float none, int k, float2 (&v)[4]) { rn_parameter(p, c0 + k * step, a.C, a.pvec, none, v); };
+  auto read = [&](const RnParameter& p, float none, int k, float2 (&v)[4]) { rn_parameter<VEC>(p, c0 + k * step, a.C, none, v); };
   // w1 or b1 times the gate of a row.
   auto product = [&](const RnParameter& p, float none, const RnParameter& gate, int k, float2 (&v)[4]) {
     read(p, none, k, v);
@@ -552,7 +551,7 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   };
   auto get = [&](int set, float2 (&v)[4]) { rn_get(parameters_s + 2 * set * threads + threadIdx.x, threads, v); };
   float2 none[4] = {}, w2[4];
-  rn_parameter(a.w2, c, C, a.pvec, 1.f, w2);
+  rn_parameter<VEC>(a.w2, c, C, 1.f, w2);
   put(kW2, w2);
   put(kDw1, none);
   if (LAYER) put(kDb1, none);
@@ -572,7 +571,7 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   auto turn = [&](uint32_t row) {
     const uint32_t g = fast_div(row, a.by_gate);
     float2 q[4], v[4], d[4];
-    rn_parameter(rn_gate_row(a, row), c, C, a.pvec, 1.f, q);
+    rn_parameter<VEC>(rn_gate_row(a, row), c, C, 1.f, q);
     get(kDw1, d);
 #pragma unroll
     for (int i = 0; i < 4; ++i) d[i] = f_fma(q[i], sum[i], d[i]);
@@ -584,11 +583,11 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
       put(kDb1, d);
     }
     if (a.dgate) {
-      rn_parameter(a.w1, c, C, a.pvec, 1.f, v);
+      rn_parameter<VEC>(a.w1, c, C, 1.f, v);
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = f_mul(v[i], sum[i]);
       if (LAYER) {
-        rn_parameter(a.b1, c, C, a.pvec, 0.f, d);
+        rn_parameter<VEC>(a.b1, c, C, 0.f, d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = f_fma(d[i], sum_b[i], v[i]);
       }
@@ -602,13 +601,13 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
   for (int place = 0; first < end; ++first, place ^= 1) {
     if (other) {
       float2 q[4], w[4];
-      rn_parameter(rn_gate_row(a, first), c, C, a.pvec, 1.f, q);
-      rn_parameter(a.w1, c, C, a.pvec, 1.f, w);
+      rn_parameter<VEC>(rn_gate_row(a, first), c, C, 1.f, q);
+      rn_parameter<VEC>(a.w1, c, C, 1.f, w);
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
       put(kGw, w);
       if (LAYER) {
-        rn_parameter(a.b1, c, C, a.pvec, 0.f, w);
+        rn_parameter<VEC>(a.b1, c, C, 0.f, w);
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[i] = f_mul(w[i], q[i]);
         put(kGb, w);
