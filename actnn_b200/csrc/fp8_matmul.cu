@@ -14,6 +14,9 @@
 // 64 for scales, four sets of 16, so that none is overwritten while instructions that read it may be under way.  Split sums
 // are joined in the order of the blocks, so a shape's results are reproducible.
 //
+// 16384 x 4096 x 8192: 406 us in long runs, 2.7 PFLOP/s, the power cap; 8192 x 2048 x 4096 and its two gradients 59 to 62 each (2.3);
+// 200 x 4096 x 4096: 14, bound by what an SM gets from the L2 (51 bytes a cycle, 24 KB a stage) and latency (the weight's bytes from HBM 2.6).
+//
 // Every wait is bounded, with the integer product's rules: a block whose wait runs out writes nothing more, is counted, lets its copies
 // and instructions end and leaves; the epilogue's warps leave together; of blocks that share a reduction none writes.
 #include <algorithm>

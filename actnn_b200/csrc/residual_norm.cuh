@@ -16,6 +16,10 @@
 // With a = keep g w1 / (1 - p), dn1 is a t, so that the means of the second norm's gradient follow from sums that do not wait for
 // those of the first: mean(dn1 n1) = (sum a c n1 - p2 mean dn2 sum a n1 - p2 mean(dn2 n2) sum a n1 n2) / C.  A row takes one
 // joint reduction, not two.
+//
+// 8192 x 4096 bf16 with dropout: forward 80 us, backward 100, the join 6 (51 and 51 at the copy rate); 16384 x 8192 f16 without: 254, 382, 8
+// (205 each); 12608 x 768 float32, layer kind: 32, 36, 6.  Both directions are bound by instructions, some 470 a warp's 256 channels
+// backward: dropout's generator takes 70 of them, and registers allow 16 warps an SM backward.
 #pragma once
 
 #include <algorithm>
@@ -514,9 +518,11 @@ template <int N> ACTNN_DEV float rn_warp_sums(float (&v)[N]) {
 // cluster send theirs to one another, counted as they arrive by a barrier in memory: a barrier of the cluster would wait for
 // the results of the row before to reach the L2 as well.  A wait that runs out is counted, and the rows from there on get NaN.
 //
-// What bounds it are instructions (16 warps an SM is what registers allow), so the gate g and w1 enter as their product, and what
+// What bounds it are instructions, so the gate g and w1 enter as their product, and what
 // depends on the rows of one gate alone is summed once: with S = sum m t n1 and S' = sum m t, dw1 = g S, db1 = g S', dg = w1 S + b1 S'.
 // These products, in shared memory as float32, are a thread's own: g w1, g b1 and w2, and dw1 and db1 over the gates.
+// (With gate, w1 and each gradient's sums apart: 8192 x 4096 116 us, 16384 x 8192 500.  The second half of a row's work done after the
+// next row's first half, past the barrier: 138 us, what it holds in registers and copies costs more.)
 template <typename T, bool VEC, bool CODED, bool LAYER>
 __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a, unsigned* gave_up) {
   constexpr int N = LAYER ? 8 : 4, kWarps = kRnMostThreads / 32;
