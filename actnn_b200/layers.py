@@ -400,6 +400,10 @@ class QFp8Linear(nn.Linear):
         self.frozen = None                    # the weight moves or changes its type: freeze again
         return super()._apply(fn, recurse)
 
+    def _load_from_state_dict(self, *args, **kwargs):
+        self.frozen = None                    # another weight
+        return super()._load_from_state_dict(*args, **kwargs)
+
     def forward(self, input):
         if self.frozen is not None:
             if torch.is_grad_enabled() and input.requires_grad:

@@ -468,3 +468,37 @@ def test_refusals(cuda_device, monkeypatch, half):
             call()
         with pytest.raises(RuntimeError, match=word), torch.no_grad():
             call()
+
+
+@pytest.mark.parametrize("kind,post", [("rms", True), ("layer", True), ("layer", False)])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("c", [1, 30, 96, 257, 1024, 5000, 8192, 20000])
+def test_what_is_not_given_is_ones_and_zeros(cuda_device, c, dtype, kind, post):
+    from actnn_b200 import ops
+    x, f, dr, dh = (randn(3, 5, c, dtype=dtype, seed=i) for i in range(4))
+    ones, zeros = torch.ones(c, dtype=dtype, device="cuda"), torch.zeros(c, dtype=dtype, device="cuda")
+    layer = kind == "layer"
+    given = (ones, zeros if layer else None, ones if post else None, zeros if layer and post else None, ones)
+    results = []
+    for params in (given, (None,) * 5):
+        leaves = [v.clone().requires_grad_() for v in (x, f)]
+        out = ops.residual_norm.apply(*leaves, *params, scale=SCALE, p=0.2, kind=kind, post=post, key=KEY)
+        results.append([o.detach() for o in out] + list(torch.autograd.grad(out, leaves, (dr, dh))))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("c", [96, 1024, 8192])
+def test_parameters_that_are_not_on_16_bytes(cuda_device, c):
+    from actnn_b200 import ops
+    case = Case((3, 7), c, (3, 1), "layer", True, 0.1, torch.bfloat16)
+
+    def off(t):
+        return torch.empty(t.numel() + 1, dtype=t.dtype, device="cuda")[1:].view(t.shape).copy_(t)
+
+    results = []
+    for leaves in (case.leaves(), case.leaves()[:2] + [off(v) for v in case.leaves()[2:]]):
+        leaves = [v.detach().requires_grad_() for v in leaves]
+        out = ops.residual_norm.apply(*leaves, **case.options)
+        results.append([o.detach() for o in out] + list(torch.autograd.grad(out, leaves, (case.dr, case.dh))))
+    for a, b in zip(*results):                           # the same sums in the same order; fused or not where the compiler chose
+        near(b, a.double(), a.double().abs() + 1, STEPS)
