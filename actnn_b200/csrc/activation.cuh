@@ -7,6 +7,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "load_one.cuh"
 
 namespace actnn {
 
@@ -104,7 +105,7 @@ template <typename T> struct Vec<T, 1> { T v; };
 template <typename T, int V> ACTNN_DEV Vec<T, V> load_vec(const T* p) {
   Vec<T, V> r;
   if constexpr (V == 1) {
-    r.v = __ldg(p);
+    r.v = load_one(p);
   } else if constexpr (V * sizeof(T) == 4) {
     asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(r.w[0]) : "l"(p));
   } else if constexpr (V * sizeof(T) == 8) {

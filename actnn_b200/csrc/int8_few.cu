@@ -75,7 +75,7 @@ int8_few_kernel(const T* __restrict__ x, const int8_t* __restrict__ weights, con
     if (vec && e + 8 <= K) return load_again<T>(p + e);
     Vec<T, 8> v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = e + i < K ? __ldg(p + e + i) : from_float<T>(0.f);
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = e + i < K ? load_one(p + e + i) : from_float<T>(0.f);
     return v;
   };
   if (t < tokens) {

@@ -18,6 +18,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "load_one.cuh"
 
 namespace actnn {
 
@@ -32,10 +33,10 @@ template <> ACTNN_DEV float round_to<__nv_bfloat16>(float x) {
 template <typename T> ACTNN_DEV float load_scalar(const T* p, int64_t i);
 template <> ACTNN_DEV float load_scalar<float>(const float* p, int64_t i) { return __ldg(p + i); }
 template <> ACTNN_DEV float load_scalar<__half>(const __half* p, int64_t i) {
-  return __half2float(__ldg(p + i));
+  return __half2float(load_one(p + i));
 }
 template <> ACTNN_DEV float load_scalar<__nv_bfloat16>(const __nv_bfloat16* p, int64_t i) {
-  return __bfloat162float(__ldg(p + i));
+  return __bfloat162float(load_one(p + i));
 }
 template <typename T> ACTNN_DEV void store_scalar(T* p, int64_t i, float v);
 template <> ACTNN_DEV void store_scalar<float>(float* p, int64_t i, float v) { p[i] = v; }

@@ -48,7 +48,7 @@ row_codes_kernel(const T* __restrict__ x, int8_t* __restrict__ codes, float* __r
     if (VEC && e < cols) return load_vec<T, 8>(p + e);
     Vec<T, 8> v;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && e + i < cols ? __ldg(p + e + i) : from_float<T>(0.f);
+    for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(v.w)[i] = !VEC && e + i < cols ? load_one(p + e + i) : from_float<T>(0.f);
     return v;
   };
 #pragma unroll
@@ -116,7 +116,7 @@ column_sums_kernel(const T* __restrict__ x, float* __restrict__ parts, int64_t r
         w = load_vec<T, 8>(p);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(w.w)[i] = c + i < cols ? __ldg(p + i) : from_float<T>(0.f);
+        for (int i = 0; i < 8; ++i) reinterpret_cast<T*>(w.w)[i] = c + i < cols ? load_one(p + i) : from_float<T>(0.f);
       }
       float2 f[4];
       unpack_vec(w, f);
