@@ -512,11 +512,19 @@ template <int N> ACTNN_DEV float rn_warp_sums(float (&v)[N]) {
   return s;
 }
 
+// After a wait that ran out, when all blocks have sent what they send: until the phase under way at each of the two barriers is over, or a
+// limit outlasts the sums on their way here.  (Of the two parities that of the phase before is over at once.)
+ACTNN_DEV void rn_outlast(const uint64_t* bars) {
+  for (int i = 0; i < 4; ++i) mbar_wait(smem_addr(&bars[i >> 1]), i & 1);
+}
+
 // A run of rows by a block, or by a cluster of blocks of 4096 channels each.  A thread has eight channels of every row and keeps the sums of
 // their parameters' gradients; the next row's values are requested as soon as this row's are unpacked.  The warps' sums of a row go to
 // shared memory in two places in turn, so that one barrier a row is enough, and each warp joins them for itself.  The blocks of a
 // cluster send theirs to one another, counted as they arrive by a barrier in memory: a barrier of the cluster would wait for
-// the results of the row before to reach the L2 as well.  A wait that runs out is counted, and the rows from there on get NaN.
+// the results of the row before to reach the L2 as well.  A warp whose wait runs out is counted, writes NaN for that row and those behind it,
+// and sends nothing more, so that the other warps' waits for the next row run out too: had it gone on, its later sums would be
+// counted and read as those of rows that others have not done with.
 //
 // What bounds it are instructions, so the gate g and w1 enter as their product, and what
 // depends on the rows of one gate alone is summed once: with S = sum m t n1 and S' = sum m t, dw1 = g S, db1 = g S', dg = w1 S + b1 S'.
@@ -667,8 +675,8 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
         const uint32_t bar = smem_addr(&there_s[place]), at = smem_addr(part_s[place][rank * warps + warp]);
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __shfl_sync(kFull, mine, i * (32 / N));
-        if (threadIdx.x == 0) mbar_expect_tx(bar, entries * N * (int)sizeof(float));
-        if (lane < a.cluster) {
+        if (ok && threadIdx.x == 0) mbar_expect_tx(bar, entries * N * (int)sizeof(float));
+        if (ok && lane < a.cluster) {
 #pragma unroll
           for (int i = 0; i < N; i += 4) peer_send4(at + 4 * i, bar, lane, make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
         }
@@ -728,6 +736,7 @@ __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __
     if (other || first + 1 == end) turn(first);
   }
   if (a.cluster > 1) cluster_sync();                    // nobody leaves while sums are on their way to it
+  if (!ok) rn_outlast(there_s);
   auto leave = [&](const float2 (&v)[4], int slot) {
     if (slot >= 0) rn_store_eight(a.parts, ACTNN_F32, ((size_t)run * a.slots + slot) * C, c, C, v);
   };

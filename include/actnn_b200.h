@@ -567,7 +567,7 @@ int actnn_philox_state(const int64_t* seed, const int64_t* offset, uint64_t more
  * that are not wanted are NULL.  Those of parameters and gate are sums over rows in a fixed order, float32,
  * rounded once.  Workspace: 16-byte aligned, actnn_residual_norm_workspace bytes.  Blocks that share a row (C above
  * 4096) wait for one another's sums within limits: a wait that runs out is counted (actnn_bulk_wait_failures), and
- * the row's gradients and those after it are NaN.
+ * the gradients that waited are NaN, those of the run's later rows too.
  * The reference has no counterpart (its norms are batch norms, actnn/actnn/ops.py:444-500). */
 int actnn_residual_norm_forward(const void* x, const void* f, const void* weight, const void* bias,
                                 const void* post_weight, const void* post_bias, const void* gate, void* r, void* h,
