@@ -94,6 +94,14 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
+def _capturing(idx: int) -> bool:
+    """Whether the current stream of device ``idx`` is being captured into a graph."""
+    if idx == torch.cuda.current_device():
+        return torch.cuda.is_current_stream_capturing()
+    with torch.cuda.device(idx):
+        return torch.cuda.is_current_stream_capturing()
+
+
 _scratch = {}
 
 
@@ -101,8 +109,12 @@ def scratch(device: torch.device, nbytes: int) -> torch.Tensor:
     """A uint8 scratch buffer of at least ``nbytes`` for kernels launched on the CURRENT stream
     of ``device``.  One grow-only buffer per (device, stream): the kernels that share it run in
     stream order, so the next user only starts when the previous one is done.  Saves a trip to
-    the allocator in every layer of every step."""
+    the allocator in every layer of every step.  While the stream is being captured: a buffer of the graph's own.  The kept one
+    would be written by every replay, also at the same time as another graph's on another stream, and after a larger one has
+    taken its place and its memory is somebody else's."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
+    if _capturing(idx):
+        return torch.empty((max(int(nbytes), 1) + 255) // 256 * 256, dtype=torch.uint8, device=device)
     key = (idx, stream_of_index(idx))
     buf = _scratch.get(key)
     if buf is None or buf.numel() < nbytes:
@@ -121,12 +133,7 @@ def ticket(device: torch.device) -> torch.Tensor:
     could not be shared with a graph: made during a capture it is only cleared when that graph runs, and a
     replay on another stream would use it at the same time."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx == torch.cuda.current_device():
-        capturing = torch.cuda.is_current_stream_capturing()
-    else:
-        with torch.cuda.device(idx):
-            capturing = torch.cuda.is_current_stream_capturing()
-    if capturing:
+    if _capturing(idx):
         return torch.zeros(256, dtype=torch.uint8, device=device)
     key = (idx, stream_of_index(idx))
     buf = _tickets.get(key)
