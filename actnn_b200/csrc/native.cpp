@@ -862,9 +862,10 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
 };
 
 // x, weight, bias -> x weight^T + bias in 8-bit floating point.  Kept are the codes that the gradients multiply: those of x along the
-// tokens, those of the weight along the output channels, and of these only what a gradient asked for needs.
+// tokens, those of the weight along the output channels, and of these only what a gradient asked for needs.  `grad`: whether there can be
+// any (here it cannot be seen, and a leaf asks for its gradient all the same).
 struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const OptTensor& bias, bool grad) {
     check_values(x, "x");
     check_values(weight, "weight");
     TORCH_CHECK(weight.dim() == 2 && x.dim() >= 1 && x.size(-1) == weight.size(1), "shapes ", x.sizes(), " and ", weight.sizes(),
@@ -876,7 +877,7 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
     c10::cuda::CUDAGuard guard(x.device());
     int64_t rows = 1;
     for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
-    const bool keep_x = weight.requires_grad(), keep_w = x.requires_grad();
+    const bool keep_x = grad && weight.requires_grad(), keep_w = grad && x.requires_grad();
     Tensor out = make(with_last(x, n), x.scalar_type(), x);
     const Tensor b = with ? bias->to(x.scalar_type()).contiguous() : Tensor();
     FpTiles cx, cw;
@@ -915,14 +916,14 @@ struct Fp8Linear : torch::autograd::Function<Fp8Linear> {
       if (want_x) gx.zero_();
       if (want_w) gw.zero_();
       if (want_b) gb = go.sum(0).to((at::ScalarType)bias_type);
-      return {gx, gw, gb};
+      return {gx, gw, gb, Tensor()};
     }
     const auto [flat, ld] = as_rows(go);
     const FpTiles c = fp8_tile_codes(flat, rows, n, ld, want_x, want_w, want_b, false);
     if (want_x) fp8_product(c.here, {saved[2], saved[3]}, Tensor(), gx, rows, k, n);
     if (want_w) fp8_product(c.there, {saved[0], saved[1]}, Tensor(), gw, n, k, rows);
     if (want_b) gb = fp8_join_sums(c.parts, (at::ScalarType)bias_type);
-    return {gx, gw, gb};
+    return {gx, gw, gb, Tensor()};
   }
 };
 
@@ -1035,7 +1036,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return norm_forward(x, groups, w, b, eps, activation_kind(name), false, false).y;
   });
   m.def("fp8_linear", &fp8_linear);
-  m.def("fp8_linear_train", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return Fp8Linear::apply(x, w, b); });
+  m.def("fp8_linear_train", [](const Tensor& x, const Tensor& w, const OptTensor& b) { return Fp8Linear::apply(x, w, b, at::GradMode::is_enabled()); });
   m.def("seeded_dropout", [](const Tensor& x, double p, const OptKey& key) { return SeededDropout::apply(x, p, key); });
   m.def("residual_norm", [](const Tensor& x, const Tensor& f, const OptTensor& weight, const OptTensor& bias, const OptTensor& post_weight,
                             const OptTensor& post_bias, const OptTensor& gate, double scale, double p, double eps, int64_t layer, bool post,

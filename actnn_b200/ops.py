@@ -793,12 +793,12 @@ class group_norm:
 # ---------------------------------------------------------------------------------------
 class _Fp8Linear(Function):
     @staticmethod
-    def forward(ctx, input, weight, bias=None):
+    def forward(ctx, input, weight, bias, grad):              # grad: whether gradients are recorded, which cannot be seen here
         with _autocast_off():
             if weight.dim() != 2 or input.dim() < 1 or input.shape[-1] != weight.shape[1]:
                 raise RuntimeError("shapes %s and %s cannot be multiplied" % (tuple(input.shape), tuple(weight.shape)))
             x = input.reshape(input.shape[:-1].numel(), input.shape[-1])
-            need_x, need_w = ctx.needs_input_grad[:2]
+            need_x, need_w = (grad and need for need in ctx.needs_input_grad[:2])
             here, there, _ = ext_fp8.tile_codes(x, True, True) if need_w else (ext_fp8.quantize(x), None, None)
             whole = ext_fp8.quantize_weight(weight, both=need_x)
             output = ext_fp8.matmul(*here, *whole[:2], bias, input.dtype).view(input.shape[:-1] + weight.shape[:1])
@@ -817,7 +817,7 @@ class _Fp8Linear(Function):
             grad_input = ext_fp8.matmul(*here, *weight, None, dtype).view(shape) if need_x else None
             grad_weight = ext_fp8.matmul(*there, _kept(tokens[0]).view(ext_fp8.CODES), tokens[1], None, wdtype) if need_w else None
             grad_bias = ext_fp8.join_sums(parts, bdtype) if need_b else None
-        return grad_input, grad_weight, grad_bias
+        return grad_input, grad_weight, grad_bias, None
 
 
 class fp8_linear:
@@ -834,7 +834,7 @@ class fp8_linear:
         nat = _lib.native()
         if nat and not config.swap:
             return nat.fp8_linear_train(input, weight, bias)
-        return _Fp8Linear.apply(input, weight, bias)
+        return _Fp8Linear.apply(input, weight, bias, torch.is_grad_enabled())
 
 
 class _SeededDropout(Function):
