@@ -13,6 +13,7 @@ The reference's norms are batch norms (actnn/actnn/ops.py:444-500); it has no co
 import ctypes
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 from ._checks import FLOAT_TYPES, check_cuda_values
@@ -28,6 +29,12 @@ def norm_kind(kind):
         return KINDS[kind]
     except (KeyError, TypeError):
         raise RuntimeError("kind must be one of layer, rms, got %r" % (kind,)) from None
+
+
+def _no_tangents(**tensors):
+    for name, t in tensors.items():
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise RuntimeError("%s has a forward-mode tangent, which residual_norm does not pass on" % name)
 
 
 def _inputs(x, branch):
@@ -83,6 +90,7 @@ def run(x, branch, weight=None, bias=None, post_weight=None, post_bias=None, gat
     _inputs(x, branch)
     if branch.dtype != x.dtype:
         raise RuntimeError("x and branch must have the same type")
+    _no_tangents(x=x, branch=branch, weight=weight, bias=bias, post_weight=post_weight, post_bias=post_bias, gate=gate)
     params, pdtype = _parameters(x, weight, bias, post_weight, post_bias, post, layer)
     each = gate_rows(x, gate)
     gate = None if gate is None else gate.detach().contiguous()
@@ -103,7 +111,7 @@ def run(x, branch, weight=None, bias=None, post_weight=None, post_bias=None, gat
 
 
 def inference(x, branch, weight=None, bias=None, post_weight=None, post_bias=None, gate=None, scale=1.0, eps=1e-5, kind="rms", post=True):
-    """``(r, h)`` alone, without dropout."""
+    """``(r, h)`` alone, without dropout.  No gradient passes through it: training goes through ``ops.residual_norm``."""
     nat = _lib.native()
     if nat:
         return nat.residual_norm_value(x, branch, weight, bias, post_weight, post_bias, gate, float(scale), 0.0, float(eps), norm_kind(kind),

@@ -648,6 +648,11 @@ void check_pair(const Tensor& x, const Tensor& f) {
   TORCH_CHECK(x.dim() >= 1 && x.sizes() == f.sizes(), "x and branch must have the same shape of at least one dimension, got ", x.sizes(), " and ", f.sizes());
 }
 
+// What passes autograd by refuses a forward-mode tangent instead of dropping it.
+void check_no_tangent(const OptTensor& t, const char* name) {
+  TORCH_CHECK(!t.has_value() || !t->defined() || !t->_fw_grad(0).defined(), name, " has a forward-mode tangent, which residual_norm does not pass on");
+}
+
 // with_minmax: also min and max of every 256 outputs, not differentiable
 struct Relu : torch::autograd::Function<Relu> {
   static variable_list forward(AutogradContext* ctx, const Tensor& x, bool with_minmax) {
@@ -1051,6 +1056,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
                                   const OptKey& key) {
     check_pair(x, f);
     TORCH_CHECK(x.scalar_type() == f.scalar_type(), "x and branch must have the same type");
+    check_no_tangent(x, "x"), check_no_tangent(f, "branch"), check_no_tangent(weight, "weight"), check_no_tangent(bias, "bias");
+    check_no_tangent(post_weight, "post_weight"), check_no_tangent(post_bias, "post_bias"), check_no_tangent(gate, "gate");
     c10::cuda::CUDAGuard guard(x.device());
     const Residual q = residual_of(x, given(weight), given(bias), given(post_weight), given(post_bias), given(gate), scale, p, eps, (int)layer, post);
     const ResidualOut o = residual_forward(x.detach(), f.detach(), q, p > 0 ? make_key(key, x) : Key{}, false, false);
