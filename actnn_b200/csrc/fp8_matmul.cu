@@ -11,7 +11,7 @@
 // reduction split over a cluster where the tiles are too few; pairs of blocks on 256 channels where they are many.  Scales lie in global
 // memory as the instructions read them, 512 bytes for 128 rows and four blocks: they come with the first stage of the four,
 // go to tensor memory by tcgen05.cp, and each of the next stages names its byte of a column.  Two accumulators of 224 columns leave
-// 64 for scales, four sets of 16, so that none is overwritten while instructions that read it may be under way.  Split sums
+// 64 for scales, four sets of 12; a wide one of 448 as many, three of 20: none is overwritten while instructions that read it may be under way.  Split sums
 // are joined in the order of the blocks, so a shape's results are reproducible.
 //
 // 16384 x 4096 x 8192: 406 us in long runs, 2.7 PFLOP/s, the power cap; 8192 x 2048 x 4096 and its two gradients 59 to 62 each (2.3);
@@ -237,7 +237,7 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
         scales_to_tmem<PAIR>(at_w, from);
         scales_to_tmem<PAIR>(at_w + 4, from + 512);
         if (a.atoms > 1) scales_to_tmem<PAIR>(at_w + 8, from + 1024);
-        if (a.atoms > 2) scales_to_tmem<PAIR>(at_w + 12, from + 1536);
+        if (WIDE && a.atoms > 2) scales_to_tmem<PAIR>(at_w + 12, from + 1536);
         if (WIDE && a.atoms > 3) scales_to_tmem<PAIR>(at_w + 16, from + 2048);
       };
       auto multiply = [&](int at, int k, int half) {
@@ -458,7 +458,7 @@ void plan(FpArgs& a) {
     const int step = wide ? 64 : a.T <= 16 && !boxes ? 16 : 32;
     tokens = (tokens + step - 1) / step * step;
     if (tokens < a.T) tokens = (tokens + 63) / 64 * 64;
-    if (tokens > (wide ? kFpWide : splits > 1 ? 256 : kFpTokens) || (wide && tokens < 256)) return;
+    if (tokens > (wide ? kFpWide : kFpTokens) || (wide && tokens < 256)) return;
     const int channels = pair ? 2 * kFpChannels : kFpChannels;
     const int64_t channel_tiles = (a.N + channels - 1) / channels, tiles = channel_tiles * ((a.T + tokens - 1) / tokens);
     const int64_t blocks = tiles * splits * (pair ? 2 : 1), waves = (blocks + sms - 1) / sms;
