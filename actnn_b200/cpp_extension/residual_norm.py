@@ -125,6 +125,8 @@ def backward(grad_r, grad_h, saved, stats, weight=None, bias=None, post_weight=N
     returned as codes, or ``(x, branch)``.  One of the two gradients may be ``None``."""
     layer, p, (seed, offset) = norm_kind(kind), check_probability(p), check_key(key)
     like = grad_r if grad_r is not None else grad_h
+    if like is None:
+        raise RuntimeError("one of grad_r and grad_h must be given")
     for g, name in ((grad_r, "grad_r"), (grad_h, "grad_h")):
         if g is not None:
             check_cuda_values(g, name, like.device)
