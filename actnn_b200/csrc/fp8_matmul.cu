@@ -14,7 +14,8 @@
 // 64 for scales, four sets of 12; a wide one of 448 as many, three of 20: none is overwritten while instructions that read it may be under way.  Split sums
 // are joined in the order of the blocks, so a shape's results are reproducible.
 //
-// 16384 x 4096 x 8192: 406 us in long runs, 2.7 PFLOP/s, the power cap; 8192 x 2048 x 4096 and its two gradients 59 to 62 each (2.3);
+// 16384 x 4096 x 8192: 407 us in short runs, 2.7 PFLOP/s, 476 in long ones, where the power cap sets the clock; 8192 x 2048 x 4096 and its two
+// gradients 60 to 64 each (2.2), in long runs 68 to 73;
 // 200 x 4096 x 4096: 14, bound by what an SM gets from the L2 (51 bytes a cycle, 24 KB a stage) and latency (the weight's bytes from HBM 2.6).
 //
 // Every wait is bounded, with the integer product's rules: a block whose wait runs out writes nothing more, is counted, lets its copies
@@ -442,10 +443,10 @@ fp8_matmul_kernel(const __grid_constant__ CUtensorMap weights, const __grid_cons
 // ------------------------------------------------------------------ host
 // The cut: tokens of a tile, blocks that share a reduction, pairs or single blocks, two accumulators or a wide one, by what they are
 // expected to take (us): a stage, which is no shorter than its instructions take to issue, and what a tile takes besides.  Fitted to
-// times of all cuts in long runs, where the power cap sets the clock: 16384 x 4096 x 8192, 448 tokens wide 462, 192 by pairs 484, by single
-// blocks 546; 8192 x 2048 x 4096, 192 by pairs 72, 384 wide 74, 192 by single blocks 78; 4096 x 512 x 16384, 192 by single blocks 51, by
-// pairs 65, 448 wide 68; 1024 x 4096 x 4096, 256 wide 20.5, 128 by pairs 24.3; 100 x 8192 x 2048, 64 shared by four 10.5, by two 14.6, alone
-// 19.9.  Eight blocks that share a reduction find room for few such clusters at a time: 100 x 8192 x 2048 18.2 in two rounds.
+// times of all cuts in long runs, where the power cap sets the clock; they are now: 16384 x 4096 x 8192, 448 tokens wide 476, 384 wide 479, 192 by
+// pairs 493, by single blocks 564; 8192 x 2048 x 4096, 192 by pairs 73, 384 wide 76, 448 wide 80, 192 by single blocks 81; 4096 x 512 x 16384,
+// 192 by single blocks 53, by pairs 64, 448 wide 68; 1024 x 4096 x 4096, 256 wide 20.5, 128 by pairs 25; 100 x 8192 x 2048, 64 shared by
+// four 12.3, by two 16.4, alone 22.5.  Eight blocks that share a reduction find room for few such clusters at a time, and are offered where all do.
 void plan(FpArgs& a) {
   const int sms = device_info().sm_count;
   const int64_t least = a.T <= kFpTokens ? 1 : (a.T + kFpTokens / 64 * 64 - 1) / (kFpTokens / 64 * 64);

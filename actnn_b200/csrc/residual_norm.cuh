@@ -21,9 +21,10 @@
 // a mean (rms) has p = 0, so that its own channel is NaN and the row's others are zero.  The gradients of such a row are NaN, and no other row's are
 // touched.
 //
-// 8192 x 4096 bf16 with dropout: forward 80 us, backward 100, the join 6 (51 and 51 at the copy rate); 16384 x 8192 f16 without: 254, 382, 8
-// (205 each); 12608 x 768 float32, layer kind: 32, 36, 6.  Both directions are bound by instructions, some 470 a warp's 256 channels
-// backward: dropout's generator takes 70 of them, and registers allow 16 warps an SM backward.
+// 8192 x 4096 bf16 with dropout: forward 80 us, backward 102, the join 6 (51 and 51 at the copy rate); 16384 x 8192 f16 without: 251, 355, 8
+// (205 each); 12608 x 768 float32, layer kind: 32, 37, 6 (27 each).  Forward is bound by instructions (issue slots 71 % busy); backward by
+// some 470 of them a warp's 256 channels, of which dropout's generator takes 70, and by a row's barrier: registers allow one block of 16 warps an
+// SM, which stand at it together (issue slots 56 % busy).
 #pragma once
 
 #include <algorithm>
@@ -530,11 +531,11 @@ ACTNN_DEV void rn_outlast(const uint64_t* bars) {
 // and sends nothing more, so that the other warps' waits for the next row run out too: had it gone on, its later sums would be
 // counted and read as those of rows that others have not done with.
 //
-// What bounds it are instructions, so the gate g and w1 enter as their product, and what
+// Fewer instructions: the gate g and w1 enter as their product, and what
 // depends on the rows of one gate alone is summed once: with S = sum m t n1 and S' = sum m t, dw1 = g S, db1 = g S', dg = w1 S + b1 S'.
 // These products, in shared memory as float32, are a thread's own: g w1, g b1 and w2, and dw1 and db1 over the gates.
-// (With gate, w1 and each gradient's sums apart: 8192 x 4096 116 us, 16384 x 8192 500.  The second half of a row's work done after the
-// next row's first half, past the barrier: 138 us, what it holds in registers and copies costs more.)
+// (With gate, w1 and each gradient's sums apart: 8192 x 4096 116 us where 102 are taken now, 16384 x 8192 500 (355).  The second half of a row's
+// work done after the next row's first half, past the barrier: 138 us, what it holds in registers and copies costs more.)
 template <typename T, bool VEC, bool CODED, bool LAYER>
 __global__ void __launch_bounds__(kRnMostThreads, 1) rn_backward_kernel(const __grid_constant__ RnArgs a, unsigned* gave_up) {
   constexpr int N = LAYER ? 8 : 4, kWarps = kRnMostThreads / 32;
